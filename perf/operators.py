@@ -342,8 +342,8 @@ def _quantise(x, fine):
     x = torch.where(fine.unsqueeze(-1), x.float(), torch.zeros((), device=x.device))
     top = x.abs().amax(-1)
     m, e = torch.frexp(top)
-    e = (e - 9 + (m > 0.875).to(e.dtype)).clamp(-117, 119)
-    e = torch.where(top == 0, torch.full_like(e, -117), e)
+    e = (e - 9 + (m > 0.875).to(e.dtype)).clamp(-60, 60)
+    e = torch.where(top == 0, torch.full_like(e, -60), e)
     y = (x * _power(-e).unsqueeze(-1)).clamp(-E4M3_MAX, E4M3_MAX)
     return y.to(torch.float8_e4m3fn).view(torch.uint8), torch.where(fine, e, 128).to(torch.int16)
 
@@ -515,7 +515,7 @@ def _exact_rows(x):
     x = x.double()
     top = x.abs().amax(-1, keepdim=True)
     two = lambda n: ((n.long() + 1023) << 52).view(torch.float64)  # noqa: E731  2^n, exactly
-    power = torch.ceil(torch.log2(top / E4M3_MAX)).clamp(-116, 118)
+    power = torch.ceil(torch.log2(top / E4M3_MAX)).clamp(-59, 59)
     power = torch.where(top > E4M3_MAX * two(power), power + 1, power)
     power = torch.where(top <= E4M3_MAX * two(power - 1), power - 1, power)
     y = x / two(power)
