@@ -1,0 +1,628 @@
+"""The streaming operators against their definitions in float64 (oracle/streaming.py)."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from oracle import streaming as O
+from vasc_amd import ops
+from vasc_amd.streaming import BlockCache
+
+pytestmark = pytest.mark.gpu
+
+HALF = {torch.bfloat16: 2.0 ** -9 * 2, torch.float16: 2.0 ** -12 * 2, torch.float32: 2.0 ** -25 * 2}  # half a step
+
+
+def _gen(seed):
+    return torch.Generator().manual_seed(seed)
+
+
+def _np(t):
+    return t.detach().double().cpu().numpy()
+
+
+def _i32(x):
+    return torch.tensor(x, dtype=torch.int32, device="cuda")
+
+
+def _randn(g, *shape, dtype=torch.bfloat16):
+    return torch.randn(*shape, generator=g).to(dtype)
+
+
+def _table(g, B, mp, spare=3):
+    """(page table with pages in random order, pages of the cache)."""
+    pages = B * mp + spare
+    return torch.randperm(pages, generator=g)[:B * mp].view(B, mp).to(torch.int32).cuda(), pages
+
+
+# ------------------------------------------------------------------ rotary
+def _freq(sections, bases):
+    return torch.cat([b ** (-torch.arange(0, s, 2, dtype=torch.float64) / s) for s, b in zip(sections, bases)])
+
+
+def _rotary_bound(x, ref, sections, dtype):
+    """Output rounding, and float32 arithmetic on the pair: cos and sin within 2^-22 of exact (the correction term leaves
+    sincosf's last place and the reduction's 2^-24), two products and a sum of three roundings."""
+    x = _np(x)
+    size = np.abs(x).copy()
+    at = 0
+    for d in sections:
+        h = d // 2
+        s = np.abs(x[..., at:at + h]) + np.abs(x[..., at + h:at + d])
+        size[..., at:at + h] = size[..., at + h:at + d] = s
+        at += d
+    size[..., at:] = 0
+    return HALF[dtype] * np.abs(ref) + (2.0 ** -22 + 3 * 2.0 ** -24) * size * (1 + HALF[dtype]) + 2.0 ** -25
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("D,sections,T", [(64, (16, 24, 24), 37), (128, (32, 48, 48), 9), (64, (32, 32), 1),
+                                          (64, (6, 28, 28), 130), (80, (16, 16, 16, 16), 21), (64, (2, 6, 10), 50),
+                                          (64, (64,), 600)])
+def test_rotary_matches_float64(dtype, D, sections, T):
+    g = _gen(D + T)
+    B, Hq, Hk = 2, 5, 3
+    q, k = _randn(g, B, T, Hq, D, dtype=dtype).cuda().transpose(1, 2), _randn(g, B, Hk, T, D, dtype=dtype).cuda()
+    pos = torch.randint(-50, 5000, (B, T, len(sections)), generator=g)
+    freq = _freq(sections, (10000.0, 100.0, 100.0, 50.0))
+    qo, ko = ops.rotary_axes(q, k, pos.cuda(), sections, freq.cuda())
+    for x, y in ((q, qo), (k, ko)):
+        ref = O.rotate(_np(x), pos.numpy(), sections, freq.numpy())
+        assert y.shape == x.shape and y.dtype == dtype
+        assert (np.abs(_np(y) - ref) <= _rotary_bound(x, ref, sections, dtype)).all()
+        assert torch.equal(y[..., sum(sections):], x[..., sum(sections):])
+    assert qo.stride() == q.stride() and ko.stride() == k.stride()
+
+
+def test_rotary_far_positions_and_shared_rows():
+    """Positions of 2^31 - 1: a float32 angle would be off by tens of radians. One row of positions for all sequences."""
+    g = _gen(3)
+    sections = (16, 24, 24)
+    x = _randn(g, 3, 2, 40, 64, dtype=torch.float32).cuda()
+    pos = torch.randint(2 ** 30, 2 ** 31 - 1, (40, 3), generator=g)
+    pos[0] = 2 ** 31 - 1
+    pos[1] = -2 ** 31
+    freq = _freq(sections, (10000.0, 100.0, 100.0))
+    y, none = ops.rotary_axes(x, None, pos.cuda(), sections, freq.cuda())
+    assert none is None
+    ref = O.rotate(_np(x), pos.numpy()[None], sections, freq.numpy())
+    # the float64 angle itself is rounded: 2^31 * 2^-53 on both sides
+    bound = _rotary_bound(x, ref, sections, torch.float32) + 2 ** -21 * (np.abs(_np(x)).max() * 2)
+    assert (np.abs(_np(y) - ref) <= bound).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_rotary_gradients(dtype):
+    """Against the formula (the inverse turn), with shared and broadcast inputs, one gradient missing, and differences."""
+    g = _gen(11)
+    sections, D, T = (16, 24, 24), 72, 33
+    freq = _freq(sections, (10000.0, 100.0, 100.0)).cuda()
+    pos = torch.randint(0, 900, (2, T, 3), generator=g).cuda()
+    q = _randn(g, 2, 4, T, D, dtype=dtype).cuda().requires_grad_()
+    k = _randn(g, 1, 1, T, D, dtype=dtype).cuda().requires_grad_()
+    gq, gk = _randn(g, 2, 4, T, D, dtype=dtype).cuda(), _randn(g, 2, 3, T, D, dtype=dtype).cuda()
+    qo, ko = ops.rotary_axes(q, k.expand(2, 3, T, D), pos, sections, freq)
+    dq, dk = torch.autograd.grad([qo, ko], [q, k], [gq, gk])
+    ref = O.rotate(_np(gq), pos.cpu().numpy(), sections, freq.cpu().numpy(), -1.0)
+    assert (np.abs(_np(dq) - ref) <= _rotary_bound(gq, ref, sections, dtype)).all()
+    each = O.rotate(_np(gk), pos.cpu().numpy(), sections, freq.cpu().numpy(), -1.0)
+    # six gradients summed by torch (a rounding for each of at most two sums of partial results, and their own)
+    bound = _rotary_bound(gk, each, sections, dtype).sum((0, 1)) + 6 * HALF[dtype] * np.abs(each).sum((0, 1))
+    assert (np.abs(_np(dk)[0, 0] - each.sum((0, 1))) <= bound).all()
+    # only one of the outputs is used
+    _, ko = ops.rotary_axes(q, k.expand(2, 3, T, D), pos, sections, freq)
+    dq, dk2 = torch.autograd.grad([ko], [q, k], [gk], allow_unused=True)
+    assert dq is None and torch.equal(dk2, dk)
+    if dtype == torch.float32:  # differences: the map is linear, so a difference of a long step is its rounding off
+        d = _randn(g, 2, 4, T, D, dtype=dtype).cuda()
+        with torch.no_grad():
+            up = ops.rotary_axes(q + d, None, pos, sections, freq)[0].double()
+            dn = ops.rotary_axes(q - d, None, pos, sections, freq)[0].double()
+        qo = ops.rotary_axes(q, None, pos, sections, freq)[0]
+        dq, = torch.autograd.grad(qo, q, gq)
+        lhs = ((up - dn) / 2 * gq.double()).sum().item()
+        rhs = (dq.double() * d.double()).sum().item()
+        n = gq.numel()
+        assert abs(lhs - rhs) <= 2.0 ** -20 * math.sqrt(n) * 40
+    # broadcast gradient (stride 0 everywhere)
+    qo = ops.rotary_axes(q, None, pos, sections, freq)[0]
+    dq, = torch.autograd.grad(qo.sum(), q)
+    ref = O.rotate(np.ones(q.shape), pos.cpu().numpy(), sections, freq.cpu().numpy(), -1.0)
+    assert (np.abs(_np(dq) - ref) <= _rotary_bound(torch.ones(q.shape), ref, sections, dtype)).all()
+
+
+def test_rotary_odd_strides_and_empty():
+    """Rows that start at odd elements, a transposed layout, no tokens, no heads."""
+    g = _gen(5)
+    sections = (8, 8)
+    freq = _freq(sections, (100.0, 100.0))
+    pos = torch.randint(0, 40, (1, 19, 2), generator=g)
+    wide = _randn(g, 2, 3, 19, 37).cuda()
+    for x in (wide[..., 1:21], wide[..., 2:34], wide.permute(0, 2, 3, 1)[:, :, :19, :].transpose(1, 2)[..., :2]):
+        if x.shape[-1] < 16:
+            with pytest.raises(ValueError, match="sections"):
+                ops.rotary_axes(x, None, pos.cuda(), sections, freq.cuda())
+            continue
+        y = ops.rotary_axes(x, None, pos.cuda(), sections, freq.cuda())[0]
+        ref = O.rotate(_np(x), pos.numpy(), sections, freq.numpy())
+        assert (np.abs(_np(y) - ref) <= _rotary_bound(x, ref, sections, torch.bfloat16)).all()
+    e = torch.zeros(2, 3, 0, 32, device="cuda")
+    out, _ = ops.rotary_axes(e, None, pos[:, :0].cuda(), sections, freq.cuda())
+    assert out.shape == e.shape
+
+
+# ------------------------------------------------------------------ the cache: write and read
+def _fill(cache, g, table, lens, k=None, v=None):
+    """Random history; returns the held values, float64 [B][H,len,D]."""
+    B, H, D, L = len(lens), cache.heads, cache.head_dim, max(max(lens), 1)
+    k = _randn(g, B, H, L, D) if k is None else k
+    v = _randn(g, B, H, L, D) if v is None else v
+    ops.cache_write(cache, k.cuda(), v.cuda(), table, _i32([0] * B), count=_i32(lens))
+    held = [O.quantise(_np(k[b, :, :n]), _np(v[b, :, :n])) for b, n in enumerate(lens)]
+    return held
+
+
+def _same(a, b):
+    return np.array_equal(a, b, equal_nan=True)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("D,H", [(64, 3), (128, 2)])
+def test_write_then_read(dtype, D, H):
+    """Values of many magnitudes at ragged places, from strided rows; every other byte of the cache stays."""
+    g = _gen(D)
+    B, T, mp = 4, 150, 6
+    table, pages = _table(g, B, mp)
+    start, count = [0, 61, 130, 64], [150, 70, 0, 1]
+    cache = BlockCache(pages, H, D)
+    for t in (cache.kc, cache.vc):  # finite codes everywhere
+        t.copy_(torch.randint(0, 0x7e, t.shape, generator=g, dtype=torch.uint8))
+    for t in (cache.ks, cache.vs):
+        t.copy_(torch.randint(110, 140, t.shape, generator=g, dtype=torch.uint8))
+    cache.mean.copy_(torch.randn(cache.mean.shape, generator=g))
+    before = {n: getattr(cache, n).clone() for n in ("kc", "vc", "ks", "vs", "mean")}
+    mag = torch.exp2(torch.randint(-12, 12, (B, T, H, 1), generator=g).float())
+    k = (torch.randn(B, T, H, D, generator=g) * mag).to(dtype).cuda().transpose(1, 2)
+    v = (torch.randn(B, T, H, D, generator=g) * mag.flip(1)).to(dtype).cuda().transpose(1, 2)
+    old_k, old_v = ops.cache_read(cache, table, _i32([0] * B), mp * 64, dtype=torch.float32)
+    ops.cache_write(cache, k, v, table, _i32(start), count=_i32(count))
+    rk, rv = ops.cache_read(cache, table, _i32(start), T, count=_i32(count), dtype=torch.float32)
+    all_k, all_v = ops.cache_read(cache, table, _i32([0] * B), mp * 64, dtype=torch.float32)
+    touched = set()
+    for b in range(B):
+        s, n = start[b], count[b]
+        ko, vo = O.quantise(_np(k[b, :, :n]), _np(v[b, :, :n]))
+        assert _same(_np(rk[b, :, :n]), ko) and _same(_np(rv[b, :, :n]), vo)
+        assert not rk[b, :, n:].any() and not rv[b, :, n:].any()
+        want_k, want_v = _np(old_k[b]), _np(old_v[b])
+        want_k[:, s:s + n], want_v[:, s:s + n] = ko, vo
+        assert _same(_np(all_k[b]), want_k) and _same(_np(all_v[b]), want_v)
+        for j in range(s // 64, (s + n - 1) // 64 + 1 if n else s // 64):
+            p = int(table[b, j])
+            touched.add(p)
+            part = want_k[:, j * 64:min(j * 64 + 64, s + n)]
+            mean = O.round_bf16((part.sum(1) / part.shape[1]).astype(np.float32))
+            assert _same(_np(cache.mean[p]), mean.astype(np.float64))
+    rest = [p for p in range(pages) if p not in touched]
+    for n, t in before.items():
+        assert torch.equal(getattr(cache, n)[rest], t[rest]), n
+
+
+@pytest.mark.parametrize("D", [64, 128])
+def test_write_edge_values(D):
+    """Rows at the borders of the format: powers of two, 448 * 2^e and one step past it, e4m3 ties and subnormals, zero,
+    the exponents' ends, float32's largest and smallest; tokens that are not finite."""
+    step = 1 + 2.0 ** -10
+    rows = [[448.0], [448.0 * step], [1.75, 0.4375], [1.75 * step, 1.0], [0.0], [-0.0], [2.0 ** -70, 2.0 ** -69],
+            [2.0 ** -126, 2.0 ** -149], [3.0e38, 1.0], [448 * 2.0 ** 60, 2.0 ** 53], [2.0 ** 127],
+            [17.0, 19.0, 21.0, 23.0, -17.0], [448.0, 2.0 ** -9, 2.0 ** -10, 3 * 2.0 ** -10, 2.0 ** -11],
+            [float("inf")], [1.0, float("nan")], [-float("inf"), 1.0]]
+    x = torch.zeros(1, 1, len(rows), D)
+    for i, r in enumerate(rows):
+        x[0, 0, i, :len(r)] = torch.tensor(r, dtype=torch.float64).float()
+        x[0, 0, i, D - 1] = x[0, 0, i, 0]
+    y = torch.full_like(x, 0.5)
+    y[0, 0, 2, 5] = float("nan")  # a value that is not finite marks the token's key too
+    table = _i32([[1]])
+    for a, b in ((x, y), (y, x)):
+        cache = BlockCache(2, 1, D)
+        ops.cache_write(cache, a.cuda(), b.cuda(), table, _i32([0]))
+        k, v = ops.cache_read(cache, table, _i32([0]), len(rows), dtype=torch.float32)
+        ko, vo = O.quantise(_np(a), _np(b))
+        assert _same(_np(k), ko) and _same(_np(v), vo)
+        assert cache.mean[1].isnan().all()  # NaN tokens in the page
+        ops.cache_write(cache, a[:, :, :2].cuda(), b[:, :, :2].cuda(), table, _i32([0]))  # written again, shorter
+        mean = O.round_bf16((ko[0, 0, :2].sum(0) / 2).astype(np.float32))
+        assert _same(_np(cache.mean[1, 0]), mean.astype(np.float64))
+        k16, _ = ops.cache_read(cache, table, _i32([0]), len(rows), dtype=torch.float16)
+        with np.errstate(over="ignore"):
+            assert _same(_np(k16), ko.astype(np.float16).astype(np.float64))
+
+
+def test_write_in_any_portions_gives_the_same_bytes():
+    g = _gen(17)
+    H, D, n = 2, 64, 200
+    k, v = _randn(g, 1, H, n, D).cuda(), _randn(g, 1, H, n, D).cuda()
+    table, pages = _table(g, 1, 4)
+    caches = []
+    for cuts in ([n], list(range(1, n + 1)), [3, 63, 64, 65, 127, 130, 192, n]):
+        c, at = BlockCache(pages, H, D), 0
+        for e in cuts:
+            ops.cache_write(c, k[:, :, at:e], v[:, :, at:e], table, _i32([at]))
+            at = e
+        caches.append(c)
+    for c in caches[1:]:
+        for name in ("kc", "vc", "ks", "vs", "mean"):
+            assert torch.equal(getattr(c, name), getattr(caches[0], name)), name
+
+
+def test_write_and_read_outside_the_table():
+    """Entries that are no page, a start past the table or below 0, more tokens than the table holds: nothing is written
+    there, and zeros are read."""
+    g = _gen(23)
+    cache = BlockCache(3, 1, 64)
+    table = _i32([[0, -1], [7, 1], [2, 3], [-5, -5], [5, 4]])
+    k, v = _randn(g, 5, 1, 200, 64).cuda(), _randn(g, 5, 1, 200, 64).cuda()
+    ops.cache_write(cache, k, v, table, _i32([0, 0, 0, 10, -3]))
+    rk, rv = ops.cache_read(cache, table, _i32([0, 0, 0, 10, -3]), 200, dtype=torch.float32)
+    for b, (lo, hi) in enumerate(((0, 64), (64, 128), (0, 64), (0, 0), (0, 0))):
+        ko, vo = O.quantise(_np(k[b, :, lo:hi]), _np(v[b, :, lo:hi]))
+        assert _same(_np(rk[b, :, lo:hi]), ko) and _same(_np(rv[b, :, lo:hi]), vo)
+        for r in (rk, rv):
+            assert not r[b, :, :lo].any() and not r[b, :, hi:].any()
+    before = cache.kc.clone()
+    ops.cache_write(cache, k, v, table, _i32([128, 2 ** 31 - 1, 1000, -2 ** 31, -1]))
+    assert torch.equal(before, cache.kc)
+    far, _ = ops.cache_read(cache, table, _i32([128, 2 ** 31 - 1, 1000, -2 ** 31, -1]), 70)
+    assert not far.any()
+
+
+# ------------------------------------------------------------------ choice
+def _check_select(q, cache, table, lens, held, keep, block_q, sink, recent, causal, n_q=None):
+    B, Hq, T, D = q.shape
+    H, mp = cache.heads, table.shape[1]
+    G, U = Hq // H, -(-T // block_q)
+    index, count, score = ops.cache_select(q, cache, table, _i32(lens), keep, block_q=block_q, sink=sink, recent=recent,
+                                           causal=causal, q_count=None if n_q is None else _i32(n_q), want_score=True)
+    assert index.shape == (B, H, U, min(mp, sink + keep + recent + ((block_q + 62) // 64 if causal else 0)))
+    i2, c2 = ops.cache_select(q, cache, table, _i32(lens), keep, block_q=block_q, sink=sink, recent=recent, causal=causal,
+                              q_count=None if n_q is None else _i32(n_q))
+    assert torch.equal(index, i2) and torch.equal(count, c2)
+    qn, index, count, score = _np(q), index.cpu().numpy(), count.cpu().numpy(), score.cpu().numpy()
+    for b in range(B):
+        nq = T if n_q is None else n_q[b]
+        for h in range(H):
+            means = O.page_means(held[b][0][h])
+            for u in range(U):
+                t0, t1 = u * block_q, min((u + 1) * block_q, nq)
+                seen, own = O.unit_pages(lens[b], nq, t0, t1, causal)
+                if seen == 0:
+                    want, s = [], np.zeros(0, np.float32)
+                else:
+                    rows = qn[b, h * G:(h + 1) * G, t0:t1].reshape(-1, D)
+                    want, s = O.select(rows, means, seen, own, keep, sink, recent)
+                n = count[b, h, u]
+                assert n == len(want), (b, h, u)
+                assert list(index[b, h, u, :n]) == want and (index[b, h, u, n:] == -1).all(), (b, h, u)
+                assert np.array_equal(score[b, h, u, :seen], s) and (score[b, h, u, seen:] == -np.inf).all()
+
+
+@pytest.mark.parametrize("D,H,G,T,block_q,causal", [(64, 2, 1, 1, 1, False), (128, 1, 5, 1, 1, False),
+                                                    (64, 1, 1, 300, 128, False), (128, 2, 4, 70, 32, True),
+                                                    (64, 2, 2, 130, 64, True), (64, 1, 128, 2, 1, False),
+                                                    (64, 1, 1, 9, 3, True)])
+def test_select_matches_definition(D, H, G, T, block_q, causal):
+    g = _gen(D + G + T)
+    lens = [1500, 64, 1, 0, 777, T]
+    if causal:
+        lens = [max(n, T) for n in lens]
+    table, pages = _table(g, len(lens), 25)
+    cache = BlockCache(pages, H, D)
+    held = _fill(cache, g, table, lens)
+    q = _randn(g, len(lens), H * G, T, D).cuda()
+    for keep, sink, recent in ((5, 1, 1), (0, 2, 3), (40, 0, 1)):
+        _check_select(q, cache, table, lens, held, keep, block_q, sink, recent, causal)
+
+
+@pytest.mark.parametrize("mp", [1, 255, 257, 2049, 8200])
+def test_select_long_tables(mp):
+    """Around the sizes at which the list kernel changes."""
+    g = _gen(mp)
+    H, D = 1, 64
+    table, pages = _table(g, 2, mp)
+    cache = BlockCache(pages, H, D)
+    lens = [mp * 64, mp * 64 - min(mp * 64, 100)]
+    means = torch.randn(pages, H, D, generator=g).bfloat16()
+    cache.mean.copy_(means)
+    q = _randn(g, 2, 2, 1, D).cuda()
+    for keep in (max(1, mp // 4), 3, mp - 1):
+        index, count, score = ops.cache_select(q, cache, table, _i32(lens), keep, want_score=True)
+        for b in range(2):
+            m = _np(means)[table[b].cpu().numpy(), 0]
+            want, s = O.select(_np(q)[b, :, 0], m, -(-lens[b] // 64), -(-lens[b] // 64) - 1, keep, 1, 1)
+            assert count[b, 0, 0] == len(want) and index[b, 0, 0, :len(want)].tolist() == want
+            assert np.array_equal(score[b, 0, 0, :len(s)].cpu().numpy(), s)
+
+
+def test_select_ties_nan_and_missing_pages():
+    """Equal scores go by page; NaN and missing pages come last; +0 and -0 are equal; queries past q_count choose nothing."""
+    H, D, mp = 1, 64, 600
+    cache = BlockCache(mp, H, D)
+    g = _gen(9)
+    level = torch.randint(-2, 3, (mp,), generator=g).float()
+    cache.mean[:, 0, 0] = level.cuda().bfloat16()
+    cache.mean[50, 0, 3] = float("nan")
+    cache.mean[60, 0, 0] = -0.0
+    table = torch.arange(mp, dtype=torch.int32).view(1, mp).cuda()
+    table[0, 70] = -1
+    table[0, 80] = mp
+    q = torch.zeros(1, 1, 3, D, dtype=torch.bfloat16, device="cuda")
+    q[0, 0, :, 0] = torch.tensor([1.0, -1.0, 0.0], device="cuda")
+    means = _np(cache.mean)[:, 0]
+    means[70] = means[80] = np.nan
+    for keep in (1, 100, 130, 350, 595, 598):
+        index, count = ops.cache_select(q, cache, table, _i32([mp * 64 - 5]), keep, sink=1, recent=1, q_count=_i32([2]))
+        for t in range(2):
+            want, _ = O.select(_np(q)[0, :, t], means, mp, mp - 1, keep, 1, 1)
+            assert index[0, 0, t, :len(want)].tolist() == want and count[0, 0, t] == len(want)
+        assert count[0, 0, 2] == 0 and (index[0, 0, 2] == -1).all()
+
+
+# ------------------------------------------------------------------ attention
+def _check_attend(o, q, held, lens, lists, block_q, causal, scale=None, n_q=None, H=None):
+    """o against float64 over the held values. Bound for an element: the output's rounding; weights rounded to half
+    (2^-11 of each term); an error of the float32 logits in weights and sum, (D + 8) 2^-24 of the products' magnitudes;
+    float32 sums over n keys, n 2^-24 of the terms' magnitudes, twice (weights and their sum), and 2^-20 for exp2, the
+    powers and the division; weights under 2^-36 of the largest, at most n of them."""
+    B, Hq, T, D = q.shape
+    G = Hq // H
+    scale = D ** -0.5 if scale is None else scale
+    qn, on = _np(q), _np(o)
+    assert not np.isnan(on).any()
+    worst = 0.0
+    for b in range(B):
+        nq = T if n_q is None else n_q[b]
+        for h in range(H):
+            k, v = held[b][0][h], held[b][1][h]
+            pos = np.arange(len(k))
+            for t in range(T):
+                seen = pos < lens[b]
+                if lists is not None:
+                    seen &= np.isin(pos // 64, lists[b][h][t // block_q])
+                if causal:
+                    seen &= pos <= lens[b] - nq + t
+                if t >= nq:
+                    seen &= False
+                for gi in range(G):
+                    ref, mag, logit = O.attend(qn[b, h * G + gi, t], k, v, seen, scale)
+                    n = int(seen.sum())
+                    rel = 2.0 ** -11 + 2 * ((D + 8) * 2.0 ** -24 * logit + n * 2.0 ** -24) + 2.0 ** -20
+                    bound = rel * mag + HALF[o.dtype] * (np.abs(ref) + rel * mag) + n * 2.0 ** -36 * np.abs(v).max(initial=0)
+                    if o.dtype == torch.float16:
+                        bound = bound + 2.0 ** -25
+                    err = np.abs(on[b, h * G + gi, t] - ref)
+                    assert (err <= bound).all(), (b, h, t, gi, (err - bound).max())
+                    worst = max(worst, float((err / (bound + 1e-30)).max()))
+    return worst
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("D,H,G", [(64, 2, 1), (128, 1, 4), (64, 1, 12), (128, 2, 1)])
+def test_attend_single_tokens(dtype, D, H, G):
+    g = _gen(D + G)
+    lens = [1, 63, 64, 65, 0, 700, 1300]
+    table, pages = _table(g, len(lens), 21)
+    cache = BlockCache(pages, H, D)
+    held = _fill(cache, g, table, lens)
+    q = _randn(g, len(lens), H * G, 1, D, dtype=dtype).cuda()
+    o = ops.cache_attn(q, cache, table, _i32(lens))
+    assert o.dtype == dtype
+    _check_attend(o, q, held, lens, None, 1, False, H=H)
+    assert not o[4].any()
+    for keep in (0, 3):
+        index, count = ops.cache_select(q, cache, table, _i32(lens), keep)
+        lists = [[[index[b, h, 0, :count[b, h, 0]].tolist()] for h in range(H)] for b in range(len(lens))]
+        o = ops.cache_attn(q, cache, table, _i32(lens), index, count)
+        _check_attend(o, q, held, lens, lists, 1, False, H=H)
+
+
+@pytest.mark.parametrize("D,H,G,T,block_q,L", [(64, 2, 1, 300, 128, 1200), (64, 1, 1, 40, 32, 500), (128, 1, 4, 70, 32, 600),
+                                               (64, 1, 2, 50, 16, 50), (128, 1, 8, 5, 2, 330), (128, 2, 1, 130, 64, 700)])
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_attend_chunks(D, H, G, T, block_q, L, causal, dtype):
+    g = _gen(D + T + L)
+    lens = [L, max(T, L - 77)]
+    table, pages = _table(g, 2, -(-L // 64) + 1)
+    cache = BlockCache(pages, H, D)
+    held = _fill(cache, g, table, lens)
+    q = _randn(g, 2, H * G, T, D, dtype=dtype).cuda()
+    n_q = [T, T - T // 3]
+    o = ops.cache_attn(q, cache, table, _i32(lens), causal=causal, q_count=_i32(n_q))
+    _check_attend(o, q, held, lens, None, block_q, causal, n_q=n_q, H=H)
+    index, count = ops.cache_select(q, cache, table, _i32(lens), 2, block_q=block_q, causal=causal, q_count=_i32(n_q))
+    lists = [[[index[b, h, u, :count[b, h, u]].tolist() for u in range(index.shape[2])] for h in range(H)] for b in range(2)]
+    o = ops.cache_attn(q, cache, table, _i32(lens), index, count, block_q=block_q, causal=causal, q_count=_i32(n_q))
+    _check_attend(o, q, held, lens, lists, block_q, causal, n_q=n_q, H=H)
+
+
+def test_attend_list_rules():
+    """Entries that repeat, fall back, lie outside or have no page are skipped; counts are cut to the list; rows that see
+    nothing are zero."""
+    g = _gen(31)
+    D, H, L = 64, 1, 640
+    table, pages = _table(g, 1, 12)
+    cache = BlockCache(pages, H, D)
+    held = _fill(cache, g, table, [L])
+    table[0, 4] = -1
+    q = _randn(g, 1, 1, 8, D).cuda()
+    rows = [[0, 2, 2, 5, 9, -1], [3, 1, 5, 5, 5, 5], [-1, -1, 7, 8, 9, 10], [4, 10, 11, 12, 300, 7], [0, 1, 2, 3, 4, 5],
+            [6, 7, 8, 9, 10, 11], [0, 1, 2, 3, 4, 5], [2, -7, 5, 6, 7, 8]]
+    counts = [6, 6, 6, 6, 3, 99, 0, -4]
+    want = [[0, 2, 5, 9], [3, 5], [7, 8, 9], [], [0, 1, 2], [6, 7, 8, 9], [], []]
+    o = ops.cache_attn(q, cache, table, _i32([L]), _i32(rows).view(1, 1, 8, 6), _i32(counts).view(1, 1, 8), block_q=1)
+    _check_attend(o, q, held, [L], [[want]], 1, False, H=1)
+    for t in (3, 6, 7):
+        assert not o[0, 0, t].any()
+
+
+def test_attend_masked_values_do_not_matter():
+    """NaN tokens past the length or behind a causal row change nothing; seen ones make exactly their rows NaN. Keys whose
+    logits are far apart, values whose powers are far apart, zero rows."""
+    g = _gen(37)
+    D, H, T, L = 64, 1, 40, 200
+    table, pages = _table(g, 1, 4)
+    k, v = _randn(g, 1, H, L, D), _randn(g, 1, H, L, D)
+    v[0, 0, 10:20] *= 2.0 ** 40
+    v[0, 0, 20:30] *= 2.0 ** -40
+    v[0, 0, 64:128] = 0
+    k[0, 0, 30:40] *= 40
+    cache = BlockCache(pages, H, D)
+    held = _fill(cache, g, table, [L], k, v)
+    q = _randn(g, 1, H, T, D).cuda()
+    base = ops.cache_attn(q, cache, table, _i32([L]), causal=True)
+    _check_attend(base, q, held, [L], None, 1, True, H=1)
+    v[0, 0, 190, 5] = float("nan")
+    _fill(cache, g, table, [L], k, v)
+    o = ops.cache_attn(q, cache, table, _i32([L]), causal=True)
+    # rows up to position 189 do not see token 190
+    assert torch.equal(o[0, 0, :30], base[0, 0, :30]) and o[0, 0, 30:].isnan().all()
+    o = ops.cache_attn(q[:, :, :5], cache, table, _i32([190]))
+    _check_attend(o, q[:, :, :5], [(held[0][0][:, :190], held[0][1][:, :190])], [190], None, 1, False, H=1)
+
+
+def test_attend_wide_logits_and_scale():
+    """Logits of hundreds: one key takes all; the running maximum moves many times; a scale of the caller's."""
+    g = _gen(41)
+    D, H, L = 128, 1, 900
+    table, pages = _table(g, 1, 15)
+    cache = BlockCache(pages, H, D)
+    k = _randn(g, 1, H, L, D) * torch.linspace(0.1, 6, L).view(1, 1, L, 1).bfloat16()
+    held = _fill(cache, g, table, [L], k)
+    q = (_randn(g, 1, 3, 1, D) * 4).cuda()
+    for scale in (1.0, 0.01, 0.0):
+        o = ops.cache_attn(q, cache, table, _i32([L]), scale=scale)
+        _check_attend(o, q, held, [L], None, 1, False, scale=scale, H=1)
+
+
+def test_attend_strided_tensors_and_out():
+    g = _gen(43)
+    D, H, T, L = 64, 2, 6, 333
+    table, pages = _table(g, 2, 6)
+    wide = torch.full((2, 9), -1, dtype=torch.int32, device="cuda")
+    wide[:, :6] = table
+    cache = BlockCache(pages, H, D)
+    held = _fill(cache, g, table, [L, L - 9])
+    qkv = _randn(g, 2, T, 3, H * 2, D).cuda()
+    q = qkv[:, :, 1].transpose(1, 2)
+    rows = torch.full((2, T, H * 2, D + 8), 7.0, dtype=torch.bfloat16, device="cuda")
+    out = rows[..., :D].transpose(1, 2)
+    o = ops.cache_attn(q, cache, wide[:, :6], _i32([L, L - 9]), out=out)
+    assert o.data_ptr() == rows.data_ptr() and (rows[..., D:] == 7.0).all()
+    _check_attend(o, q, held, [L, L - 9], None, 1, False, H=H)
+    again = ops.cache_attn(q, cache, wide[:, :6], torch.tensor([L, L - 9], device="cuda"))  # int64 lengths
+    assert torch.equal(again, o)
+
+
+def test_offsets_past_32_bits():
+    """A cache whose codes lie past 2^32 bytes, written, chosen from and attended to at both ends."""
+    g = _gen(47)
+    H, D = 8, 128
+    pages = (2 ** 32) // (H * 64 * D) + 40
+    cache = BlockCache(pages, H, D)
+    table = torch.stack([torch.arange(pages - 12, pages), torch.arange(12)]).to(torch.int32).cuda()
+    lens = [700, 650]
+    held = _fill(cache, g, table, lens)
+    rk, rv = ops.cache_read(cache, table, _i32([0, 0]), 700, count=_i32(lens), dtype=torch.float32)
+    for b, n in enumerate(lens):
+        assert _same(_np(rk[b, :, :n]), held[b][0]) and _same(_np(rv[b, :, :n]), held[b][1])
+    q = _randn(g, 2, H, 1, D).cuda()
+    _check_select(q, cache, table, lens, held, 3, 1, 1, 1, False)
+    o = ops.cache_attn(q, cache, table, _i32(lens))
+    _check_attend(o, q, held, lens, None, 1, False, H=H)
+
+
+# ------------------------------------------------------------------ a run of them
+def _step(cache, q, k, v, pos, table, start, lengths, freq, sections, block_q):
+    q, k = ops.rotary_axes(q, k, pos, sections, freq)
+    ops.cache_write(cache, k, v, table, start)
+    index, count = ops.cache_select(q, cache, table, lengths, 2, block_q=block_q)
+    return ops.cache_attn(q, cache, table, lengths, index, count, block_q=block_q)
+
+
+@pytest.mark.parametrize("T", [1, 37])
+def test_step_captured_in_graphs(T):
+    """rotary, write, choice and attention in two graphs with their own memory, replayed in turn with eager work between:
+    each replay equals the eager run. The lengths live on the device, so one graph serves every step."""
+    g = _gen(T)
+    H, G, D, block_q = 2, 2, 64, 32
+    sections = (16, 24, 24)
+    freq = _freq(sections, (10000.0, 100.0, 100.0)).cuda()
+    table, pages = _table(g, 2, 10)
+    steps = 5
+    qs = [_randn(g, 2, H * G, T, D).cuda() for _ in range(steps)]
+    ks = [_randn(g, 2, H, T, D).cuda() for _ in range(steps)]
+    vs = [_randn(g, 2, H, T, D).cuda() for _ in range(steps)]
+    ps = [torch.randint(0, 99, (2, T, 3), generator=g).cuda().int() for _ in range(steps)]
+    start0 = [70, 3]
+
+    def history():
+        c = BlockCache(pages, H, D)
+        gg = _gen(99)
+        k, v = _randn(gg, 2, H, 70, D).cuda(), _randn(gg, 2, H, 70, D).cuda()
+        ops.cache_write(c, k, v, table, _i32([0, 0]), count=_i32(start0))
+        return c
+
+    eager, cache = [], history()
+    for i in range(steps):
+        s = _i32(start0) + i * T
+        eager.append(_step(cache, qs[i], ks[i], vs[i], ps[i], table, s, s + T, freq, sections, block_q))
+    graphs = []
+    for _ in range(2):
+        c = history()
+        # the cache and the inputs live as long as their graph does
+        st = dict(cache=c, q=qs[0].clone(), k=ks[0].clone(), v=vs[0].clone(), pos=ps[0].clone(), start=_i32(start0),
+                  lengths=_i32(start0) + T)
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            _step(c, st["q"], st["k"], st["v"], st["pos"], table, st["start"], st["lengths"], freq, sections, block_q)
+        torch.cuda.current_stream().wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = _step(c, st["q"], st["k"], st["v"], st["pos"], table, st["start"], st["lengths"], freq, sections, block_q)
+        graphs.append((graph, st, out))
+    for i in range(steps):
+        for graph, st, out in graphs:
+            for name, src in (("q", qs), ("k", ks), ("v", vs), ("pos", ps)):
+                st[name].copy_(src[i])
+            st["start"].copy_(_i32(start0) + i * T)
+            st["lengths"].copy_(st["start"] + T)
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(out, eager[i]), i
+            torch.randn(1 << 16, device="cuda").sum().item()  # other work between replays
+
+
+def test_two_streams_at_once():
+    """Two sequences' attention on streams of their own: separate workspaces, same results as one after the other."""
+    g = _gen(53)
+    H, D, L = 2, 64, 4000
+    table, pages = _table(g, 2, 63)
+    cache = BlockCache(pages, H, D)
+    k, v = _randn(g, 2, H, L, D).cuda(), _randn(g, 2, H, L, D).cuda()
+    ops.cache_write(cache, k, v, table, _i32([0, 0]))
+    q = _randn(g, 2, H, 1, D).cuda()
+    n = _i32([L])
+    want = [ops.cache_attn(q[b:b + 1], cache, table[b:b + 1], n) for b in range(2)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    got = [[], []]
+    for _ in range(10):
+        for b, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[b].append(ops.cache_attn(q[b:b + 1], cache, table[b:b + 1], n))
+    torch.cuda.synchronize()
+    for b in range(2):
+        assert all(torch.equal(x, want[b]) for x in got[b])

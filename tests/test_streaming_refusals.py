@@ -1,0 +1,129 @@
+"""What the streaming operators refuse, on the CPU: host tensors, and bad arguments at the C boundary (which returns
+before it touches a pointer)."""
+import ctypes
+
+import pytest
+import torch
+
+from vasc_amd import _lib, ops
+from vasc_amd.streaming import BlockCache
+
+FAKE = 1 << 20  # an aligned address that nothing reads
+
+
+def _rotary(**kw):
+    a = dict(q=FAKE, Hq=2, k=None, ko=None, Hk=0, B=1, T=4, D=64, pos=FAKE, axes=3, sections=(16, 24, 24), freq=FAKE,
+             dtype=0, qst=64)
+    a.update(kw)
+    sec = (ctypes.c_int64 * max(1, len(a["sections"])))(*a["sections"])
+    _lib.call("vasc_rotary_axes", a["q"], 512, 256, a["qst"], FAKE, 512, 256, 64, a["Hq"], a["k"], 0, 0, 0, a["ko"], 0, 0, 0,
+              a["Hk"], a["B"], a["T"], a["D"], a["pos"], 12, 3, a["axes"], ctypes.cast(sec, ctypes.c_void_p), a["freq"],
+              a["dtype"], 0, None)
+
+
+@pytest.mark.parametrize("kw,match", [
+    (dict(q=None), "required"), (dict(pos=None), "required"), (dict(freq=None), "required"), (dict(k=FAKE), "together"),
+    (dict(B=0), "empty"), (dict(T=0), "empty"), (dict(Hq=0), "empty"), (dict(D=0), "outside"), (dict(D=257), "outside"),
+    (dict(axes=0), "axes"), (dict(axes=5), "axes"), (dict(sections=(15, 24, 24)), "even"),
+    (dict(sections=(0, 24, 24)), "even"), (dict(sections=(32, 24, 24)), "hold"), (dict(dtype=3), "dtype"),
+])
+def test_rotary_refuses(kw, match):
+    with pytest.raises(_lib.VascError, match=match):
+        _rotary(**kw)
+
+
+def _write(name="vasc_cache_write", **kw):
+    a = dict(k=FAKE, st=64, B=1, H=2, T=4, D=64, dtype=0, table=FAKE, ts=8, mp=8, start=FAKE, kc=FAKE, pages=9)
+    a.update(kw)
+    if name == "vasc_cache_write":
+        _lib.call(name, a["k"], 512, 256, a["st"], FAKE, 512, 256, 64, a["B"], a["H"], a["T"], a["D"], a["dtype"],
+                  a["table"], a["ts"], a["mp"], a["start"], None, a["kc"], FAKE, FAKE, FAKE, FAKE, a["pages"], None)
+    else:
+        _lib.call(name, a["kc"], FAKE, FAKE, FAKE, a["pages"], a["table"], a["ts"], a["mp"], a["start"], None, a["B"],
+                  a["H"], a["T"], a["D"], a["dtype"], a["k"], FAKE, None)
+
+
+@pytest.mark.parametrize("name", ["vasc_cache_write", "vasc_cache_read"])
+@pytest.mark.parametrize("kw,match", [
+    (dict(k=None), "NULL"), (dict(table=None), "required"), (dict(start=None), "required"), (dict(kc=None), "required"),
+    (dict(B=0), "empty"), (dict(T=0), "empty"), (dict(D=80), "not built"), (dict(dtype=7), "dtype"),
+    (dict(pages=0), "positive"), (dict(mp=0), "positive"), (dict(mp=1 << 24, ts=1 << 24), "too large"),
+    (dict(ts=4), "table_stride"), (dict(k=FAKE + 8), "aligned"), (dict(kc=FAKE + 4), "aligned"),
+    (dict(T=1 << 30), "too many"), (dict(B=1 << 24), "too many"), (dict(B=1 << 20, T=1 << 20), "too many"),
+])
+def test_write_and_read_refuse(name, kw, match):
+    with pytest.raises(_lib.VascError, match=match):
+        _write(name, **kw)
+
+
+def test_write_refuses_odd_strides():
+    with pytest.raises(_lib.VascArgumentError, match="multiples of 8"):
+        _write(st=65)
+
+
+def _select(**kw):
+    a = dict(q=FAKE, B=1, Hq=4, H=2, T=8, D=64, dtype=0, mean=FAKE, mp=8, lengths=FAKE, block_q=4, sink=1, recent=1,
+             keep=2, causal=0, width=4)
+    a.update(kw)
+    _lib.call("vasc_cache_select", a["q"], 512, 64, 256, a["B"], a["Hq"], a["H"], a["T"], a["D"], a["dtype"], a["mean"], 9,
+              FAKE, a["mp"], a["mp"], a["lengths"], None, a["block_q"], a["sink"], a["recent"], a["keep"], a["causal"],
+              FAKE, FAKE, a["width"], FAKE, None)
+
+
+@pytest.mark.parametrize("kw,match", [
+    (dict(q=None), "NULL"), (dict(mean=None), "required"), (dict(lengths=None), "required"), (dict(Hq=5), "multiple"),
+    (dict(Hq=0), "multiple"), (dict(dtype=2), "dtype"), (dict(block_q=0), "rows"), (dict(block_q=65), "rows"),
+    (dict(Hq=512), "rows"), (dict(recent=0), "recent"), (dict(keep=-1), "negative"), (dict(sink=-1), "negative"),
+    (dict(width=5), "width"), (dict(causal=1), "width"), (dict(mp=40000), "not built"), (dict(D=32), "not built"),
+    (dict(B=1 << 23, H=2, T=1 << 20), "too many"),
+])
+def test_select_refuses(kw, match):
+    with pytest.raises(_lib.VascError, match=match):
+        _select(**kw)
+
+
+def _attn(**kw):
+    a = dict(q=FAKE, o=FAKE, B=1, Hq=4, H=2, T=1, D=64, dtype=0, kc=FAKE, mp=5000, ts=5000, lengths=FAKE, block_q=1,
+             index=None, width=0, count=None, ws=None, bytes=0, qst=256, ost=256)
+    a.update(kw)
+    _lib.call("vasc_cache_attn", a["q"], 512, 64, a["qst"], a["o"], 512, 64, a["ost"], a["B"], a["Hq"], a["H"], a["T"],
+              a["D"], a["dtype"], a["kc"], FAKE, FAKE, FAKE, 9, FAKE, a["ts"], a["mp"], a["lengths"], None, a["block_q"],
+              a["index"], a["width"], a["count"], 0, 0.125, a["ws"], a["bytes"], None)
+
+
+@pytest.mark.parametrize("kw,match", [
+    (dict(q=None), "NULL"), (dict(kc=None), "NULL"), (dict(lengths=None), "NULL"), (dict(D=96), "not built"),
+    (dict(dtype=2), "dtype"), (dict(index=FAKE), "together"), (dict(index=FAKE, count=FAKE), "together"),
+    (dict(width=3), "together"), (dict(Hq=3), "sizes"), (dict(block_q=65), "sizes"), (dict(T=0), "sizes"),
+    (dict(B=1 << 24), "sizes"), (dict(q=FAKE + 2), "aligned"), (dict(o=FAKE + 4), "aligned"), (dict(qst=260), "multiples"),
+    (dict(ost=258), "multiples"), (dict(ts=7), "table_stride"), (dict(), "workspace"), (dict(ws=FAKE, bytes=64), "workspace"),
+])
+def test_attn_refuses(kw, match):
+    with pytest.raises(_lib.VascError, match=match):
+        _attn(**kw)
+
+
+def test_workspace_query():
+    size = _lib.fn("vasc_cache_attn_workspace_size")
+    assert size(1, 4, 2, 1, 64, 1, 5000, 0) > 0
+    assert size(1, 4, 2, 1, 64, 1, 5000, 4) == 0  # a short list is not split
+    for bad in ((0, 4, 2, 1, 64, 1, 10, 0), (1, 5, 2, 1, 64, 1, 10, 0), (1, 4, 2, 1, 60, 1, 10, 0), (1, 4, 2, 1, 64, 0, 10, 0),
+                (1, 4, 2, 1, 64, 65, 10, 0), (1, 4, 2, 1, 64, 1, 0, 0), (1, 4, 2, 1, 64, 1, 10, -1)):
+        assert size(*bad) == -1
+
+
+def test_host_tensors_are_refused():
+    x, i = torch.zeros(1, 2, 4, 64), torch.zeros(1, dtype=torch.int32)
+    table = torch.zeros(1, 4, dtype=torch.int32)
+    with pytest.raises(ValueError, match="GPU"):
+        ops.rotary_axes(x, None, torch.zeros(1, 4, 1, dtype=torch.int32), (16,), torch.zeros(8, dtype=torch.float64))
+    for call in (lambda: ops.cache_write(None, x, x, table, i), lambda: ops.cache_read(None, table, i, 4),
+                 lambda: ops.cache_select(x, None, table, i, 4), lambda: ops.cache_attn(x, None, table, i)):
+        with pytest.raises(ValueError, match="GPU"):
+            call()
+    with pytest.raises(ValueError, match="GPU"):
+        BlockCache(4, 2, 64, device="cpu")
+    with pytest.raises(ValueError, match="not built"):
+        BlockCache(4, 2, 96)
+    with pytest.raises(ValueError, match="pages"):
+        BlockCache(0, 2, 64)

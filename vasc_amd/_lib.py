@@ -25,7 +25,7 @@ P = c_void_p
 I64 = c_int64
 I32 = c_int32
 
-# name -> (restype, argtypes); mirrors include/vasc_hip.h and include/vasc_runner.h.
+# name -> (restype, argtypes); mirrors include/vasc_hip.h, include/vasc_runner.h and include/vasc_stream.h.
 SIGNATURES: dict[str, tuple] = {
     "vasc_last_error": (ctypes.c_char_p, []),
     "vasc_abi_version": (c_int32, []),
@@ -82,6 +82,17 @@ SIGNATURES: dict[str, tuple] = {
                                       P, P]),
     # include/vasc_runner.h
     "vasc_residual_norm": (c_int32, [P, I64, P, I64, P, P, P, c_float, P, I64, P, I64, I64, I64, P]),
+    # include/vasc_stream.h
+    "vasc_rotary_axes": (c_int32, [P, I64, I64, I64, P, I64, I64, I64, I64, P, I64, I64, I64, P, I64, I64, I64, I64,
+                                   I64, I64, I64, P, I64, I64, I32, P, P, I32, I32, P]),
+    "vasc_cache_write": (c_int32, [P, I64, I64, I64, P, I64, I64, I64, I64, I64, I64, I64, I32, P, I64, I64, P, P,
+                                   P, P, P, P, P, I64, P]),
+    "vasc_cache_read": (c_int32, [P, P, P, P, I64, P, I64, I64, P, P, I64, I64, I64, I64, I32, P, P, P]),
+    "vasc_cache_select": (c_int32, [P, I64, I64, I64, I64, I64, I64, I64, I64, I32, P, I64, P, I64, I64, P, P,
+                                    I64, I64, I64, I64, I32, P, P, I64, P, P]),
+    "vasc_cache_attn_workspace_size": (I64, [I64, I64, I64, I64, I64, I64, I64, I64]),
+    "vasc_cache_attn": (c_int32, [P, I64, I64, I64, P, I64, I64, I64, I64, I64, I64, I64, I64, I32, P, P, P, P, I64,
+                                  P, I64, I64, P, P, I64, P, I64, P, I32, c_float, P, I64, P]),
 }
 
 _lock = threading.Lock()

@@ -41,6 +41,9 @@ SOURCES = {
     "select.hip": ["-ffp-contract=off", "-Wshadow"],
     # the residual products and sums round separately, as torch's bf16 ops do
     "block.hip": ["-ffp-contract=off"],
+    "rotary.hip": [],
+    "cache.hip": [],
+    "cache_attn.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
 }
 
 

@@ -6,6 +6,7 @@ must be device tensors; nothing here falls back to the CPU.
 """
 from __future__ import annotations
 
+import ctypes
 import math
 
 import numpy as np
@@ -662,4 +663,327 @@ def restore_tokens(x_patch: torch.Tensor, x_special: torch.Tensor | None, frames
     out = torch.empty(B, N * P, H * D, device=x_patch.device, dtype=torch.bfloat16)
     _lib.call("vasc_restore_tokens", x_patch.data_ptr(), *x_patch.stride()[:3], *xs, B, H, N, P, S, D,
               out.data_ptr(), _stream())
+    return out
+
+
+# ----------------------------------------------------------------- streaming
+_DTYPE = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+
+
+def _launch(ref: torch.Tensor, name: str, *args) -> None:
+    """``_lib.call`` on the current stream of ``ref``'s device."""
+    if torch._C._cuda_getDevice() == ref.device.index:
+        _lib.call(name, *args, _stream())
+    else:
+        with torch.cuda.device(ref.device):
+            _lib.call(name, *args, _stream())
+
+
+def _together(ref: torch.Tensor, **tensors) -> None:
+    for name, t in tensors.items():
+        if t is None:
+            continue
+        _dev(t, name)
+        if t.device != ref.device:
+            raise ValueError(f"{name} is on {t.device}, expected {ref.device}")
+
+
+def _inference(**tensors) -> None:
+    if torch.is_grad_enabled():
+        for name, t in tensors.items():
+            if t.requires_grad:
+                raise ValueError(f"{name} requires a gradient: the block cache has no backward pass, "
+                                 "call it under torch.no_grad()")
+
+
+def _rows8(t: torch.Tensor, name: str, dtypes: tuple) -> torch.Tensor:
+    """``[B,H,T,D]`` of one of ``dtypes`` with unit stride on D and 16-byte aligned rows."""
+    _dev(t, name)
+    if t.dim() != 4:
+        raise ValueError(f"{name} must be [B,H,T,D], got {tuple(t.shape)}")
+    if t.dtype not in dtypes:
+        raise ValueError(f"{name} must be one of {[str(d) for d in dtypes]}, got {t.dtype}")
+    if t.stride(-1) != 1 or any(s % 8 for s in t.stride()[:3]) or t.data_ptr() % 16:
+        t = t.contiguous()
+        if t.data_ptr() % 16:  # a contiguous view that starts inside a row
+            t = t.clone()
+    return t
+
+
+def _int_rows(t: torch.Tensor | None, name: str, B: int) -> torch.Tensor | None:
+    """``[B]`` int32, contiguous."""
+    if t is None:
+        return None
+    _dev(t, name)
+    if t.dtype.is_floating_point or t.dtype == torch.bool or t.shape != (B,):
+        raise ValueError(f"{name} must hold {B} integers, got {t.dtype} {tuple(t.shape)}")
+    return t.to(torch.int32).contiguous()
+
+
+def _page_table(t: torch.Tensor, B: int) -> tuple:
+    """(tensor, stride of a sequence, pages a sequence)."""
+    _dev(t, "page_table")
+    if t.dtype.is_floating_point or t.dtype == torch.bool or t.dim() != 2 or t.shape[0] != B or t.shape[1] == 0:
+        raise ValueError(f"page_table must be [{B}, max_pages] integers, got {t.dtype} {tuple(t.shape)}")
+    t = t.to(torch.int32)
+    if t.shape[1] > 1 and t.stride(1) != 1 or t.stride(0) < t.shape[1]:
+        t = t.contiguous()
+    return t, t.stride(0) if B > 1 else t.shape[1], t.shape[1]
+
+
+def _rotary_out(x: torch.Tensor) -> torch.Tensor:
+    """An output in the memory order of ``x``: [B,T,H,D] where x's heads lie inside its tokens."""
+    B, H, T, D = x.shape
+    if x.stride(1) < x.stride(2):
+        return torch.empty(B, T, H, D, device=x.device, dtype=x.dtype).transpose(1, 2)
+    return torch.empty(B, H, T, D, device=x.device, dtype=x.dtype)
+
+
+def _rotary(q, k, pos, sections, inv_freq, inverse: bool) -> tuple:
+    q = q if q.stride(-1) == 1 else q.contiguous()
+    qo = _rotary_out(q)
+    kargs, ko, Hk = (None, 0, 0, 0, None, 0, 0, 0), None, 0
+    if k is not None:
+        k = k if k.stride(-1) == 1 else k.contiguous()
+        ko, Hk = _rotary_out(k), k.shape[1]
+        kargs = (k.data_ptr(), *k.stride()[:3], ko.data_ptr(), *ko.stride()[:3])
+    if q.numel() == 0 or (k is not None and k.numel() == 0):
+        if q.numel():
+            qo = _rotary(q, None, pos, sections, inv_freq, inverse)[0]
+        elif k is not None and k.numel():
+            ko = _rotary(k, None, pos, sections, inv_freq, inverse)[0]
+        return qo, ko
+    B, Hq, T, D = q.shape
+    sec = (ctypes.c_int64 * len(sections))(*sections)
+    _launch(q, "vasc_rotary_axes", q.data_ptr(), *q.stride()[:3], qo.data_ptr(), *qo.stride()[:3], Hq, *kargs, Hk, B, T,
+            D, pos.data_ptr(), pos.stride(0) if pos.shape[0] > 1 else 0, pos.stride(1), len(sections),
+            ctypes.cast(sec, ctypes.c_void_p), inv_freq.data_ptr(), _DTYPE[q.dtype], int(inverse))
+    return qo, ko
+
+
+class _RotaryAxes(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, pos, sections, inv_freq):
+        ctx.save_for_backward(pos, inv_freq)
+        ctx.sections = sections
+        ctx.set_materialize_grads(False)
+        return _rotary(q, k, pos, sections, inv_freq, False)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, gq, gk):
+        pos, inv_freq = ctx.saved_tensors
+        if gq is None and gk is None:
+            return None, None, None, None, None
+        if gq is None:
+            return None, _rotary(gk, None, pos, ctx.sections, inv_freq, True)[0], None, None, None
+        dq, dk = _rotary(gq, gk, pos, ctx.sections, inv_freq, True)
+        return dq, dk, None, None, None
+
+
+def rotary_axes(q: torch.Tensor, k: torch.Tensor | None, pos: torch.Tensor, sections, inv_freq: torch.Tensor):
+    """Rotary embedding over several position axes, of q and k in one launch.
+
+    q ``[B,Hq,T,D]``, k ``[B,Hk,T,D]`` or None, of one dtype (bf16, fp16 or
+    fp32), any strides over B, H, T. Axis ``a`` of ``pos [B,T,A]`` (integers
+    of 32 bits; ``[T,A]`` and ``[1,T,A]`` serve every sequence) turns the next
+    ``sections[a]`` features: pair ``(j, j + sections[a]/2)`` by the angle
+    ``pos * inv_freq``, whose float64 values ``[sum(sections)/2]`` hold the
+    axes' frequencies one after another. Features past the sections pass
+    through. Returns ``(q', k' or None)`` in the inputs' memory order;
+    differentiable in q and k.
+    """
+    _dev(q, "q")
+    _together(q, k=k, pos=pos, inv_freq=inv_freq)
+    if q.dim() != 4 or q.dtype not in _DTYPE:
+        raise ValueError(f"q must be [B,H,T,D] in bf16, fp16 or fp32, got {q.dtype} {tuple(q.shape)}")
+    B, _, T, D = q.shape
+    if k is not None and (k.dim() != 4 or k.dtype != q.dtype or k.shape[0] != B or k.shape[2:] != q.shape[2:]):
+        raise ValueError(f"k must be [{B},H,{T},{D}] of {q.dtype}, got {k.dtype} {tuple(k.shape)}")
+    sections = tuple(int(s) for s in sections)
+    if not 1 <= len(sections) <= 4 or any(s <= 0 or s % 2 for s in sections) or sum(sections) > D:
+        raise ValueError(f"sections {sections} must be 1 to 4 even sizes that sum to at most {D}")
+    if pos.dtype.is_floating_point or pos.dtype == torch.bool:
+        raise ValueError(f"pos must hold integers, got {pos.dtype}")
+    if pos.dim() == 2:
+        pos = pos.unsqueeze(0)
+    if pos.dim() != 3 or pos.shape[0] not in (1, B) or pos.shape[1:] != (T, len(sections)):
+        raise ValueError(f"pos must be [{B} or 1, {T}, {len(sections)}], got {tuple(pos.shape)}")
+    if inv_freq.dtype != torch.float64 or inv_freq.shape != (sum(sections) // 2,):
+        raise ValueError(f"inv_freq must hold {sum(sections) // 2} float64 values, got {inv_freq.dtype} "
+                         f"{tuple(inv_freq.shape)}")
+    pos = pos.to(torch.int32)
+    pos = pos if pos.stride(-1) == 1 or pos.shape[-1] == 1 else pos.contiguous()
+    inv_freq = inv_freq.detach().contiguous()
+    if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
+        return _RotaryAxes.apply(q, k, pos, sections, inv_freq)
+    return _rotary(q, k, pos, sections, inv_freq, False)
+
+
+def _cache_ptrs(cache) -> tuple:
+    return cache.kc.data_ptr(), cache.vc.data_ptr(), cache.ks.data_ptr(), cache.vs.data_ptr()
+
+
+def cache_write(cache, k: torch.Tensor, v: torch.Tensor, page_table: torch.Tensor, start: torch.Tensor,
+                count: torch.Tensor | None = None) -> None:
+    """Writes new tokens into a ``streaming.BlockCache``, in 8 bits.
+
+    k, v ``[B,H,T,D]`` (bf16, fp16 or fp32, any strides over B, H, T): token
+    ``t < count[b]`` (default T) of sequence b becomes its token
+    ``start[b] + t``. ``page_table [B,max_pages]`` holds the sequences' pages
+    (entries outside the cache: nothing is written there); no page may occur
+    twice among the pages one call writes. Each (token, head) row is rounded
+    to e4m3 values times a power of two, and every touched page's key mean is
+    renewed over its tokens up to the last one written, so the tokens before
+    ``start`` in its page must be there, and writing further back drops what
+    came after. A token whose k or v row holds a value that is not finite is
+    held as NaN in both. Nothing here waits for the GPU.
+    """
+    _dev(k, "k")
+    _inference(k=k, v=v)
+    _together(k, v=v, page_table=page_table, start=start, count=count, cache=cache.kc)
+    dtypes = (torch.bfloat16, torch.float16, torch.float32)
+    k, v = _rows8(k, "k", dtypes), _rows8(v, "v", dtypes)
+    if k.shape != v.shape or k.dtype != v.dtype:
+        raise ValueError(f"k {k.dtype} {tuple(k.shape)} and v {v.dtype} {tuple(v.shape)} differ")
+    B, H, T, D = k.shape
+    if (H, D) != (cache.heads, cache.head_dim):
+        raise ValueError(f"the cache holds {cache.heads} heads of {cache.head_dim}, k has {H} of {D}")
+    table, ts, mp = _page_table(page_table, B)
+    start, count = _int_rows(start, "start", B), _int_rows(count, "count", B)
+    if k.numel() == 0:
+        return
+    _launch(k, "vasc_cache_write", k.data_ptr(), *k.stride()[:3], v.data_ptr(), *v.stride()[:3], B, H, T, D,
+            _DTYPE[k.dtype], table.data_ptr(), ts, mp, start.data_ptr(), _ptr(count), *_cache_ptrs(cache),
+            cache.mean.data_ptr(), cache.pages)
+
+
+def cache_read(cache, page_table: torch.Tensor, start: torch.Tensor, tokens: int, count: torch.Tensor | None = None,
+               dtype: torch.dtype = torch.bfloat16) -> tuple:
+    """``(k, v) [B,H,tokens,D]`` of the cache's tokens ``start[b]..`` in
+    ``dtype`` (bf16: exactly what the cache holds). Rows from ``count[b]`` on
+    (default ``tokens``) and rows that have no page are zero."""
+    _dev(page_table, "page_table")
+    _together(page_table, start=start, count=count, cache=cache.kc)
+    if dtype not in _DTYPE:
+        raise ValueError(f"dtype must be bf16, fp16 or fp32, got {dtype}")
+    B, tokens = page_table.shape[0], int(tokens)
+    if tokens < 0:
+        raise ValueError(f"tokens must not be negative, got {tokens}")
+    table, ts, mp = _page_table(page_table, B)
+    start, count = _int_rows(start, "start", B), _int_rows(count, "count", B)
+    k = torch.empty(B, cache.heads, tokens, cache.head_dim, device=table.device, dtype=dtype)
+    v = torch.empty_like(k)
+    if k.numel():
+        _launch(k, "vasc_cache_read", *_cache_ptrs(cache), cache.pages, table.data_ptr(), ts, mp, start.data_ptr(),
+                _ptr(count), B, cache.heads, tokens, cache.head_dim, _DTYPE[dtype], k.data_ptr(), v.data_ptr())
+    return k, v
+
+
+def _cache_query(q, cache, page_table, lengths, q_count, block_q: int) -> tuple:
+    _dev(q, "q")
+    _inference(q=q)
+    _together(q, page_table=page_table, lengths=lengths, q_count=q_count, cache=cache.kc)
+    q = _rows8(q, "q", (torch.bfloat16, torch.float16))
+    B, Hq, T, D = q.shape
+    if D != cache.head_dim or Hq % cache.heads or Hq == 0:
+        raise ValueError(f"q has {Hq} heads of {D}: expected a multiple of {cache.heads} heads of {cache.head_dim}")
+    G = Hq // cache.heads
+    if not (1 <= block_q and block_q * G <= 128):
+        raise ValueError(f"block_q {block_q} with {G} query heads a key head: a unit has 1 to 128 rows")
+    table, ts, mp = _page_table(page_table, B)
+    return q, table, ts, mp, _int_rows(lengths, "lengths", B), _int_rows(q_count, "q_count", B)
+
+
+def cache_select(q: torch.Tensor, cache, page_table: torch.Tensor, lengths: torch.Tensor, keep: int, *,
+                 block_q: int = 1, sink: int = 1, recent: int = 1, causal: bool = False,
+                 q_count: torch.Tensor | None = None, want_score: bool = False) -> tuple:
+    """Pages that each unit of queries attends to, by a cheap score.
+
+    A unit is ``block_q`` consecutive query tokens of the ``G = Hq / H`` query
+    heads that share a key head (``block_q * G <= 128``); q ``[B,Hq,T,D]`` bf16
+    or fp16. A page's score is the product of the unit's mean query and the
+    page's mean key (both rounded to bf16, summed in float64). Listed are the
+    first ``sink`` pages, the last ``recent``, and the ``keep`` of highest score
+    among the others (equal scores in page order, NaN lowest). ``lengths[b]``:
+    tokens of sequence b in the cache. With ``causal`` the ``q_count[b]``
+    (default T) queries are its last tokens; a unit then sees the pages up to
+    its last row's own, and ``recent`` counts back from its first row's own
+    page (every page from there on is listed).
+
+    Returns ``(index [B,H,U,W], count [B,H,U])`` int32, ``U = ceil(T / block_q)``:
+    ascending logical pages, -1 behind them; ``W`` is the largest possible
+    count. ``want_score`` adds the scores ``[B,H,U,max_pages]`` float32 (-inf
+    for pages the unit does not see).
+    """
+    block_q, keep, sink, recent = int(block_q), int(keep), int(sink), int(recent)
+    q, table, ts, mp, lengths, q_count = _cache_query(q, cache, page_table, lengths, q_count, block_q)
+    if keep < 0 or sink < 0 or recent < 1:
+        raise ValueError(f"keep {keep} and sink {sink} must not be negative, recent {recent} at least 1")
+    B, Hq, T, D = q.shape
+    H, U = cache.heads, -(-T // block_q)
+    width = min(mp, sink + keep + recent + ((block_q + BLOCK_K - 2) // BLOCK_K if causal else 0))
+    i32 = dict(device=q.device, dtype=torch.int32)
+    index, count = torch.empty(B, H, U, width, **i32), torch.empty(B, H, U, **i32)
+    score = torch.empty(B, H, U, mp, device=q.device, dtype=torch.float32)
+    if count.numel():
+        _launch(q, "vasc_cache_select", q.data_ptr(), *q.stride()[:3], B, Hq, H, T, D, _DTYPE[q.dtype],
+                cache.mean.data_ptr(), cache.pages, table.data_ptr(), ts, mp, lengths.data_ptr(), _ptr(q_count),
+                block_q, sink, recent, keep, int(bool(causal)), score.data_ptr(), index.data_ptr(), width,
+                count.data_ptr())
+    return (index, count, score) if want_score else (index, count)
+
+
+def cache_attn(q: torch.Tensor, cache, page_table: torch.Tensor, lengths: torch.Tensor,
+               index: torch.Tensor | None = None, count: torch.Tensor | None = None, *, block_q: int | None = None,
+               causal: bool = False, q_count: torch.Tensor | None = None, scale: float | None = None,
+               out: torch.Tensor | None = None) -> torch.Tensor:
+    """Attention of q ``[B,Hq,T,D]`` (bf16 or fp16) over the cache.
+
+    ``index`` / ``count``: the lists of ``cache_select`` with the same
+    ``block_q`` (ascending logical pages; an entry not above the one before it
+    is skipped); without them every page is attended to. Keys at or past
+    ``lengths[b]`` are not seen, nor, with ``causal``, those behind the row's
+    own position ``lengths[b] - q_count[b] + t``. Rows that see no key, and
+    rows from ``q_count[b]`` on, are zero. Softmax scale ``scale`` (default
+    ``D ** -0.5``). Returns ``[B,Hq,T,D]`` of q's dtype, written to ``out``
+    when given (unit stride over D).
+    """
+    _dev(q, "q")
+    if (index is None) != (count is None):
+        raise ValueError("index and count go together")
+    if q.dim() != 4:
+        raise ValueError(f"q must be [B,H,T,D], got {tuple(q.shape)}")
+    if block_q is None:
+        if index is not None and q.shape[2] > 1:
+            raise ValueError("lists need the block_q they were made with")
+        block_q = max(1, min(q.shape[2], 128 // max(1, q.shape[1] // cache.heads)))
+    block_q = int(block_q)
+    q, table, ts, mp, lengths, q_count = _cache_query(q, cache, page_table, lengths, q_count, block_q)
+    _together(q, index=index, count=count, out=out)
+    B, Hq, T, D = q.shape
+    H, U, width = cache.heads, -(-T // block_q), 0
+    if index is not None:
+        if index.dim() != 4 or index.shape[:3] != (B, H, U) or count.shape != (B, H, U):
+            raise ValueError(f"index/count must be [{B},{H},{U},W]/[{B},{H},{U}], got {tuple(index.shape)}/"
+                             f"{tuple(count.shape)}")
+        if any(t.dtype.is_floating_point or t.dtype == torch.bool for t in (index, count)):
+            raise ValueError("index and count must be integers")
+        index, count = index.to(torch.int32).contiguous(), count.to(torch.int32).contiguous()
+        width = index.shape[3]
+    if out is None:
+        out = torch.empty(B, Hq, T, D, device=q.device, dtype=q.dtype)
+    elif (out.shape != q.shape or out.dtype != q.dtype or out.stride(3) != 1 or any(s % 4 for s in out.stride()[:3])
+          or out.data_ptr() % 8):
+        raise ValueError(f"out must be {q.dtype} {tuple(q.shape)} with unit stride over D, 8-byte aligned rows")
+    if q.numel() == 0:
+        return out
+    if index is not None and width == 0:
+        return out.zero_()
+    scale = D ** -0.5 if scale is None else float(scale)
+    size = _lib.fn("vasc_cache_attn_workspace_size")(B, Hq, H, T, D, block_q, mp, width)
+    ws = torch.empty(size, device=q.device, dtype=torch.uint8) if size > 0 else None
+    _launch(q, "vasc_cache_attn", q.data_ptr(), *q.stride()[:3], out.data_ptr(), *out.stride()[:3], B, Hq, H, T, D,
+            _DTYPE[q.dtype], *_cache_ptrs(cache), cache.pages, table.data_ptr(), ts, mp, lengths.data_ptr(),
+            _ptr(q_count), block_q, _ptr(index), width, _ptr(count), int(bool(causal)), scale, _ptr(ws), max(size, 0))
     return out
