@@ -16,9 +16,10 @@
  *   ks   uint8    [P, H, 64]     exponents of the key rows, 2^(byte - 127)
  *   vs   uint8    [P, H, 64]     exponents of the value rows
  *   mean bfloat16 [P, H, D]      mean of the page's keys
- * vc's last dimension, ks and vs hold token t of the page at
+ * vc's last dimension and vs hold token t of the page at
  *   ((t >> 2) & 3) * 16 + (t >> 4) * 4 + (t & 3),
- * the order in which the lanes of a matrix product consume them. A row's
+ * ks at (t & 15) * 4 + (t >> 4): the orders in which the lanes of a matrix
+ * product consume them. A row's
  * exponent is the smallest e in [-60, 60] with max|x| <= 448 * 2^e: every
  * value is exact in bfloat16, sums of 2^e over a softmax stay inside float32,
  * values past 448 * 2^60 saturate and those under 2^-70 are zero. A token
@@ -112,7 +113,7 @@ int64_t vasc_cache_attn_workspace_size(int64_t B, int64_t Hq, int64_t H, int64_t
  * [B,H,U] as vasc_cache_select writes them: ascending logical pages; entries
  * that are not above the one before, negative or not below max_pages are
  * skipped. block_q as there (index NULL: any block_q with block_q * G <= 128).
- * q, o [B,Hq,T,D] strided, bfloat16 or float16.
+ * q, o [B,Hq,T,D] strided, bfloat16 or float16. scale: finite.
  */
 int vasc_cache_attn(const void *q, int64_t q_sb, int64_t q_sh, int64_t q_st, void *o, int64_t o_sb, int64_t o_sh,
                     int64_t o_st, int64_t B, int64_t Hq, int64_t H, int64_t T, int64_t D, int32_t dtype,

@@ -27,19 +27,6 @@ struct RowArgs {
   int span;  // pages that T tokens can touch
 };
 
-// Four floats -> four e4m3 codes, rounded to nearest even (|x| <= 448).
-__device__ __forceinline__ uint32_t pack_e4m3(float a, float b, float c, float d) {
-  int r = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
-  r = __builtin_amdgcn_cvt_pk_fp8_f32(c, d, r, true);
-  return static_cast<uint32_t>(r);
-}
-
-__device__ __forceinline__ void unpack_e4m3(uint32_t w, float (&f)[4]) {
-  const floatx2 a = __builtin_amdgcn_cvt_pk_f32_fp8(static_cast<int>(w), false);
-  const floatx2 b = __builtin_amdgcn_cvt_pk_f32_fp8(static_cast<int>(w), true);
-  f[0] = a[0]; f[1] = a[1]; f[2] = b[0]; f[3] = b[1];
-}
-
 // Eight consecutive elements as floats.
 template <typename T>
 __device__ __forceinline__ void load8(const T *src, float (&x)[8]) {
@@ -65,12 +52,8 @@ __device__ __forceinline__ float row_max(float v) {
   return D == 128 ? fmaxf(v, xor_lane(v, 8)) : v;
 }
 
-// Exponent byte of a row whose largest magnitude is `top`: the smallest e in [-60, 60] with top <= 448 * 2^e.
-__device__ __forceinline__ int row_exponent(float top) {
-  const uint32_t u = __float_as_uint(top);
-  const int e = static_cast<int>(u >> 23) - 127 - 8 + ((u & 0x7fffffu) > 0x600000u ? 1 : 0);
-  return min(max(e, -60), 60) + 127;
-}
+// Exponent byte of a row whose largest magnitude is `top`.
+__device__ __forceinline__ int row_exponent(float top) { return power_of(top, -60, 60) + 127; }
 
 __device__ __forceinline__ void quantise8(const float (&x)[8], int byte, uint32_t (&w)[2]) {
   const float inv = __uint_as_float(static_cast<uint32_t>(254 - byte) << 23);
@@ -141,7 +124,7 @@ __global__ __launch_bounds__(256) void cache_write_kernel(const CacheArgs c, con
     if (row < w.lo) {  // held before: its part of the mean
       *reinterpret_cast<u32x2 *>(kt + row * D + col) =
           *reinterpret_cast<const u32x2 *>(c.kc + (ph * kPage + row) * D + col);
-      if (col == 0) ke[row] = c.ks[ph * kPage + page_place(row)];
+      if (col == 0) ke[row] = c.ks[ph * kPage + key_place(row)];
     } else if (row < w.hi) {
       const int64_t t = w.j * kPage + row - w.s;
       float x[8], y[8];
@@ -175,7 +158,7 @@ __global__ __launch_bounds__(256) void cache_write_kernel(const CacheArgs c, con
       *reinterpret_cast<uint32_t *>(vt + row * kS + col + 4) = vw[1];
       if (col == 0) {
         ke[row] = static_cast<uint8_t>(kb);
-        c.ks[ph * kPage + page_place(row)] = static_cast<uint8_t>(kb);
+        c.ks[ph * kPage + key_place(row)] = static_cast<uint8_t>(kb);
         c.vs[ph * kPage + page_place(row)] = static_cast<uint8_t>(vb);
       }
     }
@@ -287,7 +270,7 @@ __global__ __launch_bounds__(256) void cache_read_kernel(const CacheArgs c, cons
     float x[8] = {0, 0, 0, 0, 0, 0, 0, 0}, y[8] = {0, 0, 0, 0, 0, 0, 0, 0};
     if (live && t < n) {
       const u32x2 kw = *reinterpret_cast<const u32x2 *>(c.kc + (ph * kPage + row) * D + col);
-      const uint32_t kb = c.ks[ph * kPage + page_place(row)];
+      const uint32_t kb = c.ks[ph * kPage + key_place(row)];
       const float ke = pow2_byte(kb);
       const float ve = kb == 255 ? ke : pow2_byte(c.vs[ph * kPage + page_place(row)]);
 #pragma unroll

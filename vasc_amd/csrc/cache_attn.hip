@@ -1,21 +1,28 @@
 // Attention over listed pages of the 8-bit block cache.
 //
 // A unit's query rows (block_q tokens x G heads of one key head) are the
-// columns of S^T = K Q^T, 16 to a tile. K's codes are read as they lie: a
-// 16-key tile is the A operand of 16x16x32 products, lane l holding 16
-// consecutive features of key l & 15, converted in registers (e4m3 is exact in
-// bfloat16 and in half). S^T leaves each lane four consecutive keys of one
-// query row, which is what the second product's B operand wants of P^T; the
-// cache holds V transposed with the tokens in that same order, so V too goes
-// from memory to the matrix pipe without a shuffle.
+// columns of S^T = K Q^T, 16 to a tile. A 16-key tile is the A operand of
+// 16x16x32 products, lane l holding 16 consecutive features of key l & 15: its
+// codes are widened to bfloat16 in registers by a conversion that takes the
+// key's power of two along (exact: e4m3 times 2^-60..60). Float16 queries are
+// two bfloat16 parts (8 and 3 of their 11 bits), a product each. (The 8-bit
+// matrix products would save the widening, but keep only some 14 bits of a
+// sum: measured, an error of 2^-13 to 2^-16 of sum |q k|.)
+// S^T leaves each lane four consecutive keys of one query row, which is what
+// the second product's B operand wants of P^T; the cache holds V transposed
+// with the tokens in that same order, so V too goes from memory to the matrix
+// pipe without a shuffle, widened to half on the way (exact).
 //
-// Powers of two: a row's exponents scale S (keys) and enter the softmax's
-// exponent (values), e = c S + ev, so that the weights of the second product
-// are w = 2^(e - m) with m the running maximum of e, and its sum l takes them
-// without the value's power: l = sum w 2^-ev. Weights are rounded to half (11
-// bits; bfloat16's 8 would be the largest error of a float16 result). They are
-// held as 2^(11 + e - m), so that those under half's range are below 2^-36 of
-// the row's largest, and m is renewed only when it would be passed by 2^4.
+// A value row's power 2^ev enters the softmax's exponent, e = c S + ev, so the
+// weights of the second product are w = 2^(e - ref) and its sum takes them
+// without the power: l = sum w 2^-ev. The reference is the accumulator's start:
+// S begins at -ref / c, and c S' + ev is the exponent. It is set 11 below the
+// row's largest e and renewed only when that has grown by more than 4: weights
+// are held in half (11 bits; bfloat16's 8 would be the largest error of a
+// float16 result) up to 2^15, and those below its range are under 2^-36 of the
+// row's largest.
+#include <cmath>
+
 #include "stream.h"
 
 namespace vasc {
@@ -38,43 +45,31 @@ struct AttnParams {
   int block_q, causal;
   const int32_t *index, *count;
   int64_t width;
-  float scale;  // times log2(e)
+  float c;      // scale * log2(e)
   int rows;     // block_q * G
   int parts;    // workgroups that share a unit's pages
-  int tiles;    // workgroups that share a unit's rows
   float *ws;
 };
 
-template <typename Q>
-struct Mfma;
-template <>
-struct Mfma<__bf16> {
-  typedef bf16x8 vec;
-  static __device__ __forceinline__ floatx4 mul(vec a, vec b, floatx4 c) {
-    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
-  }
-  static __device__ __forceinline__ uint32_t two(uint32_t w, bool hi) {
-    return __builtin_bit_cast(uint32_t, hi ? __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, true)
-                                           : __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, false));
-  }
-};
-template <>
-struct Mfma<_Float16> {
-  typedef halfx8 vec;
-  static __device__ __forceinline__ floatx4 mul(vec a, vec b, floatx4 c) {
-    return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
-  }
-  static __device__ __forceinline__ uint32_t two(uint32_t w, bool hi) {
-    return __builtin_bit_cast(uint32_t, hi ? __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, true)
-                                           : __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, false));
-  }
-};
+// Eight e4m3 codes as halves.
+__device__ __forceinline__ uint32_t two_halves(uint32_t w, bool hi) {
+  return __builtin_bit_cast(uint32_t, hi ? __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, true)
+                                         : __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, false));
+}
+__device__ __forceinline__ halfx8 widen(uint32_t a, uint32_t b) {
+  const u32x4 w = {two_halves(a, false), two_halves(a, true), two_halves(b, false), two_halves(b, true)};
+  return __builtin_bit_cast(halfx8, w);
+}
 
-// Eight e4m3 codes as the eight 16-bit values of an operand.
-template <typename Q>
-__device__ __forceinline__ typename Mfma<Q>::vec widen(uint32_t a, uint32_t b) {
-  const u32x4 w = {Mfma<Q>::two(a, false), Mfma<Q>::two(a, true), Mfma<Q>::two(b, false), Mfma<Q>::two(b, true)};
-  return __builtin_bit_cast(typename Mfma<Q>::vec, w);
+// Eight e4m3 codes times a power of two, as bfloat16.
+__device__ __forceinline__ uint32_t two_scaled(uint32_t w, float power, bool hi) {
+  return __builtin_bit_cast(uint32_t, hi ? __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, power, true)
+                                         : __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, power, false));
+}
+__device__ __forceinline__ bf16x8 widen_scaled(uint32_t a, uint32_t b, float power) {
+  const u32x4 w = {two_scaled(a, power, false), two_scaled(a, power, true), two_scaled(b, power, false),
+                   two_scaled(b, power, true)};
+  return __builtin_bit_cast(bf16x8, w);
 }
 
 __device__ __forceinline__ uint32_t pack_half2(float a, float b) {
@@ -97,18 +92,21 @@ __device__ __forceinline__ float row4_sum(float v) {
 template <typename Q, int D, int kTiles, int kRowWaves>
 __global__ __launch_bounds__(256, 2) void cache_attn_kernel(const AttnParams p) {
   constexpr int kPageWaves = 4 / kRowWaves;
-  constexpr int kK = D / 64;    // 16-byte loads of a key per lane
-  constexpr int kDT = D / 16;   // feature tiles of the output
+  constexpr int kDT = D / 16;  // feature tiles of the output
   constexpr int kRows = kRowWaves * kTiles * 16;
-  typedef typename Mfma<Q>::vec vec;
-  __shared__ float lo[kPageWaves > 1 ? kPageWaves : 1][kPageWaves > 1 ? kRows : 1][kPageWaves > 1 ? D + 2 : 1];
+  constexpr int kK = D / 64;   // 16-byte loads of a key per lane, two products each
+  constexpr int kParts = __is_same(Q, __bf16) ? 1 : 2;
+  // the query operands, 16 bytes a lane: [row tile][part][product]; after the pages, the page waves' sums
+  constexpr int kOps = kParts * kK * 2;
+  typedef float Sums[kRows][D + 2];
+  constexpr size_t kQBytes = kRowWaves * kTiles * kOps * 1024, kSBytes = (kPageWaves - 1) * sizeof(Sums);
+  __shared__ __align__(16) uint8_t shared[kQBytes > kSBytes ? kQBytes : kSBytes];
+  bf16x8 *query = reinterpret_cast<bf16x8 *>(shared);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int col = lane & 15, g = lane >> 4;
   const int rw = wave % kRowWaves, pw = wave / kRowWaves;
-  // workgroup -> (sequence and key head, part, unit, row tile): the units of a part read the same pages
+  // workgroup -> (sequence and key head, part, unit): the units of a part read the same pages
   int id = static_cast<int>(xcd_remap(blockIdx.x, gridDim.x));
-  const int tile = id % p.tiles;
-  id /= p.tiles;
   const int u = id % p.U;
   id /= p.U;
   const int part = id % p.parts;
@@ -123,42 +121,63 @@ __global__ __launch_bounds__(256, 2) void cache_attn_kernel(const AttnParams p) 
   const UnitView view = unit_view(L, nq, t0, t1, p.max_pages, p.causal);
   const int64_t cut = clamp_tokens(L, p.max_pages);
 
-  // the rows of this wave's tiles: query operand, and one past the last key that the row sees
-  vec qf[kTiles][kK * 2];
-  int64_t limit[kTiles];
-  int64_t low = cut;  // keys below it are seen by every row of the wave that counts
+  // the rows of this wave's tiles: one past the last key that the row sees, and the query operands
+  int limit[kTiles];
+  int low = static_cast<int>(cut), high = 0;  // keys below `low` are seen by every row of the wave that counts, from `high` on by none
 #pragma unroll
   for (int i = 0; i < kTiles; ++i) {
-    const int r = ((tile * kRowWaves + rw) * kTiles + i) * 16 + col;
+    const int r = (rw * kTiles + i) * 16 + col;
     const int tl = r / p.G, gh = r - tl * p.G;
     const int64_t t = t0 + tl;
     const bool live = r < p.rows && t < t1;
-    limit[i] = live ? cut : 0;
+    limit[i] = live ? static_cast<int>(cut) : 0;  // below 2^30
     if (live && p.causal) {
       const int64_t own = L - nq + t + 1;
-      limit[i] = own < cut ? (own > 0 ? own : 0) : cut;
+      limit[i] = static_cast<int>(own < cut ? (own > 0 ? own : 0) : cut);
     }
     if (live && limit[i] < low) low = limit[i];
+    if (limit[i] > high) high = limit[i];
+    if (pw > 0) continue;  // the page waves share the operands
     const Q *src = static_cast<const Q *>(p.q) + b * p.qsb + (static_cast<int64_t>(h) * p.G + gh) * p.qsh + t * p.qst + g * 16;
 #pragma unroll
-    for (int x = 0; x < kK; ++x)
+    for (int y = 0; y < kK * 2; ++y) {
+      float x[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+      if (limit[i] > 0) {
+        struct alignas(16) Eight { Q v[8]; };
+        const Eight v = *reinterpret_cast<const Eight *>(src + (y >> 1) * 64 + (y & 1) * 8);
 #pragma unroll
-      for (int y = 0; y < 2; ++y)
-        qf[i][x * 2 + y] = live ? *reinterpret_cast<const vec *>(src + x * 64 + y * 8) : vec{};
+        for (int e = 0; e < 8; ++e) x[e] = to_f32(v.v[e]);
+      }
+#pragma unroll
+      for (int piece = 0; piece < kParts; ++piece) {
+        bf16x8 w;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          w[e] = static_cast<__bf16>(x[e]);
+          if (kParts > 1 && __builtin_isfinite(x[e])) x[e] -= static_cast<float>(w[e]);
+        }
+        query[((rw * kTiles + i) * kOps + piece * kK * 2 + y) * 64 + lane] = w;
+      }
+    }
   }
-  // the lowest limit over the wave's rows: pages below it need no mask
 #pragma unroll
   for (int off = 1; off < 64; off <<= 1) {
-    const int64_t other = __shfl_xor(static_cast<long long>(low), off);
-    if (other < low) low = other;
+    low = min(low, __shfl_xor(low, off));
+    high = max(high, __shfl_xor(high, off));
   }
+  low = __builtin_amdgcn_readfirstlane(low);
+  high = __builtin_amdgcn_readfirstlane(high);
+  __syncthreads();
 
   floatx4 acc[kTiles][kDT];
-  float m[kTiles], l[kTiles];
+  // ref: the exponent's reference; start: -ref / c; renew: the exponent that renews it (any, before the first key)
+  float ref[kTiles], start[kTiles], renew[kTiles], l[kTiles];
+  constexpr float kUnset = -3.0e38f;
+  const float inv_c = 1.f / p.c;
 #pragma unroll
   for (int i = 0; i < kTiles; ++i) {
-    m[i] = -__builtin_inff();
-    l[i] = 0.f;
+    ref[i] = start[i] = l[i] = 0.f;
+    renew[i] = kUnset;
 #pragma unroll
     for (int d = 0; d < kDT; ++d) acc[i][d] = floatx4{0, 0, 0, 0};
   }
@@ -173,119 +192,168 @@ __global__ __launch_bounds__(256, 2) void cache_attn_kernel(const AttnParams p) 
     entries = view.seen == 0 ? 0 : (n < 0 ? 0 : (n < p.width ? n : p.width));
   }
   const int64_t share = cdiv(entries, p.parts);
-  const int64_t e0 = part * share, e1 = e0 + share < entries ? e0 + share : entries;
+  const int64_t e0 = part * share;
+  const int64_t e1 = high == 0 ? e0 : (e0 + share < entries ? e0 + share : entries);
 
+  const uint8_t *kbase = p.kc + static_cast<int64_t>(h) * (kPage * D) + col * D + g * 16;
+  const uint8_t *vbase = p.vc + static_cast<int64_t>(h) * (kPage * D) + col * kPage + g * 16;
+  const uint8_t *ksbase = p.ks + static_cast<int64_t>(h) * kPage + col * 4;
+  const uint8_t *vsbase = p.vs + static_cast<int64_t>(h) * kPage + g * 16;
   for (int64_t base = e0; base < e1; base += 64) {
-    // lane i resolves entry base + i: logical page and physical page, or -1
-    int64_t mine = base + lane;
-    int page = -1, pid = -1;
+    // lane i resolves entry base + i: logical and physical page; a place without a page reads page 0 and sees none of it
+    const int64_t mine = base + lane;
+    int page = -1, pid = 0;
     if (mine < e1) {
       page = list ? list[mine] : static_cast<int>(mine);
       if (list && mine > 0 && list[mine - 1] >= page) page = -1;
-      if (page >= 0 && page < view.seen) {
+      if (page >= view.seen) page = -1;
+      if (page >= 0) {
         pid = p.table[b * p.table_stride + page];
-        if (pid < 0 || pid >= p.pages) pid = -1;
+        if (pid < 0 || pid >= p.pages) {
+          pid = 0;
+          page = -1;
+        }
       }
     }
     const int n = static_cast<int>(e1 - base < 64 ? e1 - base : 64);
-    for (int i = pw; i < n; i += kPageWaves) {
-      const int ppage = __builtin_amdgcn_readlane(pid, i);
-      const int lpage = __builtin_amdgcn_readlane(page, i);
-      if (ppage < 0) continue;
-      const int64_t ph = static_cast<int64_t>(ppage) * p.H + h;
-      const uint8_t *kp = p.kc + ph * (kPage * D) + col * D + g * 16;
-      const uint8_t *vp = p.vc + ph * (kPage * D) + col * kPage + g * 16;
-      u32x4 kr[4][kK], vr[kDT];
+    u32x4 kr[4][kK];
+    uint32_t kb = 0;
+    auto load_keys = [&](int i) {
+      const int64_t at = static_cast<int64_t>(__builtin_amdgcn_readlane(pid, i)) * p.H;
 #pragma unroll
       for (int t = 0; t < 4; ++t)
 #pragma unroll
-        for (int x = 0; x < kK; ++x) kr[t][x] = *reinterpret_cast<const u32x4 *>(kp + t * 16 * D + x * 64);
-      const u32x4 kb = *reinterpret_cast<const u32x4 *>(p.ks + ph * kPage + g * 16);
-      const u32x4 vb = *reinterpret_cast<const u32x4 *>(p.vs + ph * kPage + g * 16);
+        for (int y = 0; y < kK; ++y)
+          kr[t][y] = *reinterpret_cast<const u32x4 *>(kbase + at * (kPage * D) + t * 16 * D + y * 64);
+      kb = *reinterpret_cast<const uint32_t *>(ksbase + at * kPage);
+    };
+    if (pw < n) load_keys(pw);
+    for (int i = pw; i < n; i += kPageWaves) {
+      const int lpage = __builtin_amdgcn_readlane(page, i);
+      const int64_t at = static_cast<int64_t>(__builtin_amdgcn_readlane(pid, i)) * p.H;
+      // the query operands are read again for every page: held over the loop they would cost 8 to 64 registers
+      asm volatile("" ::: "memory");
+      u32x4 vr[kDT];
 #pragma unroll
-      for (int d = 0; d < kDT; ++d) vr[d] = *reinterpret_cast<const u32x4 *>(vp + d * 16 * kPage);
+      for (int d = 0; d < kDT; ++d)
+        vr[d] = *reinterpret_cast<const u32x4 *>(vbase + at * (kPage * D) + d * 16 * kPage);
+      const u32x4 vb = *reinterpret_cast<const u32x4 *>(vsbase + at * kPage);
 
       floatx4 s[kTiles][4];
 #pragma unroll
-      for (int i2 = 0; i2 < kTiles; ++i2)
+      for (int t = 0; t < 4; ++t) {
+        const float power = pow2_byte((kb >> (8 * t)) & 255u);
 #pragma unroll
-        for (int t = 0; t < 4; ++t) s[i2][t] = floatx4{0, 0, 0, 0};
+        for (int y = 0; y < kK * 2; ++y) {
+          const u32x4 w = kr[t][y >> 1];
+          const bf16x8 a = y & 1 ? widen_scaled(w[2], w[3], power) : widen_scaled(w[0], w[1], power);
 #pragma unroll
-      for (int t = 0; t < 4; ++t)
+          for (int x = 0; x < kTiles; ++x)
 #pragma unroll
-        for (int x = 0; x < kK; ++x) {
-          const u32x4 w = kr[t][x];
-          const vec a0 = widen<Q>(w[0], w[1]), a1 = widen<Q>(w[2], w[3]);
-#pragma unroll
-          for (int i2 = 0; i2 < kTiles; ++i2) {
-            s[i2][t] = Mfma<Q>::mul(a0, qf[i2][x * 2], s[i2][t]);
-            s[i2][t] = Mfma<Q>::mul(a1, qf[i2][x * 2 + 1], s[i2][t]);
-          }
+            for (int piece = 0; piece < kParts; ++piece) {
+              const bf16x8 q = query[((rw * kTiles + x) * kOps + piece * kK * 2 + y) * 64 + lane];
+              const floatx4 c = y == 0 && piece == 0 ? floatx4{start[x], start[x], start[x], start[x]} : s[x][t];
+              s[x][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, q, c, 0, 0, 0);
+            }
         }
-      const int64_t key0 = static_cast<int64_t>(lpage) * kPage;
-      const bool masked = key0 + kPage > low;
+      }
+      // the next page's keys arrive while this one's weights are made
+      if (i + kPageWaves < n) load_keys(i + kPageWaves);
+
+      const int key0 = lpage * kPage;
+      const bool masked = lpage < 0 || key0 + kPage > low;
+      // exponents, in place: the byte's bias of 127 goes with the reference
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        const uint32_t vw = vb[t];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float ev = static_cast<float>((vw >> (8 * j)) & 255u);
+#pragma unroll
+          for (int x = 0; x < kTiles; ++x) s[x][t][j] = fmaf(s[x][t][j], p.c, ev);
+        }
+      }
+      if (masked) {
+#pragma unroll
+        for (int x = 0; x < kTiles; ++x) {
+          const int lim = (lpage < 0 ? 0 : limit[x] - key0) - g * 4;
+#pragma unroll
+          for (int t = 0; t < 4; ++t)
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              if (t * 16 + j >= lim) s[x][t][j] = -__builtin_inff();
+        }
+      }
+      bool renewing = false;
+      float top[kTiles];
+#pragma unroll
+      for (int x = 0; x < kTiles; ++x) {
+        float a = fmaxf(s[x][0][0], s[x][0][1]);
+#pragma unroll
+        for (int j = 2; j < 16; j += 2) a = fmaxf(fmaxf(a, s[x][j >> 2][j & 3]), s[x][j >> 2][(j & 3) + 1]);
+        top[x] = row4_max(a);
+        renewing = renewing || top[x] > renew[x];
+      }
+      if (__ballot(renewing)) {
+#pragma unroll
+        for (int x = 0; x < kTiles; ++x) {
+          const bool need = top[x] > renew[x];
+          const float by = need ? top[x] - kHeadroom : 0.f;
+          const float a = need && renew[x] != kUnset ? __builtin_amdgcn_exp2f(-by) : 1.f;
+          l[x] *= a;
+#pragma unroll
+          for (int d = 0; d < kDT; ++d) acc[x][d] *= a;
+#pragma unroll
+          for (int t = 0; t < 4; ++t)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) s[x][t][j] -= by;
+          ref[x] += by;
+          start[x] = -ref[x] * inv_c;
+          if (need) renew[x] = kHeadroom + kSlack;
+        }
+      }
+      uint32_t packed[kTiles][8];
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        const uint32_t iw = 0xfefefefeu - vb[t];  // the opposite powers
+        float un[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) un[j] = pow2_byte((iw >> (8 * j)) & 255u);
+#pragma unroll
+        for (int x = 0; x < kTiles; ++x) {
+          float w[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            w[j] = __builtin_amdgcn_exp2f(s[x][t][j]);
+            l[x] = fmaf(w[j], un[j], l[x]);
+          }
+          packed[x][t * 2] = pack_half2(w[0], w[1]);
+          packed[x][t * 2 + 1] = pack_half2(w[2], w[3]);
+        }
+      }
       halfx8 w[kTiles][2];
 #pragma unroll
-      for (int i2 = 0; i2 < kTiles; ++i2) {
-        float e[16];
-        float top = -__builtin_inff();
-        const int lim = static_cast<int>(limit[i2] - key0 < kPage ? (limit[i2] > key0 ? limit[i2] - key0 : 0) : kPage);
-#pragma unroll
-        for (int t = 0; t < 4; ++t) {
-          const uint32_t kw = kb[t], vw = vb[t];
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const float c = pow2_byte((kw >> (8 * j)) & 255u) * p.scale;
-            const float ev = static_cast<float>((vw >> (8 * j)) & 255u) - 127.f;
-            float x = fmaf(s[i2][t][j], c, ev);
-            if (masked) x = t * 16 + g * 4 + j < lim ? x : -__builtin_inff();
-            e[t * 4 + j] = x;
-            top = fmaxf(top, x);
-          }
-        }
-        top = row4_max(top);
-        if (__ballot(top > m[i2] + kSlack)) {
-          const float mn = fmaxf(m[i2], top);
-          const float a = mn == m[i2] ? 1.f : __builtin_amdgcn_exp2f(m[i2] - mn);
-          l[i2] *= a;
-#pragma unroll
-          for (int d = 0; d < kDT; ++d) acc[i2][d] *= a;
-          m[i2] = mn;
-        }
-        const float ref = m[i2] == -__builtin_inff() ? 0.f : m[i2] - kHeadroom;
-        uint32_t packed[8];
-        float sum = 0.f;
-#pragma unroll
-        for (int t = 0; t < 4; ++t) {
-          const uint32_t vw = vb[t];
-          float x[4];
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            x[j] = __builtin_amdgcn_exp2f(e[t * 4 + j] - ref);
-            sum = fmaf(x[j], pow2_byte(254u - ((vw >> (8 * j)) & 255u)), sum);
-          }
-          packed[t * 2] = pack_half2(x[0], x[1]);
-          packed[t * 2 + 1] = pack_half2(x[2], x[3]);
-        }
-        l[i2] += sum;
-        w[i2][0] = __builtin_bit_cast(halfx8, u32x4{packed[0], packed[1], packed[2], packed[3]});
-        w[i2][1] = __builtin_bit_cast(halfx8, u32x4{packed[4], packed[5], packed[6], packed[7]});
+      for (int x = 0; x < kTiles; ++x) {
+        w[x][0] = __builtin_bit_cast(halfx8, u32x4{packed[x][0], packed[x][1], packed[x][2], packed[x][3]});
+        w[x][1] = __builtin_bit_cast(halfx8, u32x4{packed[x][4], packed[x][5], packed[x][6], packed[x][7]});
       }
 #pragma unroll
       for (int d = 0; d < kDT; ++d) {
         const u32x4 v = vr[d];
-        const halfx8 a0 = widen<_Float16>(v[0], v[1]), a1 = widen<_Float16>(v[2], v[3]);
+        const halfx8 a0 = widen(v[0], v[1]), a1 = widen(v[2], v[3]);
 #pragma unroll
-        for (int i2 = 0; i2 < kTiles; ++i2) {
-          acc[i2][d] = Mfma<_Float16>::mul(a0, w[i2][0], acc[i2][d]);
-          acc[i2][d] = Mfma<_Float16>::mul(a1, w[i2][1], acc[i2][d]);
+        for (int x = 0; x < kTiles; ++x) {
+          acc[x][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a0, w[x][0], acc[x][d], 0, 0, 0);
+          acc[x][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a1, w[x][1], acc[x][d], 0, 0, 0);
         }
       }
     }
   }
+  float m[kTiles];
 #pragma unroll
   for (int i = 0; i < kTiles; ++i) {
     l[i] = row4_sum(l[i]);
+    m[i] = renew[i] == kUnset ? -__builtin_inff() : ref[i];
     if (limit[i] == 0) {  // no key, or no row: pages that all counting rows see were not masked for it
       m[i] = -__builtin_inff();
       l[i] = 0.f;
@@ -296,10 +364,12 @@ __global__ __launch_bounds__(256, 2) void cache_attn_kernel(const AttnParams p) 
 
   // the page waves' parts, joined in LDS by the first of them
   if constexpr (kPageWaves > 1) {
+    Sums *lo = reinterpret_cast<Sums *>(shared);  // of page waves 1..
+    __syncthreads();  // the query operands have been read
     if (pw > 0) {
 #pragma unroll
       for (int i = 0; i < kTiles; ++i) {
-        float *dst = lo[pw][(rw * kTiles + i) * 16 + col];
+        float *dst = lo[pw - 1][(rw * kTiles + i) * 16 + col];
         if (g == 0) {
           dst[D] = m[i];
           dst[D + 1] = l[i];
@@ -316,14 +386,14 @@ __global__ __launch_bounds__(256, 2) void cache_attn_kernel(const AttnParams p) 
     for (int i = 0; i < kTiles; ++i) {
       float mx = m[i];
 #pragma unroll
-      for (int x = 1; x < kPageWaves; ++x) mx = fmaxf(mx, lo[x][(rw * kTiles + i) * 16 + col][D]);
+      for (int x = 1; x < kPageWaves; ++x) mx = fmaxf(mx, lo[x - 1][(rw * kTiles + i) * 16 + col][D]);
       const float a = m[i] == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(m[i] - mx);
       l[i] *= a;
 #pragma unroll
       for (int d = 0; d < kDT; ++d) acc[i][d] *= a;
 #pragma unroll
       for (int x = 1; x < kPageWaves; ++x) {
-        const float *src = lo[x][(rw * kTiles + i) * 16 + col];
+        const float *src = lo[x - 1][(rw * kTiles + i) * 16 + col];
         const float mo = src[D];
         const float c = mo == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(mo - mx);
         l[i] = fmaf(src[D + 1], c, l[i]);
@@ -337,7 +407,7 @@ __global__ __launch_bounds__(256, 2) void cache_attn_kernel(const AttnParams p) 
   }
 #pragma unroll
   for (int i = 0; i < kTiles; ++i) {
-    const int r = ((tile * kRowWaves + rw) * kTiles + i) * 16 + col;
+    const int r = (rw * kTiles + i) * 16 + col;
     if (r >= p.rows) continue;
     const int tl = r / p.G, gh = r - tl * p.G;
     const int64_t t = t0 + tl;
@@ -400,32 +470,44 @@ __global__ __launch_bounds__(256) void cache_join_kernel(const AttnParams p) {
 }
 
 struct Shape {
-  int kind;   // 0: 16 rows, four page waves; 1: 32 rows likewise; 2: 64 rows, four row waves; 3: 128 rows
-  int tiles, parts;
+  int kind;   // 16 rows a wave, 32, or 64 or 128 a workgroup
+  int parts;
 };
 
-// Up to 32 rows a workgroup is bound by the cache's bytes, so its waves share the pages; beyond, by the products, so
-// they share the rows. The pages are split over workgroups until about four of them run on each CU, with at least
-// eight pages each (two for a page wave).
-Shape attn_shape(int64_t units, int64_t rows, int64_t pages) {
+// Up to 32 rows a wave holds all of a unit's rows and the four waves share its pages; beyond, they share the rows too.
+// A unit's pages are split over `parts` workgroups so that the rounds of resident workgroups (their registers allow 4 to
+// 2 on a CU) times the pages of one, with its start and the joining of its sums as so many pages more, come out least.
+Shape attn_shape(int64_t units, int64_t rows, int64_t pages, int64_t D) {
   Shape s;
   s.kind = rows <= 16 ? 0 : rows <= 32 ? 1 : rows <= 64 ? 2 : 3;
-  s.tiles = 1;
-  int64_t parts = cdiv(1024, units);
-  const int64_t most = cdiv(pages, 8);
-  if (parts > most) parts = most;
-  s.parts = static_cast<int>(parts < 1 ? 1 : parts > 256 ? 256 : parts);
+  const int64_t resident = 256 * (D == 128 ? 2 : s.kind == 0 ? 4 : 3);
+  const int page_waves = s.kind < 2 ? 4 : s.kind == 2 ? 2 : 1;
+  constexpr int64_t kStart = 4;
+  int64_t best = 0, best_cost = 0;
+  for (int64_t parts = 1; parts <= 256; ++parts) {
+    const int64_t share = cdiv(cdiv(pages, parts), page_waves);
+    if (parts > 1 && cdiv(pages, parts - 1) == cdiv(pages, parts)) continue;
+    const int64_t cost = cdiv(units * parts, resident) * (share + kStart + (parts > 1 ? 1 : 0));
+    if (best == 0 || cost < best_cost) {
+      best = parts;
+      best_cost = cost;
+    }
+    if (units * parts >= 8 * resident || parts >= pages) break;
+  }
+  s.parts = static_cast<int>(best);
   return s;
 }
 
 template <typename Q, int D>
 int launch_attn(const AttnParams &p, const Shape &s, hipStream_t st) {
-  const dim3 grid(static_cast<unsigned>(p.B * p.H * p.U * s.parts * s.tiles));
+  const dim3 grid(static_cast<unsigned>(p.B * p.H * p.U * s.parts));
+  // D = 128 has no registers for 64 rows a wave
+  constexpr int kWide = 2;
   switch (s.kind) {
     case 0: hipLaunchKernelGGL((cache_attn_kernel<Q, D, 1, 1>), grid, dim3(256), 0, st, p); break;
     case 1: hipLaunchKernelGGL((cache_attn_kernel<Q, D, 2, 1>), grid, dim3(256), 0, st, p); break;
-    case 2: hipLaunchKernelGGL((cache_attn_kernel<Q, D, 1, 4>), grid, dim3(256), 0, st, p); break;
-    default: hipLaunchKernelGGL((cache_attn_kernel<Q, D, 2, 4>), grid, dim3(256), 0, st, p); break;
+    case 2: hipLaunchKernelGGL((cache_attn_kernel<Q, D, kWide, 4 / kWide>), grid, dim3(256), 0, st, p); break;
+    default: hipLaunchKernelGGL((cache_attn_kernel<Q, D, kWide, 8 / kWide>), grid, dim3(256), 0, st, p); break;
   }
   int rc = check_launch("vasc_cache_attn");
   if (rc || s.parts == 1) return rc;
@@ -454,7 +536,7 @@ extern "C" int64_t vasc_cache_attn_workspace_size(int64_t B, int64_t Hq, int64_t
   using namespace vasc;
   if (!attn_sizes(B, Hq, H, T, D, block_q, max_pages, width)) return -1;
   const int64_t units = B * H * cdiv(T, block_q), rows = block_q * (Hq / H);
-  return workspace_bytes(units, rows, D, attn_shape(units, rows, width ? width : max_pages).parts);
+  return workspace_bytes(units, rows, D, attn_shape(units, rows, width ? width : max_pages, D).parts);
 }
 
 extern "C" int vasc_cache_attn(const void *q, int64_t q_sb, int64_t q_sh, int64_t q_st, void *o, int64_t o_sb,
@@ -493,13 +575,15 @@ extern "C" int vasc_cache_attn(const void *q, int64_t q_sb, int64_t q_sh, int64_
   p.block_q = static_cast<int>(block_q);
   p.causal = causal;
   p.index = index; p.width = width; p.count = count;
-  p.scale = scale * 1.4426950408889634f;
+  VASC_REQUIRE(scale - scale == 0.f && (scale == 0.f || (fabsf(scale) > 1e-30f && fabsf(scale) < 1e30f)),
+               "scale must be 0 or of magnitude 1e-30 to 1e30");
+  // the reference is divided by c: a scale of 0 is one too small to show
+  p.c = scale == 0.f ? 1e-30f : scale * 1.4426950408889634f;
   p.rows = p.block_q * p.G;
   const int64_t units = B * H * p.U;
-  const Shape s = attn_shape(units, p.rows, width ? width : max_pages);
+  const Shape s = attn_shape(units, p.rows, width ? width : max_pages, D);
   p.parts = s.parts;
-  p.tiles = s.tiles;
-  VASC_REQUIRE(units < (int64_t(1) << 31) / (s.parts * s.tiles), "too many units");
+  VASC_REQUIRE(units < (int64_t(1) << 31) / s.parts, "too many units");
   const int64_t need = workspace_bytes(units, p.rows, D, s.parts);
   VASC_REQUIRE(need == 0 || (workspace && workspace_bytes_given >= need), "workspace of %lld bytes, %lld needed",
                (long long)workspace_bytes_given, (long long)need);
