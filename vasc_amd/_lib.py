@@ -129,7 +129,7 @@ class VascArgumentError(VascError, ValueError):
 
 def call(name: str, *args) -> None:
     """Call an int-status entry point and raise on failure."""
-    lib = load()
+    lib = _lib or load()
     rc = getattr(lib, name)(*args)
     if rc != VASC_OK:
         msg = lib.vasc_last_error().decode(errors="replace")

@@ -475,26 +475,30 @@ struct Shape {
 };
 
 // Up to 32 rows a wave holds all of a unit's rows and the four waves share its pages; beyond, they share the rows too.
-// A unit's pages are split over `parts` workgroups so that the rounds of resident workgroups (their registers allow 4 to
-// 2 on a CU) times the pages of one, with its start and the joining of its sums as so many pages more, come out least.
+// A unit's pages are split over `parts` workgroups, as many as one to four rounds of resident workgroups take (their
+// registers allow 4 to 2 on a CU), where that is estimated to save more than the start of another round and the joining
+// of the sums cost. Measured, in us: a wave's page where few run 0.3, the start 3, the join 5 (up to 32 rows); with 64
+// or 128 rows 4, 4 and 8.
 Shape attn_shape(int64_t units, int64_t rows, int64_t pages, int64_t D) {
   Shape s;
   s.kind = rows <= 16 ? 0 : rows <= 32 ? 1 : rows <= 64 ? 2 : 3;
-  const int64_t resident = 256 * (D == 128 ? 2 : s.kind == 0 ? 4 : 3);
-  const int page_waves = s.kind < 2 ? 4 : s.kind == 2 ? 2 : 1;
-  constexpr int64_t kStart = 4;
-  int64_t best = 0, best_cost = 0;
-  for (int64_t parts = 1; parts <= 256; ++parts) {
-    const int64_t share = cdiv(cdiv(pages, parts), page_waves);
-    if (parts > 1 && cdiv(pages, parts - 1) == cdiv(pages, parts)) continue;
-    const int64_t cost = cdiv(units * parts, resident) * (share + kStart + (parts > 1 ? 1 : 0));
-    if (best == 0 || cost < best_cost) {
-      best = parts;
-      best_cost = cost;
+  const int64_t resident = 256 * (D == 128 || s.kind > 1 ? 2 : s.kind == 0 ? 4 : 3);
+  const int64_t waves = s.kind < 2 ? 4 : (s.kind == 2 ? 2 : 1) * (D == 64 ? 2 : 1);  // that share a workgroup's pages
+  const double page_us = s.kind < 2 ? 0.3 : 4.0, start_us = s.kind < 2 ? 3.0 : 4.0, join_us = s.kind < 2 ? 5.0 : 8.0;
+  double best = 0;
+  s.parts = 0;
+  for (int64_t rounds = 0; rounds <= 4; ++rounds) {
+    int64_t parts = rounds == 0 ? 1 : rounds * resident / units;
+    if (parts < 1) continue;
+    if (parts > 256) parts = 256;
+    const int64_t share = cdiv(cdiv(pages, parts), waves);  // pages of a wave
+    parts = cdiv(pages, share * waves);                     // the fewest with that share
+    const double us = cdiv(units * parts, resident) * (share * page_us + start_us) + (parts > 1 ? join_us : 0.0);
+    if (s.parts == 0 || us < best) {
+      best = us;
+      s.parts = static_cast<int>(parts);
     }
-    if (units * parts >= 8 * resident || parts >= pages) break;
   }
-  s.parts = static_cast<int>(best);
   return s;
 }
 
@@ -502,7 +506,7 @@ template <typename Q, int D>
 int launch_attn(const AttnParams &p, const Shape &s, hipStream_t st) {
   const dim3 grid(static_cast<unsigned>(p.B * p.H * p.U * s.parts));
   // D = 128 has no registers for 64 rows a wave
-  constexpr int kWide = 2;
+  constexpr int kWide = D == 64 ? 4 : 2;
   switch (s.kind) {
     case 0: hipLaunchKernelGGL((cache_attn_kernel<Q, D, 1, 1>), grid, dim3(256), 0, st, p); break;
     case 1: hipLaunchKernelGGL((cache_attn_kernel<Q, D, 2, 1>), grid, dim3(256), 0, st, p); break;

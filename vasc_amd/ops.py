@@ -7,6 +7,7 @@ must be device tensors; nothing here falls back to the CPU.
 from __future__ import annotations
 
 import ctypes
+import functools
 import math
 
 import numpy as np
@@ -667,84 +668,98 @@ def restore_tokens(x_patch: torch.Tensor, x_special: torch.Tensor | None, frames
 
 
 # ----------------------------------------------------------------- streaming
+# A single query token's kernels take a few microseconds, so these wrappers
+# count theirs: one look at each tensor, and no torch call that copies nothing.
 _DTYPE = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+_ROWS = (torch.bfloat16, torch.float16, torch.float32)
+_QUERIES = (torch.bfloat16, torch.float16)
 
 
-def _launch(ref: torch.Tensor, name: str, *args) -> None:
-    """``_lib.call`` on the current stream of ``ref``'s device."""
-    if torch._C._cuda_getDevice() == ref.device.index:
-        _lib.call(name, *args, _stream())
+def _launch(dev: int, name: str, *args) -> None:
+    """``_lib.call`` on the current stream of GPU ``dev``."""
+    if torch._C._cuda_getDevice() == dev:
+        _lib.call(name, *args, torch._C._cuda_getCurrentRawStream(dev))
     else:
-        with torch.cuda.device(ref.device):
-            _lib.call(name, *args, _stream())
+        with torch.cuda.device(dev):
+            _lib.call(name, *args, torch._C._cuda_getCurrentRawStream(dev))
 
 
-def _together(ref: torch.Tensor, **tensors) -> None:
-    for name, t in tensors.items():
-        if t is None:
-            continue
-        _dev(t, name)
-        if t.device != ref.device:
-            raise ValueError(f"{name} is on {t.device}, expected {ref.device}")
+def _gpu(t, name: str, dev: int = -1) -> int:
+    """The GPU that holds ``t``; it has to be ``dev`` where that is given."""
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+        raise ValueError(f"{name} must be a GPU tensor (the HIP path has no CPU fallback)")
+    at = t.get_device()
+    if dev >= 0 and at != dev:
+        raise ValueError(f"{name} is on cuda:{at}, expected cuda:{dev}")
+    return at
 
 
-def _inference(**tensors) -> None:
-    if torch.is_grad_enabled():
-        for name, t in tensors.items():
-            if t.requires_grad:
-                raise ValueError(f"{name} requires a gradient: the block cache has no backward pass, "
-                                 "call it under torch.no_grad()")
+def _inference(t: torch.Tensor, name: str) -> None:
+    if t.requires_grad and torch.is_grad_enabled():
+        raise ValueError(f"{name} requires a gradient: the block cache has no backward pass, "
+                         "call it under torch.no_grad()")
 
 
-def _rows8(t: torch.Tensor, name: str, dtypes: tuple) -> torch.Tensor:
-    """``[B,H,T,D]`` of one of ``dtypes`` with unit stride on D and 16-byte aligned rows."""
-    _dev(t, name)
+def _rows8(t: torch.Tensor, name: str, dtypes: tuple) -> tuple:
+    """(tensor, strides) of ``[B,H,T,D]`` with unit stride on D and 16-byte aligned rows."""
     if t.dim() != 4:
         raise ValueError(f"{name} must be [B,H,T,D], got {tuple(t.shape)}")
     if t.dtype not in dtypes:
         raise ValueError(f"{name} must be one of {[str(d) for d in dtypes]}, got {t.dtype}")
-    if t.stride(-1) != 1 or any(s % 8 for s in t.stride()[:3]) or t.data_ptr() % 16:
+    sb, sh, st, sd = t.stride()
+    if sd != 1 or (sb | sh | st) & 7 or t.data_ptr() & 15:
         t = t.contiguous()
-        if t.data_ptr() % 16:  # a contiguous view that starts inside a row
+        if t.data_ptr() & 15:  # contiguous, but a view that starts inside a row
             t = t.clone()
-    return t
+        sb, sh, st, sd = t.stride()
+        if (sb | sh | st) & 7:  # a head dimension that is no multiple of 8
+            raise ValueError(f"{name} has rows of {t.shape[3]} elements, expected a multiple of 8")
+    return t, sb, sh, st
 
 
-def _int_rows(t: torch.Tensor | None, name: str, B: int) -> torch.Tensor | None:
-    """``[B]`` int32, contiguous."""
+def _int_rows(t, name: str, B: int, dev: int):
+    """``[B]`` int32, contiguous (None stays)."""
     if t is None:
         return None
-    _dev(t, name)
-    if t.dtype.is_floating_point or t.dtype == torch.bool or t.shape != (B,):
+    _gpu(t, name, dev)
+    if t.shape != (B,) or t.dtype.is_floating_point or t.dtype is torch.bool:
         raise ValueError(f"{name} must hold {B} integers, got {t.dtype} {tuple(t.shape)}")
-    return t.to(torch.int32).contiguous()
+    if t.dtype is not torch.int32:
+        t = t.to(torch.int32)
+    return t if t.is_contiguous() else t.contiguous()
 
 
-def _page_table(t: torch.Tensor, B: int) -> tuple:
+def _page_table(t, B: int, dev: int) -> tuple:
     """(tensor, stride of a sequence, pages a sequence)."""
-    _dev(t, "page_table")
-    if t.dtype.is_floating_point or t.dtype == torch.bool or t.dim() != 2 or t.shape[0] != B or t.shape[1] == 0:
+    _gpu(t, "page_table", dev)
+    if t.dim() != 2 or t.shape[0] != B or t.shape[1] == 0 or t.dtype.is_floating_point or t.dtype is torch.bool:
         raise ValueError(f"page_table must be [{B}, max_pages] integers, got {t.dtype} {tuple(t.shape)}")
-    t = t.to(torch.int32)
-    if t.shape[1] > 1 and t.stride(1) != 1 or t.stride(0) < t.shape[1]:
+    if t.dtype is not torch.int32:
+        t = t.to(torch.int32)
+    mp = t.shape[1]
+    sb, sp = t.stride()
+    if (mp > 1 and sp != 1) or (B > 1 and sb < mp):
         t = t.contiguous()
-    return t, t.stride(0) if B > 1 else t.shape[1], t.shape[1]
+        sb = mp
+    return t, sb if B > 1 else mp, mp
 
 
 def _rotary_out(x: torch.Tensor) -> torch.Tensor:
     """An output in the memory order of ``x``: [B,T,H,D] where x's heads lie inside its tokens."""
     B, H, T, D = x.shape
     if x.stride(1) < x.stride(2):
-        return torch.empty(B, T, H, D, device=x.device, dtype=x.dtype).transpose(1, 2)
+        return torch.empty_strided((B, H, T, D), (T * H * D, D, H * D, 1), device=x.device, dtype=x.dtype)
     return torch.empty(B, H, T, D, device=x.device, dtype=x.dtype)
 
 
 def _rotary(q, k, pos, sections, inv_freq, inverse: bool) -> tuple:
-    q = q if q.stride(-1) == 1 else q.contiguous()
+    if q.stride(3) != 1:
+        q = q.contiguous()
     qo = _rotary_out(q)
     kargs, ko, Hk = (None, 0, 0, 0, None, 0, 0, 0), None, 0
     if k is not None:
-        k = k if k.stride(-1) == 1 else k.contiguous()
+        if k.stride(3) != 1:
+            k = k.contiguous()
         ko, Hk = _rotary_out(k), k.shape[1]
         kargs = (k.data_ptr(), *k.stride()[:3], ko.data_ptr(), *ko.stride()[:3])
     if q.numel() == 0 or (k is not None and k.numel() == 0):
@@ -754,10 +769,9 @@ def _rotary(q, k, pos, sections, inv_freq, inverse: bool) -> tuple:
             ko = _rotary(k, None, pos, sections, inv_freq, inverse)[0]
         return qo, ko
     B, Hq, T, D = q.shape
-    sec = (ctypes.c_int64 * len(sections))(*sections)
-    _launch(q, "vasc_rotary_axes", q.data_ptr(), *q.stride()[:3], qo.data_ptr(), *qo.stride()[:3], Hq, *kargs, Hk, B, T,
-            D, pos.data_ptr(), pos.stride(0) if pos.shape[0] > 1 else 0, pos.stride(1), len(sections),
-            ctypes.cast(sec, ctypes.c_void_p), inv_freq.data_ptr(), _DTYPE[q.dtype], int(inverse))
+    _launch(q.get_device(), "vasc_rotary_axes", q.data_ptr(), *q.stride()[:3], qo.data_ptr(), *qo.stride()[:3], Hq,
+            *kargs, Hk, B, T, D, pos.data_ptr(), pos.stride(0) if pos.shape[0] > 1 else 0, pos.stride(1), len(sections),
+            _section_sizes(sections, D), inv_freq.data_ptr(), _DTYPE[q.dtype], inverse)
     return qo, ko
 
 
@@ -781,6 +795,14 @@ class _RotaryAxes(torch.autograd.Function):
         return dq, dk, None, None, None
 
 
+@functools.lru_cache(maxsize=64)
+def _section_sizes(sections: tuple, D: int):
+    """The checked sections of a head dimension as a C array."""
+    if not 1 <= len(sections) <= 4 or any(s <= 0 or s % 2 for s in sections) or sum(sections) > D:
+        raise ValueError(f"sections {sections} must be 1 to 4 even sizes that sum to at most {D}")
+    return (ctypes.c_int64 * len(sections))(*sections)
+
+
 def rotary_axes(q: torch.Tensor, k: torch.Tensor | None, pos: torch.Tensor, sections, inv_freq: torch.Tensor):
     """Rotary embedding over several position axes, of q and k in one launch.
 
@@ -793,35 +815,36 @@ def rotary_axes(q: torch.Tensor, k: torch.Tensor | None, pos: torch.Tensor, sect
     through. Returns ``(q', k' or None)`` in the inputs' memory order;
     differentiable in q and k.
     """
-    _dev(q, "q")
-    _together(q, k=k, pos=pos, inv_freq=inv_freq)
+    dev = _gpu(q, "q")
     if q.dim() != 4 or q.dtype not in _DTYPE:
         raise ValueError(f"q must be [B,H,T,D] in bf16, fp16 or fp32, got {q.dtype} {tuple(q.shape)}")
     B, _, T, D = q.shape
-    if k is not None and (k.dim() != 4 or k.dtype != q.dtype or k.shape[0] != B or k.shape[2:] != q.shape[2:]):
-        raise ValueError(f"k must be [{B},H,{T},{D}] of {q.dtype}, got {k.dtype} {tuple(k.shape)}")
-    sections = tuple(int(s) for s in sections)
-    if not 1 <= len(sections) <= 4 or any(s <= 0 or s % 2 for s in sections) or sum(sections) > D:
-        raise ValueError(f"sections {sections} must be 1 to 4 even sizes that sum to at most {D}")
-    if pos.dtype.is_floating_point or pos.dtype == torch.bool:
-        raise ValueError(f"pos must hold integers, got {pos.dtype}")
+    if k is not None:
+        _gpu(k, "k", dev)
+        if k.dim() != 4 or k.dtype != q.dtype or k.shape[0] != B or k.shape[2:] != q.shape[2:]:
+            raise ValueError(f"k must be [{B},H,{T},{D}] of {q.dtype}, got {k.dtype} {tuple(k.shape)}")
+    sections = tuple(sections)
+    _section_sizes(sections, D)
+    _gpu(pos, "pos", dev)
+    if pos.dtype is not torch.int32:
+        if pos.dtype.is_floating_point or pos.dtype is torch.bool:
+            raise ValueError(f"pos must hold integers, got {pos.dtype}")
+        pos = pos.to(torch.int32)
     if pos.dim() == 2:
         pos = pos.unsqueeze(0)
-    if pos.dim() != 3 or pos.shape[0] not in (1, B) or pos.shape[1:] != (T, len(sections)):
-        raise ValueError(f"pos must be [{B} or 1, {T}, {len(sections)}], got {tuple(pos.shape)}")
-    if inv_freq.dtype != torch.float64 or inv_freq.shape != (sum(sections) // 2,):
+    A = len(sections)
+    if pos.shape != (B, T, A) and pos.shape != (1, T, A):
+        raise ValueError(f"pos must be [{B} or 1, {T}, {A}], got {tuple(pos.shape)}")
+    if pos.stride(2) != 1 and A > 1:
+        pos = pos.contiguous()
+    _gpu(inv_freq, "inv_freq", dev)
+    if inv_freq.dtype is not torch.float64 or inv_freq.shape != (sum(sections) // 2,):
         raise ValueError(f"inv_freq must hold {sum(sections) // 2} float64 values, got {inv_freq.dtype} "
                          f"{tuple(inv_freq.shape)}")
-    pos = pos.to(torch.int32)
-    pos = pos if pos.stride(-1) == 1 or pos.shape[-1] == 1 else pos.contiguous()
-    inv_freq = inv_freq.detach().contiguous()
+    inv_freq = inv_freq.detach().contiguous() if inv_freq.requires_grad or not inv_freq.is_contiguous() else inv_freq
     if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
         return _RotaryAxes.apply(q, k, pos, sections, inv_freq)
     return _rotary(q, k, pos, sections, inv_freq, False)
-
-
-def _cache_ptrs(cache) -> tuple:
-    return cache.kc.data_ptr(), cache.vc.data_ptr(), cache.ks.data_ptr(), cache.vs.data_ptr()
 
 
 def cache_write(cache, k: torch.Tensor, v: torch.Tensor, page_table: torch.Tensor, start: torch.Tensor,
@@ -839,23 +862,28 @@ def cache_write(cache, k: torch.Tensor, v: torch.Tensor, page_table: torch.Tenso
     came after. A token whose k or v row holds a value that is not finite is
     held as NaN in both. Nothing here waits for the GPU.
     """
-    _dev(k, "k")
-    _inference(k=k, v=v)
-    _together(k, v=v, page_table=page_table, start=start, count=count, cache=cache.kc)
-    dtypes = (torch.bfloat16, torch.float16, torch.float32)
-    k, v = _rows8(k, "k", dtypes), _rows8(v, "v", dtypes)
-    if k.shape != v.shape or k.dtype != v.dtype:
-        raise ValueError(f"k {k.dtype} {tuple(k.shape)} and v {v.dtype} {tuple(v.shape)} differ")
-    B, H, T, D = k.shape
-    if (H, D) != (cache.heads, cache.head_dim):
+    dev = _gpu(k, "k")
+    _gpu(v, "v", dev)
+    _inference(k, "k")
+    _inference(v, "v")
+    if cache.device_index != dev:
+        raise ValueError(f"the cache is on cuda:{cache.device_index}, k on cuda:{dev}")
+    k, ksb, ksh, kst = _rows8(k, "k", _ROWS)
+    v, vsb, vsh, vst = _rows8(v, "v", _ROWS)
+    B, H, T, D = shape = k.shape
+    if shape != v.shape or k.dtype != v.dtype:
+        raise ValueError(f"k {k.dtype} {tuple(shape)} and v {v.dtype} {tuple(v.shape)} differ")
+    if H != cache.heads or D != cache.head_dim:
         raise ValueError(f"the cache holds {cache.heads} heads of {cache.head_dim}, k has {H} of {D}")
-    table, ts, mp = _page_table(page_table, B)
-    start, count = _int_rows(start, "start", B), _int_rows(count, "count", B)
-    if k.numel() == 0:
+    table, ts, mp = _page_table(page_table, B, dev)
+    start, count = _int_rows(start, "start", B, dev), _int_rows(count, "count", B, dev)
+    if start is None:
+        raise ValueError("start is required")
+    if B == 0 or T == 0:
         return
-    _launch(k, "vasc_cache_write", k.data_ptr(), *k.stride()[:3], v.data_ptr(), *v.stride()[:3], B, H, T, D,
-            _DTYPE[k.dtype], table.data_ptr(), ts, mp, start.data_ptr(), _ptr(count), *_cache_ptrs(cache),
-            cache.mean.data_ptr(), cache.pages)
+    _launch(dev, "vasc_cache_write", k.data_ptr(), ksb, ksh, kst, v.data_ptr(), vsb, vsh, vst, B, H, T, D,
+            _DTYPE[k.dtype], table.data_ptr(), ts, mp, start.data_ptr(), _ptr(count), *cache.pointers,
+            cache.mean_pointer, cache.pages)
 
 
 def cache_read(cache, page_table: torch.Tensor, start: torch.Tensor, tokens: int, count: torch.Tensor | None = None,
@@ -863,36 +891,41 @@ def cache_read(cache, page_table: torch.Tensor, start: torch.Tensor, tokens: int
     """``(k, v) [B,H,tokens,D]`` of the cache's tokens ``start[b]..`` in
     ``dtype`` (bf16: exactly what the cache holds). Rows from ``count[b]`` on
     (default ``tokens``) and rows that have no page are zero."""
-    _dev(page_table, "page_table")
-    _together(page_table, start=start, count=count, cache=cache.kc)
+    dev = _gpu(page_table, "page_table")
+    if cache.device_index != dev:
+        raise ValueError(f"the cache is on cuda:{cache.device_index}, page_table on cuda:{dev}")
     if dtype not in _DTYPE:
         raise ValueError(f"dtype must be bf16, fp16 or fp32, got {dtype}")
-    B, tokens = page_table.shape[0], int(tokens)
+    B, H, D, tokens = page_table.shape[0], cache.heads, cache.head_dim, int(tokens)
     if tokens < 0:
         raise ValueError(f"tokens must not be negative, got {tokens}")
-    table, ts, mp = _page_table(page_table, B)
-    start, count = _int_rows(start, "start", B), _int_rows(count, "count", B)
-    k = torch.empty(B, cache.heads, tokens, cache.head_dim, device=table.device, dtype=dtype)
-    v = torch.empty_like(k)
-    if k.numel():
-        _launch(k, "vasc_cache_read", *_cache_ptrs(cache), cache.pages, table.data_ptr(), ts, mp, start.data_ptr(),
-                _ptr(count), B, cache.heads, tokens, cache.head_dim, _DTYPE[dtype], k.data_ptr(), v.data_ptr())
+    table, ts, mp = _page_table(page_table, B, dev)
+    start, count = _int_rows(start, "start", B, dev), _int_rows(count, "count", B, dev)
+    if start is None:
+        raise ValueError("start is required")
+    k = torch.empty(B, H, tokens, D, device=table.device, dtype=dtype)
+    v = torch.empty(B, H, tokens, D, device=table.device, dtype=dtype)
+    if B and tokens:
+        _launch(dev, "vasc_cache_read", *cache.pointers, cache.pages, table.data_ptr(), ts, mp, start.data_ptr(),
+                _ptr(count), B, H, tokens, D, _DTYPE[dtype], k.data_ptr(), v.data_ptr())
     return k, v
 
 
-def _cache_query(q, cache, page_table, lengths, q_count, block_q: int) -> tuple:
-    _dev(q, "q")
-    _inference(q=q)
-    _together(q, page_table=page_table, lengths=lengths, q_count=q_count, cache=cache.kc)
-    q = _rows8(q, "q", (torch.bfloat16, torch.float16))
+def _cache_query(q, cache, page_table, lengths, q_count, block_q: int, dev: int) -> tuple:
+    _inference(q, "q")
+    if cache.device_index != dev:
+        raise ValueError(f"the cache is on cuda:{cache.device_index}, q on cuda:{dev}")
+    q, sb, sh, st = _rows8(q, "q", _QUERIES)
     B, Hq, T, D = q.shape
     if D != cache.head_dim or Hq % cache.heads or Hq == 0:
         raise ValueError(f"q has {Hq} heads of {D}: expected a multiple of {cache.heads} heads of {cache.head_dim}")
-    G = Hq // cache.heads
-    if not (1 <= block_q and block_q * G <= 128):
-        raise ValueError(f"block_q {block_q} with {G} query heads a key head: a unit has 1 to 128 rows")
-    table, ts, mp = _page_table(page_table, B)
-    return q, table, ts, mp, _int_rows(lengths, "lengths", B), _int_rows(q_count, "q_count", B)
+    if not (1 <= block_q and block_q * (Hq // cache.heads) <= 128):
+        raise ValueError(f"block_q {block_q} with {Hq // cache.heads} query heads a key head: a unit has 1 to 128 rows")
+    table, ts, mp = _page_table(page_table, B, dev)
+    lengths = _int_rows(lengths, "lengths", B, dev)
+    if lengths is None:
+        raise ValueError("lengths is required")
+    return q, (q.data_ptr(), sb, sh, st), table, ts, mp, lengths, _int_rows(q_count, "q_count", B, dev)
 
 
 def cache_select(q: torch.Tensor, cache, page_table: torch.Tensor, lengths: torch.Tensor, keep: int, *,
@@ -916,22 +949,28 @@ def cache_select(q: torch.Tensor, cache, page_table: torch.Tensor, lengths: torc
     count. ``want_score`` adds the scores ``[B,H,U,max_pages]`` float32 (-inf
     for pages the unit does not see).
     """
-    block_q, keep, sink, recent = int(block_q), int(keep), int(sink), int(recent)
-    q, table, ts, mp, lengths, q_count = _cache_query(q, cache, page_table, lengths, q_count, block_q)
+    dev = _gpu(q, "q")
+    block_q, keep, sink, recent, causal = int(block_q), int(keep), int(sink), int(recent), bool(causal)
+    q, qargs, table, ts, mp, lengths, q_count = _cache_query(q, cache, page_table, lengths, q_count, block_q, dev)
     if keep < 0 or sink < 0 or recent < 1:
         raise ValueError(f"keep {keep} and sink {sink} must not be negative, recent {recent} at least 1")
     B, Hq, T, D = q.shape
     H, U = cache.heads, -(-T // block_q)
     width = min(mp, sink + keep + recent + ((block_q + BLOCK_K - 2) // BLOCK_K if causal else 0))
-    i32 = dict(device=q.device, dtype=torch.int32)
-    index, count = torch.empty(B, H, U, width, **i32), torch.empty(B, H, U, **i32)
-    score = torch.empty(B, H, U, mp, device=q.device, dtype=torch.float32)
-    if count.numel():
-        _launch(q, "vasc_cache_select", q.data_ptr(), *q.stride()[:3], B, Hq, H, T, D, _DTYPE[q.dtype],
-                cache.mean.data_ptr(), cache.pages, table.data_ptr(), ts, mp, lengths.data_ptr(), _ptr(q_count),
-                block_q, sink, recent, keep, int(bool(causal)), score.data_ptr(), index.data_ptr(), width,
-                count.data_ptr())
+    device = q.device
+    index = torch.empty(B, H, U, width, device=device, dtype=torch.int32)
+    count = torch.empty(B, H, U, device=device, dtype=torch.int32)
+    score = torch.empty(B, H, U, mp, device=device, dtype=torch.float32)
+    if B and T:
+        _launch(dev, "vasc_cache_select", *qargs, B, Hq, H, T, D, _DTYPE[q.dtype], cache.mean_pointer, cache.pages,
+                table.data_ptr(), ts, mp, lengths.data_ptr(), _ptr(q_count), block_q, sink, recent, keep, causal,
+                score.data_ptr(), index.data_ptr(), width, count.data_ptr())
     return (index, count, score) if want_score else (index, count)
+
+
+@functools.lru_cache(maxsize=256)
+def _attn_workspace(*sizes: int) -> int:
+    return _lib.fn("vasc_cache_attn_workspace_size")(*sizes)
 
 
 def cache_attn(q: torch.Tensor, cache, page_table: torch.Tensor, lengths: torch.Tensor,
@@ -949,7 +988,7 @@ def cache_attn(q: torch.Tensor, cache, page_table: torch.Tensor, lengths: torch.
     ``D ** -0.5``). Returns ``[B,Hq,T,D]`` of q's dtype, written to ``out``
     when given (unit stride over D).
     """
-    _dev(q, "q")
+    dev = _gpu(q, "q")
     if (index is None) != (count is None):
         raise ValueError("index and count go together")
     if q.dim() != 4:
@@ -959,31 +998,39 @@ def cache_attn(q: torch.Tensor, cache, page_table: torch.Tensor, lengths: torch.
             raise ValueError("lists need the block_q they were made with")
         block_q = max(1, min(q.shape[2], 128 // max(1, q.shape[1] // cache.heads)))
     block_q = int(block_q)
-    q, table, ts, mp, lengths, q_count = _cache_query(q, cache, page_table, lengths, q_count, block_q)
-    _together(q, index=index, count=count, out=out)
-    B, Hq, T, D = q.shape
-    H, U, width = cache.heads, -(-T // block_q), 0
+    q, qargs, table, ts, mp, lengths, q_count = _cache_query(q, cache, page_table, lengths, q_count, block_q, dev)
+    B, Hq, T, D = shape = q.shape
+    H, width = cache.heads, 0
     if index is not None:
+        U = -(-T // block_q)
+        _gpu(index, "index", dev)
+        _gpu(count, "count", dev)
         if index.dim() != 4 or index.shape[:3] != (B, H, U) or count.shape != (B, H, U):
             raise ValueError(f"index/count must be [{B},{H},{U},W]/[{B},{H},{U}], got {tuple(index.shape)}/"
                              f"{tuple(count.shape)}")
-        if any(t.dtype.is_floating_point or t.dtype == torch.bool for t in (index, count)):
-            raise ValueError("index and count must be integers")
-        index, count = index.to(torch.int32).contiguous(), count.to(torch.int32).contiguous()
+        if index.dtype is not torch.int32 or count.dtype is not torch.int32:
+            if any(t.dtype.is_floating_point or t.dtype is torch.bool for t in (index, count)):
+                raise ValueError("index and count must be integers")
+            index, count = index.to(torch.int32), count.to(torch.int32)
+        index, count = index.contiguous(), count.contiguous()
         width = index.shape[3]
     if out is None:
-        out = torch.empty(B, Hq, T, D, device=q.device, dtype=q.dtype)
-    elif (out.shape != q.shape or out.dtype != q.dtype or out.stride(3) != 1 or any(s % 4 for s in out.stride()[:3])
-          or out.data_ptr() % 8):
-        raise ValueError(f"out must be {q.dtype} {tuple(q.shape)} with unit stride over D, 8-byte aligned rows")
-    if q.numel() == 0:
+        out = torch.empty(shape, device=q.device, dtype=q.dtype)
+        osb, osh, ost = Hq * T * D, T * D, D
+    else:
+        _gpu(out, "out", dev)
+        if out.shape != shape or out.dtype != q.dtype:
+            raise ValueError(f"out must be {q.dtype} {tuple(shape)}, got {out.dtype} {tuple(out.shape)}")
+        osb, osh, ost, osd = out.stride()
+        if osd != 1 or (osb | osh | ost) & 3 or out.data_ptr() & 7:
+            raise ValueError("out needs unit stride over D and 8-byte aligned rows")
+    if B == 0 or T == 0:
         return out
     if index is not None and width == 0:
         return out.zero_()
-    scale = D ** -0.5 if scale is None else float(scale)
-    size = _lib.fn("vasc_cache_attn_workspace_size")(B, Hq, H, T, D, block_q, mp, width)
+    size = _attn_workspace(B, Hq, H, T, D, block_q, mp, width)
     ws = torch.empty(size, device=q.device, dtype=torch.uint8) if size > 0 else None
-    _launch(q, "vasc_cache_attn", q.data_ptr(), *q.stride()[:3], out.data_ptr(), *out.stride()[:3], B, Hq, H, T, D,
-            _DTYPE[q.dtype], *_cache_ptrs(cache), cache.pages, table.data_ptr(), ts, mp, lengths.data_ptr(),
-            _ptr(q_count), block_q, _ptr(index), width, _ptr(count), int(bool(causal)), scale, _ptr(ws), max(size, 0))
+    _launch(dev, "vasc_cache_attn", *qargs, out.data_ptr(), osb, osh, ost, B, Hq, H, T, D, _DTYPE[q.dtype],
+            *cache.pointers, cache.pages, table.data_ptr(), ts, mp, lengths.data_ptr(), _ptr(q_count), block_q,
+            _ptr(index), width, _ptr(count), bool(causal), D ** -0.5 if scale is None else scale, _ptr(ws), size)
     return out

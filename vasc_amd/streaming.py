@@ -31,11 +31,21 @@ class BlockCache:
         self.pages, self.heads, self.head_dim = int(pages), int(heads), int(head_dim)
         u8 = dict(device=device, dtype=torch.uint8)
         page = ops.BLOCK_K
-        self.kc = torch.zeros(pages, heads, page, head_dim, **u8)
-        self.vc = torch.zeros(pages, heads, head_dim, page, **u8)
-        self.ks = torch.zeros(pages, heads, page, **u8)
-        self.vs = torch.zeros(pages, heads, page, **u8)
-        self.mean = torch.zeros(pages, heads, head_dim, device=device, dtype=torch.bfloat16)
+        self._kc = torch.zeros(pages, heads, page, head_dim, **u8)
+        self._vc = torch.zeros(pages, heads, head_dim, page, **u8)
+        self._ks = torch.zeros(pages, heads, page, **u8)
+        self._vs = torch.zeros(pages, heads, page, **u8)
+        self._mean = torch.zeros(pages, heads, head_dim, device=device, dtype=torch.bfloat16)
+        self.device_index = self._kc.get_device()
+        # the buffers stay where they are, so a call need not ask for their addresses again
+        self.pointers = tuple(t.data_ptr() for t in (self._kc, self._vc, self._ks, self._vs))
+        self.mean_pointer = self._mean.data_ptr()
+
+    kc = property(lambda self: self._kc)
+    vc = property(lambda self: self._vc)
+    ks = property(lambda self: self._ks)
+    vs = property(lambda self: self._vs)
+    mean = property(lambda self: self._mean)
 
     @property
     def nbytes(self) -> int:
