@@ -369,6 +369,28 @@ def test_select_ties_nan_and_missing_pages():
         assert count[0, 0, 2] == 0 and (index[0, 0, 2] == -1).all()
 
 
+@pytest.mark.parametrize("mp", [200, 600, 4000, 9000])
+def test_select_equal_and_close_scores(mp):
+    """All scores equal (the list is the first pages), equal in two halves, and apart in their last bits only."""
+    g = _gen(mp)
+    cache = BlockCache(mp, 1, 64)
+    table = torch.arange(mp, dtype=torch.int32).view(1, mp).cuda()
+    q = torch.zeros(1, 1, 1, 64, dtype=torch.bfloat16, device="cuda")
+    q[..., 0], q[..., 1] = 1.0, 2.0 ** -9
+    for kind in range(3):
+        m = torch.zeros(mp, 64)
+        if kind == 1:
+            m[::2, 0] = -1.0
+        if kind == 2:
+            m[:, 0] = -1.0
+            m[:, 1] = torch.randint(0, 200, (mp,), generator=g).float() * 2.0 ** -7
+        cache.mean[:, 0] = m.bfloat16().cuda()
+        for keep in (1, 7, mp // 2 - 1, mp // 2, mp - 3):
+            index, count = ops.cache_select(q, cache, table, _i32([mp * 64]), keep)
+            want, _ = O.select(_np(q)[0, :, 0], _np(cache.mean)[:, 0], mp, mp - 1, keep, 1, 1)
+            assert count.item() == len(want) and index[0, 0, 0, :len(want)].tolist() == want
+
+
 # ------------------------------------------------------------------ attention
 def _check_attend(o, q, held, lens, lists, block_q, causal, scale=None, n_q=None, H=None):
     """o against float64 over the held values. Bound for an element: the output's rounding; weights rounded to half

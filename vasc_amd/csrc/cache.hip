@@ -302,7 +302,7 @@ struct SelectParams {
   const int32_t *table;
   int64_t table_stride, max_pages;
   const int32_t *lengths, *n_q;
-  int block_q, causal, chunks;
+  int block_q, causal, chunks, rounds;
   int64_t sink, recent, keep, width;
   float *score;
   int32_t *index, *count;
@@ -328,69 +328,147 @@ __device__ __forceinline__ Unit unit_of(const SelectParams &p, int row) {
   return n;
 }
 
-constexpr int kScorePages = 256;  // pages of a scoring workgroup
-
-// Scores of a unit against 256 pages: the bf16 mean of its query rows times each page's bf16 key mean, products and sums
+// Scores of a unit against its pages: the bf16 mean of its query rows times each page's bf16 key mean, products and sums
 // in float64. Those products are exact and their sums all but always, so the order of a sum does not show in the score.
+//
+// Bound: the float64 pipe (a conversion, a product and a seventh of an exchange for each feature and page) and the latency
+// of what depends on what (lengths, page table and queries, means). So all that can is in flight together: a workgroup
+// asks for its pages' places before it has seen the lengths and for their means before it sums the queries; the sums of
+// kScoreBatch pages cross the lanes together, each step leaving a lane half the pages; and a workgroup takes as many
+// rounds of pages as leave the chip some four workgroups a CU.
+constexpr int kScoreBatch = 8;
+
+// Sums v[0..8) over the lanes that differ in the bits [lo, hi) of the lane number; a lane is left with the sum of element
+// (its low three of those bits) in v[0].
+__device__ __forceinline__ void scatter_sum(double (&v)[8], int lo, int hi) {
+  int width = 8;
+#pragma unroll
+  for (int o = lo; o < hi; o <<= 1) {
+    if (width > 1) {
+      width >>= 1;
+      const bool up = __lane_id() & o;
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (i < width) {
+          const double keep = up ? v[2 * i + 1] : v[2 * i], send = up ? v[2 * i] : v[2 * i + 1];
+          v[i] = keep + xor_lane(send, o);
+        }
+    } else {
+      v[0] += xor_lane(v[0], o);
+    }
+  }
+}
+
 template <typename T, int D>
 __global__ __launch_bounds__(256) void cache_score_kernel(const SelectParams p) {
-  constexpr int kLanes = D / 8, kRows = 256 / kLanes;
-  __shared__ double part[kRows][D];
+  constexpr int kLanes = D / 8, kRows = 256 / kLanes;  // lanes of a row or page; rows or pages of a step
+  constexpr int kRound = kScoreBatch * kRows;
+  const int kPages = kRound * p.rounds;
+  __shared__ double part[4][D];
   __shared__ float qm[D];
-  const int tid = threadIdx.x;
+  const int tid = threadIdx.x, lane = tid % kLanes, grp = tid / kLanes;
   const int64_t row = static_cast<int>(blockIdx.x) / p.chunks;
-  const int64_t first = static_cast<int64_t>(static_cast<int>(blockIdx.x) % p.chunks) * kScorePages;
+  const int first = static_cast<int>(blockIdx.x) % p.chunks * kPages;
+  const int end = static_cast<int>(first + kPages < p.max_pages ? first + kPages : p.max_pages);
+  const int64_t b = row / (static_cast<int64_t>(p.U) * p.H);
+  int pid[kScoreBatch];
+#pragma unroll
+  for (int i = 0; i < kScoreBatch; ++i) {
+    const int j = first + grp + i * kRows;
+    pid[i] = j < end ? p.table[b * p.table_stride + j] : -1;
+  }
   const Unit n = unit_of(p, static_cast<int>(row));
+  const int seen = static_cast<int>(n.view.seen);
   float *out = p.score + row * p.max_pages;
-  const int64_t end = first + kScorePages < p.max_pages ? first + kScorePages : p.max_pages;
-  if (first >= n.view.seen) {
-    for (int64_t j = first + tid; j < end; j += 256) out[j] = -__builtin_inff();
+  if (first >= seen) {
+    for (int j = first + tid; j < end; j += 256) out[j] = -__builtin_inff();
     return;
   }
-  const int lane = tid % kLanes, grp = tid / kLanes;
-  const int rows = static_cast<int>((n.t1 - n.t0) * p.G);
+  const int rows = static_cast<int>(n.t1 - n.t0) * p.G;
+  // up to 128 rows: at most kMost a lane group
+  constexpr int kMost = 128 / kRows;
+  typedef uint32_t words __attribute__((ext_vector_type(4)));
+  words x[kMost];
+  const T *q = static_cast<const T *>(p.q) + n.b * p.qsb + n.h * p.G * p.qsh + n.t0 * p.qst + lane * 8;
+#pragma unroll
+  for (int i = 0; i < kMost; ++i) {
+    const int r = grp + i * kRows, tl = r / p.G;
+    x[i] = words{0, 0, 0, 0};
+    if (r < rows) x[i] = *reinterpret_cast<const words *>(q + tl * p.qst + (r - tl * p.G) * p.qsh);
+  }
+  u32x4 m[kScoreBatch];
+#pragma unroll
+  for (int i = 0; i < kScoreBatch; ++i) {
+    if (first + grp + i * kRows >= seen || pid[i] >= p.pages) pid[i] = -1;
+    m[i] = u32x4{0, 0, 0, 0};
+    if (pid[i] >= 0)
+      m[i] = *reinterpret_cast<const u32x4 *>(p.mean + (static_cast<int64_t>(pid[i]) * p.H + n.h) * D + lane * 8);
+  }
   {
     double s[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-    const T *q = static_cast<const T *>(p.q) + n.b * p.qsb + n.h * p.G * p.qsh + n.t0 * p.qst + lane * 8;
-    for (int r = grp; r < rows; r += kRows) {
-      float x[8];
-      load8(q + (r / p.G) * p.qst + (r % p.G) * p.qsh, x);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) s[i] += static_cast<double>(x[i]);
+    for (int i = 0; i < kMost; ++i) {
+      if (i * kRows >= rows) break;
+      struct alignas(16) Eight { T v[8]; };
+      const Eight v = __builtin_bit_cast(Eight, x[i]);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) s[e] += static_cast<double>(to_f32(v.v[e]));
     }
-#pragma unroll
-    for (int i = 0; i < 8; ++i) part[grp][lane * 8 + i] = s[i];
+    // lanes of different rows: D = 64 leaves a feature a lane, D = 128 two
+    scatter_sum(s, kLanes, 64);
+    const int at = (tid & 63) / kLanes;
+    if (D == 64) {
+      part[tid >> 6][lane * 8 + at] = s[0];
+    } else {
+      part[tid >> 6][lane * 8 + at] = s[0];
+      part[tid >> 6][lane * 8 + at + 4] = s[1];
+    }
   }
   __syncthreads();
-  if (tid < D) {
-    double s = 0;
-    for (int i = 0; i < kRows && i < rows; ++i) s += part[i][tid];
-    qm[tid] = round_bf16(static_cast<float>(s / rows));
-  }
+  if (tid < D)
+    qm[tid] = round_bf16(static_cast<float>((part[0][tid] + part[1][tid] + part[2][tid] + part[3][tid]) / rows));
   __syncthreads();
   double qd[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) qd[i] = static_cast<double>(qm[lane * 8 + i]);
-  for (int64_t j = first + grp; j < end; j += kRows) {
-    int64_t pid = -1;
-    if (j < n.view.seen) {
-      pid = p.table[n.b * p.table_stride + j];
-      if (pid >= p.pages) pid = -1;
-    }
-    double s = 0;
-    if (pid >= 0) {
-      const u32x4 m = *reinterpret_cast<const u32x4 *>(p.mean + (pid * p.H + n.h) * D + lane * 8);
+  for (int j0 = first;;) {
+    double sum[kScoreBatch];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const uint32_t word = m[i >> 1];
-        s = fma(qd[i], static_cast<double>(__uint_as_float(i & 1 ? word & 0xffff0000u : word << 16)), s);
+    for (int i = 0; i < kScoreBatch; ++i) {
+      sum[i] = 0;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const uint32_t word = m[i][e >> 1];
+        sum[i] = fma(qd[e], static_cast<double>(__uint_as_float(e & 1 ? word & 0xffff0000u : word << 16)), sum[i]);
       }
     }
+    scatter_sum(sum, 1, kLanes);
+    // lane i of the group (of its first eight) has page i of the batch
+    uint32_t gone = 0;
 #pragma unroll
-    for (int o = 1; o < kLanes; o <<= 1) s += xor_lane(s, o);
-    float f = static_cast<float>(s);
-    if (pid < 0 || f != f) f = -__builtin_inff();
-    if (lane == 0) out[j] = f;
+    for (int i = 0; i < kScoreBatch; ++i) gone |= (pid[i] < 0 ? 1u : 0u) << i;
+    const int i = lane & 7, j = j0 + grp + i * kRows;
+    float f = static_cast<float>(sum[0]);
+    if ((gone >> i & 1) || f != f) f = -__builtin_inff();
+    if (lane < 8 && j < end) out[j] = f;
+    j0 += kRound;
+    if (j0 >= end) break;
+    if (j0 >= seen) {
+      for (int k = j0 + tid; k < end; k += 256) out[k] = -__builtin_inff();
+      break;
+    }
+#pragma unroll
+    for (int k = 0; k < kScoreBatch; ++k) {
+      const int page = j0 + grp + k * kRows;
+      pid[k] = page < seen && page < end ? p.table[b * p.table_stride + page] : -1;
+    }
+#pragma unroll
+    for (int k = 0; k < kScoreBatch; ++k) {
+      if (pid[k] >= p.pages) pid[k] = -1;
+      m[k] = u32x4{0, 0, 0, 0};
+      if (pid[k] >= 0)
+        m[k] = *reinterpret_cast<const u32x4 *>(p.mean + (static_cast<int64_t>(pid[k]) * p.H + n.h) * D + lane * 8);
+    }
   }
 }
 
@@ -401,69 +479,167 @@ __device__ __forceinline__ uint32_t score_key(float f) {
 }
 
 // The list of one unit. Wave w holds the scores of pages [w * 64 E, (w + 1) * 64 E) in registers, page base + i * 64 + lane
-// in element i. The keep-th largest is found bit by bit from the top, one count of all elements a bit; a count that
-// meets `keep` exactly ends it.
+// in element i, and looks for the last chosen of them: (cut, cut_page), such that a page is chosen with a higher score, or
+// the same one and no higher a number.
+//
+// One wave finds the keep-th largest bit by bit from the top, a count of all elements a bit; a count that meets `keep`
+// exactly ends it. More waves would pay a barrier a bit (9.9 us for 128 lists of 2048 pages): they sort into 2048 bins by
+// the next 11 bits instead, until the bin that holds the cut has at most kRanked members (scores of one sign and size spread
+// over some dozens of bins, so most lists need one turn), which are then ranked among themselves.
+constexpr int kBins = 2048, kRanked = 128;
+
 template <int kWaves, int E>
 __global__ __launch_bounds__(kWaves * 64) void cache_list_kernel(const SelectParams p) {
-  __shared__ int sums[2][kWaves], wave_total[kWaves], wave_equal[kWaves];
+  constexpr int kThreads = kWaves * 64;
+  constexpr int kOwn = kBins / (kWaves > 1 ? kThreads : kBins);  // bins of a thread
+  __shared__ uint32_t bins[kWaves > 1 ? kBins : 1];
+  __shared__ __align__(16) uint64_t ranked[kWaves > 1 ? kRanked : 1];
+  static_assert(kWaves == 1 || kRanked <= kThreads, "a thread a member");
+  __shared__ int wave_total[kWaves], wave_equal[kWaves];
+  __shared__ int found[4];  // the cut's bin, what is left to choose in it, its members; the next free place of `ranked`
+  __shared__ uint64_t last;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int64_t row = blockIdx.x;
-  const Unit n = unit_of(p, blockIdx.x);
   const float *score = p.score + row * p.max_pages;
-  const int64_t seen = n.view.seen;
-  const int64_t base = static_cast<int64_t>(wave) * 64 * E;
-  const int64_t tail = n.view.own - (p.recent - 1);  // pages from here on are listed
-  uint32_t key[E];
-  uint32_t forced = 0;
-  static_assert(E <= 32, "one bit an element");
+  const int base = wave * 64 * E;
+  float value[E];  // asked for before the lengths are known: all of max_pages are written
 #pragma unroll
   for (int i = 0; i < E; ++i) {
-    const int64_t j = base + i * 64 + lane;
+    const int j = base + i * 64 + lane;
+    value[i] = j < p.max_pages ? score[j] : 0.f;
+  }
+  const Unit n = unit_of(p, blockIdx.x);
+  const int seen = static_cast<int>(n.view.seen), sink = static_cast<int>(p.sink);
+  const int tail = static_cast<int>(n.view.own - (p.recent - 1));  // pages from here on are listed
+  uint32_t key[E];  // 0: not free to choose
+  uint32_t forced = 0;
+  static_assert(E <= 32, "one bit an element");
+  int free_pages = 0;
+#pragma unroll
+  for (int i = 0; i < E; ++i) {
+    const int j = base + i * 64 + lane;
     key[i] = 0;
     if (j < seen) {
-      if (j < p.sink || j >= tail)
+      if (j < sink || j >= tail)
         forced |= 1u << i;
       else
-        key[i] = score_key(score[j]);
+        key[i] = score_key(value[i]);
     }
   }
-  int turn = 0;
-  auto total = [&](uint32_t at_least) {
-    int c = 0;
-#pragma unroll
-    for (int i = 0; i < E; ++i) c += __popcll(__ballot(key[i] >= at_least));
-    if (lane == 0) sums[turn][wave] = c;
-    __syncthreads();
-    int s = 0;
-#pragma unroll
-    for (int w = 0; w < kWaves; ++w) s += sums[turn][w];
-    turn ^= 1;  // the next count writes the other half: one barrier a count
-    return s;
-  };
-  const int free_pages = total(1);
-  uint32_t cut = 1;  // chosen: key > cut, and the first `ties` of key == cut; or key >= cut
-  int ties = -1;     // -1: all that equal the cut
+  {
+    const int end = tail < seen ? tail : seen;  // the free pages are [sink, end)
+    free_pages = end > sink ? end - sink : 0;
+  }
+  uint32_t cut = 1;              // chosen: above the cut, or
+  int cut_page = 1 << 30;        // on it and no higher a page, or
+  int ties = 0;                  // on it and (ties > 0) among the first of those
   if (p.keep < free_pages) {
-    const int keep = static_cast<int>(p.keep);
-    uint32_t t = 0;
-    bool exact = false;
-    if (keep == 0) {
-      t = 0xffffffffu;  // no score has this key (it would be a NaN)
-      exact = true;
+    int want = static_cast<int>(p.keep);
+    if (want == 0) {
+      cut = 0xffffffffu;  // no score has this key (it would be a NaN)
+    } else if (kWaves == 1) {
+      uint32_t t = 0;
+      int at = 0;
+      bool exact = false;
+      for (int bit = 31; bit >= 0 && !exact; --bit) {
+        const uint32_t cand = t | (1u << bit);
+        int c = 0;
+#pragma unroll
+        for (int i = 0; i < E; ++i) c += __popcll(__ballot(key[i] >= cand));
+        if (c >= want) {
+          t = cand;
+          at = c;
+        }
+        exact = c == want;
+      }
+      cut = t;
+      if (!exact && at > want) {
+        int above = 0;
+#pragma unroll
+        for (int i = 0; i < E; ++i) above += __popcll(__ballot(key[i] > cut));
+        ties = want - above;
+      }
+    } else {
+      uint32_t prefix = 0, mask = 0;  // the cut's bits found so far
+      for (int shift = 21; ; shift = shift == 21 ? 10 : 0) {
+        const uint32_t digits = shift == 0 ? 1023u : 2047u;
+        for (int i = tid; i < kBins; i += kThreads) bins[i] = 0;
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < E; ++i)
+          if (key[i] != 0 && (key[i] & mask) == prefix) atomicAdd(&bins[(key[i] >> shift) & digits], 1u);
+        __syncthreads();
+        int own = 0;
+#pragma unroll
+        for (int i = 0; i < kOwn; ++i) own += bins[tid * kOwn + i];
+        int above = own;  // this thread's bins and those over them, in the wave and then in all
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+          const int x = __shfl_down(above, o);
+          if (lane + o < 64) above += x;
+        }
+        if (lane == 0) wave_total[wave] = above;
+        __syncthreads();
+        for (int w = wave + 1; w < kWaves; ++w) above += wave_total[w];
+        above -= own;
+        if (above < want && above + own >= want) {  // one thread
+#pragma unroll
+          for (int i = kOwn - 1; i >= 0; --i) {
+            const int c = bins[tid * kOwn + i];
+            if (above < want && above + c >= want) {
+              found[0] = tid * kOwn + i;
+              found[1] = want - above;
+              found[2] = c;
+              found[3] = 0;
+            }
+            above += c;
+          }
+        }
+        __syncthreads();
+        prefix |= static_cast<uint32_t>(found[0]) << shift;
+        mask |= digits << shift;
+        want = found[1];
+        const int members = found[2];
+        if (members == want) {  // the whole bin
+          cut = prefix;
+          break;
+        }
+        if (members <= kRanked) {
+#pragma unroll
+          for (int i = 0; i < E; ++i)
+            if (key[i] != 0 && (key[i] & mask) == prefix)
+              ranked[atomicAdd(&found[3], 1)] =
+                  static_cast<uint64_t>(key[i]) << 32 | static_cast<uint32_t>(~(base + i * 64 + lane));
+          const int padded = (members + 7) & ~7;
+          if (tid >= members && tid < padded) ranked[tid] = 0;
+          __syncthreads();
+          if (tid < members) {
+            const uint64_t mine = ranked[tid];
+            int over = 0;
+            for (int i = 0; i < padded; i += 8) {
+#pragma unroll
+              for (int e = 0; e < 8; ++e) over += ranked[i + e] > mine;
+            }
+            if (over == want - 1) last = mine;
+          }
+          __syncthreads();
+          cut = static_cast<uint32_t>(last >> 32);
+          cut_page = static_cast<int>(~static_cast<uint32_t>(last));
+          break;
+        }
+        if (shift == 0) {  // equal scores, more of them than are ranked
+          cut = prefix;
+          ties = want;
+          break;
+        }
+        __syncthreads();  // `found` and the bins are written again
+      }
     }
-    for (int bit = 31; bit >= 0 && !exact; --bit) {
-      const uint32_t cand = t | (1u << bit);
-      const int c = total(cand);
-      if (c >= keep) t = cand;
-      exact = c == keep;
-    }
-    cut = t;
-    if (!exact) ties = keep - (t == 0xffffffffu ? 0 : total(t + 1));
   }
   // places: lists ascend, so every wave needs what the waves before it chose (and how many equal the cut)
   uint64_t pick[E];
   int eq_before = 0, chosen = 0;
-  if (ties >= 0) {
+  if (ties > 0) {
     int eq = 0;
 #pragma unroll
     for (int i = 0; i < E; ++i) eq += __popcll(__ballot(key[i] == cut));
@@ -473,17 +649,19 @@ __global__ __launch_bounds__(kWaves * 64) void cache_list_kernel(const SelectPar
   }
 #pragma unroll
   for (int i = 0; i < E; ++i) {
-    bool take = (forced >> i) & 1;
-    if (ties < 0) {
-      take = take || key[i] >= cut;
-    } else {
+    bool take = ((forced >> i) & 1) || key[i] > cut;
+    if (ties > 0) {
       const uint64_t eq = __ballot(key[i] == cut);
-      take = take || key[i] > cut || (key[i] == cut && eq_before + lanes_below(eq) < ties);
+      take = take || (key[i] == cut && eq_before + lanes_below(eq) < ties);
       eq_before += __popcll(eq);
+    } else {
+      // with a whole bin the cut is the least key that the bin can hold
+      take = take || (key[i] == cut && base + i * 64 + lane <= cut_page);
     }
     pick[i] = __ballot(take);
     chosen += __popcll(pick[i]);
   }
+  __syncthreads();  // wave_total is read above
   if (lane == 0) wave_total[wave] = chosen;
   __syncthreads();
   int at = 0, all = 0;
@@ -491,15 +669,16 @@ __global__ __launch_bounds__(kWaves * 64) void cache_list_kernel(const SelectPar
     if (w < wave) at += wave_total[w];
     all += wave_total[w];
   }
+  const int width = static_cast<int>(p.width);
   int32_t *list = p.index + row * p.width;
 #pragma unroll
   for (int i = 0; i < E; ++i) {
     const int place = at + lanes_below(pick[i]);
-    if ((pick[i] >> lane & 1) && place < p.width) list[place] = static_cast<int32_t>(base + i * 64 + lane);
+    if ((pick[i] >> lane & 1) && place < width) list[place] = base + i * 64 + lane;
     at += __popcll(pick[i]);
   }
-  for (int64_t i = all + tid; i < p.width; i += kWaves * 64) list[i] = -1;
-  if (tid == 0) p.count[row] = all < p.width ? all : static_cast<int32_t>(p.width);
+  for (int i = all + tid; i < width; i += kThreads) list[i] = -1;
+  if (tid == 0) p.count[row] = all < width ? all : width;
 }
 
 template <typename T, int D>
@@ -617,7 +796,9 @@ extern "C" int vasc_cache_select(const void *q, int64_t q_sb, int64_t q_sh, int6
   p.lengths = lengths; p.n_q = q_count;
   p.block_q = static_cast<int>(block_q);
   p.causal = causal;
-  p.chunks = static_cast<int>(cdiv(max_pages, kScorePages));
+  const int64_t round = kScoreBatch * (256 / (D / 8)), all = B * H * p.U * cdiv(max_pages, round);
+  p.rounds = all <= 1024 ? 1 : all >= 8192 ? 8 : static_cast<int>(cdiv(all, 1024));
+  p.chunks = static_cast<int>(cdiv(max_pages, round * p.rounds));
   p.sink = sink; p.recent = recent; p.keep = keep; p.width = width;
   p.score = score; p.index = index; p.count = count;
   VASC_REQUIRE(B * H < (int64_t(1) << 31) / p.U && B * H * p.U < (int64_t(1) << 31) / p.chunks, "too many units");
@@ -634,6 +815,7 @@ extern "C" int vasc_cache_select(const void *q, int64_t q_sb, int64_t q_sh, int6
   if ((rc = check_launch("vasc_cache_select"))) return rc;
   if (max_pages <= 256) hipLaunchKernelGGL((cache_list_kernel<1, 4>), list, dim3(64), 0, s, p);
   else if (max_pages <= 2048) hipLaunchKernelGGL((cache_list_kernel<4, 8>), list, dim3(256), 0, s, p);
+  else if (max_pages <= 4096) hipLaunchKernelGGL((cache_list_kernel<8, 8>), list, dim3(512), 0, s, p);
   else if (max_pages <= 8192) hipLaunchKernelGGL((cache_list_kernel<16, 8>), list, dim3(1024), 0, s, p);
   else hipLaunchKernelGGL((cache_list_kernel<16, 32>), list, dim3(1024), 0, s, p);
   return check_launch("vasc_cache_select");

@@ -744,34 +744,44 @@ def _page_table(t, B: int, dev: int) -> tuple:
     return t, sb if B > 1 else mp, mp
 
 
-def _rotary_out(x: torch.Tensor) -> torch.Tensor:
-    """An output in the memory order of ``x``: [B,T,H,D] where x's heads lie inside its tokens."""
-    B, H, T, D = x.shape
-    if x.stride(1) < x.stride(2):
-        return torch.empty_strided((B, H, T, D), (T * H * D, D, H * D, 1), device=x.device, dtype=x.dtype)
-    return torch.empty(B, H, T, D, device=x.device, dtype=x.dtype)
+def _rotary_out(x: torch.Tensor, D: int) -> torch.Tensor:
+    """An output in the memory order of ``x`` (strides that fall as its do), D innermost."""
+    out = torch.empty_like(x)
+    return out if out.stride(3) == 1 or D == 1 else torch.empty(x.shape, device=x.device, dtype=x.dtype)
+
+
+_NO_K = (None, 0, 0, 0, None, 0, 0, 0, 0)
 
 
 def _rotary(q, k, pos, sections, inv_freq, inverse: bool) -> tuple:
-    if q.stride(3) != 1:
-        q = q.contiguous()
-    qo = _rotary_out(q)
-    kargs, ko, Hk = (None, 0, 0, 0, None, 0, 0, 0), None, 0
-    if k is not None:
-        if k.stride(3) != 1:
-            k = k.contiguous()
-        ko, Hk = _rotary_out(k), k.shape[1]
-        kargs = (k.data_ptr(), *k.stride()[:3], ko.data_ptr(), *ko.stride()[:3])
-    if q.numel() == 0 or (k is not None and k.numel() == 0):
-        if q.numel():
-            qo = _rotary(q, None, pos, sections, inv_freq, inverse)[0]
-        elif k is not None and k.numel():
-            ko = _rotary(k, None, pos, sections, inv_freq, inverse)[0]
-        return qo, ko
     B, Hq, T, D = q.shape
-    _launch(q.get_device(), "vasc_rotary_axes", q.data_ptr(), *q.stride()[:3], qo.data_ptr(), *qo.stride()[:3], Hq,
-            *kargs, Hk, B, T, D, pos.data_ptr(), pos.stride(0) if pos.shape[0] > 1 else 0, pos.stride(1), len(sections),
-            _section_sizes(sections, D), inv_freq.data_ptr(), _DTYPE[q.dtype], inverse)
+    qsb, qsh, qst, qsd = q.stride()
+    if qsd != 1:
+        q = q.contiguous()
+        qsb, qsh, qst, _ = q.stride()
+    qo = _rotary_out(q, D)
+    ko, kargs = None, _NO_K
+    if k is not None:
+        Hk = k.shape[1]
+        ksb, ksh, kst, ksd = k.stride()
+        if ksd != 1:
+            k = k.contiguous()
+            ksb, ksh, kst, _ = k.stride()
+        ko = _rotary_out(k, D)
+        if not Hk:
+            k = None
+        else:
+            osb, osh, ost, _ = ko.stride()
+            kargs = (k.data_ptr(), ksb, ksh, kst, ko.data_ptr(), osb, osh, ost, Hk)
+    if B == 0 or T == 0 or (Hq == 0 and k is None):
+        return qo, ko
+    if Hq == 0:
+        return qo, _rotary(k, None, pos, sections, inv_freq, inverse)[0]
+    osb, osh, ost, _ = qo.stride()
+    psb, pst, _ = pos.stride()
+    _launch(q.get_device(), "vasc_rotary_axes", q.data_ptr(), qsb, qsh, qst, qo.data_ptr(), osb, osh, ost, Hq, *kargs,
+            B, T, D, pos.data_ptr(), psb if pos.shape[0] > 1 else 0, pst, len(sections), _section_sizes(sections, D),
+            inv_freq.data_ptr(), _DTYPE[q.dtype], inverse)
     return qo, ko
 
 
@@ -816,13 +826,15 @@ def rotary_axes(q: torch.Tensor, k: torch.Tensor | None, pos: torch.Tensor, sect
     differentiable in q and k.
     """
     dev = _gpu(q, "q")
-    if q.dim() != 4 or q.dtype not in _DTYPE:
-        raise ValueError(f"q must be [B,H,T,D] in bf16, fp16 or fp32, got {q.dtype} {tuple(q.shape)}")
+    dtype = q.dtype
+    if q.dim() != 4 or dtype not in _DTYPE:
+        raise ValueError(f"q must be [B,H,T,D] in bf16, fp16 or fp32, got {dtype} {tuple(q.shape)}")
     B, _, T, D = q.shape
     if k is not None:
         _gpu(k, "k", dev)
-        if k.dim() != 4 or k.dtype != q.dtype or k.shape[0] != B or k.shape[2:] != q.shape[2:]:
-            raise ValueError(f"k must be [{B},H,{T},{D}] of {q.dtype}, got {k.dtype} {tuple(k.shape)}")
+        kshape = k.shape
+        if len(kshape) != 4 or k.dtype is not dtype or kshape[0] != B or kshape[2] != T or kshape[3] != D:
+            raise ValueError(f"k must be [{B},H,{T},{D}] of {dtype}, got {k.dtype} {tuple(kshape)}")
     sections = tuple(sections)
     _section_sizes(sections, D)
     _gpu(pos, "pos", dev)
