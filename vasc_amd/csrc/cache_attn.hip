@@ -77,6 +77,12 @@ __device__ __forceinline__ uint32_t pack_half2(float a, float b) {
   return __builtin_bit_cast(uint32_t, __builtin_convertvector(f, halfx2));
 }
 
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;  // three operands at once; a NaN gives way to a number, as with fmaxf
+  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+  return r;
+}
+
 // The four lanes l, l ^ 16, l ^ 32, l ^ 48 share a query row.
 __device__ __forceinline__ float row4_max(float v) {
   v = fmaxf(v, xor_lane(v, 16));
@@ -87,135 +93,302 @@ __device__ __forceinline__ float row4_sum(float v) {
   return v + xor_lane(v, 32);
 }
 
-// A workgroup of 4 waves: kRowWaves of them side by side over the rows, the others over the pages.
-// Each wave holds kTiles tiles of 16 rows.
-template <typename Q, int D, int kTiles, int kRowWaves>
-__global__ __launch_bounds__(256, 2) void cache_attn_kernel(const AttnParams p) {
-  constexpr int kPageWaves = 4 / kRowWaves;
-  constexpr int kDT = D / 16;  // feature tiles of the output
-  constexpr int kRows = kRowWaves * kTiles * 16;
+// What a workgroup works on: workgroup -> (sequence and key head, part, unit); the units of a part read the same pages.
+struct Work {
+  int64_t b, L, nq, t0, t1, unit_row;
+  int h, u, part, cut;
+  int entries;          // pages of the unit
+  int e0, e1;           // this part's of them
+  int seen;
+  const int32_t *list;  // or NULL: the pages in order
+};
+
+__device__ __forceinline__ Work work_of(const AttnParams &p) {
+  Work w;
+  int id = static_cast<int>(xcd_remap(blockIdx.x, gridDim.x));
+  w.u = id % p.U;
+  id /= p.U;
+  w.part = id % p.parts;
+  const int bh = id / p.parts;
+  w.b = bh / p.H;
+  w.h = bh - static_cast<int>(w.b) * p.H;
+  w.L = p.lengths[w.b];
+  w.nq = p.n_q ? p.n_q[w.b] : p.T;
+  w.nq = w.nq < 0 ? 0 : (w.nq < p.T ? w.nq : p.T);
+  w.t0 = static_cast<int64_t>(w.u) * p.block_q;
+  w.t1 = w.t0 + p.block_q < w.nq ? w.t0 + p.block_q : w.nq;
+  const UnitView view = unit_view(w.L, w.nq, w.t0, w.t1, p.max_pages, p.causal);
+  w.cut = static_cast<int>(clamp_tokens(w.L, p.max_pages));  // below 2^30
+  w.seen = static_cast<int>(view.seen);
+  w.unit_row = static_cast<int64_t>(bh) * p.U + w.u;
+  w.entries = w.seen;
+  w.list = nullptr;
+  if (p.index) {
+    w.list = p.index + w.unit_row * p.width;
+    const int64_t n = p.count[w.unit_row];
+    w.entries = w.seen == 0 ? 0 : static_cast<int>(n < 0 ? 0 : (n < p.width ? n : p.width));
+  }
+  const int share = (w.entries + p.parts - 1) / p.parts;
+  w.e0 = min(w.part * share, w.entries);
+  w.e1 = min(w.e0 + share, w.entries);
+  return w;
+}
+
+// Entry `at` of the unit: its logical page (-1: none) and physical page (0 where there is none: it is read, and not seen).
+__device__ __forceinline__ void resolve(const AttnParams &p, const Work &w, int at, int &page, int &pid) {
+  page = -1;
+  pid = 0;
+  if (at >= w.e1) return;
+  page = w.list ? w.list[at] : at;
+  if (w.list && at > 0 && w.list[at - 1] >= page) page = -1;
+  if (page >= w.seen) page = -1;
+  if (page < 0) {
+    page = -1;
+    return;
+  }
+  pid = p.table[w.b * p.table_stride + page];
+  if (pid < 0 || pid >= p.pages) {
+    pid = 0;
+    page = -1;
+  }
+}
+
+// One past the last key that unit row r sees; 0 for no row.
+__device__ __forceinline__ int row_limit(const AttnParams &p, const Work &w, int r, int64_t &t, int &gh) {
+  const int tl = r / p.G;
+  gh = r - tl * p.G;
+  t = w.t0 + tl;
+  if (r >= p.rows || t >= w.t1) return 0;
+  if (!p.causal) return w.cut;
+  const int64_t own = w.L - w.nq + t + 1;
+  return static_cast<int>(own < w.cut ? (own > 0 ? own : 0) : w.cut);
+}
+
+// This lane's query operands of a row: [part][product]; zeros where there is no row.
+template <typename Q, int D, int kOps>
+__device__ __forceinline__ void query_operands(const AttnParams &p, const Work &w, int64_t t, int gh, bool live, int g,
+                                               bf16x8 (&out)[kOps]) {
+  constexpr int kMul = D / 32, kParts = kOps / kMul;
+  const Q *src = static_cast<const Q *>(p.q) + w.b * p.qsb + (static_cast<int64_t>(w.h) * p.G + gh) * p.qsh + t * p.qst + g * 16;
+#pragma unroll
+  for (int y = 0; y < kMul; ++y) {
+    float x[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+    if (live) {
+      struct alignas(16) Eight { Q v[8]; };
+      const Eight v = *reinterpret_cast<const Eight *>(src + (y >> 1) * 64 + (y & 1) * 8);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[e] = to_f32(v.v[e]);
+    }
+#pragma unroll
+    for (int piece = 0; piece < kParts; ++piece)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        out[piece * kMul + y][e] = static_cast<__bf16>(x[e]);
+        if (kParts > 1 && __builtin_isfinite(x[e])) x[e] -= static_cast<float>(out[piece * kMul + y][e]);
+      }
+  }
+}
+
+// The running softmax of a wave's row tiles.
+constexpr float kUnset = -3.0e38f;
+template <int kTiles, int kDT>
+struct Rows {
+  floatx4 acc[kTiles][kDT];
+  // ref: the exponent's reference; start: -ref / c; renew: the exponent that renews it (any, before the first key)
+  float ref[kTiles], start[kTiles], renew[kTiles], l[kTiles];
+  int limit[kTiles];
+  int low, high;  // keys below `low` are seen by every row of the wave that counts, from `high` on by none
+
+  __device__ __forceinline__ void init() {
+#pragma unroll
+    for (int i = 0; i < kTiles; ++i) {
+      ref[i] = start[i] = l[i] = 0.f;
+      renew[i] = kUnset;
+#pragma unroll
+      for (int d = 0; d < kDT; ++d) acc[i][d] = floatx4{0, 0, 0, 0};
+    }
+  }
+
+  // After limit[]: low and high over the wave.
+  __device__ __forceinline__ void bounds(int cut) {
+    low = cut;
+    high = 0;
+#pragma unroll
+    for (int i = 0; i < kTiles; ++i) {
+      if (limit[i] > 0 && limit[i] < low) low = limit[i];
+      high = max(high, limit[i]);
+    }
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) {
+      low = min(low, __shfl_xor(low, off));
+      high = max(high, __shfl_xor(high, off));
+    }
+    low = __builtin_amdgcn_readfirstlane(low);
+    high = __builtin_amdgcn_readfirstlane(high);
+  }
+
+  // Exponents of a page's keys (key t * 16 + g * 4 + j in s[x][t][j]) -> weights as the second product's operands;
+  // un(t): the opposite powers of the values of keys t * 16 + g * 4 ...
+  template <typename Un>
+  __device__ __forceinline__ void weights(floatx4 (&s)[kTiles][4], int page, int g, float inv_c, Un un,
+                                          halfx8 (&w)[kTiles][2]) {
+    if (page < 0 || page * kPage + kPage > low) {
+#pragma unroll
+      for (int x = 0; x < kTiles; ++x) {
+        const int lim = (page < 0 ? 0 : limit[x] - page * kPage) - g * 4;
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            if (t * 16 + j >= lim) s[x][t][j] = -__builtin_inff();
+      }
+    }
+    bool renewing = false;
+    float top[kTiles];
+#pragma unroll
+    for (int x = 0; x < kTiles; ++x) {
+      float a = max3(s[x][0][0], s[x][0][1], s[x][0][2]);
+#pragma unroll
+      for (int j = 3; j < 15; j += 2) a = max3(a, s[x][j >> 2][j & 3], s[x][(j + 1) >> 2][(j + 1) & 3]);
+      top[x] = row4_max(fmaxf(a, s[x][3][3]));
+      renewing = renewing || top[x] > renew[x];
+    }
+    if (__ballot(renewing)) {
+#pragma unroll
+      for (int x = 0; x < kTiles; ++x) {
+        const bool need = top[x] > renew[x];
+        const float by = need ? top[x] - kHeadroom : 0.f;
+        const float a = need && renew[x] != kUnset ? __builtin_amdgcn_exp2f(-by) : 1.f;
+        l[x] *= a;
+#pragma unroll
+        for (int d = 0; d < kDT; ++d) acc[x][d] *= a;
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) s[x][t][j] -= by;
+        ref[x] += by;
+        start[x] = -ref[x] * inv_c;
+        if (need) renew[x] = kHeadroom + kSlack;
+      }
+    }
+    uint32_t packed[kTiles][8];
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+      const floatx4 power = un(t);
+#pragma unroll
+      for (int x = 0; x < kTiles; ++x) {
+        float e[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          e[j] = __builtin_amdgcn_exp2f(s[x][t][j]);
+          l[x] = fmaf(e[j], power[j], l[x]);
+        }
+        packed[x][t * 2] = pack_half2(e[0], e[1]);
+        packed[x][t * 2 + 1] = pack_half2(e[2], e[3]);
+      }
+    }
+#pragma unroll
+    for (int x = 0; x < kTiles; ++x) {
+      w[x][0] = __builtin_bit_cast(halfx8, u32x4{packed[x][0], packed[x][1], packed[x][2], packed[x][3]});
+      w[x][1] = __builtin_bit_cast(halfx8, u32x4{packed[x][4], packed[x][5], packed[x][6], packed[x][7]});
+    }
+  }
+
+  // The lanes' sums joined; m: the reference, -inf for a row without a key.
+  __device__ __forceinline__ void finish(float (&m)[kTiles]) {
+#pragma unroll
+    for (int i = 0; i < kTiles; ++i) {
+      l[i] = row4_sum(l[i]);
+      m[i] = renew[i] == kUnset ? -__builtin_inff() : ref[i];
+      if (limit[i] == 0) {  // no key, or no row: pages that all counting rows see were not masked for it
+        m[i] = -__builtin_inff();
+        l[i] = 0.f;
+#pragma unroll
+        for (int d = 0; d < kDT; ++d) acc[i][d] = floatx4{0, 0, 0, 0};
+      }
+    }
+  }
+
+  // Results of unit rows first + 16 i + col, or this part's share of them.
+  template <typename Q>
+  __device__ __forceinline__ void store(const AttnParams &p, const Work &w, int first, int col, int g, const float (&m)[kTiles]) {
+    constexpr int D = kDT * 16;
+#pragma unroll
+    for (int i = 0; i < kTiles; ++i) {
+      const int r = first + i * 16 + col;
+      if (r >= p.rows) continue;
+      const int tl = r / p.G, gh = r - tl * p.G;
+      const int64_t t = w.t0 + tl;
+      if (t >= p.T) continue;
+      if (p.parts == 1) {
+        const float inv = l[i] == 0.f ? 0.f : 1.f / l[i];
+        Q *dst = static_cast<Q *>(p.o) + w.b * p.osb + (static_cast<int64_t>(w.h) * p.G + gh) * p.osh + t * p.ost + g * 4;
+#pragma unroll
+        for (int d = 0; d < kDT; ++d) {
+          struct alignas(8) Four { Q v[4]; } out;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) out.v[j] = from_f32<Q>(acc[i][d][j] * inv);
+          *reinterpret_cast<Four *>(dst + d * 16) = out;
+        }
+      } else {
+        // [unit row][part][D], behind them (m, l) alike
+        const int64_t at = (w.unit_row * p.rows + r) * p.parts + w.part;
+        float *dst = p.ws + at * D + g * 4;
+#pragma unroll
+        for (int d = 0; d < kDT; ++d) *reinterpret_cast<floatx4 *>(dst + d * 16) = acc[i][d];
+        if (g == 0) {
+          float *ml = p.ws + static_cast<int64_t>(p.B) * p.H * p.U * p.rows * p.parts * D + at * 2;
+          ml[0] = m[i];
+          ml[1] = l[i];
+        }
+      }
+    }
+  }
+};
+
+// Few rows (up to 32): the cache's bytes bound the kernel. Each of the 4 waves holds all of the unit's rows, kTiles tiles of
+// 16, and takes every fourth page straight from memory to its registers; their sums are joined in LDS.
+template <typename Q, int D, int kTiles>
+__global__ __launch_bounds__(256, 2) void cache_attn_few_kernel(const AttnParams p) {
+  constexpr int kWaves = 4, kDT = D / 16, kRows = kTiles * 16;
   constexpr int kK = D / 64;   // 16-byte loads of a key per lane, two products each
   constexpr int kParts = __is_same(Q, __bf16) ? 1 : 2;
-  // the query operands, 16 bytes a lane: [row tile][part][product]; after the pages, the page waves' sums
+  // the query operands, 16 bytes a lane: [row tile][part][product]; after the pages, the other waves' sums
   constexpr int kOps = kParts * kK * 2;
   typedef float Sums[kRows][D + 2];
-  constexpr size_t kQBytes = kRowWaves * kTiles * kOps * 1024, kSBytes = (kPageWaves - 1) * sizeof(Sums);
+  constexpr size_t kQBytes = kTiles * kOps * 1024, kSBytes = (kWaves - 1) * sizeof(Sums);
   __shared__ __align__(16) uint8_t shared[kQBytes > kSBytes ? kQBytes : kSBytes];
   bf16x8 *query = reinterpret_cast<bf16x8 *>(shared);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int col = lane & 15, g = lane >> 4;
-  const int rw = wave % kRowWaves, pw = wave / kRowWaves;
-  // workgroup -> (sequence and key head, part, unit): the units of a part read the same pages
-  int id = static_cast<int>(xcd_remap(blockIdx.x, gridDim.x));
-  const int u = id % p.U;
-  id /= p.U;
-  const int part = id % p.parts;
-  const int bh = id / p.parts;
-  const int64_t b = bh / p.H;
-  const int h = bh - static_cast<int>(b) * p.H;
-  const int64_t L = p.lengths[b];
-  int64_t nq = p.n_q ? p.n_q[b] : p.T;
-  nq = nq < 0 ? 0 : (nq < p.T ? nq : p.T);
-  const int64_t t0 = static_cast<int64_t>(u) * p.block_q;
-  const int64_t t1 = t0 + p.block_q < nq ? t0 + p.block_q : nq;
-  const UnitView view = unit_view(L, nq, t0, t1, p.max_pages, p.causal);
-  const int64_t cut = clamp_tokens(L, p.max_pages);
+  const Work w = work_of(p);
 
-  // the rows of this wave's tiles: one past the last key that the row sees, and the query operands
-  int limit[kTiles];
-  int low = static_cast<int>(cut), high = 0;  // keys below `low` are seen by every row of the wave that counts, from `high` on by none
+  Rows<kTiles, kDT> rows;
 #pragma unroll
   for (int i = 0; i < kTiles; ++i) {
-    const int r = (rw * kTiles + i) * 16 + col;
-    const int tl = r / p.G, gh = r - tl * p.G;
-    const int64_t t = t0 + tl;
-    const bool live = r < p.rows && t < t1;
-    limit[i] = live ? static_cast<int>(cut) : 0;  // below 2^30
-    if (live && p.causal) {
-      const int64_t own = L - nq + t + 1;
-      limit[i] = static_cast<int>(own < cut ? (own > 0 ? own : 0) : cut);
-    }
-    if (live && limit[i] < low) low = limit[i];
-    if (limit[i] > high) high = limit[i];
-    if (pw > 0) continue;  // the page waves share the operands
-    const Q *src = static_cast<const Q *>(p.q) + b * p.qsb + (static_cast<int64_t>(h) * p.G + gh) * p.qsh + t * p.qst + g * 16;
+    int64_t t;
+    int gh;
+    rows.limit[i] = row_limit(p, w, i * 16 + col, t, gh);
+    if (wave == 0) {
+      bf16x8 ops[kOps];
+      query_operands<Q, D>(p, w, t, gh, rows.limit[i] > 0, g, ops);
 #pragma unroll
-    for (int y = 0; y < kK * 2; ++y) {
-      float x[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-      if (limit[i] > 0) {
-        struct alignas(16) Eight { Q v[8]; };
-        const Eight v = *reinterpret_cast<const Eight *>(src + (y >> 1) * 64 + (y & 1) * 8);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = to_f32(v.v[e]);
-      }
-#pragma unroll
-      for (int piece = 0; piece < kParts; ++piece) {
-        bf16x8 w;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          w[e] = static_cast<__bf16>(x[e]);
-          if (kParts > 1 && __builtin_isfinite(x[e])) x[e] -= static_cast<float>(w[e]);
-        }
-        query[((rw * kTiles + i) * kOps + piece * kK * 2 + y) * 64 + lane] = w;
-      }
+      for (int o = 0; o < kOps; ++o) query[(i * kOps + o) * 64 + lane] = ops[o];
     }
   }
-#pragma unroll
-  for (int off = 1; off < 64; off <<= 1) {
-    low = min(low, __shfl_xor(low, off));
-    high = max(high, __shfl_xor(high, off));
-  }
-  low = __builtin_amdgcn_readfirstlane(low);
-  high = __builtin_amdgcn_readfirstlane(high);
+  rows.bounds(w.cut);
+  rows.init();
   __syncthreads();
 
-  floatx4 acc[kTiles][kDT];
-  // ref: the exponent's reference; start: -ref / c; renew: the exponent that renews it (any, before the first key)
-  float ref[kTiles], start[kTiles], renew[kTiles], l[kTiles];
-  constexpr float kUnset = -3.0e38f;
   const float inv_c = 1.f / p.c;
-#pragma unroll
-  for (int i = 0; i < kTiles; ++i) {
-    ref[i] = start[i] = l[i] = 0.f;
-    renew[i] = kUnset;
-#pragma unroll
-    for (int d = 0; d < kDT; ++d) acc[i][d] = floatx4{0, 0, 0, 0};
-  }
-
-  // this part's entries of the list (or of the pages in order)
-  const int64_t unit_row = static_cast<int64_t>(bh) * p.U + u;
-  int64_t entries = view.seen;
-  const int32_t *list = nullptr;
-  if (p.index) {
-    list = p.index + unit_row * p.width;
-    const int64_t n = p.count[unit_row];
-    entries = view.seen == 0 ? 0 : (n < 0 ? 0 : (n < p.width ? n : p.width));
-  }
-  const int64_t share = cdiv(entries, p.parts);
-  const int64_t e0 = part * share;
-  const int64_t e1 = high == 0 ? e0 : (e0 + share < entries ? e0 + share : entries);
-
-  const uint8_t *kbase = p.kc + static_cast<int64_t>(h) * (kPage * D) + col * D + g * 16;
-  const uint8_t *vbase = p.vc + static_cast<int64_t>(h) * (kPage * D) + col * kPage + g * 16;
-  const uint8_t *ksbase = p.ks + static_cast<int64_t>(h) * kPage + col * 4;
-  const uint8_t *vsbase = p.vs + static_cast<int64_t>(h) * kPage + g * 16;
-  for (int64_t base = e0; base < e1; base += 64) {
-    // lane i resolves entry base + i: logical and physical page; a place without a page reads page 0 and sees none of it
-    const int64_t mine = base + lane;
-    int page = -1, pid = 0;
-    if (mine < e1) {
-      page = list ? list[mine] : static_cast<int>(mine);
-      if (list && mine > 0 && list[mine - 1] >= page) page = -1;
-      if (page >= view.seen) page = -1;
-      if (page >= 0) {
-        pid = p.table[b * p.table_stride + page];
-        if (pid < 0 || pid >= p.pages) {
-          pid = 0;
-          page = -1;
-        }
-      }
-    }
-    const int n = static_cast<int>(e1 - base < 64 ? e1 - base : 64);
+  const uint8_t *kbase = p.kc + static_cast<int64_t>(w.h) * (kPage * D) + col * D + g * 16;
+  const uint8_t *vbase = p.vc + static_cast<int64_t>(w.h) * (kPage * D) + col * kPage + g * 16;
+  const uint8_t *ksbase = p.ks + static_cast<int64_t>(w.h) * kPage + col * 4;
+  const uint8_t *vsbase = p.vs + static_cast<int64_t>(w.h) * kPage + g * 16;
+  for (int base = w.e0; base < w.e1; base += 64) {
+    int page, pid;  // lane i has those of entry base + i
+    resolve(p, w, base + lane, page, pid);
+    const int n = min(w.e1 - base, 64);
     u32x4 kr[4][kK];
     uint32_t kb = 0;
     auto load_keys = [&](int i) {
@@ -227,8 +400,8 @@ __global__ __launch_bounds__(256, 2) void cache_attn_kernel(const AttnParams p) 
           kr[t][y] = *reinterpret_cast<const u32x4 *>(kbase + at * (kPage * D) + t * 16 * D + y * 64);
       kb = *reinterpret_cast<const uint32_t *>(ksbase + at * kPage);
     };
-    if (pw < n) load_keys(pw);
-    for (int i = pw; i < n; i += kPageWaves) {
+    if (wave < n) load_keys(wave);
+    for (int i = wave; i < n; i += kWaves) {
       const int lpage = __builtin_amdgcn_readlane(page, i);
       const int64_t at = static_cast<int64_t>(__builtin_amdgcn_readlane(pid, i)) * p.H;
       // the query operands are read again for every page: held over the loop they would cost 8 to 64 registers
@@ -245,23 +418,22 @@ __global__ __launch_bounds__(256, 2) void cache_attn_kernel(const AttnParams p) 
         const float power = pow2_byte((kb >> (8 * t)) & 255u);
 #pragma unroll
         for (int y = 0; y < kK * 2; ++y) {
-          const u32x4 w = kr[t][y >> 1];
-          const bf16x8 a = y & 1 ? widen_scaled(w[2], w[3], power) : widen_scaled(w[0], w[1], power);
+          const u32x4 k = kr[t][y >> 1];
+          const bf16x8 a = y & 1 ? widen_scaled(k[2], k[3], power) : widen_scaled(k[0], k[1], power);
 #pragma unroll
           for (int x = 0; x < kTiles; ++x)
 #pragma unroll
             for (int piece = 0; piece < kParts; ++piece) {
-              const bf16x8 q = query[((rw * kTiles + x) * kOps + piece * kK * 2 + y) * 64 + lane];
-              const floatx4 c = y == 0 && piece == 0 ? floatx4{start[x], start[x], start[x], start[x]} : s[x][t];
+              const bf16x8 q = query[(x * kOps + piece * kK * 2 + y) * 64 + lane];
+              const float start = rows.start[x];
+              const floatx4 c = y == 0 && piece == 0 ? floatx4{start, start, start, start} : s[x][t];
               s[x][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, q, c, 0, 0, 0);
             }
         }
       }
       // the next page's keys arrive while this one's weights are made
-      if (i + kPageWaves < n) load_keys(i + kPageWaves);
+      if (i + kWaves < n) load_keys(i + kWaves);
 
-      const int key0 = lpage * kPage;
-      const bool masked = lpage < 0 || key0 + kPage > low;
       // exponents, in place: the byte's bias of 127 goes with the reference
 #pragma unroll
       for (int t = 0; t < 4; ++t) {
@@ -273,168 +445,195 @@ __global__ __launch_bounds__(256, 2) void cache_attn_kernel(const AttnParams p) 
           for (int x = 0; x < kTiles; ++x) s[x][t][j] = fmaf(s[x][t][j], p.c, ev);
         }
       }
-      if (masked) {
-#pragma unroll
-        for (int x = 0; x < kTiles; ++x) {
-          const int lim = (lpage < 0 ? 0 : limit[x] - key0) - g * 4;
-#pragma unroll
-          for (int t = 0; t < 4; ++t)
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-              if (t * 16 + j >= lim) s[x][t][j] = -__builtin_inff();
-        }
-      }
-      bool renewing = false;
-      float top[kTiles];
-#pragma unroll
-      for (int x = 0; x < kTiles; ++x) {
-        float a = fmaxf(s[x][0][0], s[x][0][1]);
-#pragma unroll
-        for (int j = 2; j < 16; j += 2) a = fmaxf(fmaxf(a, s[x][j >> 2][j & 3]), s[x][j >> 2][(j & 3) + 1]);
-        top[x] = row4_max(a);
-        renewing = renewing || top[x] > renew[x];
-      }
-      if (__ballot(renewing)) {
-#pragma unroll
-        for (int x = 0; x < kTiles; ++x) {
-          const bool need = top[x] > renew[x];
-          const float by = need ? top[x] - kHeadroom : 0.f;
-          const float a = need && renew[x] != kUnset ? __builtin_amdgcn_exp2f(-by) : 1.f;
-          l[x] *= a;
-#pragma unroll
-          for (int d = 0; d < kDT; ++d) acc[x][d] *= a;
-#pragma unroll
-          for (int t = 0; t < 4; ++t)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) s[x][t][j] -= by;
-          ref[x] += by;
-          start[x] = -ref[x] * inv_c;
-          if (need) renew[x] = kHeadroom + kSlack;
-        }
-      }
-      uint32_t packed[kTiles][8];
-#pragma unroll
-      for (int t = 0; t < 4; ++t) {
+      halfx8 wt[kTiles][2];
+      rows.weights(s, lpage, g, inv_c, [&](int t) {
         const uint32_t iw = 0xfefefefeu - vb[t];  // the opposite powers
-        float un[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) un[j] = pow2_byte((iw >> (8 * j)) & 255u);
-#pragma unroll
-        for (int x = 0; x < kTiles; ++x) {
-          float w[4];
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            w[j] = __builtin_amdgcn_exp2f(s[x][t][j]);
-            l[x] = fmaf(w[j], un[j], l[x]);
-          }
-          packed[x][t * 2] = pack_half2(w[0], w[1]);
-          packed[x][t * 2 + 1] = pack_half2(w[2], w[3]);
-        }
-      }
-      halfx8 w[kTiles][2];
-#pragma unroll
-      for (int x = 0; x < kTiles; ++x) {
-        w[x][0] = __builtin_bit_cast(halfx8, u32x4{packed[x][0], packed[x][1], packed[x][2], packed[x][3]});
-        w[x][1] = __builtin_bit_cast(halfx8, u32x4{packed[x][4], packed[x][5], packed[x][6], packed[x][7]});
-      }
+        return floatx4{pow2_byte(iw & 255u), pow2_byte((iw >> 8) & 255u), pow2_byte((iw >> 16) & 255u), pow2_byte(iw >> 24)};
+      }, wt);
 #pragma unroll
       for (int d = 0; d < kDT; ++d) {
         const u32x4 v = vr[d];
         const halfx8 a0 = widen(v[0], v[1]), a1 = widen(v[2], v[3]);
 #pragma unroll
         for (int x = 0; x < kTiles; ++x) {
-          acc[x][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a0, w[x][0], acc[x][d], 0, 0, 0);
-          acc[x][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a1, w[x][1], acc[x][d], 0, 0, 0);
+          rows.acc[x][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a0, wt[x][0], rows.acc[x][d], 0, 0, 0);
+          rows.acc[x][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a1, wt[x][1], rows.acc[x][d], 0, 0, 0);
         }
       }
     }
   }
   float m[kTiles];
-#pragma unroll
-  for (int i = 0; i < kTiles; ++i) {
-    l[i] = row4_sum(l[i]);
-    m[i] = renew[i] == kUnset ? -__builtin_inff() : ref[i];
-    if (limit[i] == 0) {  // no key, or no row: pages that all counting rows see were not masked for it
-      m[i] = -__builtin_inff();
-      l[i] = 0.f;
-#pragma unroll
-      for (int d = 0; d < kDT; ++d) acc[i][d] = floatx4{0, 0, 0, 0};
-    }
-  }
+  rows.finish(m);
 
-  // the page waves' parts, joined in LDS by the first of them
-  if constexpr (kPageWaves > 1) {
-    Sums *lo = reinterpret_cast<Sums *>(shared);  // of page waves 1..
-    __syncthreads();  // the query operands have been read
-    if (pw > 0) {
-#pragma unroll
-      for (int i = 0; i < kTiles; ++i) {
-        float *dst = lo[pw - 1][(rw * kTiles + i) * 16 + col];
-        if (g == 0) {
-          dst[D] = m[i];
-          dst[D + 1] = l[i];
-        }
-#pragma unroll
-        for (int d = 0; d < kDT; ++d)
-#pragma unroll
-          for (int j = 0; j < 4; ++j) dst[d * 16 + g * 4 + j] = acc[i][d][j];
-      }
-    }
-    __syncthreads();
-    if (pw > 0) return;
+  // the other waves' sums, joined by the first
+  Sums *others = reinterpret_cast<Sums *>(shared);
+  __syncthreads();  // the query operands have been read
+  if (wave > 0) {
 #pragma unroll
     for (int i = 0; i < kTiles; ++i) {
-      float mx = m[i];
-#pragma unroll
-      for (int x = 1; x < kPageWaves; ++x) mx = fmaxf(mx, lo[x - 1][(rw * kTiles + i) * 16 + col][D]);
-      const float a = m[i] == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(m[i] - mx);
-      l[i] *= a;
-#pragma unroll
-      for (int d = 0; d < kDT; ++d) acc[i][d] *= a;
-#pragma unroll
-      for (int x = 1; x < kPageWaves; ++x) {
-        const float *src = lo[x - 1][(rw * kTiles + i) * 16 + col];
-        const float mo = src[D];
-        const float c = mo == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(mo - mx);
-        l[i] = fmaf(src[D + 1], c, l[i]);
-#pragma unroll
-        for (int d = 0; d < kDT; ++d)
-#pragma unroll
-          for (int j = 0; j < 4; ++j) acc[i][d][j] = fmaf(src[d * 16 + g * 4 + j], c, acc[i][d][j]);
+      float *dst = others[wave - 1][i * 16 + col];
+      if (g == 0) {
+        dst[D] = m[i];
+        dst[D + 1] = rows.l[i];
       }
-      m[i] = mx;
+#pragma unroll
+      for (int d = 0; d < kDT; ++d)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) dst[d * 16 + g * 4 + j] = rows.acc[i][d][j];
     }
   }
+  __syncthreads();
+  if (wave > 0) return;
 #pragma unroll
   for (int i = 0; i < kTiles; ++i) {
-    const int r = (rw * kTiles + i) * 16 + col;
-    if (r >= p.rows) continue;
-    const int tl = r / p.G, gh = r - tl * p.G;
-    const int64_t t = t0 + tl;
-    if (t >= p.T) continue;
-    if (p.parts == 1) {
-      const float inv = l[i] == 0.f ? 0.f : 1.f / l[i];
-      Q *dst = static_cast<Q *>(p.o) + b * p.osb + (static_cast<int64_t>(h) * p.G + gh) * p.osh + t * p.ost + g * 4;
+    float mx = m[i];
+#pragma unroll
+    for (int x = 1; x < kWaves; ++x) mx = fmaxf(mx, others[x - 1][i * 16 + col][D]);
+    const float a = m[i] == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(m[i] - mx);
+    rows.l[i] *= a;
+#pragma unroll
+    for (int d = 0; d < kDT; ++d) rows.acc[i][d] *= a;
+#pragma unroll
+    for (int x = 1; x < kWaves; ++x) {
+      const float *src = others[x - 1][i * 16 + col];
+      const float mo = src[D];
+      const float c = mo == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(mo - mx);
+      rows.l[i] = fmaf(src[D + 1], c, rows.l[i]);
+#pragma unroll
+      for (int d = 0; d < kDT; ++d)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) rows.acc[i][d][j] = fmaf(src[d * 16 + g * 4 + j], c, rows.acc[i][d][j]);
+    }
+    m[i] = mx;
+  }
+  rows.template store<Q>(p, w, 0, col, g, m);
+}
+
+// Many rows (up to 128): the vector and matrix pipes bound the kernel. The kWaves waves lie side by side over the rows, and
+// a page is widened once for all of them: each wave turns its share of the codes into operands in LDS (keys as bfloat16 with
+// their powers, values as half, and the values' exponents as floats), 16 bytes a lane in the order in which they are read.
+// Two buffers and one barrier a page: the next page's codes are on their way to registers while this one is computed.
+template <typename Q, int D, int kTiles, int kWaves>
+__global__ __launch_bounds__(kWaves * 64, D == 64 && kWaves == 4 ? 3 : 2) void cache_attn_many_kernel(const AttnParams p) {
+  constexpr int kDT = D / 16, kK = D / 64, kMul = kK * 2;
+  constexpr int kParts = __is_same(Q, __bf16) ? 1 : 2;
+  constexpr int kOps = kParts * kMul;
+  constexpr int kKeyTasks = 4 * kK, kTasks = (kKeyTasks + kDT) / kWaves;  // 1 KB of codes each: a key tile's half, a feature tile
+  struct Page {
+    bf16x8 k[4 * kMul][64];
+    halfx8 v[kDT * 2][64];
+    float ev[kPage], un[kPage];
+  };
+  __shared__ __align__(16) Page buffer[2];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int col = lane & 15, g = lane >> 4;
+  const Work w = work_of(p);
+  const int first = wave * kTiles * 16;
+
+  Rows<kTiles, kDT> rows;
+  bf16x8 query[kTiles][kOps];
+#pragma unroll
+  for (int i = 0; i < kTiles; ++i) {
+    int64_t t;
+    int gh;
+    rows.limit[i] = row_limit(p, w, first + i * 16 + col, t, gh);
+    query_operands<Q, D>(p, w, t, gh, rows.limit[i] > 0, g, query[i]);
+  }
+  rows.bounds(w.cut);
+  rows.init();
+
+  const float inv_c = 1.f / p.c;
+  const int64_t head = static_cast<int64_t>(w.h) * (kPage * D);
+  u32x4 raw[kTasks];
+  uint32_t kb[kTasks], vb = 0;
+  int turn = 0;
+  for (int base = w.e0; base < w.e1; base += 64) {
+    int page, pid;  // lane i has those of entry base + i
+    resolve(p, w, base + lane, page, pid);
+    const int n = min(w.e1 - base, 64);
+    auto load = [&](int i) {
+      const int64_t at = static_cast<int64_t>(__builtin_amdgcn_readlane(pid, i)) * p.H;
+#pragma unroll
+      for (int k = 0; k < kTasks; ++k) {
+        const int task = wave + k * kWaves;
+        if (task < kKeyTasks) {
+          const int t = task / kK, y = task % kK;
+          raw[k] = *reinterpret_cast<const u32x4 *>(p.kc + at * (kPage * D) + head + (t * 16 + col) * D + y * 64 + g * 16);
+          kb[k] = p.ks[(at + w.h) * kPage + col * 4 + t];
+        } else {
+          const int d = task - kKeyTasks;
+          raw[k] = *reinterpret_cast<const u32x4 *>(p.vc + at * (kPage * D) + head + (d * 16 + col) * kPage + g * 16);
+        }
+      }
+      if (wave == 0) vb = p.vs[(at + w.h) * kPage + lane];
+    };
+    load(0);
+    for (int i = 0; i < n; ++i) {
+      Page &buf = buffer[turn];
+      turn ^= 1;
+#pragma unroll
+      for (int k = 0; k < kTasks; ++k) {
+        const int task = wave + k * kWaves;
+        const u32x4 x = raw[k];
+        if (task < kKeyTasks) {
+          const float power = pow2_byte(kb[k]);
+          buf.k[task * 2][lane] = widen_scaled(x[0], x[1], power);
+          buf.k[task * 2 + 1][lane] = widen_scaled(x[2], x[3], power);
+        } else {
+          const int d = task - kKeyTasks;
+          buf.v[d * 2][lane] = widen(x[0], x[1]);
+          buf.v[d * 2 + 1][lane] = widen(x[2], x[3]);
+        }
+      }
+      if (wave == 0) {
+        buf.ev[lane] = static_cast<float>(vb);  // the bias of 127 goes with the reference
+        buf.un[lane] = pow2_byte(254u - vb);
+      }
+      __syncthreads();
+      if (i + 1 < n) load(i + 1);
+      if (rows.high == 0) continue;
+      const int lpage = __builtin_amdgcn_readlane(page, i);
+
+      floatx4 s[kTiles][4];
+#pragma unroll
+      for (int t = 0; t < 4; ++t)
+#pragma unroll
+        for (int y = 0; y < kMul; ++y) {
+          const bf16x8 a = buf.k[t * kMul + y][lane];
+#pragma unroll
+          for (int x = 0; x < kTiles; ++x)
+#pragma unroll
+            for (int piece = 0; piece < kParts; ++piece) {
+              const float start = rows.start[x];
+              const floatx4 c = y == 0 && piece == 0 ? floatx4{start, start, start, start} : s[x][t];
+              s[x][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, query[x][piece * kMul + y], c, 0, 0, 0);
+            }
+        }
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        const floatx4 ev = *reinterpret_cast<const floatx4 *>(buf.ev + g * 16 + t * 4);
+#pragma unroll
+        for (int x = 0; x < kTiles; ++x)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) s[x][t][j] = fmaf(s[x][t][j], p.c, ev[j]);
+      }
+      halfx8 wt[kTiles][2];
+      rows.weights(s, lpage, g, inv_c,
+                   [&](int t) { return *reinterpret_cast<const floatx4 *>(buf.un + g * 16 + t * 4); }, wt);
 #pragma unroll
       for (int d = 0; d < kDT; ++d) {
-        struct alignas(8) Four { Q v[4]; } out;
+        const halfx8 a0 = buf.v[d * 2][lane], a1 = buf.v[d * 2 + 1][lane];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) out.v[j] = from_f32<Q>(acc[i][d][j] * inv);
-        *reinterpret_cast<Four *>(dst + d * 16) = out;
-      }
-    } else {
-      // [unit row][part][D], behind them (m, l) alike
-      const int64_t at = (unit_row * p.rows + r) * p.parts + part;
-      float *dst = p.ws + at * D + g * 4;
-#pragma unroll
-      for (int d = 0; d < kDT; ++d) *reinterpret_cast<floatx4 *>(dst + d * 16) = acc[i][d];
-      if (g == 0) {
-        float *ml = p.ws + static_cast<int64_t>(p.B) * p.H * p.U * p.rows * p.parts * D + at * 2;
-        ml[0] = m[i];
-        ml[1] = l[i];
+        for (int x = 0; x < kTiles; ++x) {
+          rows.acc[x][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a0, wt[x][0], rows.acc[x][d], 0, 0, 0);
+          rows.acc[x][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a1, wt[x][1], rows.acc[x][d], 0, 0, 0);
+        }
       }
     }
   }
+  float m[kTiles];
+  rows.finish(m);
+  rows.template store<Q>(p, w, first, col, g, m);
 }
 
 // Joins the parts of each row: 16 or 32 lanes a row, four features each.
@@ -482,9 +681,9 @@ struct Shape {
 Shape attn_shape(int64_t units, int64_t rows, int64_t pages, int64_t D) {
   Shape s;
   s.kind = rows <= 16 ? 0 : rows <= 32 ? 1 : rows <= 64 ? 2 : 3;
-  const int64_t resident = 256 * (D == 128 || s.kind > 1 ? 2 : s.kind == 0 ? 4 : 3);
-  const int64_t waves = s.kind < 2 ? 4 : (s.kind == 2 ? 2 : 1) * (D == 64 ? 2 : 1);  // that share a workgroup's pages
-  const double page_us = s.kind < 2 ? 0.3 : 4.0, start_us = s.kind < 2 ? 3.0 : 4.0, join_us = s.kind < 2 ? 5.0 : 8.0;
+  const int64_t resident = 256 * (D == 128 ? 2 : s.kind == 0 ? 4 : 3);
+  const int64_t waves = s.kind < 2 ? 4 : 1;  // that share a workgroup's pages
+  const double page_us = s.kind < 2 ? 0.3 : 2.0, start_us = s.kind < 2 ? 3.0 : 4.0, join_us = s.kind < 2 ? 5.0 : 8.0;
   double best = 0;
   s.parts = 0;
   for (int64_t rounds = 0; rounds <= 4; ++rounds) {
@@ -505,13 +704,13 @@ Shape attn_shape(int64_t units, int64_t rows, int64_t pages, int64_t D) {
 template <typename Q, int D>
 int launch_attn(const AttnParams &p, const Shape &s, hipStream_t st) {
   const dim3 grid(static_cast<unsigned>(p.B * p.H * p.U * s.parts));
-  // D = 128 has no registers for 64 rows a wave
-  constexpr int kWide = D == 64 ? 4 : 2;
+  // float16 queries of 128 features are two operands: 16 rows a wave
+  constexpr int kWaves = D == 128 && !__is_same(Q, __bf16) ? 8 : 4;
   switch (s.kind) {
-    case 0: hipLaunchKernelGGL((cache_attn_kernel<Q, D, 1, 1>), grid, dim3(256), 0, st, p); break;
-    case 1: hipLaunchKernelGGL((cache_attn_kernel<Q, D, 2, 1>), grid, dim3(256), 0, st, p); break;
-    case 2: hipLaunchKernelGGL((cache_attn_kernel<Q, D, kWide, 4 / kWide>), grid, dim3(256), 0, st, p); break;
-    default: hipLaunchKernelGGL((cache_attn_kernel<Q, D, kWide, 8 / kWide>), grid, dim3(256), 0, st, p); break;
+    case 0: hipLaunchKernelGGL((cache_attn_few_kernel<Q, D, 1>), grid, dim3(256), 0, st, p); break;
+    case 1: hipLaunchKernelGGL((cache_attn_few_kernel<Q, D, 2>), grid, dim3(256), 0, st, p); break;
+    case 2: hipLaunchKernelGGL((cache_attn_many_kernel<Q, D, 1, 4>), grid, dim3(256), 0, st, p); break;
+    default: hipLaunchKernelGGL((cache_attn_many_kernel<Q, D, 8 / kWaves, kWaves>), grid, dim3(kWaves * 64), 0, st, p); break;
   }
   int rc = check_launch("vasc_cache_attn");
   if (rc || s.parts == 1) return rc;
