@@ -673,17 +673,17 @@ struct Shape {
   int parts;
 };
 
-// Up to 32 rows a wave holds all of a unit's rows and the four waves share its pages; beyond, they share the rows too.
-// A unit's pages are split over `parts` workgroups, as many as one to four rounds of resident workgroups take (their
-// registers allow 4 to 2 on a CU), where that is estimated to save more than the start of another round and the joining
-// of the sums cost. Measured, in us: a wave's page where few run 0.3, the start 3, the join 5 (up to 32 rows); with 64
-// or 128 rows 4, 4 and 8.
+// Few rows (up to 32) or many (64, 128), and how many workgroups share a unit's pages: as many as one to four rounds of
+// resident workgroups take (their registers allow 4 to 2 on a CU), or one, whichever is estimated to take least. Measured,
+// in us: a wave's page where few run 0.3 (many rows, three workgroups a CU: 2.5; D = 128, two: 3), the start of a round
+// 3, the join 4 and 0.25 a MB of sums. A last round that is not full takes as long as the others: 144 units of a frame
+// run in 266 us with 5 parts, in 305 with 6 and in 263 with 16.
 Shape attn_shape(int64_t units, int64_t rows, int64_t pages, int64_t D) {
   Shape s;
   s.kind = rows <= 16 ? 0 : rows <= 32 ? 1 : rows <= 64 ? 2 : 3;
   const int64_t resident = 256 * (D == 128 ? 2 : s.kind == 0 ? 4 : 3);
   const int64_t waves = s.kind < 2 ? 4 : 1;  // that share a workgroup's pages
-  const double page_us = s.kind < 2 ? 0.3 : 2.0, start_us = s.kind < 2 ? 3.0 : 4.0, join_us = s.kind < 2 ? 5.0 : 8.0;
+  const double page_us = s.kind < 2 ? 0.3 : D == 128 ? 3.0 : 2.5, part_mb = static_cast<double>(units * rows * D) * 4e-6;
   double best = 0;
   s.parts = 0;
   for (int64_t rounds = 0; rounds <= 4; ++rounds) {
@@ -692,7 +692,7 @@ Shape attn_shape(int64_t units, int64_t rows, int64_t pages, int64_t D) {
     if (parts > 256) parts = 256;
     const int64_t share = cdiv(cdiv(pages, parts), waves);  // pages of a wave
     parts = cdiv(pages, share * waves);                     // the fewest with that share
-    const double us = cdiv(units * parts, resident) * (share * page_us + start_us) + (parts > 1 ? join_us : 0.0);
+    const double us = cdiv(units * parts, resident) * (share * page_us + 3.0) + (parts > 1 ? 4.0 + 0.25 * parts * part_mb : 0.0);
     if (s.parts == 0 || us < best) {
       best = us;
       s.parts = static_cast<int>(parts);
