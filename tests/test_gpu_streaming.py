@@ -648,3 +648,142 @@ def test_two_streams_at_once():
     torch.cuda.synchronize()
     for b in range(2):
         assert all(torch.equal(x, want[b]) for x in got[b])
+
+
+# ------------------------------------------------------------------ the modules
+def _module(dim=256, heads=4, rope=None, seed=0):
+    from vasc_amd.aggregator import Attention
+    torch.manual_seed(seed)
+    m = Attention(dim, heads, rope=rope).cuda().to(torch.bfloat16)
+    with torch.no_grad():
+        for n in (m.q_norm, m.k_norm):
+            n.weight.normal_(1.0, 0.2)
+            n.bias.normal_(0.0, 0.2)
+    return m
+
+
+def test_rotary_axes_module_is_the_2d_one():
+    """Two sections of half a head, one frequency: RotaryPositionEmbedding2D, whose float32 tables and products are within a
+    step of these (float32 tokens: cos and sin off by 2^-24, two products and a sum, on both sides)."""
+    from vasc_amd.aggregator import RotaryPositionEmbedding2D, RotaryPositionEmbeddingAxes
+    g = _gen(61)
+    x = torch.randn(2, 3, 50, 64, generator=g).cuda()
+    pos = torch.randint(0, 4000, (2, 50, 2), generator=g).cuda()
+    a = RotaryPositionEmbedding2D(100.0)(x, pos)
+    b = RotaryPositionEmbeddingAxes((32, 32), 100.0)(x, pos)
+    assert (a - b).abs().max().item() <= 2 * (2.0 ** -22 + 3 * 2.0 ** -24) * 2 * x.abs().max().item()
+    with pytest.raises(ValueError):
+        RotaryPositionEmbeddingAxes((31, 32))
+    with pytest.raises(ValueError):
+        RotaryPositionEmbeddingAxes((16, 16), (1.0, 2.0, 3.0))
+
+
+@pytest.mark.parametrize("axes", [2, 3])
+@pytest.mark.parametrize("special", [0, 5])
+def test_stream_attention_layer(axes, special):
+    """Three pushes of a layer against float64 attention over the held keys and values, projection in float32."""
+    from vasc_amd.aggregator import RotaryPositionEmbedding2D, RotaryPositionEmbeddingAxes
+    from vasc_amd.streaming import _layer_qkv, stream_attention
+    g = _gen(67)
+    rope = RotaryPositionEmbedding2D(100.0) if axes == 2 else RotaryPositionEmbeddingAxes((16, 24, 24), (1e4, 100.0, 100.0))
+    m = _module(rope=rope)
+    B, frames, P = 2, 2, 100
+    T = frames * P
+    table, pages = _table(g, B, 10)
+    cache = BlockCache(pages, 4, 64)
+    held = None
+    for step in range(3):
+        x = _randn(g, B, T, 256).cuda()
+        pos = torch.randint(0, 40, (B, T, axes), generator=g).int().cuda()
+        start, lengths = _i32([step * T] * B), _i32([step * T + T] * B)
+        with torch.no_grad():
+            qp, qs, k, v = _layer_qkv(m, x, pos, frames, special)
+        new = [O.quantise(_np(k[b]), _np(v[b])) for b in range(B)]
+        held = new if held is None else [tuple(np.concatenate([o, n], 1) for o, n in zip(held[b], new[b])) for b in range(B)]
+        keep = None if step == 0 else 1
+        y = stream_attention(m, x, pos, cache, table, start, lengths, keep=keep, frames=frames, special=special)
+        assert y.shape == x.shape and not y.requires_grad
+        lists = None
+        n = step * T + T
+        if keep is not None:
+            index, count = ops.cache_select(qp, cache, table, lengths, keep, block_q=128)
+            lists = [[[index[b, h, u, :count[b, h, u]].tolist() for u in range(index.shape[2])] for h in range(4)] for b in range(B)]
+            o = ops.cache_attn(qp, cache, table, lengths, index, count, block_q=128)
+        else:
+            o = ops.cache_attn(qp, cache, table, lengths)
+        _check_attend(o, qp, held, [n] * B, lists, 128, False, H=4)
+        o_s = None
+        if special:
+            o_s = ops.cache_attn(qs, cache, table, lengths)
+            _check_attend(o_s, qs, held, [n] * B, None, 1, False, H=4)
+        rows = ops.restore_tokens(o, o_s, frames, P, special)
+        with torch.no_grad():
+            assert torch.equal(y, m.proj(rows))
+
+
+def test_dense_layer_with_three_axes():
+    """Attention.forward with RoPE over (time, row, column) against torch in float32 on the same bf16 q, k, v."""
+    from vasc_amd.aggregator import RotaryPositionEmbeddingAxes
+    g = _gen(71)
+    m = _module(rope=RotaryPositionEmbeddingAxes((16, 24, 24), (1e4, 100.0, 100.0)))
+    x = _randn(g, 2, 90, 256).cuda()
+    pos = torch.randint(0, 60, (2, 90, 3), generator=g).cuda()
+    with torch.no_grad():
+        y = m(x, pos=pos)
+        qkv = m.qkv(x).view(2, 90, 3, 4, 64)
+        q, k = m.rope.rotate(m.q_norm(qkv[:, :, 0].transpose(1, 2)), m.k_norm(qkv[:, :, 1].transpose(1, 2)), pos)
+        v = qkv[:, :, 2].transpose(1, 2).float()
+        p = torch.softmax((q.float() @ k.float().transpose(2, 3).contiguous()) / 8, -1)
+        o = p @ v
+        # bf16 weights (2^-8 of each term) and output (2^-8) of the dense kernel, then the projection's 256 terms
+        slack = 2.0 ** -8 * (p @ v.abs()) + 2.0 ** -8 * o.abs()
+        w = m.proj.weight.float()
+        ref = o.transpose(1, 2).reshape(2, 90, 256) @ w.T.contiguous() + m.proj.bias.float()
+        bound = slack.transpose(1, 2).reshape(2, 90, 256) @ w.T.contiguous().abs()
+        assert ((y.float() - ref).abs() <= bound + 2.0 ** -8 * (ref.abs() + bound) + 1e-4).all()
+
+
+@pytest.mark.parametrize("axes", [2, 3])
+def test_aggregator_stream(axes):
+    """Pushes run, repeat after reset bit for bit, do not see stale cache contents, and refuse what does not fit."""
+    from vasc_amd.aggregator import Aggregator, RotaryPositionEmbeddingAxes
+    from vasc_amd.streaming import AggregatorStream
+    torch.manual_seed(4)
+    model = Aggregator(dim=512, depth=2, num_heads=8, intermediate_layer_idx=(0, 1)).cuda().to(torch.bfloat16)
+    if axes == 3:
+        rope = RotaryPositionEmbeddingAxes((16, 24, 24), (1e4, 100.0, 100.0))
+        for blk in (*model.frame_blocks, *model.global_blocks):
+            blk.attn.rope = rope
+    g = _gen(73)
+    images = torch.rand(2, 5, 3, 112, 140, generator=g).cuda()
+    stream = AggregatorStream(model, 5, sparse_ratio=0.5)
+
+    def run():
+        got = []
+        for a, b in ((0, 1), (1, 3), (3, 5)):
+            outs, s = stream.push(images[:, a:b])
+            assert s == 5 and all(o.shape == (2, b - a, 85, 1024) and o.isfinite().all() for o in outs)
+            got += outs
+        return got
+
+    first = run()
+    with pytest.raises(ValueError, match="holds"):
+        stream.push(images[:, :1])
+    stream.reset()
+    with pytest.raises(ValueError, match="another"):
+        stream.push(images[:, :1])
+        stream.push(images[:1, :1])
+    stream.reset()
+    for c in stream.caches:  # what is left in the pages is not seen again
+        c.ks.fill_(255)
+    for a, b in zip(run(), first):
+        assert torch.equal(a, b)
+    if axes == 2:
+        # one frame, every page: the whole-clip aggregator, up to the 8-bit keys and values of its global layers. A value is off
+        # by at most 2^-4 of itself, so an attention output (about unit size) by some percent; two layers scaled by 0.01.
+        dense = AggregatorStream(model, 1, sparse_ratio=0.0)
+        with torch.no_grad():
+            want, _ = model(images[:, :1])
+        got, _ = dense.push(images[:, :1])
+        for a, b in zip(got, want):
+            assert (a.float() - b.float()).abs().max() <= 0.02 * b.float().abs().max()

@@ -78,11 +78,51 @@ class RotaryPositionEmbedding2D(nn.Module):
         return out.to(tokens.dtype)
 
 
+class RotaryPositionEmbeddingAxes(nn.Module):
+    """Rotary position embedding over several axes, such as (time, row, column).
+
+    Axis ``a`` turns the next ``sections[a]`` features of a head, pairs
+    ``(j, j + sections[a]/2)``, with frequencies
+    ``frequency[a]**(-2j/sections[a])``; features past the sections pass
+    through. With two sections of half a head each it is
+    ``RotaryPositionEmbedding2D``, at any position (angles are float64, there
+    is no table). Runs on the GPU (``ops.rotary_axes``), differentiable.
+    """
+
+    def __init__(self, sections, frequency=100.0):
+        super().__init__()
+        self.sections = tuple(int(s) for s in sections)
+        if not 1 <= len(self.sections) <= 4 or any(s <= 0 or s % 2 for s in self.sections):
+            raise ValueError(f"sections {self.sections} must be 1 to 4 even sizes")
+        bases = tuple(frequency) if isinstance(frequency, (tuple, list)) else (frequency,) * len(self.sections)
+        if len(bases) != len(self.sections):
+            raise ValueError(f"{len(bases)} frequencies for {len(self.sections)} sections")
+        self.base_frequency = tuple(float(b) for b in bases)
+        self._frequencies: dict = {}
+
+    def frequencies(self, device) -> torch.Tensor:
+        """The axes' float64 frequencies one after another, ``[sum(sections)/2]``."""
+        key = str(device)
+        have = self._frequencies.get(key)
+        if have is None:
+            have = torch.cat([base ** (-torch.arange(0, s, 2, dtype=torch.float64) / s)
+                              for s, base in zip(self.sections, self.base_frequency)]).to(device)
+            self._frequencies[key] = have
+        return have
+
+    def rotate(self, q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor):
+        """q, k ``[B,H,T,D]``, positions ``[B,T,A]`` integer: both turned in one launch."""
+        return ops.rotary_axes(q, k, positions, self.sections, self.frequencies(q.device))
+
+    def forward(self, tokens: torch.Tensor, positions: torch.Tensor) -> torch.Tensor:
+        return self.rotate(tokens, None, positions)[0]
+
+
 class Attention(nn.Module):
-    """Multi-head attention of the VGGT/Pi3 blocks (qk-norm, 2D RoPE)."""
+    """Multi-head attention of the VGGT/Pi3 blocks (qk-norm, 2D RoPE, or RoPE over more axes)."""
 
     def __init__(self, dim: int = 1024, num_heads: int = 16, qkv_bias: bool = True, qk_norm: bool = True,
-                 rope: RotaryPositionEmbedding2D | None = None, norm_eps: float = 1e-6):
+                 rope: RotaryPositionEmbedding2D | RotaryPositionEmbeddingAxes | None = None, norm_eps: float = 1e-6):
         super().__init__()
         self.num_heads = num_heads
         self.head_dim = dim // num_heads
@@ -98,10 +138,15 @@ class Attention(nn.Module):
         B, T, dim = x.shape
         H, D = self.num_heads, self.head_dim
         qkv = self.qkv(x).to(torch.bfloat16).view(B, T, 3, H, D)
-        qp, _, k, _ = ops.pack_qkv(qkv[:, :, 0], qkv[:, :, 1], None, 1, T, 0,
-                                   q_norm=layer_norm_args(self.q_norm), k_norm=layer_norm_args(self.k_norm),
-                                   pos=pos if self.rope is not None else None,
-                                   rope_tables=self._tables(pos, D, x.device))
+        if isinstance(self.rope, RotaryPositionEmbeddingAxes):
+            qp, k = self.q_norm(qkv[:, :, 0].transpose(1, 2)), self.k_norm(qkv[:, :, 1].transpose(1, 2))
+            if pos is not None:
+                qp, k = self.rope.rotate(qp, k.to(qp.dtype), pos)
+        else:
+            qp, _, k, _ = ops.pack_qkv(qkv[:, :, 0], qkv[:, :, 1], None, 1, T, 0,
+                                       q_norm=layer_norm_args(self.q_norm), k_norm=layer_norm_args(self.k_norm),
+                                       pos=pos if self.rope is not None else None,
+                                       rope_tables=self._tables(pos, D, x.device))
         # V needs neither norm nor rotation: its MFMA tiles are packed straight
         # from the projection's strided rows
         vt = ops.pack_v(qkv[:, :, 2].transpose(1, 2))
@@ -172,14 +217,15 @@ class Block(nn.Module):
         self.ls2 = LayerScale(dim, init_values)
 
     def forward(self, x: torch.Tensor, pos: torch.Tensor | None = None, *, normed: torch.Tensor | None = None,
-                next_norm: nn.LayerNorm | None = None):
+                next_norm: nn.LayerNorm | None = None, attend=None):
         """``normed``: ``norm1(x)`` when the caller already has it; with
         ``next_norm`` also returns ``next_norm`` of the output (the next
         block's first norm), as ``(out, normed_out)``. On the GPU in bf16
         each residual update runs with the norm after it as one
-        ``vasc_residual_norm`` pass, rounded as the separate torch ops."""
+        ``vasc_residual_norm`` pass, rounded as the separate torch ops.
+        ``attend(attn, h, pos)`` takes the place of ``attn(h, pos=pos)``."""
         h = self.norm1(x) if normed is None else normed
-        a = self.attn(h, pos=pos)
+        a = self.attn(h, pos=pos) if attend is None else attend(self.attn, h, pos)
         if not _fused_residual(x, a, self, next_norm):
             x = x + self.ls1(a)
             x = x + self.ls2(self.mlp(self.norm2(x)))
