@@ -701,26 +701,29 @@ def _inference(t: torch.Tensor, name: str) -> None:
 
 
 def _rows8(t: torch.Tensor, name: str, dtypes: tuple) -> tuple:
-    """(tensor, strides) of ``[B,H,T,D]`` with unit stride on D and 16-byte aligned rows."""
+    """(tensor, its address, strides) of ``[B,H,T,D]`` with unit stride on D and 16-byte aligned rows."""
     if t.dim() != 4:
         raise ValueError(f"{name} must be [B,H,T,D], got {tuple(t.shape)}")
     if t.dtype not in dtypes:
         raise ValueError(f"{name} must be one of {[str(d) for d in dtypes]}, got {t.dtype}")
     sb, sh, st, sd = t.stride()
-    if sd != 1 or (sb | sh | st) & 7 or t.data_ptr() & 15:
+    ptr = t.data_ptr()
+    if sd != 1 or (sb | sh | st) & 7 or ptr & 15:
         t = t.contiguous()
         if t.data_ptr() & 15:  # contiguous, but a view that starts inside a row
             t = t.clone()
         sb, sh, st, sd = t.stride()
+        ptr = t.data_ptr()
         if (sb | sh | st) & 7:  # a head dimension that is no multiple of 8
             raise ValueError(f"{name} has rows of {t.shape[3]} elements, expected a multiple of 8")
-    return t, sb, sh, st
+    return t, ptr, sb, sh, st
 
 
 def _int_rows(t, name: str, B: int, dev: int):
     """``[B]`` int32, contiguous (None stays)."""
-    if t is None:
-        return None
+    if t is None or (isinstance(t, torch.Tensor) and t.dtype is torch.int32 and t.shape == (B,)
+                     and t.get_device() == dev and t.is_contiguous()):
+        return t
     _gpu(t, name, dev)
     if t.shape != (B,) or t.dtype.is_floating_point or t.dtype is torch.bool:
         raise ValueError(f"{name} must hold {B} integers, got {t.dtype} {tuple(t.shape)}")
@@ -731,6 +734,10 @@ def _int_rows(t, name: str, B: int, dev: int):
 
 def _page_table(t, B: int, dev: int) -> tuple:
     """(tensor, stride of a sequence, pages a sequence)."""
+    if isinstance(t, torch.Tensor) and t.dtype is torch.int32 and t.get_device() == dev:
+        shape, strides = t.shape, t.stride()
+        if len(shape) == 2 and shape[0] == B and strides[1] == 1 and strides[0] >= shape[1] > 0:
+            return t, strides[0] if B > 1 else shape[1], shape[1]
     _gpu(t, "page_table", dev)
     if t.dim() != 2 or t.shape[0] != B or t.shape[1] == 0 or t.dtype.is_floating_point or t.dtype is torch.bool:
         raise ValueError(f"page_table must be [{B}, max_pages] integers, got {t.dtype} {tuple(t.shape)}")
@@ -880,8 +887,8 @@ def cache_write(cache, k: torch.Tensor, v: torch.Tensor, page_table: torch.Tenso
     _inference(v, "v")
     if cache.device_index != dev:
         raise ValueError(f"the cache is on cuda:{cache.device_index}, k on cuda:{dev}")
-    k, ksb, ksh, kst = _rows8(k, "k", _ROWS)
-    v, vsb, vsh, vst = _rows8(v, "v", _ROWS)
+    k, *kargs = _rows8(k, "k", _ROWS)
+    v, *vargs = _rows8(v, "v", _ROWS)
     B, H, T, D = shape = k.shape
     if shape != v.shape or k.dtype != v.dtype:
         raise ValueError(f"k {k.dtype} {tuple(shape)} and v {v.dtype} {tuple(v.shape)} differ")
@@ -893,7 +900,7 @@ def cache_write(cache, k: torch.Tensor, v: torch.Tensor, page_table: torch.Tenso
         raise ValueError("start is required")
     if B == 0 or T == 0:
         return
-    _launch(dev, "vasc_cache_write", k.data_ptr(), ksb, ksh, kst, v.data_ptr(), vsb, vsh, vst, B, H, T, D,
+    _launch(dev, "vasc_cache_write", *kargs, *vargs, B, H, T, D,
             _DTYPE[k.dtype], table.data_ptr(), ts, mp, start.data_ptr(), _ptr(count), *cache.pointers,
             cache.mean_pointer, cache.pages)
 
@@ -924,20 +931,21 @@ def cache_read(cache, page_table: torch.Tensor, start: torch.Tensor, tokens: int
 
 
 def _cache_query(q, cache, page_table, lengths, q_count, block_q: int, dev: int) -> tuple:
+    """(q, its shape, its C arguments, page table x 3, lengths, q_count), checked."""
     _inference(q, "q")
     if cache.device_index != dev:
         raise ValueError(f"the cache is on cuda:{cache.device_index}, q on cuda:{dev}")
-    q, sb, sh, st = _rows8(q, "q", _QUERIES)
-    B, Hq, T, D = q.shape
-    if D != cache.head_dim or Hq % cache.heads or Hq == 0:
-        raise ValueError(f"q has {Hq} heads of {D}: expected a multiple of {cache.heads} heads of {cache.head_dim}")
-    if not (1 <= block_q and block_q * (Hq // cache.heads) <= 128):
-        raise ValueError(f"block_q {block_q} with {Hq // cache.heads} query heads a key head: a unit has 1 to 128 rows")
-    table, ts, mp = _page_table(page_table, B, dev)
+    q, *args = _rows8(q, "q", _QUERIES)
+    B, Hq, T, D = shape = q.shape
+    H = cache.heads
+    if D != cache.head_dim or Hq % H or Hq == 0:
+        raise ValueError(f"q has {Hq} heads of {D}: expected a multiple of {H} heads of {cache.head_dim}")
+    if not (1 <= block_q and block_q * (Hq // H) <= 128):
+        raise ValueError(f"block_q {block_q} with {Hq // H} query heads a key head: a unit has 1 to 128 rows")
     lengths = _int_rows(lengths, "lengths", B, dev)
     if lengths is None:
         raise ValueError("lengths is required")
-    return q, (q.data_ptr(), sb, sh, st), table, ts, mp, lengths, _int_rows(q_count, "q_count", B, dev)
+    return q, shape, args, *_page_table(page_table, B, dev), lengths, _int_rows(q_count, "q_count", B, dev)
 
 
 def cache_select(q: torch.Tensor, cache, page_table: torch.Tensor, lengths: torch.Tensor, keep: int, *,
@@ -963,10 +971,10 @@ def cache_select(q: torch.Tensor, cache, page_table: torch.Tensor, lengths: torc
     """
     dev = _gpu(q, "q")
     block_q, keep, sink, recent, causal = int(block_q), int(keep), int(sink), int(recent), bool(causal)
-    q, qargs, table, ts, mp, lengths, q_count = _cache_query(q, cache, page_table, lengths, q_count, block_q, dev)
+    q, shape, qargs, table, ts, mp, lengths, q_count = _cache_query(q, cache, page_table, lengths, q_count, block_q, dev)
     if keep < 0 or sink < 0 or recent < 1:
         raise ValueError(f"keep {keep} and sink {sink} must not be negative, recent {recent} at least 1")
-    B, Hq, T, D = q.shape
+    B, Hq, T, D = shape
     H, U = cache.heads, -(-T // block_q)
     width = min(mp, sink + keep + recent + ((block_q + BLOCK_K - 2) // BLOCK_K if causal else 0))
     device = q.device
@@ -1010,22 +1018,23 @@ def cache_attn(q: torch.Tensor, cache, page_table: torch.Tensor, lengths: torch.
             raise ValueError("lists need the block_q they were made with")
         block_q = max(1, min(q.shape[2], 128 // max(1, q.shape[1] // cache.heads)))
     block_q = int(block_q)
-    q, qargs, table, ts, mp, lengths, q_count = _cache_query(q, cache, page_table, lengths, q_count, block_q, dev)
-    B, Hq, T, D = shape = q.shape
+    q, shape, qargs, table, ts, mp, lengths, q_count = _cache_query(q, cache, page_table, lengths, q_count, block_q, dev)
+    B, Hq, T, D = shape
     H, width = cache.heads, 0
     if index is not None:
         U = -(-T // block_q)
         _gpu(index, "index", dev)
         _gpu(count, "count", dev)
-        if index.dim() != 4 or index.shape[:3] != (B, H, U) or count.shape != (B, H, U):
-            raise ValueError(f"index/count must be [{B},{H},{U},W]/[{B},{H},{U}], got {tuple(index.shape)}/"
+        ishape = index.shape
+        if len(ishape) != 4 or ishape[:3] != (B, H, U) or count.shape != (B, H, U):
+            raise ValueError(f"index/count must be [{B},{H},{U},W]/[{B},{H},{U}], got {tuple(ishape)}/"
                              f"{tuple(count.shape)}")
         if index.dtype is not torch.int32 or count.dtype is not torch.int32:
             if any(t.dtype.is_floating_point or t.dtype is torch.bool for t in (index, count)):
                 raise ValueError("index and count must be integers")
             index, count = index.to(torch.int32), count.to(torch.int32)
         index, count = index.contiguous(), count.contiguous()
-        width = index.shape[3]
+        width = ishape[3]
     if out is None:
         out = torch.empty(shape, device=q.device, dtype=q.dtype)
         osb, osh, ost = Hq * T * D, T * D, D
