@@ -113,7 +113,8 @@ int64_t vasc_cache_attn_workspace_size(int64_t B, int64_t Hq, int64_t H, int64_t
  * [B,H,U] as vasc_cache_select writes them: ascending logical pages; entries
  * that are not above the one before, negative or not below max_pages are
  * skipped. block_q as there (index NULL: any block_q with block_q * G <= 128).
- * q, o [B,Hq,T,D] strided, bfloat16 or float16. scale: finite.
+ * q, o [B,Hq,T,D] strided, bfloat16 or float16. scale: 0, or of magnitude
+ * 1e-30 to 1e30.
  */
 int vasc_cache_attn(const void *q, int64_t q_sb, int64_t q_sh, int64_t q_st, void *o, int64_t o_sb, int64_t o_sh,
                     int64_t o_st, int64_t B, int64_t Hq, int64_t H, int64_t T, int64_t D, int32_t dtype,

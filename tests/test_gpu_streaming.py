@@ -395,8 +395,11 @@ def test_select_equal_and_close_scores(mp):
 def _check_attend(o, q, held, lens, lists, block_q, causal, scale=None, n_q=None, H=None):
     """o against float64 over the held values. Bound for an element: the output's rounding; weights rounded to half
     (2^-11 of each term); an error of the float32 logits in weights and sum, (D + 8) 2^-24 of the products' magnitudes;
-    float32 sums over n keys, n 2^-24 of the terms' magnitudes, twice (weights and their sum), and 2^-20 for exp2, the
-    powers and the division; weights under 2^-36 of the largest, at most n of them."""
+    float32 sums over n keys, n 2^-24 of the terms' magnitudes, twice (weights and their sum), and 2^-14.5 for exp2,
+    the powers, the division and the exponents: logits are summed on top of a reference whose size is up to 2^8 + 2 |logit| (the
+    values' biased exponents, up to 187, and the largest logit), so each of its two roundings is up to 2^-24 (2^8 + 2
+    |logit|) ln 2 of a weight, and again in the sum: 4 * 2^-24 * 2^8 ln 2 < 2^-14.5; the logits' part
+    is in (D + 8). Weights under 2^-36 of the largest, at most n of them."""
     B, Hq, T, D = q.shape
     G = Hq // H
     scale = D ** -0.5 if scale is None else scale
@@ -419,7 +422,7 @@ def _check_attend(o, q, held, lens, lists, block_q, causal, scale=None, n_q=None
                 for gi in range(G):
                     ref, mag, logit = O.attend(qn[b, h * G + gi, t], k, v, seen, scale)
                     n = int(seen.sum())
-                    rel = 2.0 ** -11 + 2 * ((D + 8) * 2.0 ** -24 * logit + n * 2.0 ** -24) + 2.0 ** -20
+                    rel = 2.0 ** -11 + 2 * ((D + 8) * 2.0 ** -24 * logit + n * 2.0 ** -24) + 2.0 ** -14.5
                     bound = rel * mag + HALF[o.dtype] * (np.abs(ref) + rel * mag) + n * 2.0 ** -36 * np.abs(v).max(initial=0)
                     if o.dtype == torch.float16:
                         bound = bound + 2.0 ** -25
@@ -512,6 +515,30 @@ def test_attend_masked_values_do_not_matter():
     assert torch.equal(o[0, 0, :30], base[0, 0, :30]) and o[0, 0, 30:].isnan().all()
     o = ops.cache_attn(q[:, :, :5], cache, table, _i32([190]))
     _check_attend(o, q[:, :, :5], [(held[0][0][:, :190], held[0][1][:, :190])], [190], None, 1, False, H=1)
+
+
+@pytest.mark.parametrize("D,G,T", [(64, 1, 1), (128, 20, 1), (64, 1, 100), (128, 4, 30)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_attend_nan_tokens_and_queries(D, G, T, dtype):
+    """In every kernel: a NaN token makes the rows that see it NaN and no others, as does an infinite query."""
+    g = _gen(D + T)
+    table, pages = _table(g, 2, 5)
+    cache = BlockCache(pages, 1, D)
+    k, v = _randn(g, 2, 1, 300, D), _randn(g, 2, 1, 300, D)
+    k[1, 0, 150, 3] = float("inf")
+    held = _fill(cache, g, table, [300, 300], k, v)
+    q = _randn(g, 2, G, T, D, dtype=dtype).cuda()
+    o = ops.cache_attn(q, cache, table, _i32([300, 300]))
+    assert o[1].isnan().all()
+    _check_attend(o[:1], q[:1], held[:1], [300], None, 1, False, H=1)
+    o = ops.cache_attn(q, cache, table, _i32([300, 150]))
+    cut = [held[0], (held[1][0][:, :150], held[1][1][:, :150])]
+    _check_attend(o, q, cut, [300, 150], None, 1, False, H=1)
+    q[0, G - 1, T - 1, 7] = float("inf")
+    o2 = ops.cache_attn(q, cache, table, _i32([300, 150]))
+    assert o2[0, G - 1, T - 1].isnan().all()
+    o2[0, G - 1, T - 1] = o[0, G - 1, T - 1]
+    assert torch.equal(o2, o)
 
 
 def test_attend_wide_logits_and_scale():

@@ -102,7 +102,7 @@ def stream_attention(attn, x: torch.Tensor, pos: torch.Tensor | None, cache: Blo
     last ``recent``; None: all. Returns ``[B,T,dim]``. No gradients.
     """
     B, T, dim = x.shape
-    if frames < 1 or T % frames or not 0 <= special <= T // frames:
+    if frames < 1 or T < 1 or T % frames or not 0 <= special <= T // frames:
         raise ValueError(f"{T} tokens are not {frames} frames with {special} special tokens each")
     H = attn.num_heads
     q_patch, q_special, k, v = _layer_qkv(attn, x, pos, frames, special)
@@ -161,7 +161,7 @@ class AggregatorStream:
         from .aggregator import grid_positions, patch_tokens, RotaryPositionEmbeddingAxes
         m = self.model
         B, n, _, Hi, Wi = images.shape
-        if self.frames + n > self.max_frames:
+        if n < 1 or self.frames + n > self.max_frames:
             raise ValueError(f"{n} more frames after {self.frames}: the stream holds {self.max_frames}")
         x = ((images - m._resnet_mean) / m._resnet_std).view(B * n, 3, Hi, Wi).to(m.patch_embed.weight.dtype)
         tokens = patch_tokens(m.patch_embed, x)
