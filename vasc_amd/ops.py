@@ -689,7 +689,7 @@ def _gpu(t, name: str, dev: int = -1) -> int:
     if not isinstance(t, torch.Tensor) or not t.is_cuda:
         raise ValueError(f"{name} must be a GPU tensor (the HIP path has no CPU fallback)")
     at = t.get_device()
-    if dev >= 0 and at != dev:
+    if at != dev and dev >= 0:
         raise ValueError(f"{name} is on cuda:{at}, expected cuda:{dev}")
     return at
 
@@ -786,9 +786,10 @@ def _rotary(q, k, pos, sections, inv_freq, inverse: bool) -> tuple:
         return qo, _rotary(k, None, pos, sections, inv_freq, inverse)[0]
     osb, osh, ost, _ = qo.stride()
     psb, pst, _ = pos.stride()
+    sizes, axes, _ = _section_sizes(sections, D)
     _launch(q.get_device(), "vasc_rotary_axes", q.data_ptr(), qsb, qsh, qst, qo.data_ptr(), osb, osh, ost, Hq, *kargs,
-            B, T, D, pos.data_ptr(), psb if pos.shape[0] > 1 else 0, pst, len(sections), _section_sizes(sections, D),
-            inv_freq.data_ptr(), _DTYPE[q.dtype], inverse)
+            B, T, D, pos.data_ptr(), psb if pos.shape[0] > 1 else 0, pst, axes, sizes, inv_freq.data_ptr(),
+            _DTYPE[q.dtype], inverse)
     return qo, ko
 
 
@@ -814,10 +815,10 @@ class _RotaryAxes(torch.autograd.Function):
 
 @functools.lru_cache(maxsize=64)
 def _section_sizes(sections: tuple, D: int):
-    """The checked sections of a head dimension as a C array."""
+    """(the checked sections of a head dimension as a C array, their number, their pairs)."""
     if not 1 <= len(sections) <= 4 or any(s <= 0 or s % 2 for s in sections) or sum(sections) > D:
         raise ValueError(f"sections {sections} must be 1 to 4 even sizes that sum to at most {D}")
-    return (ctypes.c_int64 * len(sections))(*sections)
+    return (ctypes.c_int64 * len(sections))(*sections), len(sections), sum(sections) // 2
 
 
 def rotary_axes(q: torch.Tensor, k: torch.Tensor | None, pos: torch.Tensor, sections, inv_freq: torch.Tensor):
@@ -843,24 +844,25 @@ def rotary_axes(q: torch.Tensor, k: torch.Tensor | None, pos: torch.Tensor, sect
         if len(kshape) != 4 or k.dtype is not dtype or kshape[0] != B or kshape[2] != T or kshape[3] != D:
             raise ValueError(f"k must be [{B},H,{T},{D}] of {dtype}, got {k.dtype} {tuple(kshape)}")
     sections = tuple(sections)
-    _section_sizes(sections, D)
+    _, A, pairs = _section_sizes(sections, D)
     _gpu(pos, "pos", dev)
     if pos.dtype is not torch.int32:
         if pos.dtype.is_floating_point or pos.dtype is torch.bool:
             raise ValueError(f"pos must hold integers, got {pos.dtype}")
         pos = pos.to(torch.int32)
-    if pos.dim() == 2:
+    pshape = pos.shape
+    if len(pshape) == 2:
         pos = pos.unsqueeze(0)
-    A = len(sections)
-    if pos.shape != (B, T, A) and pos.shape != (1, T, A):
-        raise ValueError(f"pos must be [{B} or 1, {T}, {A}], got {tuple(pos.shape)}")
-    if pos.stride(2) != 1 and A > 1:
+        pshape = pos.shape
+    if pshape != (B, T, A) and pshape != (1, T, A):
+        raise ValueError(f"pos must be [{B} or 1, {T}, {A}], got {tuple(pshape)}")
+    if A > 1 and pos.stride(2) != 1:
         pos = pos.contiguous()
     _gpu(inv_freq, "inv_freq", dev)
-    if inv_freq.dtype is not torch.float64 or inv_freq.shape != (sum(sections) // 2,):
-        raise ValueError(f"inv_freq must hold {sum(sections) // 2} float64 values, got {inv_freq.dtype} "
-                         f"{tuple(inv_freq.shape)}")
-    inv_freq = inv_freq.detach().contiguous() if inv_freq.requires_grad or not inv_freq.is_contiguous() else inv_freq
+    if inv_freq.dtype is not torch.float64 or inv_freq.shape != (pairs,):
+        raise ValueError(f"inv_freq must hold {pairs} float64 values, got {inv_freq.dtype} {tuple(inv_freq.shape)}")
+    if not inv_freq.is_contiguous():
+        inv_freq = inv_freq.contiguous()
     if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
         return _RotaryAxes.apply(q, k, pos, sections, inv_freq)
     return _rotary(q, k, pos, sections, inv_freq, False)
