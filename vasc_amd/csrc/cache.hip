@@ -6,6 +6,10 @@
 // the call touches that page, so partly covered words are merged with plain
 // loads and stores, and the page's key mean is recomputed from its codes, a
 // function of what the page holds whatever calls brought it there.
+// Measured (bf16, 16 heads of 64): 32 frames of 1041 tokens written in 47 us
+// (4.4 TB/s; a large copy reaches 4.75), read back in 32 us (6.4 TB/s, partly
+// from the cache behind HBM); one token of 64 sequences, 8 heads of 128, in
+// 7.3 us: the latency of table, codes, barrier and merge.
 #include "stream.h"
 
 namespace vasc {
@@ -336,6 +340,8 @@ __device__ __forceinline__ Unit unit_of(const SelectParams &p, int row) {
 // asks for its pages' places before it has seen the lengths and for their means before it sums the queries; the sums of
 // kScoreBatch pages cross the lanes together, each step leaving a lane half the pages; and a workgroup takes as many
 // rounds of pages as leave the chip some four workgroups a CU.
+// Measured: 16 x 131072 tokens, 8 heads of 128, in 13.6 us (3.2 TB/s); nine
+// units of a frame against 2082 pages, 16 heads of 64, in 13.1 us.
 constexpr int kScoreBatch = 8;
 
 // Sums v[0..8) over the lanes that differ in the bits [lo, hi) of the lane number; a lane is left with the sum of element
@@ -486,6 +492,7 @@ __device__ __forceinline__ uint32_t score_key(float f) {
 // exactly ends it. More waves would pay a barrier a bit (9.9 us for 128 lists of 2048 pages): they sort into 2048 bins by
 // the next 11 bits instead, until the bin that holds the cut has at most kRanked members (scores of one sign and size spread
 // over some dozens of bins, so most lists need one turn), which are then ranked among themselves.
+// Measured: 128 lists of 2048 pages or 144 of 2082 in 9.2 us, most of it latency (531 vector instructions a wave).
 constexpr int kBins = 2048, kRanked = 128;
 
 template <int kWaves, int E>
