@@ -125,6 +125,13 @@ def test_rotary_gradients(dtype):
         rhs = (dq.double() * d.double()).sum().item()
         n = gq.numel()
         assert abs(lhs - rhs) <= 2.0 ** -20 * math.sqrt(n) * 40
+    # a second derivative: of |turn(q)|^2 / 2 along gq, which is gq itself (a turn keeps lengths)
+    qo = ops.rotary_axes(q, None, pos, sections, freq)[0]
+    grad, = torch.autograd.grad(qo, q, qo, create_graph=True)
+    again, = torch.autograd.grad(grad, q, gq)
+    bound = 2 * _rotary_bound(gq, _np(gq), sections, dtype) + 2 ** -20
+    if dtype == torch.float32:
+        assert (np.abs(_np(again) - _np(gq)) <= 8 * bound).all()
     # broadcast gradient (stride 0 everywhere)
     qo = ops.rotary_axes(q, None, pos, sections, freq)[0]
     dq, = torch.autograd.grad(qo.sum(), q)
@@ -470,6 +477,20 @@ def test_attend_chunks(D, H, G, T, block_q, L, causal, dtype):
     lists = [[[index[b, h, u, :count[b, h, u]].tolist() for u in range(index.shape[2])] for h in range(H)] for b in range(2)]
     o = ops.cache_attn(q, cache, table, _i32(lens), index, count, block_q=block_q, causal=causal, q_count=_i32(n_q))
     _check_attend(o, q, held, lens, lists, block_q, causal, n_q=n_q, H=H)
+
+
+@pytest.mark.parametrize("D,H,G,T,L", [(64, 1, 1, 1, 9000), (128, 1, 3, 1, 7000), (64, 1, 1, 90, 5000), (128, 2, 1, 2, 2600)])
+def test_attend_many_parts(D, H, G, T, L):
+    """Few units over many pages: each split over some dozens of workgroups, joined by groups that share a row."""
+    g = _gen(L)
+    table, pages = _table(g, 2, -(-L // 64))
+    cache = BlockCache(pages, H, D)
+    lens = [L, 100]  # most parts of the second have no page
+    held = _fill(cache, g, table, lens)
+    q = _randn(g, 2, H * G, T, D).cuda()
+    o = ops.cache_attn(q, cache, table, _i32(lens))
+    _check_attend(o, q, held, lens, None, 1, False, H=H)
+    assert not ops.cache_attn(q, cache, table, _i32([0, 0])).any()
 
 
 def test_attend_list_rules():

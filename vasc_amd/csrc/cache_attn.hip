@@ -644,30 +644,78 @@ __global__ __launch_bounds__(kWaves * 64, D == 64 && kWaves == 4 ? 3 : 2) void c
   rows.template store<Q>(p, w, first, col, g, m);
 }
 
-// Joins the parts of each row: 16 or 32 lanes a row, four features each.
-template <typename Q, int D>
+// Joins the parts of each row: D/4 lanes a row, four features each. Up to kFewParts parts one group of lanes takes them in
+// turn and a workgroup has a row a group; beyond, the groups of a workgroup share one row's parts, four in flight each (one
+// group took 40 us for 100 parts, each waiting for the one before).
+constexpr int kFewParts = 12;
+
+template <typename Q, int D, bool kShare>
 __global__ __launch_bounds__(256) void cache_join_kernel(const AttnParams p) {
-  constexpr int kLanes = D / 4;
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * (256 / kLanes) + threadIdx.x / kLanes;
+  constexpr int kLanes = D / 4, kGroups = 256 / kLanes;
+  __shared__ float sums[kShare ? kGroups : 1][kShare ? D + 2 : 1];
+  const int grp = threadIdx.x / kLanes, d = (threadIdx.x % kLanes) * 4;
+  const int64_t row = kShare ? blockIdx.x : static_cast<int64_t>(blockIdx.x) * kGroups + grp;
   const int64_t all = p.B * p.H * p.U * static_cast<int64_t>(p.rows);
-  if (row >= all) return;
-  const int d = (threadIdx.x % kLanes) * 4;
+  if (row >= all) return;  // kShare: never
   const int64_t unit = row / p.rows;
   const int r = static_cast<int>(row - unit * p.rows), tl = r / p.G, gh = r - tl * p.G;
   const int u = static_cast<int>(unit % p.U);
   const int64_t bh = unit / p.U, b = bh / p.H, h = bh - b * p.H;
   const int64_t t = static_cast<int64_t>(u) * p.block_q + tl;
-  if (t >= p.T) return;
+  if (t >= p.T) return;  // the same for a whole workgroup where it shares a row
   const float *o = p.ws + row * p.parts * D + d;
   const float *ml = p.ws + all * p.parts * D + row * p.parts * 2;
-  float mx = -__builtin_inff();
-  for (int i = 0; i < p.parts; ++i) mx = fmaxf(mx, ml[i * 2]);
+  constexpr int kStep = kShare ? kGroups : 1;
   floatx4 acc = {0, 0, 0, 0};
-  float l = 0.f;
-  for (int i = 0; i < p.parts; ++i) {
-    const float c = ml[i * 2] == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(ml[i * 2] - mx);
-    l = fmaf(ml[i * 2 + 1], c, l);
-    acc += *reinterpret_cast<const floatx4 *>(o + static_cast<int64_t>(i) * D) * c;
+  float l = 0.f, mx = -__builtin_inff();
+  for (int i0 = kShare ? grp : 0; i0 < p.parts; i0 += 4 * kStep) {
+    float m[4], ls[4];
+    floatx4 x[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int i = i0 + k * kStep;
+      const bool in = i < p.parts;
+      m[k] = in ? ml[i * 2] : -__builtin_inff();
+      ls[k] = in ? ml[i * 2 + 1] : 0.f;
+      x[k] = in ? *reinterpret_cast<const floatx4 *>(o + static_cast<int64_t>(i) * D) : floatx4{0, 0, 0, 0};
+    }
+    const float top = fmaxf(mx, fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])));
+    if (top == -__builtin_inff()) continue;
+    const float c = __builtin_amdgcn_exp2f(mx - top);
+    l *= c;
+    acc *= c;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const float w = __builtin_amdgcn_exp2f(m[k] - top);
+      l = fmaf(ls[k], w, l);
+      acc += x[k] * w;
+    }
+    mx = top;
+  }
+  if constexpr (kShare) {
+    *reinterpret_cast<float2 *>(&sums[grp][d]) = float2{acc[0], acc[1]};
+    *reinterpret_cast<float2 *>(&sums[grp][d + 2]) = float2{acc[2], acc[3]};
+    if (d == 0) {
+      sums[grp][D] = mx;
+      sums[grp][D + 1] = l;
+    }
+    __syncthreads();
+    if (grp > 0) return;
+    float top = mx;
+#pragma unroll
+    for (int i = 1; i < kGroups; ++i) top = fmaxf(top, sums[i][D]);
+    if (top > -__builtin_inff()) {
+      const float c = __builtin_amdgcn_exp2f(mx - top);
+      l *= c;
+      acc *= c;
+#pragma unroll
+      for (int i = 1; i < kGroups; ++i) {
+        const float w = __builtin_amdgcn_exp2f(sums[i][D] - top);
+        l = fmaf(sums[i][D + 1], w, l);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc[j] = fmaf(sums[i][d + j], w, acc[j]);
+      }
+    }
   }
   const float inv = l == 0.f ? 0.f : 1.f / l;
   struct alignas(8) Four { Q v[4]; } out;
@@ -723,7 +771,10 @@ int launch_attn(const AttnParams &p, const Shape &s, hipStream_t st) {
   int rc = check_launch("vasc_cache_attn");
   if (rc || s.parts == 1) return rc;
   const int64_t rows = p.B * p.H * p.U * static_cast<int64_t>(p.rows);
-  hipLaunchKernelGGL((cache_join_kernel<Q, D>), dim3(static_cast<unsigned>(cdiv(rows, 256 / (D / 4)))), dim3(256), 0, st, p);
+  if (s.parts > kFewParts && rows < (int64_t(1) << 16))
+    hipLaunchKernelGGL((cache_join_kernel<Q, D, true>), dim3(static_cast<unsigned>(rows)), dim3(256), 0, st, p);
+  else
+    hipLaunchKernelGGL((cache_join_kernel<Q, D, false>), dim3(static_cast<unsigned>(cdiv(rows, 256 / (D / 4)))), dim3(256), 0, st, p);
   return check_launch("vasc_cache_attn");
 }
 

@@ -794,23 +794,24 @@ def _rotary(q, k, pos, sections, inv_freq, inverse: bool) -> tuple:
 
 
 class _RotaryAxes(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, q, k, pos, sections, inv_freq):
-        ctx.save_for_backward(pos, inv_freq)
-        ctx.sections = sections
-        ctx.set_materialize_grads(False)
-        return _rotary(q, k, pos, sections, inv_freq, False)
+    """A turn is orthogonal: its gradient is the opposite turn of the gradient, which is differentiable in turn."""
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    def forward(ctx, q, k, pos, sections, inv_freq, inverse):
+        ctx.save_for_backward(pos, inv_freq)
+        ctx.sections, ctx.inverse = sections, inverse
+        ctx.set_materialize_grads(False)
+        return _rotary(q, k, pos, sections, inv_freq, inverse)
+
+    @staticmethod
     def backward(ctx, gq, gk):
-        pos, inv_freq = ctx.saved_tensors
         if gq is None and gk is None:
-            return None, None, None, None, None
+            return None, None, None, None, None, None
+        pos, inv_freq = ctx.saved_tensors
+        turn = _RotaryAxes.apply if torch.is_grad_enabled() else _rotary  # grad mode: a second derivative is asked for
         if gq is None:
-            return None, _rotary(gk, None, pos, ctx.sections, inv_freq, True)[0], None, None, None
-        dq, dk = _rotary(gq, gk, pos, ctx.sections, inv_freq, True)
-        return dq, dk, None, None, None
+            return None, turn(gk, None, pos, ctx.sections, inv_freq, not ctx.inverse)[0], None, None, None, None
+        return *turn(gq, gk, pos, ctx.sections, inv_freq, not ctx.inverse), None, None, None, None
 
 
 @functools.lru_cache(maxsize=64)
@@ -864,7 +865,7 @@ def rotary_axes(q: torch.Tensor, k: torch.Tensor | None, pos: torch.Tensor, sect
     if not inv_freq.is_contiguous():
         inv_freq = inv_freq.contiguous()
     if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
-        return _RotaryAxes.apply(q, k, pos, sections, inv_freq)
+        return _RotaryAxes.apply(q, k, pos, sections, inv_freq, False)
     return _rotary(q, k, pos, sections, inv_freq, False)
 
 
