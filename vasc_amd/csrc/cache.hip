@@ -492,7 +492,8 @@ __device__ __forceinline__ uint32_t score_key(float f) {
 // exactly ends it. More waves would pay a barrier a bit (9.9 us for 128 lists of 2048 pages): they sort into 2048 bins by
 // the next 11 bits instead, until the bin that holds the cut has at most kRanked members (scores of one sign and size spread
 // over some dozens of bins, so most lists need one turn), which are then ranked among themselves.
-// Measured: 128 lists of 2048 pages or 144 of 2082 in 9.2 us, most of it latency (531 vector instructions a wave).
+// Measured: 128 lists of 2048 pages or 144 of 2082 in 8.6 us: 4.5 until the scores are there, 1.4 for the bins, 1.5 for the
+// ranks, the rest for the list; latency throughout.
 constexpr int kBins = 2048, kRanked = 128;
 
 template <int kWaves, int E>
@@ -576,9 +577,12 @@ __global__ __launch_bounds__(kWaves * 64) void cache_list_kernel(const SelectPar
         for (int i = 0; i < E; ++i)
           if (key[i] != 0 && (key[i] & mask) == prefix) atomicAdd(&bins[(key[i] >> shift) & digits], 1u);
         __syncthreads();
-        int own = 0;
+        int mine[kOwn], own = 0;
 #pragma unroll
-        for (int i = 0; i < kOwn; ++i) own += bins[tid * kOwn + i];
+        for (int i = 0; i < kOwn; ++i) {
+          mine[i] = bins[tid * kOwn + i];
+          own += mine[i];
+        }
         int above = own;  // this thread's bins and those over them, in the wave and then in all
 #pragma unroll
         for (int o = 1; o < 64; o <<= 1) {
@@ -587,12 +591,13 @@ __global__ __launch_bounds__(kWaves * 64) void cache_list_kernel(const SelectPar
         }
         if (lane == 0) wave_total[wave] = above;
         __syncthreads();
-        for (int w = wave + 1; w < kWaves; ++w) above += wave_total[w];
+#pragma unroll
+        for (int w = 1; w < kWaves; ++w) above += w > wave ? wave_total[w] : 0;
         above -= own;
         if (above < want && above + own >= want) {  // one thread
 #pragma unroll
           for (int i = kOwn - 1; i >= 0; --i) {
-            const int c = bins[tid * kOwn + i];
+            const int c = mine[i];
             if (above < want && above + c >= want) {
               found[0] = tid * kOwn + i;
               found[1] = want - above;
@@ -620,14 +625,19 @@ __global__ __launch_bounds__(kWaves * 64) void cache_list_kernel(const SelectPar
           const int padded = (members + 7) & ~7;
           if (tid >= members && tid < padded) ranked[tid] = 0;
           __syncthreads();
-          if (tid < members) {
-            const uint64_t mine = ranked[tid];
+          // kThreads / kRanked neighbouring threads count for a member
+          constexpr int kShare = kWaves > 1 ? kThreads / kRanked : 1;
+          const int member = tid / kShare;
+          if (member < members) {
+            const uint64_t own_key = ranked[member];
             int over = 0;
-            for (int i = 0; i < padded; i += 8) {
+            for (int i = tid % kShare * 8; i < padded; i += 8 * kShare) {
 #pragma unroll
-              for (int e = 0; e < 8; ++e) over += ranked[i + e] > mine;
+              for (int e = 0; e < 8; ++e) over += ranked[i + e] > own_key;
             }
-            if (over == want - 1) last = mine;
+#pragma unroll
+            for (int o = 1; o < kShare; o <<= 1) over += xor_lane(over, o);
+            if (over == want - 1) last = own_key;
           }
           __syncthreads();
           cut = static_cast<uint32_t>(last >> 32);
@@ -672,9 +682,11 @@ __global__ __launch_bounds__(kWaves * 64) void cache_list_kernel(const SelectPar
   if (lane == 0) wave_total[wave] = chosen;
   __syncthreads();
   int at = 0, all = 0;
+#pragma unroll
   for (int w = 0; w < kWaves; ++w) {
-    if (w < wave) at += wave_total[w];
-    all += wave_total[w];
+    const int c = wave_total[w];
+    at += w < wave ? c : 0;
+    all += c;
   }
   const int width = static_cast<int>(p.width);
   int32_t *list = p.index + row * p.width;
