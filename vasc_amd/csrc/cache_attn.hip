@@ -515,8 +515,8 @@ __global__ __launch_bounds__(256, 2) void cache_attn_few_kernel(const AttnParams
 // a page is widened once for all of them: each wave turns its share of the codes into operands in LDS (keys as bfloat16 with
 // their powers, values as half, and the values' exponents as floats), 16 bytes a lane in the order in which they are read.
 // Two buffers and one barrier a page: the next page's codes are on their way to registers while this one is computed.
-// Measured: a frame of 1041 queries over 522 of 2082 pages, 16 heads of 64, 142 GFLOP in 237 us with the join (600 TFLOP/s);
-// 250 causal tokens of 32 heads of 128 over 20001, 163 GFLOP in 197 us (825). A wave's page (32 rows, D = 64) takes some
+// Measured: a frame of 1041 queries over 522 of 2082 pages, 16 heads of 64, 142 GFLOP in 225 us with the join (630 TFLOP/s);
+// 250 causal tokens of 32 heads of 128 over 20001, 163 GFLOP in 191 us (850). A wave's page (32 rows, D = 64) takes some
 // 1700 cycles: 208 vector instructions, 32 of them exp2, and 32 matrix ones; the same mix from registers alone takes 1110
 // with three waves a SIMD, the matrix pipe by itself 516. Also built, and no faster: values widened with their powers and
 // weights summed by a product with ones (253 us, D = 128 slower), the next page's first product beside this page's
@@ -617,6 +617,9 @@ __global__ __launch_bounds__(kWaves * 64, D == 64 && kWaves == 4 ? 3 : 2) void c
               s[x][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, query[x][piece * kMul + y], c, 0, 0, 0);
             }
         }
+      // The softmax goes before the other waves' products: the matrix pipe works on while its instructions are issued. Measured
+      // for the frame above, one card: 256 us without, 249 with, 254 with the products before the softmax.
+      __builtin_amdgcn_s_setprio(1);
 #pragma unroll
       for (int t = 0; t < 4; ++t) {
         const floatx4 ev = *reinterpret_cast<const floatx4 *>(buf.ev + g * 16 + t * 4);
@@ -628,6 +631,7 @@ __global__ __launch_bounds__(kWaves * 64, D == 64 && kWaves == 4 ? 3 : 2) void c
       halfx8 wt[kTiles][2];
       rows.weights(s, lpage, g, inv_c,
                    [&](int t) { return *reinterpret_cast<const floatx4 *>(buf.un + g * 16 + t * 4); }, wt);
+      __builtin_amdgcn_s_setprio(0);
 #pragma unroll
       for (int d = 0; d < kDT; ++d) {
         const halfx8 a0 = buf.v[d * 2][lane], a1 = buf.v[d * 2 + 1][lane];
