@@ -613,6 +613,48 @@ def test_offsets_past_32_bits():
     _check_attend(o, q, held, lens, None, 1, False, H=H)
 
 
+def test_rotary_backward_captured():
+    """A captured forward and backward is refused while an eager graph of its leaves lives; without one, every replay
+    equals the eager result."""
+    g = _gen(71)
+    sections, T = (16, 24, 24), 50
+    freq = _freq(sections, (10000.0, 100.0, 100.0)).cuda()
+    pos = torch.randint(0, 900, (1, T, 3), generator=g).cuda().int()
+    q, k = _randn(g, 1, 4, T, 64).cuda().requires_grad_(), _randn(g, 1, 2, T, 64).cuda().requires_grad_()
+    gq, gk = _randn(g, 1, 4, T, 64).cuda(), _randn(g, 1, 2, T, 64).cuda()
+
+    def both():
+        out = ops.rotary_axes(q, k, pos, sections, freq)
+        return [*(x.detach() for x in out), *torch.autograd.grad(out, (q, k), (gq, gk))]
+
+    eager = ops.rotary_axes(q, None, pos, sections, freq)[0]
+    refused = None
+    with torch.cuda.graph(torch.cuda.CUDAGraph()):
+        try:
+            ops.rotary_axes(q, k, pos, sections, freq)
+        except ValueError as e:
+            refused = str(e)
+    assert refused is not None and "eager graph" in refused
+    del eager
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        both()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = both()
+    for i in range(4):
+        with torch.no_grad():
+            for x in (q, k, gq, gk):
+                x.copy_(_randn(g, *x.shape))
+        graph.replay()
+        torch.cuda.synchronize()
+        want = both()
+        assert all(torch.equal(a, b) for a, b in zip(got, want)), i
+        torch.randn(1 << 16, device="cuda").sum().item()  # other work between replays
+
+
 # ------------------------------------------------------------------ a run of them
 def _step(cache, q, k, v, pos, table, start, lengths, freq, sections, block_q):
     q, k = ops.rotary_axes(q, k, pos, sections, freq)

@@ -127,3 +127,27 @@ def test_host_tensors_are_refused():
         BlockCache(4, 2, 96)
     with pytest.raises(ValueError, match="pages"):
         BlockCache(0, 2, 64)
+
+
+def test_captured_call_on_leaves_of_an_eager_graph(monkeypatch):
+    """The mark lives as long as the eager graph does, whichever of its tensors is let go first."""
+    capturing = [False]
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: capturing[0])
+    a, b = torch.ones(2, requires_grad=True), torch.ones(2, requires_grad=True)
+
+    def call(*leaves):
+        out = sum(leaves[1:], leaves[0] * 1)  # a graph over all of them
+        node = torch.cat(leaves).grad_fn
+        ops._one_graph(node)
+        return out, node
+
+    eager = call(a)
+    capturing[0] = True
+    call(b)
+    with pytest.raises(ValueError, match="eager graph"):
+        call(a, b)
+    eager = eager[0]  # the other node goes, the leaf's stays
+    with pytest.raises(ValueError, match="eager graph"):
+        call(a)
+    del eager
+    call(a, b)

@@ -814,6 +814,24 @@ class _RotaryAxes(torch.autograd.Function):
         return *turn(gq, gk, pos, ctx.sections, inv_freq, not ctx.inverse), None, None, None, None
 
 
+def _one_graph(node) -> None:
+    """Refuses a captured call on leaves that an eager call's live graph holds.
+
+    Both graphs share a leaf's accumulation node, whose stream is the eager
+    call's: the captured backward pass would wait for it from outside the
+    capture, which ends the process. The mark goes with the node, so it is
+    gone when the eager graph is.
+    """
+    captured = torch.cuda.is_current_stream_capturing()
+    for leaf, _ in node.next_functions:
+        if leaf is None or leaf.next_functions:
+            continue
+        if not captured:
+            leaf.metadata["eager"] = True
+        elif "eager" in leaf.metadata:
+            raise ValueError("q or k is a leaf of an eager graph that still lives: drop that call's outputs before capturing")
+
+
 @functools.lru_cache(maxsize=64)
 def _section_sizes(sections: tuple, D: int):
     """(the checked sections of a head dimension as a C array, their number, their pairs)."""
@@ -832,7 +850,8 @@ def rotary_axes(q: torch.Tensor, k: torch.Tensor | None, pos: torch.Tensor, sect
     ``pos * inv_freq``, whose float64 values ``[sum(sections)/2]`` hold the
     axes' frequencies one after another. Features past the sections pass
     through. Returns ``(q', k' or None)`` in the inputs' memory order;
-    differentiable in q and k.
+    differentiable in q and k. A captured call is refused while an eager
+    call's graph of the same leaves lives.
     """
     dev = _gpu(q, "q")
     dtype = q.dtype
@@ -865,7 +884,9 @@ def rotary_axes(q: torch.Tensor, k: torch.Tensor | None, pos: torch.Tensor, sect
     if not inv_freq.is_contiguous():
         inv_freq = inv_freq.contiguous()
     if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
-        return _RotaryAxes.apply(q, k, pos, sections, inv_freq, False)
+        out = _RotaryAxes.apply(q, k, pos, sections, inv_freq, False)
+        _one_graph(out[0].grad_fn)
+        return out
     return _rotary(q, k, pos, sections, inv_freq, False)
 
 
