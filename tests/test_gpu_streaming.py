@@ -6,7 +6,7 @@ import pytest
 import torch
 
 from oracle import streaming as O
-from vasc_amd import ops
+from vasc_amd import _lib, ops
 from vasc_amd.streaming import BlockCache
 
 pytestmark = pytest.mark.gpu
@@ -560,6 +560,55 @@ def test_attend_nan_tokens_and_queries(D, G, T, dtype):
     assert o2[0, G - 1, T - 1].isnan().all()
     o2[0, G - 1, T - 1] = o[0, G - 1, T - 1]
     assert torch.equal(o2, o)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("D,H,G,T,mp,parts", [(64, 1, 1, 1, 8, 1), (64, 64, 1, 1, 200, 8), (64, 1, 1, 1, 140, 35),
+                                              (128, 64, 20, 1, 200, 4), (128, 1, 20, 1, 140, 35), (64, 1, 1, 50, 8, 8),
+                                              (64, 1, 1, 100, 24, 24), (128, 1, 4, 30, 3, 3), (128, 1, 4, 30, 100, 100)])
+def test_attend_nan_in_split_pages(D, H, G, T, mp, parts, dtype):
+    """The pages of a unit on one workgroup or on some, joined a row a lane group or a row a workgroup: rows that see a NaN
+    token are NaN where it shares its part with others, fills it, fills the first parts or is all there is, and so are NaN
+    queries; every other row is as without them."""
+    block_q = max(1, min(T, 128 // G))
+    units = 2 * H * -(-T // block_q)
+    size = _lib.fn("vasc_cache_attn_workspace_size")(2, H * G, H, T, D, block_q, mp, 0)
+    assert size == (units * block_q * G * parts * (D + 2) * 4 if parts > 1 else 0)
+    g = _gen(D + T + mp)
+    table, pages = _table(g, 2, mp)
+    full = min(mp, 7) * 64
+    k, v = _randn(g, 2, H, full, D), _randn(g, 2, H, full, D)
+    q = _randn(g, 2, H * G, T, D, dtype=dtype).cuda()
+
+    def attend(bad, length, queries=q, **rule):
+        """With NaN in the tokens `bad` of the second sequence."""
+        cache = BlockCache(pages, H, D)
+        kn = k.clone()
+        kn[1, :, bad, 5] = float("nan")
+        ops.cache_write(cache, kn.cuda(), v.cuda(), table, _i32([0, 0]))
+        return ops.cache_attn(queries, cache, table, _i32([full, length]), **rule)
+
+    for bad, length in ((slice(70, 71), full), (slice(64, 128), full), (slice(0, full - 64), full), (slice(64, 65), 65),
+                        (slice(0, 1), 1), (slice(0, full), full)):
+        base, o = attend(slice(0, 0), length), attend(bad, length)
+        assert torch.equal(o[0], base[0]) and base.isfinite().all()
+        assert o[1].isnan().all(), (bad, length)
+        # masked for every row
+        cut = bad.start
+        assert torch.equal(attend(bad, cut), attend(slice(0, 0), cut)), (bad, cut)
+        if T > 1:  # the queries are the last T tokens: those before the first bad token do not see it
+            base, o = attend(slice(0, 0), length, causal=True), attend(bad, length, causal=True)
+            blind = min(max(0, bad.start - (length - T)), T)
+            assert torch.equal(o[0], base[0]) and torch.equal(o[1, :, :blind], base[1, :, :blind])
+            assert o[1, :, blind:].isnan().all(), (bad, length)
+    base = attend(slice(0, 0), full)
+    qn = q.clone()
+    qn[1, H * G - 1, T - 1, 3] = float("nan")
+    o = attend(slice(0, 0), full, qn)
+    assert o[1, H * G - 1, T - 1].isnan().all()
+    o[1, H * G - 1, T - 1] = base[1, H * G - 1, T - 1]
+    assert torch.equal(o, base)
+    assert not attend(slice(0, 0), 0, qn)[1].any()  # it sees no key
 
 
 def test_attend_wide_logits_and_scale():

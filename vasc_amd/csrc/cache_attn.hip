@@ -294,12 +294,13 @@ struct Rows {
     }
   }
 
-  // The lanes' sums joined; m: the reference, -inf for a row without a key.
+  // The lanes' sums joined; m: the reference, -inf for a row without a key, whose sums are zeros. Sums that only NaN has
+  // gone into have no reference (a maximum drops NaN), but are no empty row's: a join has to take them.
   __device__ __forceinline__ void finish(float (&m)[kTiles]) {
 #pragma unroll
     for (int i = 0; i < kTiles; ++i) {
       l[i] = row4_sum(l[i]);
-      m[i] = renew[i] == kUnset ? -__builtin_inff() : ref[i];
+      m[i] = renew[i] == kUnset && l[i] == l[i] ? -__builtin_inff() : ref[i];
       if (limit[i] == 0) {  // no key, or no row: pages that all counting rows see were not masked for it
         m[i] = -__builtin_inff();
         l[i] = 0.f;
