@@ -109,7 +109,8 @@ int64_t vasc_cache_attn_workspace_size(int64_t B, int64_t Hq, int64_t H, int64_t
  * Attention of q over the cache: o = softmax(scale * q k^T) v over the keys
  * of the listed pages (index NULL: of all pages) below lengths[b] (causal: at
  * or before the row's own position lengths[b] - q_count[b] + t). Rows that
- * see no key and rows past q_count[b] are zero. index [B,H,U,width], count
+ * see no key and rows past q_count[b] are zero; a row that sees a NaN token,
+ * or whose query is not finite, is NaN. index [B,H,U,width], count
  * [B,H,U] as vasc_cache_select writes them: ascending logical pages; entries
  * that are not above the one before, negative or not below max_pages are
  * skipped. block_q as there (index NULL: any block_q with block_q * G <= 128).

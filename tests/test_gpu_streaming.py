@@ -611,6 +611,31 @@ def test_attend_nan_in_split_pages(D, H, G, T, mp, parts, dtype):
     assert not attend(slice(0, 0), 0, qn)[1].any()  # it sees no key
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("D,G,T,mp", [(64, 1, 1, 6), (64, 1, 1, 140), (128, 20, 1, 6), (64, 1, 100, 6), (128, 4, 30, 140)])
+def test_attend_infinite_queries(D, G, T, mp, dtype):
+    """An infinite query has no softmax over any key, also where all its logits are minus infinity: its rows are NaN, or zero
+    where they see no key."""
+    g = _gen(D + T + mp)
+    L = 300
+    table, pages = _table(g, 1, mp)
+    cache = BlockCache(pages, 1, D)
+    k = _randn(g, 1, 1, L, D)
+    k[..., 7] = -k[..., 7].abs() - 0.25
+    held = _fill(cache, g, table, [L], k)
+    q = _randn(g, 1, G, T, D, dtype=dtype).cuda()
+    base = ops.cache_attn(q, cache, table, _i32([L]))
+    _check_attend(base, q, held, [L], None, 1, False, H=1)
+    for value in (float("inf"), -float("inf")):
+        bad = q.clone()
+        bad[0, 0, T - 1, 7] = value
+        o = ops.cache_attn(bad, cache, table, _i32([L]))
+        assert o[0, 0, T - 1].isnan().all()
+        o[0, 0, T - 1] = base[0, 0, T - 1]
+        assert torch.equal(o, base)
+        assert not ops.cache_attn(bad, cache, table, _i32([0])).any()
+
+
 def test_attend_wide_logits_and_scale():
     """Logits of hundreds: one key takes all; the running maximum moves many times; a scale of the caller's."""
     g = _gen(41)

@@ -164,7 +164,8 @@ __device__ __forceinline__ int row_limit(const AttnParams &p, const Work &w, int
   return static_cast<int>(own < w.cut ? (own > 0 ? own : 0) : w.cut);
 }
 
-// This lane's query operands of a row: [part][product]; zeros where there is no row.
+// This lane's query operands of a row: [part][product]; zeros where there is no row. An infinite query has no softmax, whatever
+// the sign of its logits, which a running maximum would not see where all of them are minus infinity: it goes as NaN.
 template <typename Q, int D, int kOps>
 __device__ __forceinline__ void query_operands(const AttnParams &p, const Work &w, int64_t t, int gh, bool live, int g,
                                                bf16x8 (&out)[kOps]) {
@@ -177,14 +178,17 @@ __device__ __forceinline__ void query_operands(const AttnParams &p, const Work &
       struct alignas(16) Eight { Q v[8]; };
       const Eight v = *reinterpret_cast<const Eight *>(src + (y >> 1) * 64 + (y & 1) * 8);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) x[e] = to_f32(v.v[e]);
+      for (int e = 0; e < 8; ++e) {
+        x[e] = to_f32(v.v[e]);
+        if (!__builtin_isfinite(x[e])) x[e] = __builtin_nanf("");
+      }
     }
 #pragma unroll
     for (int piece = 0; piece < kParts; ++piece)
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         out[piece * kMul + y][e] = static_cast<__bf16>(x[e]);
-        if (kParts > 1 && __builtin_isfinite(x[e])) x[e] -= static_cast<float>(out[piece * kMul + y][e]);
+        if (kParts > 1) x[e] -= static_cast<float>(out[piece * kMul + y][e]);
       }
   }
 }

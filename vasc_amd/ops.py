@@ -1028,7 +1028,8 @@ def cache_attn(q: torch.Tensor, cache, page_table: torch.Tensor, lengths: torch.
     is skipped); without them every page is attended to. Keys at or past
     ``lengths[b]`` are not seen, nor, with ``causal``, those behind the row's
     own position ``lengths[b] - q_count[b] + t``. Rows that see no key, and
-    rows from ``q_count[b]`` on, are zero. Softmax scale ``scale`` (default
+    rows from ``q_count[b]`` on, are zero; rows that see a NaN token, or whose
+    query is not finite, are NaN. Softmax scale ``scale`` (default
     ``D ** -0.5``). Returns ``[B,Hq,T,D]`` of q's dtype, written to ``out``
     when given (unit stride over D).
     """
