@@ -1,5 +1,7 @@
 """The streaming operators against their definitions in float64 (oracle/streaming.py)."""
+import copy
 import math
+import pickle
 
 import numpy as np
 import pytest
@@ -667,6 +669,33 @@ def test_attend_strided_tensors_and_out():
     _check_attend(o, q, held, [L, L - 9], None, 1, False, H=H)
     again = ops.cache_attn(q, cache, wide[:, :6], torch.tensor([L, L - 9], device="cuda"))  # int64 lengths
     assert torch.equal(again, o)
+
+
+@pytest.mark.parametrize("how", ["deepcopy", "copy", "pickle", "save"])
+def test_copied_cache(how, tmp_path):
+    """A deep copy, a pickled and a saved cache have buffers of their own, at their own addresses; a shallow copy shares them."""
+    g = _gen(59)
+    table, pages = _table(g, 1, 3)
+    cache = BlockCache(pages, 2, 64)
+    held = _fill(cache, g, table, [100])
+    if how == "save":
+        torch.save(cache, tmp_path / "cache")
+        other = torch.load(tmp_path / "cache", weights_only=False)
+    else:
+        other = {"deepcopy": copy.deepcopy, "copy": copy.copy, "pickle": lambda c: pickle.loads(pickle.dumps(c))}[how](cache)
+    buffers = ("kc", "vc", "ks", "vs")
+    assert other.pointers == tuple(getattr(other, n).data_ptr() for n in buffers)
+    assert other.mean_pointer == other.mean.data_ptr() and other.device_index == cache.device_index
+    assert (other.pointers == cache.pointers) == (how == "copy")
+    more = _randn(g, 1, 2, 30, 64).cuda()
+    before = {n: getattr(cache, n).clone() for n in (*buffers, "mean")}
+    ops.cache_write(other, more, more, table, _i32([100]))
+    assert all(torch.equal(getattr(cache, n), t) for n, t in before.items()) == (how != "copy")
+    q = _randn(g, 1, 2, 1, 64).cuda()
+    new = O.quantise(_np(more[0]), _np(more[0]))
+    both = [tuple(np.concatenate([a, b], 1) for a, b in zip(held[0], new))]
+    _check_attend(ops.cache_attn(q, other, table, _i32([130])), q, both, [130], None, 1, False, H=2)
+    _check_attend(ops.cache_attn(q, cache, table, _i32([100])), q, held, [100], None, 1, False, H=2)
 
 
 def test_offsets_past_32_bits():

@@ -1,6 +1,8 @@
 """What the streaming operators refuse, on the CPU: host tensors, and bad arguments at the C boundary (which returns
 before it touches a pointer)."""
+import copy
 import ctypes
+import pickle
 
 import pytest
 import torch
@@ -151,3 +153,19 @@ def test_captured_call_on_leaves_of_an_eager_graph(monkeypatch):
         call(a)
     del eager
     call(a, b)
+
+
+def test_copied_cache_has_addresses_of_its_own(tmp_path):
+    """A copy, a pickle or a saved cache never keeps the original's addresses: on the host it is refused (its buffers are no
+    GPU's), on a GPU they are its own buffers'."""
+    cache = BlockCache.__new__(BlockCache)
+    for name in ("_kc", "_vc", "_ks", "_vs", "_mean"):
+        setattr(cache, name, torch.zeros(2, 1, 64, 64))
+    cache.pages, cache.heads, cache.head_dim = 2, 1, 64
+    cache.device_index, cache.pointers, cache.mean_pointer = 0, (1, 2, 3, 4), 5
+    for again in (copy.deepcopy, copy.copy, lambda c: pickle.loads(pickle.dumps(c))):
+        with pytest.raises(ValueError, match="GPU"):
+            again(cache)
+    torch.save(cache, tmp_path / "cache")
+    with pytest.raises(ValueError, match="GPU"):
+        torch.load(tmp_path / "cache", weights_only=False)

@@ -46,10 +46,20 @@ class BlockCache:
         self._ks = torch.zeros(pages, heads, page, **u8)
         self._vs = torch.zeros(pages, heads, page, **u8)
         self._mean = torch.zeros(pages, heads, head_dim, device=device, dtype=torch.bfloat16)
+        self._locate()
+
+    def _locate(self) -> None:
+        """The buffers stay where they are, so a call need not ask for their addresses again."""
+        if not self._kc.is_cuda:
+            raise ValueError("the block cache lives on a GPU (the HIP path has no CPU fallback)")
         self.device_index = self._kc.get_device()
-        # the buffers stay where they are, so a call need not ask for their addresses again
         self.pointers = tuple(t.data_ptr() for t in (self._kc, self._vc, self._ks, self._vs))
         self.mean_pointer = self._mean.data_ptr()
+
+    def __setstate__(self, state: dict) -> None:
+        """A copy or an unpickled cache: the state's addresses are the original's."""
+        self.__dict__.update(state)
+        self._locate()
 
     kc = property(lambda self: self._kc)
     vc = property(lambda self: self._vc)
