@@ -141,6 +141,34 @@ def test_rotary_gradients(dtype):
     assert (np.abs(_np(dq) - ref) <= _rotary_bound(torch.ones(q.shape), ref, sections, dtype)).all()
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+def test_rotary_tangents(dtype):
+    """A forward-mode tangent is the turn of the tangent, bit for bit; the cache operators refuse one."""
+    import torch.autograd.forward_ad as fwd
+    g = _gen(13)
+    sections, T = (16, 24, 24), 21
+    freq = _freq(sections, (10000.0, 100.0, 100.0)).cuda()
+    pos = torch.randint(0, 900, (2, T, 3), generator=g).cuda()
+    q, tq = (_randn(g, 2, T, 4, 64, dtype=dtype).cuda().transpose(1, 2) for _ in range(2))
+    k, tk = (_randn(g, 2, 2, T, 64, dtype=dtype).cuda() for _ in range(2))
+    want = ops.rotary_axes(tq, tk, pos, sections, freq)
+    plain = ops.rotary_axes(q, k, pos, sections, freq)
+    with fwd.dual_level():
+        for grad in (False, True):
+            out = ops.rotary_axes(fwd.make_dual(q.clone().requires_grad_(grad), tq), fwd.make_dual(k, tk), pos, sections, freq)
+            for x, t, p in zip(out, want, plain):
+                x = fwd.unpack_dual(x)
+                assert torch.equal(x.primal, p) and torch.equal(x.tangent, t)
+        qo, ko = ops.rotary_axes(q, fwd.make_dual(k, tk), pos, sections, freq)
+        assert torch.equal(fwd.unpack_dual(ko).tangent, want[1]) and not fwd.unpack_dual(qo).tangent.any()
+        if dtype != torch.float32:
+            cache, table = BlockCache(1, 2, 64), _i32([[0], [0]])
+            with torch.no_grad(), pytest.raises(ValueError, match="tangent"):
+                ops.cache_attn(fwd.make_dual(q, tq), cache, table, _i32([0, 0]))
+            with pytest.raises(ValueError, match="tangent"):
+                ops.cache_write(cache, k, fwd.make_dual(k, tk), table, _i32([0, 0]))
+
+
 def test_rotary_odd_strides_and_empty():
     """Rows that start at odd elements, a transposed layout, no tokens, no heads."""
     g = _gen(5)

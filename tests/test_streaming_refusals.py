@@ -6,9 +6,11 @@ import pickle
 
 import pytest
 import torch
+import torch.autograd.forward_ad as fwd
 
+from oracle import streaming as O
 from vasc_amd import _lib, ops
-from vasc_amd.streaming import BlockCache
+from vasc_amd.streaming import BlockCache, stream_attention
 
 FAKE = 1 << 20  # an aligned address that nothing reads
 
@@ -169,3 +171,66 @@ def test_copied_cache_has_addresses_of_its_own(tmp_path):
     torch.save(cache, tmp_path / "cache")
     with pytest.raises(ValueError, match="GPU"):
         torch.load(tmp_path / "cache", weights_only=False)
+
+
+def _host_rotary(monkeypatch):
+    """rotary_axes on the host: the checks and the autograd function as they are, the launch in torch."""
+    def turn(q, k, pos, sections, inv_freq, inverse):
+        out = []
+        for x in (q, k):
+            y = None if x is None else torch.from_numpy(O.rotate(x.detach().numpy(), pos.numpy(), sections, inv_freq.detach().numpy(),
+                                                                 -1.0 if inverse else 1.0)).to(x.dtype)
+            out.append(y)
+        return tuple(out)
+
+    monkeypatch.setattr(ops, "_gpu", lambda t, name, dev=-1: 0)
+    monkeypatch.setattr(ops, "_rotary", turn)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    g = torch.Generator().manual_seed(0)
+    q, k, tq, tk = (torch.randn(2, 3, 5, 8, generator=g) for _ in range(4))
+    pos = torch.randint(0, 9, (1, 5, 2), generator=g, dtype=torch.int32).expand(2, 5, 2)
+    return turn, q, k, tq, tk, pos, (2, 4), torch.tensor([1.0, 0.5, 0.25], dtype=torch.float64)
+
+
+def test_rotary_carries_forward_tangents(monkeypatch):
+    """A dual tensor's tangent takes the same turn, with and without gradients; an input without one adds zeros."""
+    turn, q, k, tq, tk, pos, sections, freq = _host_rotary(monkeypatch)
+    want_q, want_k = turn(tq, tk, pos, sections, freq, False)
+
+    def tangents(q, k):
+        return [None if x is None else fwd.unpack_dual(x).tangent for x in ops.rotary_axes(q, k, pos, sections, freq)]
+
+    with fwd.dual_level():
+        for grad in (False, True):
+            a, b = (x.clone().requires_grad_(grad) for x in (q, k))
+            got = tangents(fwd.make_dual(a, tq), fwd.make_dual(b, tk))
+            assert torch.equal(got[0], want_q) and torch.equal(got[1], want_k)
+            got = tangents(a, fwd.make_dual(b, tk))
+            assert not got[0].any() and torch.equal(got[1], want_k)
+            got = tangents(fwd.make_dual(a, tq), None)
+            assert torch.equal(got[0], want_q) and got[1] is None
+            with torch.no_grad():
+                assert torch.equal(tangents(fwd.make_dual(a, tq), b)[0], want_q)
+        t = tq.clone().requires_grad_()  # a derivative of the tangent: the opposite turn
+        out = tangents(fwd.make_dual(q, t), k)[0]
+        back, = torch.autograd.grad(out, t, tk)
+        assert torch.equal(back, turn(tk, None, pos, sections, freq, True)[0])
+
+
+def test_derivatives_that_are_refused(monkeypatch):
+    _, q, k, tq, _, pos, sections, freq = _host_rotary(monkeypatch)
+    with pytest.raises(ValueError, match="inv_freq"):
+        ops.rotary_axes(q, k, pos, sections, freq.clone().requires_grad_())
+    with torch.no_grad():
+        ops.rotary_axes(q, k, pos, sections, freq.clone().requires_grad_())
+    with fwd.dual_level():
+        with pytest.raises(ValueError, match="inv_freq"):
+            ops.rotary_axes(q, k, pos, sections, fwd.make_dual(freq, freq))
+        for grad in (True, False):  # the block cache has no derivative of either kind
+            with torch.set_grad_enabled(grad), pytest.raises(ValueError, match="tangent"):
+                ops._inference(fwd.make_dual(q, tq), "q")
+        ops._inference(q, "q")
+        with pytest.raises(ValueError, match="tangent"):
+            stream_attention(None, fwd.make_dual(q, tq), None, None, None, None, None, keep=None)
+    with pytest.raises(ValueError, match="gradient"):
+        ops._inference(q.requires_grad_(), "q")

@@ -12,6 +12,7 @@ import math
 
 import numpy as np
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -694,10 +695,17 @@ def _gpu(t, name: str, dev: int = -1) -> int:
     return at
 
 
+def _tangent(t: torch.Tensor) -> bool:
+    """Whether ``t`` carries a forward-mode tangent (the level is -1 where nothing does)."""
+    return forward_ad._current_level >= 0 and forward_ad.unpack_dual(t).tangent is not None
+
+
 def _inference(t: torch.Tensor, name: str) -> None:
     if t.requires_grad and torch.is_grad_enabled():
         raise ValueError(f"{name} requires a gradient: the block cache has no backward pass, "
                          "call it under torch.no_grad()")
+    if _tangent(t):
+        raise ValueError(f"{name} carries a forward-mode tangent: the block cache has no derivative")
 
 
 def _rows8(t: torch.Tensor, name: str, dtypes: tuple) -> tuple:
@@ -794,11 +802,14 @@ def _rotary(q, k, pos, sections, inv_freq, inverse: bool) -> tuple:
 
 
 class _RotaryAxes(torch.autograd.Function):
-    """A turn is orthogonal: its gradient is the opposite turn of the gradient, which is differentiable in turn."""
+    """A turn is orthogonal: its gradient is the opposite turn of the gradient, which is differentiable in turn. It is linear:
+    its tangent is the same turn of the tangent."""
 
     @staticmethod
     def forward(ctx, q, k, pos, sections, inv_freq, inverse):
         ctx.save_for_backward(pos, inv_freq)
+        if forward_ad._current_level >= 0:
+            ctx.primals = q, k, pos, inv_freq
         ctx.sections, ctx.inverse = sections, inverse
         ctx.set_materialize_grads(False)
         return _rotary(q, k, pos, sections, inv_freq, inverse)
@@ -812,6 +823,15 @@ class _RotaryAxes(torch.autograd.Function):
         if gq is None:
             return None, turn(gk, None, pos, ctx.sections, inv_freq, not ctx.inverse)[0], None, None, None, None
         return *turn(gq, gk, pos, ctx.sections, inv_freq, not ctx.inverse), None, None, None, None
+
+    @staticmethod
+    def jvp(ctx, tq, tk, *_):
+        q, k, pos, inv_freq = ctx.primals
+        del ctx.primals
+        tq = torch.zeros_like(q) if tq is None else tq
+        tk = torch.zeros_like(k) if tk is None and k is not None else tk
+        turn = _RotaryAxes.apply if torch.is_grad_enabled() else _rotary
+        return turn(tq, tk, pos, ctx.sections, inv_freq, ctx.inverse)
 
 
 def _one_graph(node) -> None:
@@ -850,7 +870,7 @@ def rotary_axes(q: torch.Tensor, k: torch.Tensor | None, pos: torch.Tensor, sect
     ``pos * inv_freq``, whose float64 values ``[sum(sections)/2]`` hold the
     axes' frequencies one after another. Features past the sections pass
     through. Returns ``(q', k' or None)`` in the inputs' memory order;
-    differentiable in q and k. A captured call is refused while an eager
+    differentiable in q and k, backward and forward. A captured call is refused while an eager
     call's graph of the same leaves lives.
     """
     dev = _gpu(q, "q")
@@ -883,9 +903,14 @@ def rotary_axes(q: torch.Tensor, k: torch.Tensor | None, pos: torch.Tensor, sect
         raise ValueError(f"inv_freq must hold {pairs} float64 values, got {inv_freq.dtype} {tuple(inv_freq.shape)}")
     if not inv_freq.is_contiguous():
         inv_freq = inv_freq.contiguous()
-    if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
+    grad = torch.is_grad_enabled()
+    if (grad and inv_freq.requires_grad) or _tangent(inv_freq):
+        raise ValueError("inv_freq requires a gradient or carries a tangent: rotary_axes is differentiable in q and k only")
+    grad = grad and (q.requires_grad or (k is not None and k.requires_grad))
+    if grad or forward_ad._current_level >= 0:
         out = _RotaryAxes.apply(q, k, pos, sections, inv_freq, False)
-        _one_graph(out[0].grad_fn)
+        if grad:
+            _one_graph(out[0].grad_fn)
         return out
     return _rotary(q, k, pos, sections, inv_freq, False)
 

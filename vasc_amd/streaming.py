@@ -111,6 +111,7 @@ def stream_attention(attn, x: torch.Tensor, pos: torch.Tensor | None, cache: Blo
     that a block of patch queries chooses beside the first ``sink`` and the
     last ``recent``; None: all. Returns ``[B,T,dim]``. No gradients.
     """
+    ops._inference(x, "x")
     B, T, dim = x.shape
     if frames < 1 or T < 1 or T % frames or not 0 <= special <= T // frames:
         raise ValueError(f"{T} tokens are not {frames} frames with {special} special tokens each")
