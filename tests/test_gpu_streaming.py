@@ -680,6 +680,39 @@ def test_attend_wide_logits_and_scale():
         _check_attend(o, q, held, [L], None, 1, False, scale=scale, H=1)
 
 
+@pytest.mark.parametrize("L,apart", [(400, 7), (400, -56), (20000, 18)])
+@pytest.mark.parametrize("D,G,T,wide", [(64, 1, 1, False), (64, 1, 1, True), (128, 20, 1, False), (64, 1, 40, False),
+                                        (64, 2, 60, True), (128, 4, 30, False)])
+def test_attend_values_far_apart(L, apart, D, G, T, wide):
+    """One key whose value row is at the exponents' upper end, `apart` powers of two more likely than all the others, whose
+    rows are zero or at the lower end: they count in the softmax's sum with all their weight (300 of 2^-7 are 3 times the one,
+    20000 of 2^-18 are 7 % of it). It is the first key, the last, or in the middle; pages on one workgroup or split."""
+    mp = -(-L // 64) + (140 if wide else 0)
+    g = _gen(L)
+    table, pages = _table(g, 4, mp)
+    q = torch.zeros(4, G, T, D, dtype=torch.bfloat16)
+    q[..., 0] = 1.0
+    k, v = torch.zeros(4, 1, L, D), torch.zeros(4, 1, L, D)
+    for b, at in enumerate((0, L // 2 + 5, L - 1, 70)):
+        k[b, 0, at, 0] = apart
+        v[b, 0, :, 1] = 0.0 if b % 2 else 448 * 2.0 ** -60
+        v[b, 0, at] = torch.linspace(224, 448, 8).repeat(D // 8) * 2.0 ** 60
+        v[b, 0, at, 1] = -448 * 2.0 ** 60
+    cache = BlockCache(pages, 1, D)
+    ops.cache_write(cache, k.cuda(), v.cuda(), table, _i32([0] * 4))
+    hk, hv = ops.cache_read(cache, table, _i32([0] * 4), L, dtype=torch.float32)
+    assert torch.equal(hk.cpu(), k) and torch.equal(hv.cpu(), v)  # all of it is what 8 bits hold
+    held = [(_np(k[b]), _np(v[b])) for b in range(4)]
+    o = ops.cache_attn(q.cuda(), cache, table, _i32([L] * 4), scale=math.log(2.0))
+    _check_attend(o[:, :1, :1], q[:, :1, :1], held, [L] * 4, None, 1, False, scale=math.log(2.0), H=1)
+    assert (o == o[:, :1, :1]).all()
+    lists = torch.arange(-(-L // 64), dtype=torch.int32, device="cuda")[1:].expand(4, 1, T, -1)
+    count = _i32([lists.shape[3]]).expand(4, 1, T)
+    o = ops.cache_attn(q.cuda(), cache, table, _i32([L] * 4), lists, count, block_q=1, scale=math.log(2.0))
+    _check_attend(o[:, :1, :1], q[:, :1, :1], held, [L] * 4, [[[list(range(1, -(-L // 64)))]]] * 4, 1, False,
+                  scale=math.log(2.0), H=1)
+
+
 def test_attend_strided_tensors_and_out():
     g = _gen(43)
     D, H, T, L = 64, 2, 6, 333

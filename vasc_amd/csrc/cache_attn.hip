@@ -21,6 +21,13 @@
 // are held in half (11 bits; bfloat16's 8 would be the largest error of a
 // float16 result) up to 2^15, and those below its range are under 2^-36 of the
 // row's largest.
+//
+// A key whose value row is small may be lost in the second product and yet be
+// most of l: its w = 2^(e - ref) may lie under float32's 2^-126. With every
+// exponent at -30 or more, what is lost of l is below 2^-47 of it a key (w of
+// the row's largest is 2^11, its part of l 2^(11 - ev), ev at most 60). Pages
+// that hold a smaller one (rows of zeros have -60) take w 2^60 and 2^(-60 - ev)
+// for l instead, an exponential more a key; and l is scaled in two factors.
 #include <cmath>
 
 #include "stream.h"
@@ -29,6 +36,7 @@ namespace vasc {
 namespace {
 
 constexpr float kHeadroom = 11.f, kSlack = 4.f;  // kHeadroom + kSlack < 16: half's largest exponent
+constexpr uint32_t kSmall = 127 - 30;            // exponent bytes from 67 to below it are small; 0 is a slot that was never written
 
 struct AttnParams {
   const void *q;
@@ -81,6 +89,12 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   float r;  // three operands at once; a NaN gives way to a number, as with fmaxf
   asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
   return r;
+}
+
+// 2^d, d <= 0, as near * far: d may lie under -126 where a sum is scaled. far is 1 for d from -120 on.
+__device__ __forceinline__ void two_powers(float d, float &near, float &far) {
+  near = __builtin_amdgcn_exp2f(fmaxf(d, -120.f));
+  far = __builtin_amdgcn_exp2f(fminf(d + 120.f, 0.f));
 }
 
 // The four lanes l, l ^ 16, l ^ 32, l ^ 48 share a query row.
@@ -232,9 +246,9 @@ struct Rows {
   }
 
   // Exponents of a page's keys (key t * 16 + g * 4 + j in s[x][t][j]) -> weights as the second product's operands;
-  // un(t): the opposite powers of the values of keys t * 16 + g * 4 ...
+  // un(t): the opposite powers of the values of keys t * 16 + g * 4 ...; small (the wave's): one of the page's is small.
   template <typename Un>
-  __device__ __forceinline__ void weights(floatx4 (&s)[kTiles][4], int page, int g, float inv_c, Un un,
+  __device__ __forceinline__ void weights(floatx4 (&s)[kTiles][4], int page, int g, float inv_c, bool small, Un un,
                                           halfx8 (&w)[kTiles][2]) {
     if (page < 0 || page * kPage + kPage > low) {
 #pragma unroll
@@ -262,8 +276,11 @@ struct Rows {
       for (int x = 0; x < kTiles; ++x) {
         const bool need = top[x] > renew[x];
         const float by = need ? top[x] - kHeadroom : 0.f;
-        const float a = need && renew[x] != kUnset ? __builtin_amdgcn_exp2f(-by) : 1.f;
-        l[x] *= a;
+        const bool scales = need && renew[x] != kUnset;
+        const float a = scales ? __builtin_amdgcn_exp2f(-by) : 1.f;
+        float near, far;
+        two_powers(scales ? -by : 0.f, near, far);
+        l[x] = l[x] * near * far;
 #pragma unroll
         for (int d = 0; d < kDT; ++d) acc[x][d] *= a;
 #pragma unroll
@@ -276,6 +293,19 @@ struct Rows {
       }
     }
     uint32_t packed[kTiles][8];
+    float exact[kTiles];
+    if (__builtin_expect(small, false)) {
+#pragma unroll
+      for (int x = 0; x < kTiles; ++x) exact[x] = l[x];
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        const floatx4 power = un(t) * 0x1p-60f;
+#pragma unroll
+        for (int x = 0; x < kTiles; ++x)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) exact[x] = fmaf(__builtin_amdgcn_exp2f(s[x][t][j] + 60.f), power[j], exact[x]);
+      }
+    }
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
       const floatx4 power = un(t);
@@ -290,6 +320,10 @@ struct Rows {
         packed[x][t * 2] = pack_half2(e[0], e[1]);
         packed[x][t * 2 + 1] = pack_half2(e[2], e[3]);
       }
+    }
+    if (__builtin_expect(small, false)) {
+#pragma unroll
+      for (int x = 0; x < kTiles; ++x) l[x] = exact[x];
     }
 #pragma unroll
     for (int x = 0; x < kTiles; ++x) {
@@ -453,7 +487,12 @@ __global__ __launch_bounds__(256, 2) void cache_attn_few_kernel(const AttnParams
         }
       }
       halfx8 wt[kTiles][2];
-      rows.weights(s, lpage, g, inv_c, [&](int t) {
+      // bytes up to 187: 67 and more have a top bit with 0x3d, kSmall and more with 0x1f
+      static_assert(kSmall + 0x1f == 128, "the bytes' test");
+      uint32_t top = 0;
+#pragma unroll
+      for (int t = 0; t < 4; ++t) top |= (vb[t] + 0x3d3d3d3du) & ~(vb[t] + 0x1f1f1f1fu);
+      rows.weights(s, lpage, g, inv_c, __ballot(top & 0x80808080u) != 0, [&](int t) {
         const uint32_t iw = 0xfefefefeu - vb[t];  // the opposite powers
         return floatx4{pow2_byte(iw & 255u), pow2_byte((iw >> 8) & 255u), pow2_byte((iw >> 16) & 255u), pow2_byte(iw >> 24)};
       }, wt);
@@ -497,7 +536,9 @@ __global__ __launch_bounds__(256, 2) void cache_attn_few_kernel(const AttnParams
 #pragma unroll
     for (int x = 1; x < kWaves; ++x) mx = fmaxf(mx, others[x - 1][i * 16 + col][D]);
     const float a = m[i] == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(m[i] - mx);
-    rows.l[i] *= a;
+    float near, far;
+    two_powers(m[i] == -__builtin_inff() ? 0.f : m[i] - mx, near, far);
+    rows.l[i] = rows.l[i] * near * far;
 #pragma unroll
     for (int d = 0; d < kDT; ++d) rows.acc[i][d] *= a;
 #pragma unroll
@@ -505,7 +546,8 @@ __global__ __launch_bounds__(256, 2) void cache_attn_few_kernel(const AttnParams
       const float *src = others[x - 1][i * 16 + col];
       const float mo = src[D];
       const float c = mo == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(mo - mx);
-      rows.l[i] = fmaf(src[D + 1], c, rows.l[i]);
+      two_powers(mo == -__builtin_inff() ? 0.f : mo - mx, near, far);
+      rows.l[i] = fmaf(src[D + 1] * far, near, rows.l[i]);
 #pragma unroll
       for (int d = 0; d < kDT; ++d)
 #pragma unroll
@@ -536,6 +578,7 @@ __global__ __launch_bounds__(kWaves * 64, D == 64 && kWaves == 4 ? 3 : 2) void c
     bf16x8 k[4 * kMul][64];
     halfx8 v[kDT * 2][64];
     float ev[kPage], un[kPage];
+    int small;
   };
   __shared__ __align__(16) Page buffer[2];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -601,6 +644,8 @@ __global__ __launch_bounds__(kWaves * 64, D == 64 && kWaves == 4 ? 3 : 2) void c
       if (wave == 0) {
         buf.ev[lane] = static_cast<float>(vb);  // the bias of 127 goes with the reference
         buf.un[lane] = pow2_byte(254u - vb);
+        const uint64_t small = __ballot(vb - 1u < kSmall - 1u);
+        if (lane == 0) buf.small = small != 0;
       }
       __syncthreads();
       if (i + 1 < n) load(i + 1);
@@ -634,7 +679,7 @@ __global__ __launch_bounds__(kWaves * 64, D == 64 && kWaves == 4 ? 3 : 2) void c
           for (int j = 0; j < 4; ++j) s[x][t][j] = fmaf(s[x][t][j], p.c, ev[j]);
       }
       halfx8 wt[kTiles][2];
-      rows.weights(s, lpage, g, inv_c,
+      rows.weights(s, lpage, g, inv_c, __builtin_amdgcn_readfirstlane(buf.small),
                    [&](int t) { return *reinterpret_cast<const floatx4 *>(buf.un + g * 16 + t * 4); }, wt);
       __builtin_amdgcn_s_setprio(0);
 #pragma unroll
@@ -690,14 +735,15 @@ __global__ __launch_bounds__(256) void cache_join_kernel(const AttnParams p) {
     }
     const float top = fmaxf(mx, fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])));
     if (top == -__builtin_inff()) continue;
-    const float c = __builtin_amdgcn_exp2f(mx - top);
-    l *= c;
-    acc *= c;
+    float near, far;
+    two_powers(mx - top, near, far);
+    l = l * near * far;
+    acc *= __builtin_amdgcn_exp2f(mx - top);
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
-      const float w = __builtin_amdgcn_exp2f(m[k] - top);
-      l = fmaf(ls[k], w, l);
-      acc += x[k] * w;
+      two_powers(m[k] - top, near, far);
+      l = fmaf(ls[k] * far, near, l);
+      acc += x[k] * __builtin_amdgcn_exp2f(m[k] - top);
     }
     mx = top;
   }
@@ -714,13 +760,15 @@ __global__ __launch_bounds__(256) void cache_join_kernel(const AttnParams p) {
 #pragma unroll
     for (int i = 1; i < kGroups; ++i) top = fmaxf(top, sums[i][D]);
     if (top > -__builtin_inff()) {
-      const float c = __builtin_amdgcn_exp2f(mx - top);
-      l *= c;
-      acc *= c;
+      float near, far;
+      two_powers(mx - top, near, far);
+      l = l * near * far;
+      acc *= __builtin_amdgcn_exp2f(mx - top);
 #pragma unroll
       for (int i = 1; i < kGroups; ++i) {
         const float w = __builtin_amdgcn_exp2f(sums[i][D] - top);
-        l = fmaf(sums[i][D + 1], w, l);
+        two_powers(sums[i][D] - top, near, far);
+        l = fmaf(sums[i][D + 1] * far, near, l);
 #pragma unroll
         for (int j = 0; j < 4; ++j) acc[j] = fmaf(sums[i][d + j], w, acc[j]);
       }
