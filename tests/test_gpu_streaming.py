@@ -997,6 +997,52 @@ def test_dense_layer_with_three_axes():
         assert ((y.float() - ref).abs() <= bound + 2.0 ** -8 * (ref.abs() + bound) + 1e-4).all()
 
 
+@pytest.mark.parametrize("params", [torch.float32, torch.float16])
+def test_axes_rope_with_norms_of_another_type(params):
+    """Norm parameters that are not bf16 go with either rope: normed and turned in float32, rounded to bf16 once, on both sides
+    (half a step each, and float32's share as in _rotary_bound and a norm of 64 terms). Dense, sparse and streamed layers."""
+    from vasc_amd.aggregator import Attention, RotaryPositionEmbedding2D, RotaryPositionEmbeddingAxes
+    from vasc_amd.attention import adaptive_sparse_attention_forward
+    from vasc_amd.streaming import _layer_qkv, stream_attention
+    g = _gen(79)
+    torch.manual_seed(3)
+    m = Attention(256, 4).cuda()
+    m.q_norm, m.k_norm = (torch.nn.LayerNorm(64, eps=1e-6).cuda().to(params) for _ in range(2))
+    with torch.no_grad():
+        for n in (m.q_norm, m.k_norm):
+            n.weight.normal_(1.0, 0.2)
+            n.bias.normal_(0.0, 0.2)
+    B, P = 2, 6 * 7
+    x = torch.randn(B, 2 * P, 256, generator=g).cuda()
+    cell = torch.arange(P)
+    pos = torch.stack([cell // 7 + 1, cell % 7 + 1], -1).repeat(B, 2, 1).cuda()
+    got = {}
+    for name, rope in (("table", RotaryPositionEmbedding2D(100.0)), ("axes", RotaryPositionEmbeddingAxes((32, 32), 100.0))):
+        m.rope = rope
+        with torch.no_grad():
+            got[name] = _layer_qkv(m, x, pos, 2, 0)
+    for a, b in zip(got["axes"], got["table"]):
+        if a is not None:
+            a, b = a.float(), b.float()
+            side = 2.0 ** -18 * (a.abs() + a.roll(16, -1).abs() + a.roll(-16, -1).abs() + 1)
+            assert ((a - b).abs() <= 2 * 2.0 ** -8 * torch.maximum(a.abs(), b.abs()) + side).all()
+    q, _, k, v = (None if t is None else t.float() for t in got["axes"])
+    p = torch.softmax((q @ k.transpose(2, 3).contiguous()) / 8, -1)
+    o = p @ v
+    slack = 2.0 ** -8 * (p @ v.abs()) + 2.0 ** -8 * o.abs()  # as for three axes
+    with torch.no_grad():
+        w = m.proj.weight
+        flat = lambda t: t.transpose(1, 2).reshape(B, 2 * P, 256)  # noqa: E731
+        ref, bound = flat(o) @ w.T.contiguous() + m.proj.bias, flat(slack) @ w.T.contiguous().abs() + 1e-4
+        assert ((m(x, pos=pos) - ref).abs() <= bound).all()
+        sparse = adaptive_sparse_attention_forward(m, x, pos, sparse_ratio=0.0, num_special_tokens=0, num_heads=4)
+        sparse = sparse[0] if isinstance(sparse, tuple) else sparse
+        assert ((sparse - ref).abs() <= bound).all()
+        cache = BlockCache(4, 4, 64)
+        y = stream_attention(m, x, pos, cache, _i32([[0, 1], [2, 3]]), _i32([0, 0]), _i32([2 * P] * 2), keep=None, frames=2)
+    assert y.dtype == torch.float32 and y.isfinite().all()
+
+
 @pytest.mark.parametrize("axes", [2, 3])
 def test_aggregator_stream(axes):
     """Pushes run, repeat after reset bit for bit, do not see stale cache contents, and refuse what does not fit."""

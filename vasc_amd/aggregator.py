@@ -118,6 +118,18 @@ class RotaryPositionEmbeddingAxes(nn.Module):
         return self.rotate(tokens, None, positions)[0]
 
 
+def head_norm(norm: nn.Module, rows: torch.Tensor) -> torch.Tensor:
+    """``norm(rows)`` of bf16 head rows outside the layout kernel. A LayerNorm
+    whose parameters are of another type, which torch refuses to mix with bf16
+    rows, runs in float32 as in that kernel and returns float32."""
+    if isinstance(norm, nn.LayerNorm):
+        params = (norm.weight, norm.bias)
+        if any(t is not None and t.dtype != rows.dtype for t in params):
+            return nn.functional.layer_norm(rows.float(), norm.normalized_shape,
+                                            *(None if t is None else t.float() for t in params), norm.eps)
+    return norm(rows)
+
+
 class Attention(nn.Module):
     """Multi-head attention of the VGGT/Pi3 blocks (qk-norm, 2D RoPE, or RoPE over more axes)."""
 
@@ -139,7 +151,7 @@ class Attention(nn.Module):
         H, D = self.num_heads, self.head_dim
         qkv = self.qkv(x).to(torch.bfloat16).view(B, T, 3, H, D)
         if isinstance(self.rope, RotaryPositionEmbeddingAxes):
-            qp, k = self.q_norm(qkv[:, :, 0].transpose(1, 2)), self.k_norm(qkv[:, :, 1].transpose(1, 2))
+            qp, k = (head_norm(n, qkv[:, :, i].transpose(1, 2)) for i, n in enumerate((self.q_norm, self.k_norm)))
             if pos is not None:
                 qp, k = self.rope.rotate(qp, k.to(qp.dtype), pos)
         else:

@@ -106,7 +106,7 @@ def adaptive_sparse_attention_forward(self, x: torch.Tensor, pos: torch.Tensor, 
     ``proj`` reads (the reference's restore and transpose, ATT:8992-9030).
     With a PV post-cut the separate restore kernel does that step.
     """
-    from .aggregator import fused_layout_supported, layer_norm_args
+    from .aggregator import fused_layout_supported, head_norm, layer_norm_args
     from .launcher import routing_config
     from .sparse_wrapper import sparse_global_attention
 
@@ -149,7 +149,7 @@ def adaptive_sparse_attention_forward(self, x: torch.Tensor, pos: torch.Tensor, 
             k_norm=layer_norm_args(self.k_norm), pos=pos if rope is not None else None, rope_tables=tables)
     else:
         q, k, v = qkv.permute(2, 0, 3, 1, 4).unbind(0)
-        q, k = self.q_norm(q), self.k_norm(k)
+        q, k = head_norm(self.q_norm, q), head_norm(self.k_norm, k)
         if rope is not None:
             q, k = rope(q, pos), rope(k, pos)
         q_patch, q_special, k_re, v_re = ops.pack_qkv(

@@ -75,7 +75,7 @@ class BlockCache:
 
 def _layer_qkv(attn, x: torch.Tensor, pos: torch.Tensor | None, frames: int, special: int) -> tuple:
     """q of the patch and of the special tokens, k and v ``[B,H,*,D]`` in bf16, normed and turned."""
-    from .aggregator import RotaryPositionEmbeddingAxes, fused_layout_supported, layer_norm_args
+    from .aggregator import RotaryPositionEmbeddingAxes, fused_layout_supported, head_norm, layer_norm_args
     B, T, dim = x.shape
     H = attn.num_heads
     D = dim // H
@@ -87,7 +87,7 @@ def _layer_qkv(attn, x: torch.Tensor, pos: torch.Tensor | None, frames: int, spe
         return ops.pack_qkv(q, k, v, frames, T // frames, special, q_norm=layer_norm_args(attn.q_norm),
                             k_norm=layer_norm_args(attn.k_norm), pos=pos if turned else None,
                             rope_tables=rope.tables(D, x.device) if turned else None)
-    q, k = attn.q_norm(q.transpose(1, 2)), attn.k_norm(k.transpose(1, 2))
+    q, k = head_norm(attn.q_norm, q.transpose(1, 2)), head_norm(attn.k_norm, k.transpose(1, 2))
     if rope is not None and pos is not None:
         if isinstance(rope, RotaryPositionEmbeddingAxes):
             q, k = rope.rotate(q, k.to(q.dtype), pos)
