@@ -234,3 +234,13 @@ def test_derivatives_that_are_refused(monkeypatch):
             stream_attention(None, fwd.make_dual(q, tq), None, None, None, None, None, keep=None)
     with pytest.raises(ValueError, match="gradient"):
         ops._inference(q.requires_grad_(), "q")
+
+
+def test_frames_from_positions_over_three_axes():
+    """A sparse layer reads the grid from the row and column axes, the last two, whatever the time before them."""
+    from vasc_amd.aggregator import grid_positions
+    from vasc_amd.attention import _infer_frames
+    pos = grid_positions(6, 3, 4, 5, "cpu").reshape(1, 6 * 17, 2)
+    time = torch.arange(100, 106).repeat_interleave(17).view(1, -1, 1)
+    assert _infer_frames(pos, 6 * 17, 5) == (3, 4, 6, 17)
+    assert _infer_frames(torch.cat([time, pos], -1), 6 * 17, 5) == (3, 4, 6, 17)

@@ -74,13 +74,14 @@ def frame_grid(h: int, w: int):
 
 def _infer_frames(pos: torch.Tensor, n_tokens: int, S: int):
     """H, W, N, P from the RoPE positions (ATT:8343-8349): patch positions are
-    1-based (specials sit at 0), so the maxima are the grid sizes."""
+    1-based (specials sit at 0), so the maxima are the grid sizes. Row and
+    column are the last axes; a rope over more has the time before them."""
     grid = _FRAME_GRID.get()
     if grid is not None:
         H, W = grid
     else:
-        H = int(pos[0].max(0).values[0])
-        W = int(pos[0].max(0).values[1])
+        H = int(pos[0].max(0).values[-2])
+        W = int(pos[0].max(0).values[-1])
     P = H * W + S
     N = n_tokens // P
     assert N * P == n_tokens, f"{N=}, {H=}, {W=}, {S=}, {n_tokens=}"
