@@ -244,3 +244,36 @@ def test_frames_from_positions_over_three_axes():
     time = torch.arange(100, 106).repeat_interleave(17).view(1, -1, 1)
     assert _infer_frames(pos, 6 * 17, 5) == (3, 4, 6, 17)
     assert _infer_frames(torch.cat([time, pos], -1), 6 * 17, 5) == (3, 4, 6, 17)
+
+
+@pytest.mark.parametrize("view", ["leaf", "transpose", "expand", "unbind"])
+def test_captured_call_on_views_of_leaves(monkeypatch, view):
+    """What q and k are views of counts, through rotary_axes itself; a leaf of another op's graph is not seen."""
+    _, q, k, _, _, pos, sections, freq = _host_rotary(monkeypatch)
+    capturing = [False]
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: capturing[0])
+    make = dict(leaf=lambda: (q.clone().requires_grad_(),) * 2, transpose=lambda: seen(q.transpose(1, 2), lambda t: t.transpose(1, 2)),
+                expand=lambda: seen(q[:1, :1], lambda t: t.expand(2, 3, 5, 8)),
+                unbind=lambda: seen(torch.stack([q, k]), lambda t: t.view(2, 6, 5, 8).unbind(0)[0].view(2, 3, 5, 8)))
+
+    def seen(t, how):
+        leaf = t.clone().requires_grad_()
+        return leaf, lambda: how(leaf)
+
+    leaf, call = make[view]()
+    of = call if callable(call) else lambda: leaf
+    other = k.clone().requires_grad_()
+    for args in ((lambda: (of(), None)), (lambda: (other, of())), (lambda: (k, of()))):
+        capturing[0] = False
+        eager = ops.rotary_axes(*args(), pos, sections, freq)
+        capturing[0] = True
+        with pytest.raises(ValueError, match="eager graph"):
+            ops.rotary_axes(*args(), pos, sections, freq)
+        ops.rotary_axes(q.clone().requires_grad_(), None, pos, sections, freq)
+        del eager
+        ops.rotary_axes(*args(), pos, sections, freq)
+    capturing[0] = False
+    eager = ops.rotary_axes(leaf * 1 if view == "leaf" else of() * 1, None, pos, sections, freq)
+    capturing[0] = True
+    ops.rotary_axes(of(), None, pos, sections, freq)
+    del eager

@@ -834,22 +834,30 @@ class _RotaryAxes(torch.autograd.Function):
         return turn(tq, tk, pos, ctx.sections, inv_freq, ctx.inverse)
 
 
-def _one_graph(node) -> None:
+def _one_graph(node, inputs=()) -> None:
     """Refuses a captured call on leaves that an eager call's live graph holds.
 
     Both graphs share a leaf's accumulation node, whose stream is the eager
     call's: the captured backward pass would wait for it from outside the
     capture, which ends the process. The mark goes with the node, so it is
-    gone when the eager graph is.
+    gone when the eager graph is. ``inputs``: the tensors of the node's first
+    edges; an edge of a view of a leaf is followed to the leaf.
     """
     captured = torch.cuda.is_current_stream_capturing()
-    for leaf, _ in node.next_functions:
-        if leaf is None or leaf.next_functions:
+    for i, (leaf, _) in enumerate(node.next_functions):
+        if leaf is None:
             continue
+        if leaf.next_functions:
+            base = inputs[i]._base if i < len(inputs) else None
+            if base is None or not base.is_leaf:
+                continue
+            while leaf.next_functions:  # views have one input
+                leaf = leaf.next_functions[0][0]
         if not captured:
             leaf.metadata["eager"] = True
         elif "eager" in leaf.metadata:
-            raise ValueError("q or k is a leaf of an eager graph that still lives: drop that call's outputs before capturing")
+            raise ValueError("q or k is, or is a view of, a leaf of an eager graph that still lives: "
+                             "drop that call's outputs before capturing")
 
 
 @functools.lru_cache(maxsize=64)
@@ -870,8 +878,10 @@ def rotary_axes(q: torch.Tensor, k: torch.Tensor | None, pos: torch.Tensor, sect
     ``pos * inv_freq``, whose float64 values ``[sum(sections)/2]`` hold the
     axes' frequencies one after another. Features past the sections pass
     through. Returns ``(q', k' or None)`` in the inputs' memory order;
-    differentiable in q and k, backward and forward. A captured call is refused while an eager
-    call's graph of the same leaves lives.
+    differentiable in q and k, backward and forward. Where q or k is a leaf or
+    a view of one, a captured call is refused while an eager call's graph of
+    that leaf lives, on whatever stream that was; eager graphs that other
+    operators made of it, and leaves behind other operators, are not seen.
     """
     dev = _gpu(q, "q")
     dtype = q.dtype
@@ -910,7 +920,7 @@ def rotary_axes(q: torch.Tensor, k: torch.Tensor | None, pos: torch.Tensor, sect
     if grad or forward_ad._current_level >= 0:
         out = _RotaryAxes.apply(q, k, pos, sections, inv_freq, False)
         if grad:
-            _one_graph(out[0].grad_fn)
+            _one_graph(out[0].grad_fn, (q,) if k is None else (q, k))
         return out
     return _rotary(q, k, pos, sections, inv_freq, False)
 
