@@ -680,6 +680,20 @@ def test_attend_wide_logits_and_scale():
         _check_attend(o, q, held, [L], None, 1, False, scale=scale, H=1)
 
 
+def test_rows_cut_from_wider_ones():
+    """One token of one sequence and head out of rows of odd width, written and asked for: strides of dimensions of size one."""
+    g = _gen(83)
+    wide = _randn(g, 3, 1, 1, 1, 65).cuda()
+    for shift in (0, 1):  # aligned rows, and rows that are not
+        q, k, v = (t[..., shift:shift + 64] for t in wide)
+        cache, table = BlockCache(1, 1, 64), _i32([[0]])
+        ops.cache_write(cache, k, v, table, _i32([0]))
+        held = [O.quantise(_np(k[0]), _np(v[0]))]
+        _check_attend(ops.cache_attn(q, cache, table, _i32([1])), q, held, [1], None, 1, False, H=1)
+        index, count = ops.cache_select(q, cache, table, _i32([1]), 1)
+        assert index.tolist() == [[[[0]]]] and count.item() == 1
+
+
 @pytest.mark.parametrize("L,apart", [(400, 7), (400, -56), (20000, 18)])
 @pytest.mark.parametrize("D,G,T,wide", [(64, 1, 1, False), (64, 1, 1, True), (128, 20, 1, False), (64, 1, 40, False),
                                         (64, 2, 60, True), (128, 4, 30, False)])

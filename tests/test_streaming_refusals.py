@@ -277,3 +277,15 @@ def test_captured_call_on_views_of_leaves(monkeypatch, view):
     capturing[0] = True
     ops.rotary_axes(of(), None, pos, sections, freq)
     del eager
+
+
+def test_rows_of_size_one_dimensions(monkeypatch):
+    """The stride of a dimension of size one says nothing: such rows are taken, wherever they start."""
+    for x in (torch.zeros(1, 1, 1, 65)[..., :64], torch.zeros(1, 2, 3, 65)[:, 1:2, 2:3, 1:], torch.zeros(1, 3, 1, 64 + 8)[..., 3:67],
+              torch.zeros(2, 1, 4, 65)[..., :64], torch.zeros(7, 1, 1, 130)[:, :, :, 1:129]):
+        t, ptr, sb, sh, st = ops._rows8(x, "q", (torch.float32,))
+        assert t.shape == x.shape and ptr == t.data_ptr() and ptr % 16 == 0 and not (sb | sh | st) % 8
+        want = torch.empty(0).set_(t.untyped_storage(), t.storage_offset(), x.shape, (sb, sh, st, 1))
+        assert torch.equal(want, x)
+    with pytest.raises(ValueError, match="multiple of 8"):
+        ops._rows8(torch.zeros(1, 2, 3, 60), "q", (torch.float32,))

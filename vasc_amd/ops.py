@@ -720,10 +720,11 @@ def _rows8(t: torch.Tensor, name: str, dtypes: tuple) -> tuple:
         t = t.contiguous()
         if t.data_ptr() & 15:  # contiguous, but a view that starts inside a row
             t = t.clone()
-        sb, sh, st, sd = t.stride()
+        _, H, T, D = t.shape
+        if D & 7:
+            raise ValueError(f"{name} has rows of {D} elements, expected a multiple of 8")
         ptr = t.data_ptr()
-        if (sb | sh | st) & 7:  # a head dimension that is no multiple of 8
-            raise ValueError(f"{name} has rows of {t.shape[3]} elements, expected a multiple of 8")
+        sb, sh, st = H * T * D, T * D, D  # not the tensor's: those of dimensions of size 1 may be anything
     return t, ptr, sb, sh, st
 
 
