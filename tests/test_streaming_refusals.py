@@ -3,6 +3,7 @@ before it touches a pointer)."""
 import copy
 import ctypes
 import pickle
+import types
 
 import pytest
 import torch
@@ -289,3 +290,27 @@ def test_rows_of_size_one_dimensions(monkeypatch):
         assert torch.equal(want, x)
     with pytest.raises(ValueError, match="multiple of 8"):
         ops._rows8(torch.zeros(1, 2, 3, 60), "q", (torch.float32,))
+
+
+def _host_cache(monkeypatch):
+    """The cache operators' checks on the host: a cache of 2 heads of 64, and the launches that would have been made."""
+    launches = []
+    monkeypatch.setattr(ops, "_gpu", lambda t, name, dev=-1: -1)
+    monkeypatch.setattr(ops, "_launch", lambda dev, name, *args: launches.append((name, args)))
+    return types.SimpleNamespace(heads=2, head_dim=64, device_index=-1, pages=4, pointers=(FAKE,) * 4, mean_pointer=FAKE), launches
+
+
+def test_out_that_overlaps_itself_or_needs_a_gradient(monkeypatch):
+    cache, launches = _host_cache(monkeypatch)
+    q, table, n = torch.zeros(2, 4, 3, 64, dtype=torch.bfloat16), torch.zeros(2, 4, dtype=torch.int32), torch.ones(2, dtype=torch.int32)
+    one = torch.zeros(1, 1, 1, 64, dtype=torch.bfloat16)
+    for out in (one.expand(2, 4, 3, 64), torch.zeros(2, 1, 3, 64, dtype=torch.bfloat16).expand(2, 4, 3, 64)):
+        with pytest.raises(ValueError, match="overlap"):
+            ops.cache_attn(q, cache, table, n, out=out)
+    with pytest.raises(ValueError, match="gradient"):
+        ops.cache_attn(q, cache, table, n, out=torch.zeros_like(q).requires_grad_())
+    assert not launches
+    with torch.no_grad():
+        ops.cache_attn(q, cache, table, n, out=torch.zeros_like(q).requires_grad_())
+    ops.cache_attn(q[:1, :2, :1], cache, table[:1], n[:1], out=one.expand(1, 2, 1, 64)[:, :1].expand(1, 2, 1, 64).clone())
+    assert len(launches) == 2
