@@ -314,3 +314,18 @@ def test_out_that_overlaps_itself_or_needs_a_gradient(monkeypatch):
         ops.cache_attn(q, cache, table, n, out=torch.zeros_like(q).requires_grad_())
     ops.cache_attn(q[:1, :2, :1], cache, table[:1], n[:1], out=one.expand(1, 2, 1, 64)[:, :1].expand(1, 2, 1, 64).clone())
     assert len(launches) == 2
+
+
+def test_out_of_size_one_dimensions(monkeypatch):
+    """An out whose dimensions of size one have odd strides is taken, with strides that the kernel accepts."""
+    cache, launches = _host_cache(monkeypatch)
+    table, n = torch.zeros(1, 4, dtype=torch.int32), torch.ones(1, dtype=torch.int32)
+    q = torch.zeros(1, 2, 1, 64, dtype=torch.bfloat16)
+    wide = torch.zeros(1, 2, 3, 68, dtype=torch.bfloat16)
+    for out in (torch.zeros(1, 2, 64, 1, dtype=torch.bfloat16).transpose(2, 3).contiguous(), wide[:, :, 1:2, :64],
+                torch.zeros(129, dtype=torch.bfloat16)[:128].as_strided((1, 2, 1, 64), (129, 64, 65, 1))):
+        assert ops.cache_attn(q, cache, table, n, out=out) is out
+        strides = launches[-1][1][5:8]
+        assert launches[-1][1][4] == out.data_ptr() and not any(st % 4 for st in strides) and strides[1] == out.stride(1)
+    with pytest.raises(ValueError, match="aligned rows"):
+        ops.cache_attn(q, cache, table, n, out=torch.zeros(200, dtype=torch.bfloat16).as_strided((1, 2, 1, 64), (128, 65, 64, 1)))

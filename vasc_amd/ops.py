@@ -1104,8 +1104,8 @@ def cache_attn(q: torch.Tensor, cache, page_table: torch.Tensor, lengths: torch.
         if out.shape != shape or out.dtype != q.dtype:
             raise ValueError(f"out must be {q.dtype} {tuple(shape)}, got {out.dtype} {tuple(out.shape)}")
         _inference(out, "out")
-        osb, osh, ost, osd = out.stride()
-        if any(st == 0 and n > 1 for n, st in zip(shape, (osb, osh, ost))):
+        osb, osh, ost, osd = (st if n > 1 else D for n, st in zip(shape, out.stride()))
+        if not (osb and osh and ost):
             raise ValueError("out's rows overlap (an expanded tensor)")
         if osd != 1 or (osb | osh | ost) & 3 or out.data_ptr() & 7:
             raise ValueError("out needs unit stride over D and 8-byte aligned rows")
