@@ -329,3 +329,24 @@ def test_out_of_size_one_dimensions(monkeypatch):
         assert launches[-1][1][4] == out.data_ptr() and not any(st % 4 for st in strides) and strides[1] == out.stride(1)
     with pytest.raises(ValueError, match="aligned rows"):
         ops.cache_attn(q, cache, table, n, out=torch.zeros(200, dtype=torch.bfloat16).as_strided((1, 2, 1, 64), (128, 65, 64, 1)))
+
+
+def test_integers_past_32_bits(monkeypatch):
+    """Lengths, starts, page tables and lists of 64 bits keep their sense: what is out of range stays out of range."""
+    cache, launches = _host_cache(monkeypatch)
+    far = torch.tensor([2 ** 32 + 5, -2 ** 32 + 5, 2 ** 31, -2 ** 31 - 1, 2 ** 63 - 1, -2 ** 63, 7, -1])
+    got = ops._int_rows(far, "start", 8, -1)
+    most = 2 ** 31 - 1
+    assert got.dtype == torch.int32 and got.tolist() == [most, -1, most, -1, most, -1, 7, -1]
+    assert ops._int_rows(far[6:].to(torch.int8), "start", 2, -1).tolist() == [7, -1]
+    table, stride, pages = ops._page_table(far.view(2, 4), 2, -1)
+    assert table.dtype == torch.int32 and (stride, pages) == (4, 4) and table.flatten().tolist() == got.tolist()
+    q = torch.zeros(1, 2, 1, 64, dtype=torch.bfloat16)
+    seen = []
+    monkeypatch.setattr(ops, "_ptr", lambda t: seen.append(t))
+    ops.cache_attn(q, cache, table[:1], got[6:7], far.view(1, 1, 1, 8).expand(1, 2, 1, 8), far[:1].view(1, 1, 1).expand(1, 2, 1))
+    lists = [t for t in seen if t is not None and t.dim() > 2]
+    assert lists[0][0, 0, 0].tolist() == got.tolist() and lists[1].flatten().tolist() == [most] * 2
+    for bad in (torch.zeros(8), torch.zeros(8, dtype=torch.bool), torch.zeros(8, dtype=torch.complex64)):
+        with pytest.raises(ValueError, match="integers"):
+            ops._int_rows(bad, "start", 8, -1)

@@ -728,16 +728,26 @@ def _rows8(t: torch.Tensor, name: str, dtypes: tuple) -> tuple:
     return t, ptr, sb, sh, st
 
 
+def _int32(t: torch.Tensor, name: str) -> torch.Tensor:
+    """``t`` as int32; integers that it cannot hold become -1 or 2^31 - 1, which are out of range in the same sense."""
+    if t.dtype is torch.int32:
+        return t
+    if t.dtype.is_floating_point or t.dtype.is_complex or t.dtype is torch.bool:
+        raise ValueError(f"{name} must hold integers, got {t.dtype}")
+    if t.dtype.itemsize >= 4:
+        t = t.to(torch.int64).clamp(-1, 2 ** 31 - 1)
+    return t.to(torch.int32)
+
+
 def _int_rows(t, name: str, B: int, dev: int):
     """``[B]`` int32, contiguous (None stays)."""
     if t is None or (isinstance(t, torch.Tensor) and t.dtype is torch.int32 and t.shape == (B,)
                      and t.get_device() == dev and t.is_contiguous()):
         return t
     _gpu(t, name, dev)
-    if t.shape != (B,) or t.dtype.is_floating_point or t.dtype is torch.bool:
-        raise ValueError(f"{name} must hold {B} integers, got {t.dtype} {tuple(t.shape)}")
-    if t.dtype is not torch.int32:
-        t = t.to(torch.int32)
+    t = _int32(t, name)
+    if t.shape != (B,):
+        raise ValueError(f"{name} must hold {B} integers, got {tuple(t.shape)}")
     return t if t.is_contiguous() else t.contiguous()
 
 
@@ -748,10 +758,9 @@ def _page_table(t, B: int, dev: int) -> tuple:
         if len(shape) == 2 and shape[0] == B and strides[1] == 1 and strides[0] >= shape[1] > 0:
             return t, strides[0] if B > 1 else shape[1], shape[1]
     _gpu(t, "page_table", dev)
-    if t.dim() != 2 or t.shape[0] != B or t.shape[1] == 0 or t.dtype.is_floating_point or t.dtype is torch.bool:
-        raise ValueError(f"page_table must be [{B}, max_pages] integers, got {t.dtype} {tuple(t.shape)}")
-    if t.dtype is not torch.int32:
-        t = t.to(torch.int32)
+    t = _int32(t, "page_table")
+    if t.dim() != 2 or t.shape[0] != B or t.shape[1] == 0:
+        raise ValueError(f"page_table must be [{B}, max_pages] integers, got {tuple(t.shape)}")
     mp = t.shape[1]
     sb, sp = t.stride()
     if (mp > 1 and sp != 1) or (B > 1 and sb < mp):
@@ -1090,11 +1099,7 @@ def cache_attn(q: torch.Tensor, cache, page_table: torch.Tensor, lengths: torch.
         if len(ishape) != 4 or ishape[:3] != (B, H, U) or count.shape != (B, H, U):
             raise ValueError(f"index/count must be [{B},{H},{U},W]/[{B},{H},{U}], got {tuple(ishape)}/"
                              f"{tuple(count.shape)}")
-        if index.dtype is not torch.int32 or count.dtype is not torch.int32:
-            if any(t.dtype.is_floating_point or t.dtype is torch.bool for t in (index, count)):
-                raise ValueError("index and count must be integers")
-            index, count = index.to(torch.int32), count.to(torch.int32)
-        index, count = index.contiguous(), count.contiguous()
+        index, count = _int32(index, "index").contiguous(), _int32(count, "count").contiguous()
         width = ishape[3]
     if out is None:
         out = torch.empty(shape, device=q.device, dtype=q.dtype)
