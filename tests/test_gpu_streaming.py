@@ -946,6 +946,23 @@ def test_rotary_axes_module_is_the_2d_one():
         RotaryPositionEmbeddingAxes((16, 16), (1.0, 2.0, 3.0))
 
 
+def test_rope_module_across_modes(tmp_path):
+    """First called in inference mode, then trained with; saved, loaded onto the host and moved back."""
+    from vasc_amd.aggregator import RotaryPositionEmbeddingAxes
+    g = _gen(89)
+    rope = RotaryPositionEmbeddingAxes((32, 32))
+    x, pos = _randn(g, 1, 2, 9, 64).cuda(), torch.randint(0, 40, (1, 9, 2), generator=g).cuda()
+    with torch.inference_mode():
+        want = rope(x, pos).clone()
+    leaf = x.clone().requires_grad_()
+    y = rope(leaf, pos)
+    y.sum().backward()
+    assert torch.equal(y, want) and leaf.grad.isfinite().all()
+    torch.save(rope, tmp_path / "rope")
+    back = torch.load(tmp_path / "rope", map_location="cpu", weights_only=False).cuda()
+    assert torch.equal(back(x, pos), want)
+
+
 @pytest.mark.parametrize("axes", [2, 3])
 @pytest.mark.parametrize("special", [0, 5])
 def test_stream_attention_layer(axes, special):

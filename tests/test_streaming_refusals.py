@@ -350,3 +350,16 @@ def test_integers_past_32_bits(monkeypatch):
     for bad in (torch.zeros(8), torch.zeros(8, dtype=torch.bool), torch.zeros(8, dtype=torch.complex64)):
         with pytest.raises(ValueError, match="integers"):
             ops._int_rows(bad, "start", 8, -1)
+
+
+def test_frequencies_made_in_inference_mode_or_loaded_elsewhere(tmp_path):
+    """A rope first called in inference mode is trained with later, and one that was saved is loaded for another device."""
+    from vasc_amd.aggregator import RotaryPositionEmbeddingAxes
+    rope = RotaryPositionEmbeddingAxes((4, 8), 100.0)
+    with torch.inference_mode():
+        first = rope.frequencies("cpu")
+    assert not first.is_inference() and rope.frequencies("cpu") is first
+    torch.save(rope, tmp_path / "rope")
+    other = torch.load(tmp_path / "rope", map_location="meta", weights_only=False)
+    for again in (other, copy.deepcopy(rope), pickle.loads(pickle.dumps(rope))):
+        assert again.frequencies("cpu").device.type == "cpu" and torch.equal(again.frequencies("cpu"), first)

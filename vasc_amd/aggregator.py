@@ -105,10 +105,15 @@ class RotaryPositionEmbeddingAxes(nn.Module):
         key = str(device)
         have = self._frequencies.get(key)
         if have is None:
-            have = torch.cat([base ** (-torch.arange(0, s, 2, dtype=torch.float64) / s)
-                              for s, base in zip(self.sections, self.base_frequency)]).to(device)
+            with torch.inference_mode(False):  # a training call may be the next
+                have = torch.cat([base ** (-torch.arange(0, s, 2, dtype=torch.float64) / s)
+                                  for s, base in zip(self.sections, self.base_frequency)]).to(device)
             self._frequencies[key] = have
         return have
+
+    def __getstate__(self) -> dict:
+        """Without the devices' tensors: a saved module may be loaded for other ones."""
+        return {**self.__dict__, "_frequencies": {}}
 
     def rotate(self, q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor):
         """q, k ``[B,H,T,D]``, positions ``[B,T,A]`` integer: both turned in one launch."""
