@@ -11,7 +11,7 @@ import torch.autograd.forward_ad as fwd
 
 from oracle import streaming as O
 from vasc_amd import _lib, ops
-from vasc_amd.streaming import BlockCache, stream_attention
+from vasc_amd.streaming import AggregatorStream, BlockCache, stream_attention
 
 FAKE = 1 << 20  # an aligned address that nothing reads
 
@@ -363,3 +363,45 @@ def test_frequencies_made_in_inference_mode_or_loaded_elsewhere(tmp_path):
     other = torch.load(tmp_path / "rope", map_location="meta", weights_only=False)
     for again in (other, copy.deepcopy(rope), pickle.loads(pickle.dumps(rope))):
         assert again.frequencies("cpu").device.type == "cpu" and torch.equal(again.frequencies("cpu"), first)
+
+
+def test_layers_run_on_their_tensors_device(monkeypatch):
+    """The layout kernels launch on the current device's stream: a layer whose tokens are on another one makes that current."""
+    current, seen = [0], []
+
+    class Device:
+        def __init__(self, dev):
+            self.dev = dev if isinstance(dev, int) else dev.index
+
+        def __enter__(self):
+            self.before, current[0] = current[0], self.dev
+
+        def __exit__(self, *_):
+            current[0] = self.before
+
+    def stop(*_):
+        seen.append(current[0])
+        raise KeyError("stopped")
+
+    monkeypatch.setattr(torch.cuda, "device", Device)
+    monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: current[0])
+    where = {"x": 3, "pos": 3, "images": 3}
+    monkeypatch.setattr(ops, "_gpu", lambda t, name, dev=-1: where[name])
+    attn = types.SimpleNamespace(num_heads=2, qkv=stop)
+    x = torch.zeros(1, 4, 128)
+    with pytest.raises(KeyError):
+        stream_attention(attn, x, torch.zeros(1, 4, 2), None, None, None, None, keep=None)
+    model = types.SimpleNamespace(_resnet_mean=0, _resnet_std=1, patch_embed=types.SimpleNamespace(
+        weight=x, bias=None, kernel_size=(2, 2), stride=(1, 1), padding=0, __call__=stop))
+    model.patch_embed = type("Conv", (), dict(vars(model.patch_embed), __call__=lambda self, x: stop()))()
+    with pytest.raises(KeyError):
+        AggregatorStream(model, 4).push(torch.zeros(1, 1, 3, 4, 4))
+    assert seen == [3, 3] and current == [0]
+
+
+def test_streamed_layer_refuses_tensors_elsewhere():
+    x = torch.zeros(1, 4, 128)
+    with pytest.raises(ValueError, match="x must be a GPU"):
+        stream_attention(None, x, None, None, None, None, None, keep=None)
+    with pytest.raises(ValueError, match="images must be a GPU"):
+        AggregatorStream(None, 4).push(torch.zeros(1, 1, 3, 4, 4))

@@ -6,6 +6,7 @@ must be device tensors; nothing here falls back to the CPU.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import functools
 import math
@@ -683,6 +684,11 @@ def _launch(dev: int, name: str, *args) -> None:
     else:
         with torch.cuda.device(dev):
             _lib.call(name, *args, torch._C._cuda_getCurrentRawStream(dev))
+
+
+def on_device(dev: int):
+    """A context in which GPU ``dev`` is the current one."""
+    return contextlib.nullcontext() if torch._C._cuda_getDevice() == dev else torch.cuda.device(dev)
 
 
 def _gpu(t, name: str, dev: int = -1) -> int:

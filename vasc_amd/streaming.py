@@ -112,26 +112,30 @@ def stream_attention(attn, x: torch.Tensor, pos: torch.Tensor | None, cache: Blo
     last ``recent``; None: all. Returns ``[B,T,dim]``. No gradients.
     """
     ops._inference(x, "x")
+    dev = ops._gpu(x, "x")
+    if pos is not None:
+        ops._gpu(pos, "pos", dev)
     B, T, dim = x.shape
     if frames < 1 or T < 1 or T % frames or not 0 <= special <= T // frames:
         raise ValueError(f"{T} tokens are not {frames} frames with {special} special tokens each")
     H = attn.num_heads
-    q_patch, q_special, k, v = _layer_qkv(attn, x, pos, frames, special)
-    ops.cache_write(cache, k, v, page_table, start)
-    if keep is None:
-        o_patch = ops.cache_attn(q_patch, cache, page_table, lengths)
-    else:
-        index, count = ops.cache_select(q_patch, cache, page_table, lengths, keep, block_q=block_q, sink=sink,
-                                        recent=recent)
-        o_patch = ops.cache_attn(q_patch, cache, page_table, lengths, index, count, block_q=block_q)
-    o_special = ops.cache_attn(q_special, cache, page_table, lengths) if q_special is not None else None
-    if o_patch.shape[2]:
-        out = ops.restore_tokens(o_patch, o_special, frames, T // frames, special)
-    else:  # frames of special tokens only, which are in order
-        out = o_special.transpose(1, 2).reshape(B, T, H * (dim // H))
-    out = attn.proj(out.to(x.dtype))
-    drop = getattr(attn, "proj_drop", None)
-    return drop(out) if drop is not None else out
+    with ops.on_device(dev):
+        q_patch, q_special, k, v = _layer_qkv(attn, x, pos, frames, special)
+        ops.cache_write(cache, k, v, page_table, start)
+        if keep is None:
+            o_patch = ops.cache_attn(q_patch, cache, page_table, lengths)
+        else:
+            index, count = ops.cache_select(q_patch, cache, page_table, lengths, keep, block_q=block_q, sink=sink,
+                                            recent=recent)
+            o_patch = ops.cache_attn(q_patch, cache, page_table, lengths, index, count, block_q=block_q)
+        o_special = ops.cache_attn(q_special, cache, page_table, lengths) if q_special is not None else None
+        if o_patch.shape[2]:
+            out = ops.restore_tokens(o_patch, o_special, frames, T // frames, special)
+        else:  # frames of special tokens only, which are in order
+            out = o_special.transpose(1, 2).reshape(B, T, H * (dim // H))
+        out = attn.proj(out.to(x.dtype))
+        drop = getattr(attn, "proj_drop", None)
+        return drop(out) if drop is not None else out
 
 
 class AggregatorStream:
@@ -169,6 +173,10 @@ class AggregatorStream:
     @torch.no_grad()
     def push(self, images: torch.Tensor):
         """images ``[B,n,3,H,W]`` in [0, 1] -> (list of per-layer outputs, patch_start_idx)."""
+        with ops.on_device(ops._gpu(images, "images")):
+            return self._push(images)
+
+    def _push(self, images: torch.Tensor):
         from .aggregator import grid_positions, patch_tokens, RotaryPositionEmbeddingAxes
         m = self.model
         B, n, _, Hi, Wi = images.shape
