@@ -1118,3 +1118,173 @@ def test_aggregator_stream(axes):
         got, _ = dense.push(images[:, :1])
         for a, b in zip(got, want):
             assert (a.float() - b.float()).abs().max() <= 0.02 * b.float().abs().max()
+
+
+def _float64_norm(x, norm):
+    x = x - x.mean(-1, keepdims=True)
+    return x / np.sqrt((x * x).mean(-1, keepdims=True) + norm.eps) * _np(norm.weight) + _np(norm.bias)
+
+
+def _layer_positions(B, first, n, grid, special, axes):
+    """Positions of n frames from `first` on, written out: (frame,) row, column, special tokens at 0, 0."""
+    rows = []
+    for f in range(first, first + n):
+        cells = [(0, 0)] * special + [(r + 1, c + 1) for r in range(grid[0]) for c in range(grid[1])]
+        rows += [((f,) if axes == 3 else ()) + cell for cell in cells]
+    return np.broadcast_to(np.array(rows), (B, len(rows), axes))
+
+
+@pytest.mark.parametrize("sparse_ratio", [0.0, 0.6])
+@pytest.mark.parametrize("axes", [2, 3])
+def test_aggregator_stream_against_float64(axes, sparse_ratio, monkeypatch):
+    """Every global block of every push, from the projection's rows up: norms, positions (time from the stream's start), the
+    keys and values held, and attention over all that was seen or over the pages chosen, in float64 with code of its own.
+    Frame blocks pass the tokens through (their scales are 0), so the first one shows the special tokens of first and later
+    frames; a global block adds its attention to them (scales 1 and 0, an identity for the projection).
+
+    Keys: a bf16 rounding (2^-8) and an e4m3 one (2^-4 of the value, or half the smallest step 2^-9 of the row's power,
+    which is below top / 224), float32's share as in _rotary_bound and a norm of 64 terms. Output: a rounding of q in every logit,
+    2^-8 of sum |q k| scale, in weights and their sum; the rounding of half weights and the rest, 2^-10; bf16 of the
+    attention and of the sum with the tokens, 2^-8 each. With three axes the norms are torch's, which round to bf16 before the
+    turn: a pair's two roundings, 2^-8 of each value, turn with it, so either value is off by at most 2^-8 (|lo| + |hi|) more
+    (|cos| and |sin| up to 1); the layout kernel of two axes rounds once."""
+    from vasc_amd.aggregator import Aggregator, RotaryPositionEmbeddingAxes
+    from vasc_amd.streaming import AggregatorStream
+    torch.manual_seed(8)
+    C, H, D, grid, S = 512, 8, 64, (8, 10), 5
+    P = S + grid[0] * grid[1]
+    model = Aggregator(dim=C, depth=2, num_heads=H, intermediate_layer_idx=(0, 1)).cuda().to(torch.bfloat16)
+    sections, bases = ((16, 24, 24), (1e4, 100.0, 100.0)) if axes == 3 else ((32, 32), (100.0, 100.0))
+    with torch.no_grad():
+        model.camera_token.normal_()
+        model.register_token.normal_()
+        for blk in model.frame_blocks:
+            blk.ls1.gamma.zero_()
+            blk.ls2.gamma.zero_()
+        for blk in model.global_blocks:
+            blk.ls1.gamma.fill_(1)
+            blk.ls2.gamma.zero_()
+            blk.attn.proj.weight.copy_(torch.eye(C))
+            blk.attn.proj.bias.zero_()
+            blk.norm1.weight.normal_(1.0, 0.2)
+            blk.norm1.bias.normal_(0.0, 0.2)
+            for n in (blk.attn.q_norm, blk.attn.k_norm):
+                n.weight.normal_(1.5, 0.3)
+                n.bias.normal_(0.0, 0.3)
+    if axes == 3:
+        rope = RotaryPositionEmbeddingAxes(sections, bases)
+        for blk in (*model.frame_blocks, *model.global_blocks):
+            blk.attn.rope = rope
+    freq = _freq(sections, bases).numpy()
+
+    def early(rows):
+        """What a rounding before the turn adds to each value."""
+        off, at = np.zeros_like(rows), 0
+        for d in sections if axes == 3 else ():
+            pair = np.abs(rows[..., at:at + d // 2]) + np.abs(rows[..., at + d // 2:at + d])
+            off[..., at:at + d // 2] = off[..., at + d // 2:at + d] = 2.0 ** -8 * pair
+            at += d
+        return off
+
+    seen_qkv, lists = [], []
+    for blk in model.global_blocks:
+        blk.attn.qkv.register_forward_hook(lambda m, args, out: seen_qkv.append((args[0], out)))
+    choose = ops.cache_select
+    monkeypatch.setattr(ops, "cache_select", lambda *a, **kw: lists.append(choose(*a, **kw)) or lists[-1])
+    B, total = 2, 5
+    images = torch.rand(B, total, 3, grid[0] * 14, grid[1] * 14, generator=_gen(97)).cuda()
+    stream = AggregatorStream(model, total, sparse_ratio=sparse_ratio)
+    missed_time = missed_attention = False
+    for lo, hi in ((0, 1), (1, 3), (3, 5)):
+        seen_qkv.clear()
+        lists.clear()
+        n, L = hi - lo, hi * P
+        outs, _ = stream.push(images[:, lo:hi])
+        first = _np(outs[0][..., :C])  # [B,n,P,C]
+        for f in range(n):
+            which = 0 if lo + f == 0 else 1
+            assert np.array_equal(first[:, f, 0], np.broadcast_to(_np(model.camera_token[:, which, 0]), (B, C)))
+            assert np.array_equal(first[:, f, 1:S], np.broadcast_to(_np(model.register_token[:, which]), (B, S - 1, C)))
+        assert (first[:, :, S:].std((0, 1, 2)) > 0).all()
+        assert torch.equal(outs[1][..., :C], outs[0][..., C:])
+        pos = _layer_positions(B, lo, n, grid, S, axes)
+        pages = -(-L // 64)
+        keep = None if sparse_ratio == 0 else max(0, max(1, int(pages * (1 - sparse_ratio))) - 2)
+        for i, blk in enumerate(model.global_blocks):
+            x, y = (_np(outs[i][..., s]).reshape(B, n * P, C) for s in (slice(0, C), slice(C, 2 * C)))
+            h, qkv = (_np(t).reshape(B, n * P, -1) for t in seen_qkv[i])
+            want = _float64_norm(x, blk.norm1)
+            assert (np.abs(h - want) <= 2.0 ** -8 * np.abs(want) + 2.0 ** -16 * (1 + np.abs(want))).all()
+            q, k, v = (qkv.reshape(B, n * P, 3, H, D)[:, :, j].transpose(0, 2, 1, 3) for j in range(3))
+            q, k = _float64_norm(q, blk.attn.q_norm), _float64_norm(k, blk.attn.k_norm)
+            side = 2.0 ** -17 * (1 + np.abs(k).max())
+            k0, q_off, k_off = k, early(q), early(k)
+            q, k = O.rotate(q, pos, sections, freq), O.rotate(k, pos, sections, freq)
+            q_off += 2.0 ** -8 * np.abs(q)
+            zero = _i32([0] * B)
+            hk, hv = (_np(t) for t in ops.cache_read(stream.caches[i], stream.page_table, zero, L, dtype=torch.float32))
+            # a push is held in the global layers' order, its patches and behind them its special tokens
+            t = np.arange(n * P)
+            held = np.concatenate([t[t % P >= S], t[t % P < S]])
+            assert np.array_equal(hv[:, :, lo * P:], O.quantise(v, v)[1][:, :, held])
+
+            def off(kk):
+                kk = kk[:, :, held]
+                top = np.abs(kk).max(-1, keepdims=True) * (1 + 2.0 ** -8)
+                bound = (2.0 ** -4 * (1 + 2.0 ** -8) + 2.0 ** -8) * np.abs(kk) + top / 224 * 2.0 ** -10 + side + 1.07 * k_off[:, :, held]
+                return (np.abs(hk[:, :, lo * P:] - kk) > bound).any()
+
+            assert not off(k)
+            if axes == 3:  # the check sees a time that is off by one
+                later = pos + np.array([1, 0, 0])
+                missed_time = missed_time or not off(O.rotate(k0, later, sections, freq))
+            for b in range(B):
+                for head in range(H):
+                    logits = q[b, head] @ hk[b, head].T / 8
+                    live = np.ones((n * P, L), bool)
+                    if keep is not None:
+                        index, count = (z.cpu().numpy() for z in lists[i])
+                        patch = t % P >= S
+                        unit = (t // P * (P - S) + t % P - S) // 128
+                        for u in range(index.shape[2]):
+                            got = index[b, head, u, :count[b, head, u]].tolist()
+                            assert len(got) == min(pages, keep + 2) and got[0] == 0 and got[-1] == pages - 1
+                            live[patch & (unit == u)] = np.isin(np.arange(L) // 64, got)
+                    logits[~live] = -np.inf
+                    p = np.exp(logits - logits.max(-1, keepdims=True))
+                    p /= p.sum(-1, keepdims=True)
+                    o, mag = p @ hv[b, head], p @ np.abs(hv[b, head])
+                    off_logit = (q_off[b, head] @ np.abs(hk[b, head]).T).max(-1, keepdims=True) / 8 + side
+                    off_o = (np.expm1(2 * off_logit) + 2.0 ** -10) * mag
+                    off_o = off_o + 2.0 ** -8 * (np.abs(o) + off_o)
+                    xs, ys = (t[b][:, head * D:(head + 1) * D] for t in (x, y))
+                    bound = off_o + 2.0 ** -8 * (np.abs(xs + o) + off_o)
+                    assert (np.abs(ys - (xs + o)) <= bound).all(), (lo, i, b, head)
+                    missed_attention = missed_attention or not (np.abs(ys - xs) > bound).any()
+    assert not missed_time and not missed_attention
+
+
+def test_aggregator_stream_forked():
+    """A deep copy goes its own way: neither sees the other's frames."""
+    from vasc_amd.aggregator import Aggregator
+    from vasc_amd.streaming import AggregatorStream
+    torch.manual_seed(9)
+    model = Aggregator(dim=512, depth=2, num_heads=8, intermediate_layer_idx=(0, 1)).cuda().to(torch.bfloat16)
+    with torch.no_grad():
+        for blk in model.global_blocks:
+            blk.ls1.gamma.fill_(1)
+    images = torch.rand(1, 4, 3, 112, 140, generator=_gen(101)).cuda()
+
+    def straight(order):
+        stream = AggregatorStream(model, 3)
+        return [stream.push(images[:, i:i + 1])[0] for i in order]
+
+    one, two = straight((0, 1, 2)), straight((0, 3, 2))
+    stream = AggregatorStream(model, 3)
+    stream.push(images[:, :1])
+    fork = copy.deepcopy(stream)
+    for order in (1, 2):
+        a, b = stream.push(images[:, order:order + 1])[0], fork.push(images[:, [3, 2][order - 1]:][:, :1])[0]
+        for x, y, wx, wy in zip(a, b, one[order], two[order]):
+            assert torch.equal(x, wx) and torch.equal(y, wy)
+    assert not torch.equal(one[2][1], two[2][1])

@@ -109,7 +109,9 @@ def stream_attention(attn, x: torch.Tensor, pos: torch.Tensor | None, cache: Blo
     cache before the call, ``lengths [B]``: after it (``start + T``); both stay
     on the device, so that a captured call serves every step. ``keep``: pages
     that a block of patch queries chooses beside the first ``sink`` and the
-    last ``recent``; None: all. Returns ``[B,T,dim]``. No gradients.
+    last ``recent``; None: all. A call's tokens are held in the global layers'
+    order, all patches before all special tokens. Returns ``[B,T,dim]``. No
+    gradients.
     """
     ops._inference(x, "x")
     dev = ops._gpu(x, "x")
