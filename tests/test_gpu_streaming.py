@@ -680,6 +680,26 @@ def test_attend_wide_logits_and_scale():
         _check_attend(o, q, held, [L], None, 1, False, scale=scale, H=1)
 
 
+def test_integers_of_64_bits():
+    """Starts, lengths, tables and lists past 32 bits on the GPU: nothing is written or seen there; within it, as int32."""
+    g = _gen(107)
+    cache = BlockCache(3, 1, 64)
+    k = _randn(g, 2, 1, 70, 64).cuda()
+    far = torch.tensor([[2 ** 32, 2 ** 33 + 1], [1, -2 ** 32 + 2]], device="cuda")
+    ops.cache_write(cache, k, k, far, torch.tensor([2 ** 32, -2 ** 32], device="cuda"))
+    assert not cache.kc.any()
+    ops.cache_write(cache, k, k, far, torch.tensor([0, 0], device="cuda"))
+    assert not cache.kc[[0, 2]].any() and cache.kc[1].any()
+    held = [(np.zeros((1, 0, 64)),) * 2, O.quantise(_np(k[1, :, :64]), _np(k[1, :, :64]))]
+    q = _randn(g, 2, 1, 1, 64).cuda()
+    lists, count = torch.tensor([0, 2 ** 32 + 1, 1], device="cuda").expand(2, 1, 1, 3), torch.tensor([3], device="cuda").expand(2, 1, 1)
+    for length in (64, 2 ** 40):
+        n = torch.tensor([length] * 2, device="cuda")
+        assert not ops.cache_attn(q[:1], cache, far[:1], n[:1]).any()
+        _check_attend(ops.cache_attn(q, cache, far, n, lists, count), q, held, [0, 64], [[[[]]], [[[0]]]], 1, False, H=1)
+    assert not ops.cache_attn(q, cache, far, torch.tensor([-2 ** 32 + 64] * 2, device="cuda")).any()
+
+
 def test_rows_cut_from_wider_ones():
     """One token of one sequence and head out of rows of odd width, written and asked for: strides of dimensions of size one."""
     g = _gen(83)

@@ -735,7 +735,8 @@ def _rows8(t: torch.Tensor, name: str, dtypes: tuple) -> tuple:
 
 
 def _int32(t: torch.Tensor, name: str) -> torch.Tensor:
-    """``t`` as int32; integers that it cannot hold become -1 or 2^31 - 1, which are out of range in the same sense."""
+    """``t`` as int32 (which is best kept so: others cost a launch or two); integers that it cannot hold become -1 or 2^31 - 1,
+    which are out of range in the same sense."""
     if t.dtype is torch.int32:
         return t
     if t.dtype.is_floating_point or t.dtype.is_complex or t.dtype is torch.bool:
