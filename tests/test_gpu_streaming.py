@@ -700,6 +700,21 @@ def test_integers_of_64_bits():
     assert not ops.cache_attn(q, cache, far, torch.tensor([-2 ** 32 + 64] * 2, device="cuda")).any()
 
 
+@pytest.mark.parametrize("D,G,T,mp", [(64, 1, 1, 6), (64, 1, 1, 140), (128, 20, 1, 6), (64, 1, 100, 6), (128, 4, 30, 6)])
+def test_attend_scales(D, G, T, mp):
+    """Scales below zero, hardly above it and far above one, in every kernel."""
+    g = _gen(D + T + mp)
+    L = 300
+    table, pages = _table(g, 1, mp)
+    cache = BlockCache(pages, 1, D)
+    held = _fill(cache, g, table, [L])
+    q = _randn(g, 1, G, T, D).cuda()
+    for scale in (-0.125, 1e-29, -1e-29, 3.0):
+        o = ops.cache_attn(q, cache, table, _i32([L]), scale=scale)
+        # of the bound, what grows with the logits goes by their magnitude
+        _check_attend(o, q if scale > 0 else -q, held, [L], None, 1, False, scale=abs(scale), H=1)
+
+
 def test_rows_cut_from_wider_ones():
     """One token of one sequence and head out of rows of odd width, written and asked for: strides of dimensions of size one."""
     g = _gen(83)
@@ -1024,6 +1039,60 @@ def test_stream_attention_layer(axes, special):
         rows = ops.restore_tokens(o, o_s, frames, P, special)
         with torch.no_grad():
             assert torch.equal(y, m.proj(rows))
+
+
+@pytest.mark.parametrize("axes", [2, 3])
+def test_stream_attention_of_special_tokens_only(axes):
+    """Frames whose tokens are all special attend to everything, with and without a choice of pages."""
+    from vasc_amd.aggregator import RotaryPositionEmbedding2D, RotaryPositionEmbeddingAxes
+    from vasc_amd.streaming import stream_attention
+    g = _gen(109)
+    m = _module(rope=RotaryPositionEmbedding2D(100.0) if axes == 2 else RotaryPositionEmbeddingAxes((16, 24, 24)))
+    x, pos = _randn(g, 2, 3 * 30, 256).cuda(), torch.randint(0, 40, (2, 90, axes), generator=g).int().cuda()
+    table, pages = _table(g, 2, 2)
+    want = stream_attention(m, x, pos, BlockCache(pages, 4, 64), table, _i32([0, 0]), _i32([90, 90]), keep=None)
+    for keep in (None, 1):
+        got = stream_attention(m, x, pos, BlockCache(pages, 4, 64), table, _i32([0, 0]), _i32([90, 90]), keep=keep, frames=3,
+                               special=30)
+        # the same rows in units of another size: bf16 of the attention and of the projection, whose sums it moves by as much
+        assert (got.float() - want.float()).abs().max() <= 2.0 ** -6 * want.float().abs().max()
+
+
+@pytest.mark.parametrize("axes", [2, 3])
+def test_stream_attention_captured(axes):
+    """One captured layer serves every step: the lengths and the inputs are device tensors that move on."""
+    from vasc_amd.aggregator import RotaryPositionEmbedding2D, RotaryPositionEmbeddingAxes
+    from vasc_amd.streaming import stream_attention
+    g = _gen(113)
+    m = _module(rope=RotaryPositionEmbedding2D(100.0) if axes == 2 else RotaryPositionEmbeddingAxes((16, 24, 24)))
+    B, T, steps = 2, 105, 5
+    table, pages = _table(g, B, -(-steps * T // 64))
+    xs = [_randn(g, B, T, 256).cuda() for _ in range(steps)]
+    ps = [torch.randint(0, 40, (B, T, axes), generator=g).int().cuda() for _ in range(steps)]
+
+    def layer(cache, x, pos, start, lengths):
+        return stream_attention(m, x, pos, cache, table, start, lengths, keep=2, special=5)
+
+    cache = BlockCache(pages, 4, 64)
+    eager = [layer(cache, xs[i], ps[i], _i32([i * T] * B), _i32([i * T + T] * B)) for i in range(steps)]
+    st = dict(cache=BlockCache(pages, 4, 64), x=xs[0].clone(), pos=ps[0].clone(), start=_i32([0] * B), lengths=_i32([T] * B))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        layer(**st)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = layer(**st)
+    for i in range(steps):
+        st["x"].copy_(xs[i])
+        st["pos"].copy_(ps[i])
+        st["start"].fill_(i * T)
+        st["lengths"].copy_(st["start"] + T)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, eager[i]), i
+        torch.randn(1 << 16, device="cuda").sum().item()  # other work between replays
 
 
 def test_dense_layer_with_three_axes():
