@@ -19,17 +19,16 @@
  * vc's last dimension and vs hold token t of the page at
  *   ((t >> 2) & 3) * 16 + (t >> 4) * 4 + (t & 3),
  * ks at (t & 15) * 4 + (t >> 4): the orders in which the lanes of a matrix
- * product consume them. A row's
- * exponent is the smallest e in [-60, 60] with max|x| <= 448 * 2^e: every
- * value is exact in bfloat16, sums of 2^e over a softmax stay inside float32,
- * values past 448 * 2^60 saturate and those under 2^-70 are zero. A token
- * whose key or value row of a head holds a value that is not finite has key
- * exponent byte 255 there and zero codes: both rows read back as NaN. A cache
- * starts as zeros.
+ * product consume them. A row's exponent is the smallest e in [-60, 60] with
+ * max|x| <= 448 * 2^e: every value is exact in bfloat16, values past 448 * 2^60
+ * saturate and those under 2^-70 are zero. A token whose key or value row of a
+ * head holds a value that is not finite has key exponent byte 255 there and
+ * zero codes: both rows read back as NaN. A cache starts as zeros.
  *
  * Sequence b's page j is page_table[b * table_stride + j], j < max_pages
  * (int32). Entries outside [0, P) are no page: nothing is written there, and
- * their tokens are never seen. Lengths past max_pages * 64 are cut to it.
+ * their tokens are never seen. Lengths past max_pages * 64 are cut to it (the
+ * positions of causal rows are not).
  */
 #ifndef VASC_STREAM_H
 #define VASC_STREAM_H
@@ -112,10 +111,10 @@ int64_t vasc_cache_attn_workspace_size(int64_t B, int64_t Hq, int64_t H, int64_t
  * see no key and rows past q_count[b] are zero; a row that sees a NaN token,
  * or whose query is not finite, is NaN. index [B,H,U,width], count
  * [B,H,U] as vasc_cache_select writes them: ascending logical pages; entries
- * that are not above the one before, negative or not below max_pages are
- * skipped. block_q as there (index NULL: any block_q with block_q * G <= 128).
+ * that are not above the one before them in the list (skipped or not),
+ * negative or not below max_pages are skipped. block_q as there (index NULL: any block_q with block_q * G <= 128).
  * q, o [B,Hq,T,D] strided, bfloat16 or float16. scale: 0, or of magnitude
- * 1e-30 to 1e30.
+ * 1e-30 to 1e30. Logits of finite values that pass float32 are not held.
  */
 int vasc_cache_attn(const void *q, int64_t q_sb, int64_t q_sh, int64_t q_st, void *o, int64_t o_sb, int64_t o_sh,
                     int64_t o_st, int64_t B, int64_t Hq, int64_t H, int64_t T, int64_t D, int32_t dtype,

@@ -203,7 +203,9 @@ __global__ __launch_bounds__(256) void cache_write_kernel(const CacheArgs c, con
       *at = word[q];
     }
   }
-  // the page's key mean: float64 sums of exact values, so the order of the rows does not show
+  // The page's key mean, summed in float64 in an order that the slots fix (a group of threads takes every kGroups-th, the
+  // groups are added in turn), whatever calls brought the rows: the same bytes in any portions. The order would not show by
+  // itself only where the page's exponents lie within some 40 of one another, as then all sums are exact.
   {
     const int dcol = (tid % (D / 4)) * 4, grp = tid / (D / 4);
     double s[4] = {0, 0, 0, 0};
@@ -340,8 +342,8 @@ __device__ __forceinline__ Unit unit_of(const SelectParams &p, int row) {
 // asks for its pages' places before it has seen the lengths and for their means before it sums the queries; the sums of
 // kScoreBatch pages cross the lanes together, each step leaving a lane half the pages; and a workgroup takes as many
 // rounds of pages as leave the chip some four workgroups a CU.
-// Measured: 16 x 131072 tokens, 8 heads of 128, in 13.6 us (3.2 TB/s); nine
-// units of a frame against 2082 pages, 16 heads of 64, in 13.1 us.
+// Measured: 16 x 131072 tokens, 8 heads of 128, in 14.0 us (3.1 TB/s); nine
+// units of a frame against 2082 pages, 16 heads of 64, in 12.5 us.
 constexpr int kScoreBatch = 8;
 
 // Sums v[0..8) over the lanes that differ in the bits [lo, hi) of the lane number; a lane is left with the sum of element
@@ -492,7 +494,9 @@ __device__ __forceinline__ uint32_t score_key(float f) {
 // exactly ends it. More waves would pay a barrier a bit (9.9 us for 128 lists of 2048 pages): they sort into 2048 bins by
 // the next 11 bits instead, until the bin that holds the cut has at most kRanked members (scores of one sign and size spread
 // over some dozens of bins, so most lists need one turn), which are then ranked among themselves.
-// Measured: 128 lists of 2048 pages or 144 of 2082 in 8.6 us: 4.5 until the scores are there, 1.4 for the bins, 1.5 for the
+// Past 8192 pages a thread holds 32 elements: 8 lists (with their scores, 8 heads of 128) take 17.5 us for 8192 pages, 38
+// for 8193, 51 for 32768.
+// Measured: 128 lists of 2048 pages or 144 of 2082 in 8.3 us: 4.5 until the scores are there, 1.4 for the bins, 1.5 for the
 // ranks, the rest for the list; latency throughout.
 constexpr int kBins = 2048, kRanked = 128;
 

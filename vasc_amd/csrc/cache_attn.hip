@@ -387,8 +387,8 @@ struct Rows {
 
 // Few rows (up to 32): the cache's bytes bound the kernel. Each of the 4 waves holds all of the unit's rows, kTiles tiles of
 // 16, and takes every fourth page straight from memory to its registers; their sums are joined in LDS.
-// Measured: single tokens of 16 sequences, 8 x 4 heads of 128, 258 pages each, 545 MB in 103 us (5.3 TB/s; a large copy
-// reaches 4.75); more and shorter parts cost more in starts than they even out (4 pages a wave: 126 us).
+// Measured: single tokens of 16 sequences, 8 x 4 heads of 128, 258 pages each, 545 MB in 105 us (5.2 TB/s; a large copy
+// reaches 4.84); more and shorter parts cost more in starts than they even out (4 pages a wave: 126 us).
 template <typename Q, int D, int kTiles>
 __global__ __launch_bounds__(256, 2) void cache_attn_few_kernel(const AttnParams p) {
   constexpr int kWaves = 4, kDT = D / 16, kRows = kTiles * 16;
@@ -562,12 +562,15 @@ __global__ __launch_bounds__(256, 2) void cache_attn_few_kernel(const AttnParams
 // a page is widened once for all of them: each wave turns its share of the codes into operands in LDS (keys as bfloat16 with
 // their powers, values as half, and the values' exponents as floats), 16 bytes a lane in the order in which they are read.
 // Two buffers and one barrier a page: the next page's codes are on their way to registers while this one is computed.
-// Measured: a frame of 1041 queries over 522 of 2082 pages, 16 heads of 64, 142 GFLOP in 225 us with the join (630 TFLOP/s);
-// 250 causal tokens of 32 heads of 128 over 20001, 163 GFLOP in 191 us (850). A wave's page (32 rows, D = 64) takes some
-// 1700 cycles: 208 vector instructions, 32 of them exp2, and 32 matrix ones; the same mix from registers alone takes 1110
-// with three waves a SIMD, the matrix pipe by itself 516. Also built, and no faster: values widened with their powers and
-// weights summed by a product with ones (253 us, D = 128 slower), the next page's first product beside this page's
-// exponentials (registers leave two waves a SIMD: 245 us), 64 rows a wave (265 us).
+// Measured: a frame of 1041 queries over 522 of 2082 pages, 16 heads of 64, 142 GFLOP in 229 us with the join (620 TFLOP/s);
+// 250 causal tokens of 32 heads of 128 over 20001, 163 GFLOP in 196 us (830). A wave's page (32 rows, D = 64) takes some
+// 1800 cycles: some 220 vector instructions, 32 of them exp2, and 32 matrix ones; the same mix from registers alone takes 1110
+// with three waves a SIMD, the matrix pipe by itself 516. The widening is 16 of them; the softmax's care is most: a maximum of
+// 16 exponents a row (16 max3, two steps between lanes a tile, a ballot), 32 multiply-adds for the scale and the values' powers
+// and 32 for the sum. The library's attention over bf16 blocks does the same tile without these in 943 cycles (no maximum a
+// block, sums as matrix products, four waves a SIMD). Also built, while the kernel took 248 us, and no faster: values widened
+// with their powers and weights summed by a product with ones (253 us, D = 128 slower), the next page's first product beside
+// this page's exponentials (registers leave two waves a SIMD: 245 us), 64 rows a wave (265 us). All three kept the maximum.
 template <typename Q, int D, int kTiles, int kWaves>
 __global__ __launch_bounds__(kWaves * 64, D == 64 && kWaves == 4 ? 3 : 2) void cache_attn_many_kernel(const AttnParams p) {
   constexpr int kDT = D / 16, kK = D / 64, kMul = kK * 2;
@@ -668,7 +671,7 @@ __global__ __launch_bounds__(kWaves * 64, D == 64 && kWaves == 4 ? 3 : 2) void c
             }
         }
       // The softmax goes before the other waves' products: the matrix pipe works on while its instructions are issued. Measured
-      // for the frame above, one card: 256 us without, 249 with, 254 with the products before the softmax.
+      // in turn on one card: the frame above 241 us without, 230 with, the causal chunk 202 and 194.
       __builtin_amdgcn_s_setprio(1);
 #pragma unroll
       for (int t = 0; t < 4; ++t) {
@@ -789,8 +792,11 @@ struct Shape {
 // Few rows (up to 32) or many (64, 128), and how many workgroups share a unit's pages: as many as one to four rounds of
 // resident workgroups take (their registers allow 4 to 2 on a CU), or one, whichever is estimated to take least. Measured,
 // in us: a wave's page where few run 0.3 (many rows, three workgroups a CU: 2.5; D = 128, two: 3), the start of a round
-// 3, the join 4 and 0.25 a MB of sums. A last round that is not full takes as long as the others: 144 units of a frame
-// run in 266 us with 5 parts, in 305 with 6 and in 263 with 16.
+// 3, the join 4 and 0.25 a MB of sums. A last round that is not full takes as long as the others. With other parts than the
+// rule's, in us: 144 units of a frame (the rule takes 5) 234 with 5, 279 with 4, 289 with 6, 237 with 10, 259 with 16;
+// a causal chunk of 128 units (4) 208 with 4, 303 with 2, 219 with 8; 128 units of single tokens, 258 pages (4) 108 with 4,
+// 138 with 1, 107 with 2, 112 with 8; of 521 pages (8) 85 with 8, 82 with 4, 83 with 16. The pages are the list's width or the
+// table's, as the lengths are on the device: short sequences in a long table leave parts empty.
 Shape attn_shape(int64_t units, int64_t rows, int64_t pages, int64_t D) {
   Shape s;
   s.kind = rows <= 16 ? 0 : rows <= 32 ? 1 : rows <= 64 ? 2 : 3;

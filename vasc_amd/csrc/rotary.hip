@@ -11,7 +11,10 @@
 // the strides and the pointers allow.
 // Measured (bf16, 16 + 16 heads of 64, sections 16 + 24 + 24, so V = 4): 24
 // frames of 1041 tokens in 46 us, 4.45 TB/s where a large copy reaches 4.75;
-// one frame in 6.3 us, the latency of positions, sines, barrier and rows.
+// one frame in 6.0 us, the latency of positions, sines, barrier and rows.
+// A section whose half is odd leaves V = 1: the clip again and again, partly
+// from the cache behind HBM, 34 us with V = 4, 58 with sections 6 + 28 + 30,
+// 75 with 6 + 28 + 28, whose 33 pieces a row leave 25 of 256 threads idle.
 #include "common.h"
 #include "stream.h"
 
