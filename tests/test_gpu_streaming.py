@@ -1377,3 +1377,36 @@ def test_aggregator_stream_forked():
         for x, y, wx, wy in zip(a, b, one[order], two[order]):
             assert torch.equal(x, wx) and torch.equal(y, wy)
     assert not torch.equal(one[2][1], two[2][1])
+
+
+@pytest.mark.parametrize("axes", [2, 3])
+@pytest.mark.parametrize("how", ["bf16", "float32", "autocast"])
+def test_aggregator_stream_types_and_layouts(how, axes):
+    """float32 models, with autocast or without, as the whole-clip aggregator takes them; a model without a camera token; frames
+    of any memory order, whose results are those of contiguous ones."""
+    import contextlib
+    from vasc_amd.aggregator import Aggregator, RotaryPositionEmbeddingAxes
+    from vasc_amd.streaming import AggregatorStream
+    torch.manual_seed(11)
+    model = Aggregator(dim=512, depth=2, num_heads=8, intermediate_layer_idx=(0, 1), camera_token=how != "float32").cuda()
+    model = model.to(torch.bfloat16) if how == "bf16" else model
+    if axes == 3:
+        rope = RotaryPositionEmbeddingAxes((16, 24, 24), (1e4, 100.0, 100.0))
+        for blk in (*model.frame_blocks, *model.global_blocks):
+            blk.attn.rope = rope
+    images = torch.rand(2, 3, 3, 70, 84, generator=_gen(127)).cuda()
+    other = images.permute(1, 0, 3, 4, 2).contiguous().permute(1, 0, 4, 2, 3)
+    cast = torch.autocast("cuda", torch.bfloat16) if how == "autocast" else contextlib.nullcontext()
+    got = []
+    with cast:
+        for x in (images, other):
+            stream = AggregatorStream(model, 3, sparse_ratio=0.5)
+            got.append([o for a, b in ((0, 1), (1, 3)) for o in stream.push(x[:, a:b])[0]])
+        if axes == 2:
+            with torch.no_grad():
+                want, _ = model(images[:, :1].contiguous())
+            dense = AggregatorStream(model, 1, sparse_ratio=0.0).push(images[:, :1])[0]
+            for a, b in zip(dense, want):
+                assert a.dtype == b.dtype and (a.float() - b.float()).abs().max() <= 0.02 * b.float().abs().max()
+    for a, b in zip(*got):
+        assert a.isfinite().all() and torch.equal(a, b)

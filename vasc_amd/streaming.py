@@ -184,7 +184,7 @@ class AggregatorStream:
         B, n, _, Hi, Wi = images.shape
         if n < 1 or self.frames + n > self.max_frames:
             raise ValueError(f"{n} more frames after {self.frames}: the stream holds {self.max_frames}")
-        x = ((images - m._resnet_mean) / m._resnet_std).view(B * n, 3, Hi, Wi).to(m.patch_embed.weight.dtype)
+        x = ((images - m._resnet_mean) / m._resnet_std).reshape(B * n, 3, Hi, Wi).to(m.patch_embed.weight.dtype)
         tokens = patch_tokens(m.patch_embed, x)
 
         def expand(token):  # the stream's first frame has tokens of its own
