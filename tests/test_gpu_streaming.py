@@ -1410,3 +1410,29 @@ def test_aggregator_stream_types_and_layouts(how, axes):
                 assert a.dtype == b.dtype and (a.float() - b.float()).abs().max() <= 0.02 * b.float().abs().max()
     for a, b in zip(*got):
         assert a.isfinite().all() and torch.equal(a, b)
+
+
+def test_sparse_layer_with_three_axes():
+    """The sparse layer over (time, row, column) positions, nothing left out: float32 attention on the same q, k, v, special
+    tokens among the keys, as test_dense_layer_with_three_axes bounds it."""
+    from vasc_amd.aggregator import RotaryPositionEmbeddingAxes
+    from vasc_amd.attention import adaptive_sparse_attention_forward
+    g = _gen(131)
+    m = _module(rope=RotaryPositionEmbeddingAxes((16, 24, 24), (1e4, 100.0, 100.0)))
+    B, n, grid, S = 2, 3, (6, 7), 5
+    P = S + grid[0] * grid[1]
+    x = _randn(g, B, n * P, 256).cuda()
+    pos = torch.from_numpy(_layer_positions(B, 40, n, grid, S, 3).copy()).cuda()
+    with torch.no_grad():
+        y = adaptive_sparse_attention_forward(m, x, pos, sparse_ratio=0.0, num_special_tokens=S, num_heads=4)
+        y = y[0] if isinstance(y, tuple) else y
+        qkv = m.qkv(x).view(B, n * P, 3, 4, 64)
+        q, k = m.rope.rotate(m.q_norm(qkv[:, :, 0].transpose(1, 2)), m.k_norm(qkv[:, :, 1].transpose(1, 2)), pos)
+        v = qkv[:, :, 2].transpose(1, 2).float()
+        p = torch.softmax((q.float() @ k.float().transpose(2, 3).contiguous()) / 8, -1)
+        o = p @ v
+        slack = 2.0 ** -8 * (p @ v.abs()) + 2.0 ** -8 * o.abs()
+        w = m.proj.weight.float()
+        flat = lambda t: t.transpose(1, 2).reshape(B, n * P, 256)  # noqa: E731
+        ref, bound = flat(o) @ w.T.contiguous() + m.proj.bias.float(), flat(slack) @ w.T.contiguous().abs()
+    assert ((y.float() - ref).abs() <= bound + 2.0 ** -8 * (ref.abs() + bound) + 1e-4).all()
