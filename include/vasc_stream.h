@@ -1,8 +1,8 @@
 /*
  * Streaming ops of libvasc_hip.so: the operators of a global layer whose
  * frames (or single query tokens) arrive one after another. Keys and values
- * stay in an 8-bit block cache; queries attend to cache blocks that a cheap
- * score chooses. They have no counterpart in the reference, which sees a
+ * stay in a block cache of 8 bits or 4; queries attend to cache blocks that a
+ * cheap score chooses. They have no counterpart in the reference, which sees a
  * whole clip at once; vasc_amd/streaming.py calls them.
  *
  * Conventions as in vasc_hip.h: raw device pointers, int64 sizes and element
@@ -24,6 +24,26 @@
  * saturate and those under 2^-70 are zero. A token whose key or value row of a
  * head holds a value that is not finite has key exponent byte 255 there and
  * zero codes: both rows read back as NaN. A cache starts as zeros.
+ *
+ * The 4-bit block cache holds e2m1 codes (0, 0.5, 1, 1.5, 2, 3, 4, 6; the sign
+ * in the fourth bit), a power of two for each 32 features of a token's row:
+ *   kc uint8 [P, H, 64 D/2], features f, f + 1 of token t in one byte (f in its
+ *      low half) at t * 64 + f/2 (D 128), or at ((t >> 5) * 16 + (t & 15)) * 64
+ *      + (f >> 4) * 16 + ((t >> 4) & 1) * 8 + (f & 15)/2 (D 64)
+ *   vc uint8 [P, H, 64 D/2], feature f of token t, whose place p is vs's, at
+ *      ((f >> 5) * 64 + (f & 15) * 4 + (p >> 4)) * 16 + ((f >> 4) & 1) * 8
+ *      + (p & 15)/2, in the low half where p is even
+ *   ks uint8 [P, H, D/32, 64]  exponents of the key rows' groups, ks's order
+ *   vs uint8 [P, H, 64]        exponents of the value rows' largest groups
+ *   vo uint8 [P, H, 4, D/32, 2, 4]  at [p >> 4, group, (p >> 3) & 1] a word
+ *      with 15 less what the token's group lies below vs, in the four bits from
+ *      (p & 7)/2 * 4 + (p & 1) * 16 on
+ *   mean as above.
+ * A group's exponent is the smallest e in [-60, 60] with max|x| <= 7 * 2^e, of
+ * a value row at least its largest less 14; values past 6 * 2^e saturate.
+ * Codes are the nearest, ties to the even code. NaN tokens as above, byte 255
+ * in all of the row's groups. vasc_cache4_* take such a cache, and
+ * vasc_cache_select its means.
  *
  * Sequence b's page j is page_table[b * table_stride + j], j < max_pages
  * (int32). Entries outside [0, P) are no page: nothing is written there, and
@@ -122,6 +142,77 @@ int vasc_cache_attn(const void *q, int64_t q_sb, int64_t q_sh, int64_t q_st, voi
                     const int32_t *page_table, int64_t table_stride, int64_t max_pages, const int32_t *lengths,
                     const int32_t *q_count, int64_t block_q, const int32_t *index, int64_t width, const int32_t *count,
                     int32_t causal, float scale, void *workspace, int64_t workspace_bytes, void *stream);
+
+/* vasc_cache_write, vasc_cache_read and vasc_cache_attn for a 4-bit cache; the workspace is vasc_cache_attn's. */
+int vasc_cache4_write(const void *k, int64_t k_sb, int64_t k_sh, int64_t k_st, const void *v, int64_t v_sb, int64_t v_sh,
+                      int64_t v_st, int64_t B, int64_t H, int64_t T, int64_t D, int32_t dtype,
+                      const int32_t *page_table, int64_t table_stride, int64_t max_pages, const int32_t *start,
+                      const int32_t *count, uint8_t *kc, uint8_t *vc, uint8_t *ks, uint8_t *vs, uint8_t *vo,
+                      uint16_t *mean, int64_t pages, void *stream);
+int vasc_cache4_read(const uint8_t *kc, const uint8_t *vc, const uint8_t *ks, const uint8_t *vs, const uint8_t *vo,
+                     int64_t pages, const int32_t *page_table, int64_t table_stride, int64_t max_pages,
+                     const int32_t *start, const int32_t *count, int64_t B, int64_t H, int64_t T, int64_t D,
+                     int32_t dtype, void *k_out, void *v_out, void *stream);
+int vasc_cache4_attn(const void *q, int64_t q_sb, int64_t q_sh, int64_t q_st, void *o, int64_t o_sb, int64_t o_sh,
+                     int64_t o_st, int64_t B, int64_t Hq, int64_t H, int64_t T, int64_t D, int32_t dtype,
+                     const uint8_t *kc, const uint8_t *vc, const uint8_t *ks, const uint8_t *vs, const uint8_t *vo,
+                     int64_t pages, const int32_t *page_table, int64_t table_stride, int64_t max_pages,
+                     const int32_t *lengths, const int32_t *q_count, int64_t block_q, const int32_t *index,
+                     int64_t width, const int32_t *count, int32_t causal, float scale, void *workspace,
+                     int64_t workspace_bytes, void *stream);
+
+/*
+ * Copies page src[i] of a cache (bits 8 or 4; vo NULL with 8) to page dst[i],
+ * i < n; pairs with a number outside [0, pages) are skipped. No page may be
+ * written twice in one call, nor be both written and copied from.
+ */
+int vasc_cache_copy(int32_t bits, uint8_t *kc, uint8_t *vc, uint8_t *ks, uint8_t *vs, uint8_t *vo, uint16_t *mean,
+                    int64_t pages, int64_t H, int64_t D, const int32_t *src, const int32_t *dst, int64_t n, void *stream);
+
+/*
+ * Token index[b*index_sb + h*index_sh + i] of the sequence that page_table
+ * holds becomes token i < count[b] (NULL: n) of head h of the one that
+ * out_table [B, out_pages] holds, codes and exponents as they are; what is no
+ * token of page_table becomes zeros. The key means of the pages written are
+ * renewed as by vasc_cache_write. No page may occur twice among those written,
+ * nor be both written and read from.
+ */
+int vasc_cache_compact(int32_t bits, uint8_t *kc, uint8_t *vc, uint8_t *ks, uint8_t *vs, uint8_t *vo, uint16_t *mean,
+                       int64_t pages, int64_t H, int64_t D, const int32_t *page_table, int64_t table_stride,
+                       int64_t max_pages, const int32_t *index, int64_t index_sb, int64_t index_sh,
+                       const int32_t *count, int64_t B, int64_t n, const int32_t *out_table, int64_t out_stride,
+                       int64_t out_pages, void *stream);
+
+/*
+ * Page tables that share pages. refs [pages] int32 counts the entries of all
+ * tables that name a page; a page is free where it is not positive.
+ *
+ * Fork: row i < rows of out_table [rows, max_pages] gets the pages of
+ * lengths[s] tokens of row s = source[i] of page_table [B, max_pages], and -1
+ * behind them (s outside [0, B): -1 throughout); out_lengths[i] the tokens.
+ */
+int vasc_pages_fork(int32_t *refs, int64_t pages, const int32_t *page_table, int64_t table_stride, int64_t max_pages,
+                    const int32_t *lengths, int64_t B, const int32_t *source, int64_t rows, int32_t *out_table,
+                    int32_t *out_lengths, void *stream);
+
+/* Free: entries behind the pages of the first min(lengths[b], keep[b]) tokens (keep NULL: 0) become -1; that is lengths[b] now. */
+int vasc_pages_free(int32_t *refs, int64_t pages, int32_t *page_table, int64_t table_stride, int64_t max_pages,
+                    int32_t *lengths, int64_t B, const int32_t *keep, void *stream);
+
+/*
+ * Reserve: of the pages that tokens lengths[b] .. lengths[b] + count[b]
+ * (NULL: tokens; cut to what max_pages hold) touch, those that are missing
+ * (no page, or a count that is not 1) are replaced, in the order of sequences
+ * and pages, by the free pages, lowest first; a replaced page counts a holder
+ * less. granted[b]: those tokens, or 0 where the free pages do not suffice for
+ * this sequence and all before it that lack some: its row is left as it is.
+ * src[b], dst[b]: the replaced page that holds tokens before lengths[b], and
+ * its replacement, or -1.
+ */
+int64_t vasc_pages_reserve_workspace_size(int64_t pages, int64_t max_pages, int64_t B, int64_t tokens);
+int vasc_pages_reserve(int32_t *refs, int64_t pages, int32_t *page_table, int64_t table_stride, int64_t max_pages,
+                       const int32_t *lengths, int64_t B, int64_t tokens, const int32_t *count, int32_t *granted,
+                       int32_t *src, int32_t *dst, void *workspace, int64_t workspace_bytes, void *stream);
 
 #ifdef __cplusplus
 }

@@ -1,7 +1,7 @@
 """Streamed global attention in float64: the definitions behind
 ``include/vasc_stream.h``, from the formulas, one row at a time.
 
-``quantise`` is exact (every step is a power of two times a small integer),
+``quantise`` and ``quantise4`` are exact (every step is a power of two times a small integer),
 ``select`` decides on scores that float64 holds to far less than a float32
 step; ``attend`` and ``rotate`` are what the kernels are within rounding of.
 """
@@ -52,6 +52,109 @@ def quantise(k: np.ndarray, v: np.ndarray) -> tuple[np.ndarray, np.ndarray]:
             e = exponent(x[at])
             o[at] = e4m3(np.clip(np.ldexp(x[at], -e), -448.0, 448.0)) * math.ldexp(1.0, e)
     return ko, vo
+
+
+GROUP, LOWEST = 32, 14  # features under one power; powers of two that a value row's groups may lie below its largest
+
+
+def e2m1(y: np.ndarray) -> np.ndarray:
+    """The nearest e2m1 value (ties to the even code); past 6: 6."""
+    y = np.asarray(y, np.float64)
+    _, e = np.frexp(y)
+    step = np.ldexp(1.0, np.maximum(e - 1, 0) - 1)
+    return np.clip(np.rint(y / step) * step, -6.0, 6.0)
+
+
+def exponent4(group: np.ndarray) -> int:
+    """Smallest e in [E_MIN, E_MAX] with max|group| <= 7 * 2^e (E_MAX where none is)."""
+    top = float(np.abs(group).max(initial=0.0))
+    for e in range(E_MIN, E_MAX):
+        if top <= math.ldexp(7.0, e):
+            return e
+    return E_MAX
+
+
+def quantise4(k: np.ndarray, v: np.ndarray) -> tuple[np.ndarray, np.ndarray]:
+    """What the 4-bit cache holds for rows k, v ``[..., D]`` of one token and head each."""
+    k, v = np.asarray(k, np.float64), np.asarray(v, np.float64)
+    ko, vo = np.empty_like(k), np.empty_like(v)
+    for at in np.ndindex(k.shape[:-1]):
+        if not (np.isfinite(k[at]).all() and np.isfinite(v[at]).all()):
+            ko[at] = vo[at] = np.nan
+            continue
+        for x, o, below in ((k, ko, None), (v, vo, LOWEST)):
+            groups = x[at].reshape(-1, GROUP)
+            es = [exponent4(g) for g in groups]
+            if below is not None:
+                es = [max(e, max(es) - below) for e in es]
+            o[at] = np.concatenate([e2m1(np.ldexp(g, -e)) * math.ldexp(1.0, e) for g, e in zip(groups, es)])
+    return ko, vo
+
+
+class Pool:
+    """Page tables that share pages, one entry at a time: lists of rows, -1 for no page."""
+
+    def __init__(self, refs):
+        self.refs = list(refs)
+
+    def fork(self, table, lengths, source):
+        out, tokens = [], []
+        for s in source:
+            inside = 0 <= s < len(table)
+            mp = len(table[0])
+            n = max(0, min(lengths[s], mp * PAGE)) if inside else 0
+            row = [table[s][j] if inside and j * PAGE < n else -1 for j in range(mp)]
+            row = [p if 0 <= p < len(self.refs) else -1 for p in row]
+            for p in row:
+                if p >= 0:
+                    self.refs[p] += 1
+            out.append(row)
+            tokens.append(n)
+        return out, tokens
+
+    def free(self, table, lengths, keep):
+        """(table, lengths) afterwards."""
+        out, tokens = [], []
+        for row, n, k in zip(table, lengths, keep):
+            n = min(max(0, min(n, len(row) * PAGE)), max(0, k))
+            for p in row[-(-n // PAGE):]:
+                if 0 <= p < len(self.refs):
+                    self.refs[p] -= 1
+            out.append(row[:-(-n // PAGE)] + [-1] * (len(row) - -(-n // PAGE)))
+            tokens.append(n)
+        return out, tokens
+
+    def reserve(self, table, lengths, counts):
+        """(table, granted, src, dst): decided on the holders before the call."""
+        before = list(self.refs)
+        free = [p for p, r in enumerate(before) if r <= 0]
+        table = [list(row) for row in table]
+        granted, src, dst, wanted = [], [], [], 0
+        for row, n, c in zip(table, lengths, counts):
+            mp = len(row)
+            n = max(0, min(n, mp * PAGE))
+            c = max(0, min(c, mp * PAGE - n))
+            lacking = [j for j in range(n // PAGE, -(-(n + c) // PAGE) if c else 0)
+                       if not (0 <= row[j] < len(before) and before[row[j]] == 1)]
+            at, wanted = wanted, wanted + len(lacking)
+            ok = not lacking or wanted <= len(free)
+            granted.append(c if ok else 0)
+            s = d = -1
+            for i, j in enumerate(lacking):
+                held = 0 <= row[j] < len(before)
+                if not ok:
+                    row[j] = row[j] if held else -1
+                    continue
+                if held:
+                    if before[row[j]] > 0:
+                        self.refs[row[j]] -= 1
+                    if j * PAGE < n:
+                        s, d = row[j], free[at + i]
+                row[j] = free[at + i]
+                self.refs[row[j]] = 1
+            src.append(s)
+            dst.append(d)
+        return table, granted, src, dst
 
 
 def page_means(k: np.ndarray) -> np.ndarray:

@@ -1,0 +1,350 @@
+"""Pages of a block cache: copies, compaction, and page tables that share pages, against oracle/streaming.py."""
+import copy
+import pickle
+import random
+
+import numpy as np
+import pytest
+import torch
+
+from oracle import streaming as O
+from test_gpu_streaming import _check_attend, _gen, _i32, _np, _randn, _same, _table
+from vasc_amd import ops
+from vasc_amd.streaming import BlockCache, PagePool
+
+pytestmark = pytest.mark.gpu
+
+QUANTISE = {8: O.quantise, 4: O.quantise4}
+
+
+def _names(cache):
+    return [n for n in ("kc", "vc", "ks", "vs", "vo", "mean") if getattr(cache, n) is not None]
+
+
+def _noise(cache, g):
+    """Finite codes everywhere, so that a byte that moves where it should not is seen."""
+    for n in _names(cache):
+        t = getattr(cache, n)
+        if n == "mean":
+            t.copy_(torch.randn(t.shape, generator=g))
+        else:
+            lo, hi = (110, 140) if n in ("ks", "vs") else (0, 0x7e)
+            t.copy_(torch.randint(lo, hi, t.shape, generator=g, dtype=torch.uint8))
+
+
+# ------------------------------------------------------------------ copies
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("D,H", [(64, 1), (128, 3), (64, 16)])
+def test_copy(bits, D, H):
+    g = _gen(D + H)
+    cache = BlockCache(40, H, D, bits=bits)
+    _noise(cache, g)
+    before = {n: getattr(cache, n).clone() for n in _names(cache)}
+    pairs = [(3, 20), (3, 21), (39, 0), (-1, 22), (5, -1), (40, 23), (6, 40), (7, 7), (2 ** 31 - 1, 24)]
+    src, dst = _i32([a for a, _ in pairs]), _i32([b for _, b in pairs])
+    ops.cache_copy(cache, src, dst)
+    moved = {20: 3, 21: 3, 0: 39}
+    for n, t in before.items():
+        want = t.clone()
+        for d, s in moved.items():
+            want[d] = t[s]
+        assert torch.equal(getattr(cache, n), want), n
+    ops.cache_copy(cache, src[:0], dst[:0])
+    ops.cache_copy(cache, torch.tensor([2 ** 40, 2], device="cuda"), torch.tensor([25, 26], device="cuda"))
+    assert torch.equal(cache.kc[25], before["kc"][25]) and torch.equal(cache.kc[26], before["kc"][2])
+
+
+# ------------------------------------------------------------------ compaction
+def _check_compact(cache, held, table, index, out_table, counts, before, g):
+    """Everything of the cache after cache_compact: `held` float64 [B][k, v][H,L,D]."""
+    B, H = len(held), cache.heads
+    n = index.shape[-1]
+    idx = index if index.dim() == 3 else index.unsqueeze(1).expand(-1, H, -1)
+    k, v = ops.cache_read(cache, out_table, _i32([0] * B), n, dtype=torch.float32)
+    touched = set()
+    for b in range(B):
+        c = max(0, min(counts[b], n))
+        for h in range(H):
+            at = idx[b, h, :c].cpu().numpy()
+            inside = (at >= 0) & (at < held[b][0].shape[1])
+            kk = np.where(inside[:, None], held[b][0][h][np.where(inside, at, 0)], 0)
+            vv = np.where(inside[:, None], held[b][1][h][np.where(inside, at, 0)], 0)
+            assert _same(_np(k[b, h, :c]), kk) and _same(_np(v[b, h, :c]), vv), (b, h)
+            for j in range(-(-c // 64)):
+                p = int(out_table[b, j])
+                touched.add(p)
+                part = kk[j * 64:j * 64 + 64]
+                mean = O.round_bf16((part.sum(0) / len(part)).astype(np.float32))
+                assert _same(_np(cache.mean[p, h]), mean.astype(np.float64))
+    for name, t in before.items():
+        rest = [p for p in range(cache.pages) if p not in touched]
+        assert torch.equal(getattr(cache, name)[rest].view(torch.uint8), t[rest].view(torch.uint8)), name  # NaN means alike
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("D,H", [(64, 3), (128, 2)])
+@pytest.mark.parametrize("per_head", [False, True])
+@pytest.mark.parametrize("run", [1, 5, 64, 200])
+def test_compact(bits, D, H, per_head, run):
+    """Runs and single tokens, whole and ragged pages, none and all kept; slots behind the last token stay."""
+    g = _gen(D + run)
+    lens = [520, 1, 300, 0, 64]
+    B, mp, n = len(lens), 9, 330
+    table, pages = _table(g, B, mp, spare=B * 7)
+    cache = BlockCache(pages, H, D, bits=bits)
+    _noise(cache, g)
+    k, v = _randn(g, B, H, 520, D), _randn(g, B, H, 520, D)
+    k[2, 0, 17, 3] = float("nan")
+    ops.cache_write(cache, k.cuda(), v.cuda(), table, _i32([0] * B), count=_i32(lens))
+    held = [QUANTISE[bits](_np(k[b, :, :m]), _np(v[b, :, :m])) for b, m in enumerate(lens)]
+    used = set(table.flatten().tolist())
+    out = _i32([p for p in range(pages) if p not in used][:B * 6]).view(B, 6)
+    counts = [330, 1, 129, 0, 64]
+    index = torch.full((B, H, n), -1, dtype=torch.int32)
+    for b, m in enumerate(lens):
+        for h in range(H):
+            order = torch.randperm(-(-m // run) or 1, generator=g)
+            at = torch.cat([torch.arange(r * run, min((r + 1) * run, m)) for r in order.tolist()])[:counts[b]]
+            if run != 5:
+                at = at.sort().values
+            index[b, h, :len(at)] = at.int()
+    index = index if per_head else index[:, 0]
+    before = {nm: getattr(cache, nm).clone() for nm in _names(cache)}
+    old_k, _ = ops.cache_read(cache, out, _i32([0] * B), 384, dtype=torch.float32)
+    ops.cache_compact(cache, table, index.cuda(), out, count=_i32(counts))
+    _check_compact(cache, held, table, index, out, counts, before, g)
+    new_k, _ = ops.cache_read(cache, out, _i32([0] * B), 384, dtype=torch.float32)
+    for b, c in enumerate(counts):
+        assert torch.equal(new_k[b, :, c:], old_k[b, :, c:])
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+def test_compact_of_what_is_not_there(bits):
+    """Entries that are no token of the table are zeros; tables with holes; out_table entries that are no page; counts outside;
+    lists of 64 bits, strided and expanded ones, the same token twice."""
+    g = _gen(7)
+    cache = BlockCache(12, 2, 64, bits=bits)
+    _noise(cache, g)
+    k, v = _randn(g, 1, 2, 192, 64), _randn(g, 1, 2, 192, 64)
+    ops.cache_write(cache, k.cuda(), v.cuda(), _i32([[0, 1, 2]]), _i32([0]))
+    ko, vo = QUANTISE[bits](_np(k[0]), _np(v[0]))
+    table = _i32([[0, -1, 2]])
+    index = torch.tensor([[5, -1, 64, 130, 192, 2 ** 33, 5, 191]], device="cuda")
+    hole = np.array([True, False, False, True, False, False, True, True])
+    before = {nm: getattr(cache, nm).clone() for nm in _names(cache)}
+    ops.cache_compact(cache, table, index, _i32([[4]]))
+    rk, rv = ops.cache_read(cache, _i32([[4]]), _i32([0]), 8, dtype=torch.float32)
+    at = np.where(hole, index[0].cpu().numpy(), 0)
+    assert _same(_np(rk[0]), np.where(hole[:, None], ko[:, at], 0)) and _same(_np(rv[0]), np.where(hole[:, None], vo[:, at], 0))
+    for name, t in before.items():
+        assert torch.equal(getattr(cache, name)[5:], t[5:])
+    before = {nm: getattr(cache, nm).clone() for nm in _names(cache)}
+    long = torch.arange(100, device="cuda").view(1, 100)
+    ops.cache_compact(cache, table, long, _i32([[-1, 12]]))
+    ops.cache_compact(cache, table, long, _i32([[6, 7]]), count=_i32([-3]))
+    ops.cache_compact(cache, table, long[:, :0], _i32([[6, 7]]))
+    assert all(torch.equal(getattr(cache, nm), t) for nm, t in before.items())
+    wide = torch.arange(300, device="cuda").view(1, 300)[:, ::3]  # every third, a stride of three
+    ops.cache_compact(cache, _i32([[0, 1, 2]]), wide[:, :60].unsqueeze(1).expand(1, 2, 60), _i32([[6]]), count=_i32([2 ** 31 - 1]))
+    rk, _ = ops.cache_read(cache, _i32([[6]]), _i32([0]), 60, dtype=torch.float32)
+    assert _same(_np(rk[0]), ko[:, :180:3])
+
+
+def test_compact_then_attend():
+    """A sequence that forgets tokens attends as one that never had them."""
+    g = _gen(11)
+    for bits in (4, 8):
+        H, D, L = 2, 128, 500
+        cache = BlockCache(20, H, D, bits=bits)
+        k, v, q = _randn(g, 1, H, L, D).cuda(), _randn(g, 1, H, L, D).cuda(), _randn(g, 1, H * 2, 1, D).cuda()
+        table = _i32([list(range(8))])
+        ops.cache_write(cache, k, v, table, _i32([0]))
+        index = torch.randperm(L, generator=g)[:333].sort().values
+        out = _i32([list(range(10, 16))])
+        ops.cache_compact(cache, table, index.view(1, -1).cuda(), out)
+        o = ops.cache_attn(q, cache, out, _i32([333]))
+        other = BlockCache(6, H, D, bits=bits)
+        ops.cache_write(other, k[:, :, index], v[:, :, index], _i32([list(range(6))]), _i32([0]))
+        assert torch.equal(o, ops.cache_attn(q, other, _i32([list(range(6))]), _i32([333])))
+        assert torch.equal(cache.mean[10:16], other.mean)
+
+
+# ------------------------------------------------------------------ page tables
+def _state(pool, *tensors):
+    return [pool.refs.tolist(), *(t.tolist() for t in tensors)]
+
+
+@pytest.mark.parametrize("seed", range(6))
+def test_pool_random_walk(seed):
+    """Forks, reservations (some past the pool), rollbacks and frees in any order, each against the oracle."""
+    r = random.Random(seed)
+    pages, mp = r.choice([40, 300, 5000]), r.choice([3, 9, 70])
+    pool, ref = PagePool(pages), O.Pool([0] * pages)
+    B = r.choice([1, 3, 11])
+    table, lengths = torch.full((B, mp), -1, device="cuda", dtype=torch.int32), _i32([0] * B)
+    rows, tokens = [[-1] * mp for _ in range(B)], [0] * B
+    for turn in range(14):
+        what = r.choice(["reserve", "reserve", "fork", "free"])
+        if what == "reserve":
+            T = r.choice([1, 1, 63, 64, 65, 400])
+            count = None if r.random() < 0.5 else [r.randint(-1, T + 1) for _ in rows]
+            granted, src, dst = ops.pages_reserve(pool, table, lengths, T, None if count is None else _i32(count))
+            rows, g2, s2, d2 = ref.reserve(rows, tokens, [min(T, c) for c in count] if count else [T] * len(rows))
+            assert (granted.tolist(), src.tolist(), dst.tolist()) == (g2, s2, d2)
+            if r.random() < 0.8:  # the tokens are written, or not
+                lengths += granted
+                tokens = [n + c for n, c in zip(tokens, g2)]
+        elif what == "fork":
+            source = [r.randint(-1, len(rows)) for _ in range(r.choice([1, 4, 13]))]
+            new, new_lengths = ops.pages_fork(pool, table, lengths, _i32(source))
+            new_rows, new_tokens = ref.fork(rows, tokens, source)
+            ops.pages_free(pool, table, lengths)
+            assert ref.free(rows, tokens, [0] * len(rows))[0] == table.tolist() and not lengths.any()
+            table, lengths, rows, tokens = new, new_lengths, new_rows, new_tokens
+        else:
+            keep = [r.choice([0, 2 ** 31 - 1, r.randint(-2, mp * 64)]) for _ in rows]
+            ops.pages_free(pool, table, lengths, _i32(keep))
+            rows, tokens = ref.free(rows, tokens, keep)
+        assert _state(pool, table, lengths) == [ref.refs, rows, tokens], (turn, what)
+    ops.pages_free(pool, table, lengths)
+    assert not pool.refs.any() and pool.available() == pages
+
+
+def test_reserve_large():
+    """Pools of many chunks whose free pages are rare, single sequences that need many pages, many that need one."""
+    r = random.Random(3)
+    for pages, mp, B, T in ((70000, 600, 3, 30000), (20000, 4, 700, 1), (4096, 80, 2, 4000), (4097, 80, 1, 4097), (64, 2, 70, 1)):
+        for busy in (0.0, 0.5, 0.97):
+            refs = [int(r.random() < busy) for _ in range(pages)]
+            pool, ref = PagePool(pages), O.Pool(refs)
+            pool.refs.copy_(_i32(refs))
+            table, rows = torch.full((B, mp), -1, device="cuda", dtype=torch.int32), [[-1] * mp for _ in range(B)]
+            lengths = [0] * B
+            out = ops.pages_reserve(pool, table, _i32(lengths), T)
+            rows, *want = ref.reserve(rows, lengths, [T] * B)
+            assert [t.tolist() for t in out] == want
+            assert _state(pool, table) == [ref.refs, rows]
+
+
+def test_reserve_odd_tables():
+    """Entries outside the pool, pages that nobody counts, lengths past the table and below zero, rows of a wider table, 64-bit
+    lengths; a row that gets nothing stays as it was."""
+    pages = 10
+    refs = [1, 2, 0, 1, 1, 0, 0, 1, 3, 0]
+    rows = [[0, 1, -1], [3, 99, -7], [4, 2, 8], [7, -1, -1], [1, 8, 8]]
+    lengths = [70, 64, 130, 200, -4]
+    counts = [64, 128, 10, 5, 3]
+    pool, ref = PagePool(pages), O.Pool(refs)
+    pool.refs.copy_(_i32(refs))
+    wide = torch.full((5, 8), 77, device="cuda", dtype=torch.int32)
+    table = wide[:, 2:5]
+    table.copy_(_i32(rows))
+    got = ops.pages_reserve(pool, table, torch.tensor(lengths, device="cuda"), 200, torch.tensor(counts, device="cuda"))
+    new, *want = ref.reserve(rows, lengths, counts)
+    assert [t.tolist() for t in got] == want and want[0][0] == 64 and want[0][2] == 0 and want[0][3] == 0
+    assert _state(pool, table) == [ref.refs, new]
+    assert (wide[:, :2] == 77).all() and (wide[:, 5:] == 77).all()
+    empty = ops.pages_reserve(pool, table, _i32(lengths), 0)
+    assert [t.tolist() for t in empty] == [[0] * 5, [-1] * 5, [-1] * 5]
+    assert [t.numel() for t in ops.pages_reserve(pool, table[:0], _i32([]), 3)] == [0, 0, 0]
+    none, n = ops.pages_fork(pool, table[:0], _i32([]), _i32([0, 1]))
+    assert (none == -1).all() and not n.any()
+    assert ops.pages_fork(pool, table, _i32(lengths), _i32([]))[0].shape == (0, 3)
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+def test_branches_write_apart(bits):
+    """Three sequences fork into seven; each branch reserves, copies, writes tokens of its own and attends: as a cache that
+    holds its tokens alone. The parents still attend to theirs."""
+    g = _gen(13)
+    H, D, mp = 2, 64, 8
+    pool, cache = PagePool(60), BlockCache(60, H, D, bits=bits)
+    lens = [130, 64, 37]
+    table, n = torch.full((3, mp), -1, device="cuda", dtype=torch.int32), _i32([0, 0, 0])
+    k, v = _randn(g, 3, H, 130, D).cuda(), _randn(g, 3, H, 130, D).cuda()
+    granted, src, dst = ops.pages_reserve(pool, table, n, 130, _i32(lens))
+    ops.cache_write(cache, k, v, table, n, count=granted)
+    n += granted
+    q = _randn(g, 3, H, 1, D).cuda()
+    parents = ops.cache_attn(q, cache, table, n)
+    source = [0, 2, 0, 1, 1, 2, 0]
+    for T in (1, 100):
+        branch, m = ops.pages_fork(pool, table, n, _i32(source))
+        nk, nv, nq = (_randn(g, 7, H, T, D).cuda() for _ in range(3))
+        granted, src, dst = ops.pages_reserve(pool, branch, m, T)
+        assert granted.tolist() == [T] * 7 and (src >= 0).tolist() == [lens[s] % 64 > 0 for s in source]
+        ops.cache_copy(cache, src, dst)
+        ops.cache_write(cache, nk, nv, branch, m, count=granted)
+        o = ops.cache_attn(nq, cache, branch, m + granted)
+        for i, s in enumerate(source):
+            alone = BlockCache(mp, H, D, bits=bits)
+            row = _i32([list(range(mp))])
+            ops.cache_write(alone, torch.cat([k[s:s + 1, :, :lens[s]], nk[i:i + 1]], 2),
+                            torch.cat([v[s:s + 1, :, :lens[s]], nv[i:i + 1]], 2), row, _i32([0]))
+            assert torch.equal(o[i:i + 1], ops.cache_attn(nq[i:i + 1], alone, row, _i32([lens[s] + T])))
+        assert torch.equal(ops.cache_attn(q, cache, table, n), parents)
+        ops.pages_free(pool, branch, m)
+    assert pool.refs.sum() == 3 + 1 + 1 and pool.available() == 55
+
+
+def test_turn_captured_in_graphs():
+    """Fork, reserve, copy, write, attend and free in two graphs, replayed in turn with eager work between."""
+    g = _gen(19)
+    H, D, mp, pages = 1, 64, 6, 64
+
+    def make():
+        pool, cache = PagePool(pages), BlockCache(pages, H, D, bits=4)
+        table, n = torch.full((2, mp), -1, device="cuda", dtype=torch.int32), _i32([0, 0])
+        gg = _gen(5)
+        k, v = _randn(gg, 2, H, 100, D).cuda(), _randn(gg, 2, H, 100, D).cuda()
+        granted, _, _ = ops.pages_reserve(pool, table, n, 100, _i32([100, 70]))
+        ops.cache_write(cache, k, v, table, n, count=granted)
+        return dict(pool=pool, cache=cache, table=table, n=granted.clone(), source=_i32([0, 1, 1, 0]),
+                    k=_randn(gg, 4, H, 3, D).cuda(), q=_randn(gg, 4, H, 1, D).cuda())
+
+    def turn(s):
+        branch, m = ops.pages_fork(s["pool"], s["table"], s["n"], s["source"])
+        granted, src, dst = ops.pages_reserve(s["pool"], branch, m, 3)
+        ops.cache_copy(s["cache"], src, dst)
+        ops.cache_write(s["cache"], s["k"], s["k"], branch, m, count=granted)
+        o = ops.cache_attn(s["q"], s["cache"], branch, m + granted)
+        seen = branch.clone()
+        ops.pages_free(s["pool"], branch, m)
+        return o, seen, granted, s["pool"].refs.clone()
+
+    graphs = []
+    for _ in range(2):
+        s = make()
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            turn(s)
+        torch.cuda.current_stream().wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = turn(s)
+        graphs.append((graph, s, out))
+    e = make()
+    for i in range(4):
+        source, k = _i32([i % 2, 1, i - 1, 0]), _randn(g, 4, H, 3, D).cuda()
+        e["source"], e["k"] = source, k
+        want = turn(e)
+        for graph, s, out in graphs:
+            s["source"].copy_(source)
+            s["k"].copy_(k)
+            graph.replay()
+            torch.cuda.synchronize()
+            for a, b in zip(out, want):
+                assert torch.equal(a, b), i
+            torch.randn(1 << 16, device="cuda").sum().item()
+
+
+@pytest.mark.parametrize("how", ["deepcopy", "copy", "pickle"])
+def test_copied_pool(how):
+    pool = PagePool(8)
+    pool.refs[3] = 2
+    other = {"deepcopy": copy.deepcopy, "copy": copy.copy, "pickle": lambda c: pickle.loads(pickle.dumps(c))}[how](pool)
+    assert other.pointer == other.refs.data_ptr() and (other.pointer == pool.pointer) == (how == "copy")
+    table = torch.full((1, 2), -1, device="cuda", dtype=torch.int32)
+    ops.pages_reserve(other, table, _i32([0]), 128)
+    assert table.tolist() == [[0, 1]] and (pool.refs[0].item() == 1) == (how == "copy")

@@ -44,6 +44,9 @@ SOURCES = {
     "rotary.hip": [],
     "cache.hip": [],
     "cache_attn.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
+    "cache4.hip": [],
+    "cache4_attn.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
+    "pages.hip": [],
 }
 
 

@@ -10,44 +10,10 @@
 // (4.4 TB/s; a large copy reaches 4.75), read back in 32 us (6.4 TB/s, partly
 // from the cache behind HBM); one token of 64 sequences, 8 heads of 128, in
 // 7.3 us: the latency of table, codes, barrier and merge.
-#include "stream.h"
+#include "cache_page.h"
 
 namespace vasc {
 namespace {
-
-struct CacheArgs {
-  uint8_t *kc, *vc, *ks, *vs;
-  uint16_t *mean;
-  int64_t pages;
-  const int32_t *table;
-  int64_t table_stride, max_pages;
-};
-
-struct RowArgs {
-  const void *k, *v;  // read: the outputs
-  int64_t ksb, ksh, kst, vsb, vsh, vst;
-  const int32_t *start, *count;
-  int64_t B, H, T;
-  int span;  // pages that T tokens can touch
-};
-
-// Eight consecutive elements as floats.
-template <typename T>
-__device__ __forceinline__ void load8(const T *src, float (&x)[8]) {
-  struct alignas(sizeof(T) == 4 ? 16 : 8 * sizeof(T)) Eight { T v[8]; };
-  const Eight e = *reinterpret_cast<const Eight *>(src);
-#pragma unroll
-  for (int i = 0; i < 8; ++i) x[i] = to_f32(e.v[i]);
-}
-
-template <typename T>
-__device__ __forceinline__ void store8(T *dst, const float (&x)[8]) {
-  struct alignas(sizeof(T) == 4 ? 16 : 8 * sizeof(T)) Eight { T v[8]; };
-  Eight e;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) e.v[i] = from_f32<T>(x[i]);
-  *reinterpret_cast<Eight *>(dst) = e;
-}
 
 // Max over the D/8 neighbouring lanes that hold a row.
 template <int D>
@@ -57,7 +23,7 @@ __device__ __forceinline__ float row_max(float v) {
 }
 
 // Exponent byte of a row whose largest magnitude is `top`.
-__device__ __forceinline__ int row_exponent(float top) { return power_of(top, -60, 60) + 127; }
+__device__ __forceinline__ int row_exponent(float top) { return power_of<8>(top, -60, 60) + 127; }
 
 __device__ __forceinline__ void quantise8(const float (&x)[8], int byte, uint32_t (&w)[2]) {
   const float inv = __uint_as_float(static_cast<uint32_t>(254 - byte) << 23);
@@ -71,40 +37,6 @@ __device__ __forceinline__ void quantise8(const float (&x)[8], int byte, uint32_
 // Row stride of the value tile in LDS: consecutive groups of four rows start four banks apart.
 template <int D>
 constexpr int tile_stride() { return D + 4; }
-
-struct PageWork {
-  int64_t b, h, j;   // sequence, head, logical page
-  int64_t pid;       // physical page, or -1
-  int64_t s;         // position of the call's first token
-  int lo, hi;        // slots of the page that the call's tokens cover
-};
-
-// The page of this workgroup: false where the call has no token in it.
-__device__ __forceinline__ bool page_work(const CacheArgs &c, const RowArgs &r, int64_t tokens, PageWork &w) {
-  const uint32_t id = blockIdx.x, span = r.span, ph = id / span;
-  const int64_t jj = id - ph * span;
-  w.b = ph / static_cast<uint32_t>(r.H);
-  w.h = ph - static_cast<uint32_t>(w.b) * static_cast<uint32_t>(r.H);
-  w.s = r.start[w.b];
-  if (w.s < 0) return false;
-  w.j = w.s / kPage + jj;
-  const int64_t lo = w.s - w.j * kPage, hi = w.s + tokens - w.j * kPage;
-  w.lo = static_cast<int>(lo > 0 ? lo : 0);
-  w.hi = static_cast<int>(hi < kPage ? hi : kPage);
-  if (w.hi <= w.lo) return false;
-  w.pid = -1;
-  if (w.j < c.max_pages) {
-    const int64_t pid = c.table[w.b * c.table_stride + w.j];
-    if (pid >= 0 && pid < c.pages) w.pid = pid;
-  }
-  return true;
-}
-
-__device__ __forceinline__ int64_t new_tokens(const RowArgs &r, int64_t b) {
-  if (!r.count) return r.T;
-  const int64_t n = r.count[b];
-  return n < 0 ? 0 : (n < r.T ? n : r.T);
-}
 
 template <typename T, int D>
 __global__ __launch_bounds__(256) void cache_write_kernel(const CacheArgs c, const RowArgs r) {
@@ -236,21 +168,8 @@ __global__ __launch_bounds__(256) void cache_read_kernel(const CacheArgs c, cons
   PageWork w;
   const int64_t b = blockIdx.x / (static_cast<uint32_t>(r.span) * static_cast<uint32_t>(r.H));
   const int64_t n = new_tokens(r, b);
-  bool live = r.start[b] >= 0;
-  if (!page_work(c, r, r.T, w)) {
-    if (live) return;
-    // a negative start reads nothing: its rows are zero, 64 to a workgroup
-    w.s = 0;
-    w.j = blockIdx.x % r.span;
-    w.h = (blockIdx.x / r.span) % r.H;
-    w.b = b;
-    w.lo = 0;
-    const int64_t hi = r.T - w.j * kPage;
-    w.hi = static_cast<int>(hi < kPage ? hi : kPage);
-    w.pid = -1;
-    if (w.hi <= 0) return;
-  }
-  live = live && w.pid >= 0;
+  bool live;
+  if (!read_work(c, r, b, w, live)) return;
   const int64_t ph = w.pid * r.H + w.h;
   const int col = (tid % kLanes) * 8;
   if (live) {
@@ -713,25 +632,6 @@ void launch_read(const CacheArgs &c, const RowArgs &r, hipStream_t s) {
   hipLaunchKernelGGL((cache_read_kernel<T, D>), dim3(static_cast<unsigned>(r.B * r.H * r.span)), dim3(256), 0, s, c, r);
 }
 
-int check_cache(const void *kc, const void *vc, const void *ks, const void *vs, int64_t pages, const int32_t *table,
-                int64_t table_stride, int64_t max_pages, int64_t D) {
-  VASC_REQUIRE(kc && vc && ks && vs && table, "the cache and the page table are required");
-  VASC_REQUIRE(pages > 0 && max_pages > 0, "pages and max_pages must be positive");
-  VASC_REQUIRE(max_pages < (int64_t(1) << 24), "max_pages %lld too large", (long long)max_pages);
-  VASC_REQUIRE(table_stride >= max_pages || table_stride == 0, "table_stride %lld below max_pages", (long long)table_stride);
-  VASC_SUPPORTED(D == 64 || D == 128, "D %lld not built (64, 128)", (long long)D);
-  for (const void *x : {kc, vc, ks, vs})
-    VASC_REQUIRE((reinterpret_cast<uintptr_t>(x) & 15) == 0, "the cache must be 16-byte aligned");
-  return VASC_OK;
-}
-
-int check_rows(const char *name, const void *x, int64_t sb, int64_t sh, int64_t st) {
-  VASC_REQUIRE(x, "%s is NULL", name);
-  VASC_REQUIRE((reinterpret_cast<uintptr_t>(x) & 15) == 0 && sb % 8 == 0 && sh % 8 == 0 && st % 8 == 0,
-               "%s needs 16-byte aligned rows and strides that are multiples of 8", name);
-  return VASC_OK;
-}
-
 }  // namespace
 }  // namespace vasc
 
@@ -746,13 +646,9 @@ extern "C" int vasc_cache_write(const void *k, int64_t k_sb, int64_t k_sh, int64
   if ((rc = check_rows("k", k, k_sb, k_sh, k_st))) return rc;
   if ((rc = check_rows("v", v, v_sb, v_sh, v_st))) return rc;
   VASC_REQUIRE(mean && start, "mean and start are required");
-  VASC_REQUIRE(B > 0 && H > 0 && T > 0, "empty tensor");
-  VASC_SUPPORTED(dtype >= 0 && dtype <= 2, "dtype %d not built", dtype);
   RowArgs r = {k, v, k_sb, k_sh, k_st, v_sb, v_sh, v_st, start, count, B, H, T, 0};
-  VASC_REQUIRE(T < (int64_t(1) << 30), "too many tokens");
-  r.span = static_cast<int>((T + 2 * kPage - 2) / kPage);
-  VASC_REQUIRE(H < (1 << 16) && B < (int64_t(1) << 24) && B * H * r.span < (int64_t(1) << 31), "too many tokens");
-  const CacheArgs c = {kc, vc, ks, vs, mean, pages, page_table, table_stride, max_pages};
+  if ((rc = check_tokens(r, dtype))) return rc;
+  const CacheArgs c = {kc, vc, ks, vs, mean, pages, page_table, table_stride, max_pages, nullptr};
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   if (D == 64)
     (dtype == 0 ? launch_write<__bf16, 64> : dtype == 1 ? launch_write<_Float16, 64> : launch_write<float, 64>)(c, r, s);
@@ -771,14 +667,10 @@ extern "C" int vasc_cache_read(const uint8_t *kc, const uint8_t *vc, const uint8
   if ((rc = check_rows("ko", ko, 0, 0, D))) return rc;
   if ((rc = check_rows("vo", vo, 0, 0, D))) return rc;
   VASC_REQUIRE(start, "start is required");
-  VASC_REQUIRE(B > 0 && H > 0 && T > 0, "empty tensor");
-  VASC_SUPPORTED(dtype >= 0 && dtype <= 2, "dtype %d not built", dtype);
-  VASC_REQUIRE(T < (int64_t(1) << 30), "too many tokens");
   RowArgs r = {ko, vo, 0, 0, 0, 0, 0, 0, start, count, B, H, T, 0};
-  r.span = static_cast<int>((T + 2 * kPage - 2) / kPage);
-  VASC_REQUIRE(H < (1 << 16) && B < (int64_t(1) << 24) && B * H * r.span < (int64_t(1) << 31), "too many tokens");
+  if ((rc = check_tokens(r, dtype))) return rc;
   const CacheArgs c = {const_cast<uint8_t *>(kc), const_cast<uint8_t *>(vc), const_cast<uint8_t *>(ks),
-                       const_cast<uint8_t *>(vs), nullptr, pages, page_table, table_stride, max_pages};
+                       const_cast<uint8_t *>(vs), nullptr, pages, page_table, table_stride, max_pages, nullptr};
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   if (D == 64)
     (dtype == 0 ? launch_read<__bf16, 64> : dtype == 1 ? launch_read<_Float16, 64> : launch_read<float, 64>)(c, r, s);

@@ -1,0 +1,129 @@
+// Shared by the writing, reading and moving of cache pages (cache.hip, cache4.hip, pages.hip): a call's tokens, and the
+// page of a workgroup.
+#pragma once
+
+#include "stream.h"
+
+namespace vasc {
+namespace {
+
+struct CacheArgs {
+  uint8_t *kc, *vc, *ks, *vs;
+  uint16_t *mean;
+  int64_t pages;
+  const int32_t *table;
+  int64_t table_stride, max_pages;
+  uint8_t *vo;  // of the 4-bit cache
+};
+
+struct RowArgs {
+  const void *k, *v;  // read: the outputs
+  int64_t ksb, ksh, kst, vsb, vsh, vst;
+  const int32_t *start, *count;
+  int64_t B, H, T;
+  int span;  // pages that T tokens can touch
+};
+
+// Eight consecutive elements as floats.
+template <typename T>
+__device__ __forceinline__ void load8(const T *src, float (&x)[8]) {
+  struct alignas(sizeof(T) == 4 ? 16 : 8 * sizeof(T)) Eight { T v[8]; };
+  const Eight e = *reinterpret_cast<const Eight *>(src);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) x[i] = to_f32(e.v[i]);
+}
+
+template <typename T>
+__device__ __forceinline__ void store8(T *dst, const float (&x)[8]) {
+  struct alignas(sizeof(T) == 4 ? 16 : 8 * sizeof(T)) Eight { T v[8]; };
+  Eight e;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) e.v[i] = from_f32<T>(x[i]);
+  *reinterpret_cast<Eight *>(dst) = e;
+}
+
+struct PageWork {
+  int64_t b, h, j;   // sequence, head, logical page
+  int64_t pid;       // physical page, or -1
+  int64_t s;         // position of the call's first token
+  int lo, hi;        // slots of the page that the call's tokens cover
+};
+
+// The page of this workgroup: false where the call has no token in it.
+__device__ __forceinline__ bool page_work(const CacheArgs &c, const RowArgs &r, int64_t tokens, PageWork &w) {
+  const uint32_t id = blockIdx.x, span = r.span, ph = id / span;
+  const int64_t jj = id - ph * span;
+  w.b = ph / static_cast<uint32_t>(r.H);
+  w.h = ph - static_cast<uint32_t>(w.b) * static_cast<uint32_t>(r.H);
+  w.s = r.start[w.b];
+  if (w.s < 0) return false;
+  w.j = w.s / kPage + jj;
+  const int64_t lo = w.s - w.j * kPage, hi = w.s + tokens - w.j * kPage;
+  w.lo = static_cast<int>(lo > 0 ? lo : 0);
+  w.hi = static_cast<int>(hi < kPage ? hi : kPage);
+  if (w.hi <= w.lo) return false;
+  w.pid = -1;
+  if (w.j < c.max_pages) {
+    const int64_t pid = c.table[w.b * c.table_stride + w.j];
+    if (pid >= 0 && pid < c.pages) w.pid = pid;
+  }
+  return true;
+}
+
+__device__ __forceinline__ int64_t new_tokens(const RowArgs &r, int64_t b) {
+  if (!r.count) return r.T;
+  const int64_t n = r.count[b];
+  return n < 0 ? 0 : (n < r.T ? n : r.T);
+}
+
+// The page of this workgroup of a read of r.T tokens of sequence b; live: whether it holds anything (else its rows are zero).
+__device__ __forceinline__ bool read_work(const CacheArgs &c, const RowArgs &r, int64_t b, PageWork &w, bool &live) {
+  live = r.start[b] >= 0;
+  if (!page_work(c, r, r.T, w)) {
+    if (live) return false;
+    // a negative start reads nothing: its rows are zero, 64 to a workgroup
+    w.s = 0;
+    w.j = blockIdx.x % r.span;
+    w.h = (blockIdx.x / r.span) % r.H;
+    w.b = b;
+    w.lo = 0;
+    const int64_t hi = r.T - w.j * kPage;
+    w.hi = static_cast<int>(hi < kPage ? hi : kPage);
+    w.pid = -1;
+    if (w.hi <= 0) return false;
+  }
+  live = live && w.pid >= 0;
+  return true;
+}
+
+int check_cache(const void *kc, const void *vc, const void *ks, const void *vs, int64_t pages, const int32_t *table,
+                int64_t table_stride, int64_t max_pages, int64_t D) {
+  VASC_REQUIRE(kc && vc && ks && vs && table, "the cache and the page table are required");
+  VASC_REQUIRE(pages > 0 && max_pages > 0, "pages and max_pages must be positive");
+  VASC_REQUIRE(max_pages < (int64_t(1) << 24), "max_pages %lld too large", (long long)max_pages);
+  VASC_REQUIRE(table_stride >= max_pages || table_stride == 0, "table_stride %lld below max_pages", (long long)table_stride);
+  VASC_SUPPORTED(D == 64 || D == 128, "D %lld not built (64, 128)", (long long)D);
+  for (const void *x : {kc, vc, ks, vs})
+    VASC_REQUIRE((reinterpret_cast<uintptr_t>(x) & 15) == 0, "the cache must be 16-byte aligned");
+  return VASC_OK;
+}
+
+int check_rows(const char *name, const void *x, int64_t sb, int64_t sh, int64_t st) {
+  VASC_REQUIRE(x, "%s is NULL", name);
+  VASC_REQUIRE((reinterpret_cast<uintptr_t>(x) & 15) == 0 && sb % 8 == 0 && sh % 8 == 0 && st % 8 == 0,
+               "%s needs 16-byte aligned rows and strides that are multiples of 8", name);
+  return VASC_OK;
+}
+
+// Sizes and type of the tokens; fills r.span.
+int check_tokens(RowArgs &r, int32_t dtype) {
+  VASC_REQUIRE(r.B > 0 && r.H > 0 && r.T > 0, "empty tensor");
+  VASC_SUPPORTED(dtype >= 0 && dtype <= 2, "dtype %d not built", dtype);
+  VASC_REQUIRE(r.T < (int64_t(1) << 30), "too many tokens");
+  r.span = static_cast<int>((r.T + 2 * kPage - 2) / kPage);
+  VASC_REQUIRE(r.H < (1 << 16) && r.B < (int64_t(1) << 24) && r.B * r.H * r.span < (int64_t(1) << 31), "too many tokens");
+  return VASC_OK;
+}
+
+}  // namespace
+}  // namespace vasc

@@ -1,4 +1,4 @@
-// Shared by the streaming operators (rotary.hip, cache.hip, cache_attn.hip).
+// Shared by the streaming operators (rotary.hip, cache*.hip, pages.hip).
 #pragma once
 
 #include "../../include/vasc_stream.h"
@@ -38,11 +38,35 @@ __device__ __forceinline__ void unpack_e4m3(uint32_t w, float (&f)[4]) {
   f[0] = a[0]; f[1] = a[1]; f[2] = b[0]; f[3] = b[1];
 }
 
-// Smallest e in [least, most] with top <= 448 * 2^e (`most` where none is).
+// Smallest e in [least, most] with top <= 1.75 * 2^(e + kTop) (`most` where none is): kTop 8 for 448, 2 for 7.
+template <int kTop>
 __device__ __forceinline__ int power_of(float top, int least, int most) {
   const uint32_t u = __float_as_uint(top);
-  const int e = static_cast<int>(u >> 23) - 127 - 8 + ((u & 0x7fffffu) > 0x600000u ? 1 : 0);
+  const int e = static_cast<int>(u >> 23) - 127 - kTop + ((u & 0x7fffffu) > 0x600000u ? 1 : 0);
   return min(max(e, least), most);
+}
+
+// The 4-bit cache, within the bytes of a page and head. Of the keys: features [f, f + 8) of token t.
+template <int D>
+__device__ __forceinline__ int key4_at(int t, int f) {
+  return D == 128 ? t * 64 + f / 2
+                  : ((t >> 5) * 16 + (t & 15)) * 64 + (f >> 4) * 16 + ((t >> 4) & 1) * 8 + (f & 15) / 2;
+}
+// Of the values: the eight bytes of feature f that hold lane group g's tokens, in the order of page_place.
+__device__ __forceinline__ int value4_at(int f, int g) {
+  return ((f >> 5) * 64 + (f & 15) * 4 + g) * 16 + ((f >> 4) & 1) * 8;
+}
+// Slot of lane group g's i-th token (of 16).
+__device__ __forceinline__ int token4_of(int g, int i) { return (i >> 2) * 16 + g * 4 + (i & 3); }
+// Bit of token k (of eight) in a word of value offsets: the even ones in the low half, the odd ones in the high.
+__device__ __forceinline__ int offset4_bit(int k) { return (k >> 1) * 4 + (k & 1) * 16; }
+
+// Eight e2m1 codes as floats.
+__device__ __forceinline__ void unpack_e2m1(uint32_t w, float (&f)[8]) {
+  const floatx2 a = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.0f, 0), b = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.0f, 1);
+  const floatx2 c = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.0f, 2), d = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.0f, 3);
+  f[0] = a[0]; f[1] = a[1]; f[2] = b[0]; f[3] = b[1];
+  f[4] = c[0]; f[5] = c[1]; f[6] = d[0]; f[7] = d[1];
 }
 
 // 2^(byte - 127); byte 255 gives infinity, which times a zero code is NaN.

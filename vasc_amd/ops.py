@@ -942,17 +942,25 @@ def rotary_axes(q: torch.Tensor, k: torch.Tensor | None, pos: torch.Tensor, sect
     return _rotary(q, k, pos, sections, inv_freq, False)
 
 
+_CACHE_ENTRIES = {(n, name): f"vasc_cache{four}_{name}" for n, four in ((4, ""), (5, "4")) for name in ("write", "read", "attn")}
+
+
+def _cache_entry(cache, name: str) -> str:
+    """The entry point for a cache's form: four buffers with 8 bits, five with 4."""
+    return _CACHE_ENTRIES[len(cache.pointers), name]
+
+
 def cache_write(cache, k: torch.Tensor, v: torch.Tensor, page_table: torch.Tensor, start: torch.Tensor,
                 count: torch.Tensor | None = None) -> None:
-    """Writes new tokens into a ``streaming.BlockCache``, in 8 bits.
+    """Writes new tokens into a ``streaming.BlockCache``, in 8 bits or 4.
 
     k, v ``[B,H,T,D]`` (bf16, fp16 or fp32, any strides over B, H, T): token
     ``t < count[b]`` (default T) of sequence b becomes its token
     ``start[b] + t``. ``page_table [B,max_pages]`` holds the sequences' pages
     (entries outside the cache: nothing is written there); no page may occur
     twice among the pages one call writes. Each (token, head) row is rounded
-    to e4m3 values times a power of two, and every touched page's key mean is
-    renewed over its tokens up to the last one written, so the tokens before
+    to e4m3 values times a power of two (4 bits: each 32 features of it to
+    e2m1 values times one), and every touched page's key mean is renewed over its tokens up to the last one written, so the tokens before
     ``start`` in its page must be there, and writing further back drops what
     came after. A token whose k or v row holds a value that is not finite is
     held as NaN in both. Nothing here waits for the GPU.
@@ -976,7 +984,7 @@ def cache_write(cache, k: torch.Tensor, v: torch.Tensor, page_table: torch.Tenso
         raise ValueError("start is required")
     if B == 0 or T == 0:
         return
-    _launch(dev, "vasc_cache_write", *kargs, *vargs, B, H, T, D,
+    _launch(dev, _cache_entry(cache, "write"), *kargs, *vargs, B, H, T, D,
             _DTYPE[k.dtype], table.data_ptr(), ts, mp, start.data_ptr(), _ptr(count), *cache.pointers,
             cache.mean_pointer, cache.pages)
 
@@ -1001,7 +1009,7 @@ def cache_read(cache, page_table: torch.Tensor, start: torch.Tensor, tokens: int
     k = torch.empty(B, H, tokens, D, device=table.device, dtype=dtype)
     v = torch.empty(B, H, tokens, D, device=table.device, dtype=dtype)
     if B and tokens:
-        _launch(dev, "vasc_cache_read", *cache.pointers, cache.pages, table.data_ptr(), ts, mp, start.data_ptr(),
+        _launch(dev, _cache_entry(cache, "read"), *cache.pointers, cache.pages, table.data_ptr(), ts, mp, start.data_ptr(),
                 _ptr(count), B, H, tokens, D, _DTYPE[dtype], k.data_ptr(), v.data_ptr())
     return k, v
 
@@ -1127,7 +1135,179 @@ def cache_attn(q: torch.Tensor, cache, page_table: torch.Tensor, lengths: torch.
         return out.zero_()
     size = _attn_workspace(B, Hq, H, T, D, block_q, mp, width)
     ws = torch.empty(size, device=q.device, dtype=torch.uint8) if size > 0 else None
-    _launch(dev, "vasc_cache_attn", *qargs, out.data_ptr(), osb, osh, ost, B, Hq, H, T, D, _DTYPE[q.dtype],
+    _launch(dev, _cache_entry(cache, "attn"), *qargs, out.data_ptr(), osb, osh, ost, B, Hq, H, T, D, _DTYPE[q.dtype],
             *cache.pointers, cache.pages, table.data_ptr(), ts, mp, lengths.data_ptr(), _ptr(q_count), block_q,
             _ptr(index), width, _ptr(count), bool(causal), D ** -0.5 if scale is None else scale, _ptr(ws), size)
+    return out
+
+
+# ----------------------------------------------------------------- cache pages
+def _same_gpu(owner, name: str, dev: int) -> None:
+    if owner.device_index != dev:
+        raise ValueError(f"the {name} is on cuda:{owner.device_index}, the tensors on cuda:{dev}")
+
+
+def _in_place(t, name: str, shape: tuple, dev: int) -> torch.Tensor:
+    """An int32 tensor that a call changes: rows apart from one another, unit stride within."""
+    _gpu(t, name, dev)
+    if t.dtype is not torch.int32 or t.dim() != len(shape) or any(n not in (s, -1) for s, n in zip(t.shape, shape)):
+        raise ValueError(f"{name} is changed in place and must be int32 {list(shape)}, got {t.dtype} {tuple(t.shape)}")
+    strides = t.stride()
+    if (t.shape[-1] > 1 and strides[-1] != 1) or (len(shape) == 2 and t.shape[0] > 1 and strides[0] < t.shape[1]):
+        raise ValueError(f"{name} is changed in place and needs contiguous rows that do not overlap")
+    return t
+
+
+def _row_stride(t: torch.Tensor) -> int:
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+def cache_copy(cache, src: torch.Tensor, dst: torch.Tensor) -> None:
+    """Copies whole pages within a ``streaming.BlockCache``: page ``src[i]`` to page ``dst[i]``.
+
+    src, dst ``[n]`` integers; pairs with a number outside the cache (such as
+    the -1 of ``pages_reserve``) are skipped. No page may be written twice in
+    one call, nor be both written and copied from.
+    """
+    dev = _gpu(src, "src")
+    _same_gpu(cache, "cache", dev)
+    if src.dim() != 1:
+        raise ValueError(f"src must be [n], got {tuple(src.shape)}")
+    n = src.shape[0]
+    src, dst = _int_rows(src, "src", n, dev), _int_rows(dst, "dst", n, dev)
+    if dst is None:
+        raise ValueError("dst is required")
+    if n:
+        kc, vc, ks, vs, *vo = cache.pointers
+        _launch(dev, "vasc_cache_copy", cache.bits, kc, vc, ks, vs, vo[0] if vo else None, cache.mean_pointer, cache.pages,
+                cache.heads, cache.head_dim, src.data_ptr(), dst.data_ptr(), n)
+
+
+def cache_compact(cache, page_table: torch.Tensor, index: torch.Tensor, out_table: torch.Tensor,
+                  count: torch.Tensor | None = None) -> None:
+    """Moves chosen tokens of each sequence to the front of other pages.
+
+    Token ``index[b,i]`` of the sequence that ``page_table [B,max_pages]``
+    holds becomes token ``i < count[b]`` (default all) of the one that
+    ``out_table [B,pages]`` holds, k and v as they are held, with no rounding.
+    index ``[B,n]``, or ``[B,H,n]`` with a list for each head; an entry that is
+    no token of the table is held as zeros. Key means of the pages written
+    are renewed over their tokens up to the last one; a page's slots behind
+    that stay as they are. No page may occur twice among those written, nor
+    be both written and read from; the pages of ``page_table`` still hold what
+    they held (``pages_free`` gives them back).
+    """
+    dev = _gpu(index, "index")
+    _same_gpu(cache, "cache", dev)
+    if index.dim() not in (2, 3) or (index.dim() == 3 and index.shape[1] != cache.heads):
+        raise ValueError(f"index must be [B,n] or [B,{cache.heads},n], got {tuple(index.shape)}")
+    B, n = index.shape[0], index.shape[-1]
+    index = _int32(index, "index")
+    if (n > 1 and index.stride(-1) != 1) or any(st < 0 for st in index.stride()):
+        index = index.contiguous()
+    isb, ish = index.stride(0), index.stride(1) if index.dim() == 3 else 0
+    table, ts, mp = _page_table(page_table, B, dev)
+    out, os, omp = _page_table(out_table, B, dev)
+    count = _int_rows(count, "count", B, dev)
+    if n > omp * BLOCK_K:
+        raise ValueError(f"out_table holds {omp * BLOCK_K} tokens a sequence, index has {n}")
+    if B and n:
+        kc, vc, ks, vs, *vo = cache.pointers
+        _launch(dev, "vasc_cache_compact", cache.bits, kc, vc, ks, vs, vo[0] if vo else None, cache.mean_pointer, cache.pages,
+                cache.heads, cache.head_dim, table.data_ptr(), ts, mp, index.data_ptr(), isb, ish, _ptr(count), B, n,
+                out.data_ptr(), os, omp)
+
+
+def pages_fork(pool, page_table: torch.Tensor, lengths: torch.Tensor, source: torch.Tensor) -> tuple:
+    """Sequences that share the pages of others: ``(page_table', lengths')``.
+
+    Row i of the new table ``[n,max_pages]`` has the pages that hold the
+    ``lengths[s]`` tokens of sequence ``s = source[i]`` of ``page_table
+    [B,max_pages]``, and -1 behind them; the pool counts a holder more for
+    each. Any sequence may be the source of several rows or of none; a source
+    outside [0, B) gives an empty row. The old table still holds its pages:
+    ``pages_free`` gives them back. ``pages_reserve`` before a write replaces
+    the shared pages that it would touch.
+    """
+    dev = _gpu(page_table, "page_table")
+    _same_gpu(pool, "pool", dev)
+    B = page_table.shape[0]
+    table, ts, mp = _page_table(page_table, B, dev)
+    lengths = _int_rows(lengths, "lengths", B, dev)
+    if lengths is None or not isinstance(source, torch.Tensor) or source.dim() != 1:
+        raise ValueError("lengths and source [n] are required")
+    n = source.shape[0]
+    source = _int_rows(source, "source", n, dev)
+    out = torch.empty(n, mp, device=table.device, dtype=torch.int32)
+    out_lengths = torch.empty(n, device=table.device, dtype=torch.int32)
+    if not B:
+        out.fill_(-1)
+        out_lengths.zero_()
+    elif n:
+        _launch(dev, "vasc_pages_fork", pool.pointer, pool.pages, table.data_ptr(), ts, mp, lengths.data_ptr(), B,
+                source.data_ptr(), n, out.data_ptr(), out_lengths.data_ptr())
+    return out, out_lengths
+
+
+def pages_free(pool, page_table: torch.Tensor, lengths: torch.Tensor, keep: torch.Tensor | None = None) -> None:
+    """Gives back the pages behind each sequence's first ``keep[b]`` tokens (default 0: all).
+
+    page_table ``[B,max_pages]`` and lengths ``[B]``, int32, change in place:
+    entries behind the kept tokens become -1, reserved ones among them, and
+    ``lengths[b]`` at most ``keep[b]``. The pool counts a holder less for each;
+    a page that has none is free.
+    """
+    dev = _gpu(page_table, "page_table")
+    _same_gpu(pool, "pool", dev)
+    _in_place(page_table, "page_table", (-1, -1), dev)
+    B, mp = page_table.shape
+    _in_place(lengths, "lengths", (B,), dev)
+    keep = _int_rows(keep, "keep", B, dev)
+    if B and mp:
+        _launch(dev, "vasc_pages_free", pool.pointer, pool.pages, page_table.data_ptr(), _row_stride(page_table), mp,
+                lengths.data_ptr(), B, _ptr(keep))
+
+
+@functools.lru_cache(maxsize=256)
+def _reserve_workspace(*sizes: int) -> int:
+    return _lib.fn("vasc_pages_reserve_workspace_size")(*sizes)
+
+
+def pages_reserve(pool, page_table: torch.Tensor, lengths: torch.Tensor, tokens: int,
+                  count: torch.Tensor | None = None) -> tuple:
+    """Pages for the next ``tokens`` tokens (``count[b]`` of them) of each sequence: ``(granted, src, dst)``.
+
+    page_table ``[B,max_pages]``, int32, changes in place. Of the pages that
+    tokens ``lengths[b]..`` touch, the ones that a sequence lacks, or that
+    others hold too, are replaced by free pages, the lowest first, in the
+    order of sequences and tokens; a shared page then counts a holder less.
+    Where it holds tokens before ``lengths[b]`` it has to be copied before
+    the write: from ``src[b]`` to ``dst[b]`` (-1: nothing to copy), which
+    ``cache_copy`` takes, for every cache that the table serves.
+
+    ``granted[b]``: the tokens that may be written, for ``cache_write``'s
+    ``count``: all of them that the table's row can hold, or 0 where the pool
+    does not have enough for this sequence and those before it that lack some;
+    such a row stays as it is. All three ``[B]`` int32. Nothing waits for the GPU.
+    """
+    dev = _gpu(page_table, "page_table")
+    _same_gpu(pool, "pool", dev)
+    _in_place(page_table, "page_table", (-1, -1), dev)
+    B, mp = page_table.shape
+    tokens = int(tokens)
+    if tokens < 0:
+        raise ValueError(f"tokens must not be negative, got {tokens}")
+    lengths, count = _int_rows(lengths, "lengths", B, dev), _int_rows(count, "count", B, dev)
+    if lengths is None:
+        raise ValueError("lengths is required")
+    granted, src, dst = out = torch.empty(3, B, device=page_table.device, dtype=torch.int32).unbind(0)
+    if not (B and mp and tokens):
+        granted.zero_()
+        src.fill_(-1)
+        dst.fill_(-1)
+        return out
+    size = _reserve_workspace(pool.pages, mp, B, tokens)
+    ws = torch.empty(max(size, 0), device=page_table.device, dtype=torch.uint8)
+    _launch(dev, "vasc_pages_reserve", pool.pointer, pool.pages, page_table.data_ptr(), _row_stride(page_table), mp,
+            lengths.data_ptr(), B, tokens, _ptr(count), granted.data_ptr(), src.data_ptr(), dst.data_ptr(), ws.data_ptr(), size)
     return out

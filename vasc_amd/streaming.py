@@ -21,29 +21,41 @@ from .pipeline import ratio_to_topk
 
 
 class BlockCache:
-    """8-bit keys and values of ``heads`` key heads, ``pages`` pages of 64 tokens.
+    """Keys and values of ``heads`` key heads in 8 bits or 4, ``pages`` pages of 64 tokens.
 
-    ``kc`` / ``vc``: e4m3 codes (values transposed within a page), ``ks`` /
-    ``vs``: the rows' powers of two, ``mean``: each page's mean key in bf16
-    (``include/vasc_stream.h`` has the layout). ``ops.cache_write`` fills it,
-    ``ops.cache_read`` / ``cache_select`` / ``cache_attn`` read it. Which pages
-    belong to whom is the caller's page table. The cache starts as zeros.
+    ``kc`` / ``vc``: the codes, e4m3 or e2m1 (values transposed within a
+    page), ``ks`` / ``vs``: the rows' powers of two, with 4 bits one for each 32
+    features of a key row, and ``vo`` for those of a value row; ``mean``: each
+    page's mean key in bf16 (``include/vasc_stream.h`` has the layout).
+    ``ops.cache_write`` fills it, ``ops.cache_read`` / ``cache_select`` /
+    ``cache_attn`` read it, ``cache_copy`` / ``cache_compact`` move what it holds.
+    Which pages belong to whom is the caller's page table, which a ``PagePool``
+    can keep. The cache starts as zeros.
     """
 
-    def __init__(self, pages: int, heads: int, head_dim: int, device="cuda"):
+    def __init__(self, pages: int, heads: int, head_dim: int, device="cuda", bits: int = 8):
         if pages < 1 or heads < 1:
             raise ValueError(f"a cache needs pages and heads, got {pages} and {heads}")
         if head_dim not in (64, 128):
             raise ValueError(f"head_dim {head_dim} not built (64, 128)")
+        if bits not in (4, 8):
+            raise ValueError(f"bits {bits} not built (4, 8)")
         device = torch.device(device)
         if device.type != "cuda":
             raise ValueError("the block cache lives on a GPU (the HIP path has no CPU fallback)")
-        self.pages, self.heads, self.head_dim = int(pages), int(heads), int(head_dim)
+        self.pages, self.heads, self.head_dim, self._bits = int(pages), int(heads), int(head_dim), int(bits)
         u8 = dict(device=device, dtype=torch.uint8)
         page = ops.BLOCK_K
-        self._kc = torch.zeros(pages, heads, page, head_dim, **u8)
-        self._vc = torch.zeros(pages, heads, head_dim, page, **u8)
-        self._ks = torch.zeros(pages, heads, page, **u8)
+        if bits == 8:
+            self._kc = torch.zeros(pages, heads, page, head_dim, **u8)
+            self._vc = torch.zeros(pages, heads, head_dim, page, **u8)
+            self._ks = torch.zeros(pages, heads, page, **u8)
+            self._vo = None
+        else:
+            self._kc = torch.zeros(pages, heads, page * head_dim // 2, **u8)
+            self._vc = torch.zeros(pages, heads, page * head_dim // 2, **u8)
+            self._ks = torch.zeros(pages, heads, head_dim // 32, page, **u8)
+            self._vo = torch.zeros(pages, heads, head_dim, **u8)
         self._vs = torch.zeros(pages, heads, page, **u8)
         self._mean = torch.zeros(pages, heads, head_dim, device=device, dtype=torch.bfloat16)
         self._locate()
@@ -53,24 +65,65 @@ class BlockCache:
         if not self._kc.is_cuda:
             raise ValueError("the block cache lives on a GPU (the HIP path has no CPU fallback)")
         self.device_index = self._kc.get_device()
-        self.pointers = tuple(t.data_ptr() for t in (self._kc, self._vc, self._ks, self._vs))
+        self.pointers = tuple(t.data_ptr() for t in (self._kc, self._vc, self._ks, self._vs, self._vo) if t is not None)
         self.mean_pointer = self._mean.data_ptr()
 
     def __setstate__(self, state: dict) -> None:
         """A copy or an unpickled cache: the state's addresses are the original's."""
-        self.__dict__.update(state)
+        self.__dict__.update({"_bits": 8, "_vo": None, **state})
         self._locate()
 
+    bits = property(lambda self: self._bits)
     kc = property(lambda self: self._kc)
     vc = property(lambda self: self._vc)
     ks = property(lambda self: self._ks)
     vs = property(lambda self: self._vs)
+    vo = property(lambda self: self._vo)
     mean = property(lambda self: self._mean)
 
     @property
     def nbytes(self) -> int:
-        """Bytes of device memory: 2 + 2/D bytes a value pair, and the means."""
-        return sum(t.numel() * t.element_size() for t in (self.kc, self.vc, self.ks, self.vs, self.mean))
+        """Bytes of device memory: a value pair has 2 + 2/D bytes, with 4 bits 1 + 3/64 + 1/D, and a page its means."""
+        return sum(t.numel() * t.element_size() for t in (self.kc, self.vc, self.ks, self.vs, self.vo, self.mean)
+                   if t is not None)
+
+
+class PagePool:
+    """Who holds the pages of one or more block caches that a page table serves.
+
+    ``refs [pages]`` int32 on the GPU counts each page's holders, the entries
+    of page tables that name it: a page is free where it is 0.
+    ``ops.pages_reserve`` gives sequences the lowest free pages, ``pages_fork``
+    lets sequences share pages, ``pages_free`` gives them back; a table starts
+    as -1 throughout. Nothing is kept on the host, so that a captured call
+    serves every step.
+    """
+
+    def __init__(self, pages: int, device="cuda"):
+        if not 1 <= pages < 1 << 26:
+            raise ValueError(f"a pool has 1 to 2^26 - 1 pages, got {pages}")
+        device = torch.device(device)
+        if device.type != "cuda":
+            raise ValueError("the page pool lives on a GPU (the HIP path has no CPU fallback)")
+        self.pages = int(pages)
+        self._refs = torch.zeros(pages, device=device, dtype=torch.int32)
+        self._locate()
+
+    def _locate(self) -> None:
+        if not self._refs.is_cuda:
+            raise ValueError("the page pool lives on a GPU (the HIP path has no CPU fallback)")
+        self.device_index, self.pointer = self._refs.get_device(), self._refs.data_ptr()
+
+    def __setstate__(self, state: dict) -> None:
+        """A copy or an unpickled pool: the state's address is the original's."""
+        self.__dict__.update(state)
+        self._locate()
+
+    refs = property(lambda self: self._refs)
+
+    def available(self) -> int:
+        """Free pages; waits for the GPU."""
+        return int((self._refs <= 0).sum())
 
 
 def _layer_qkv(attn, x: torch.Tensor, pos: torch.Tensor | None, frames: int, special: int) -> tuple:
