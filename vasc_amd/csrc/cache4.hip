@@ -179,6 +179,21 @@ __global__ __launch_bounds__(256) void cache4_read_kernel(const CacheArgs c, con
   const int64_t ph = w.pid * r.H + w.h;
   const uint8_t *kc = c.kc + ph * (kPage * D / 2), *vc = c.vc + ph * (kPage * D / 2);
   const uint8_t *ks = c.ks + ph * (kPage * kG), *vs = c.vs + ph * kPage, *vo = c.vo + ph * (kG * 32);
+  // everything that is read is on its way before anything is waited for
+  constexpr int kPasses = kPage / kRows;
+  const int col = tid % kLanes * 8, gr = col / 32;
+  uint32_t kw[kPasses], kb[kPasses], vb[kPasses], off[kPasses];
+#pragma unroll
+  for (int pass = 0; pass < kPasses; ++pass) {
+    const int row = pass * kRows + tid / kLanes;
+    const int place = page_place(row), i = place & 15;
+    kw[pass] = kb[pass] = vb[pass] = off[pass] = 0;
+    if (!live) continue;
+    kw[pass] = *reinterpret_cast<const uint32_t *>(kc + key4_at<D>(row, col));
+    kb[pass] = ks[gr * kPage + key_place(row)];
+    vb[pass] = vs[place];
+    off[pass] = *reinterpret_cast<const uint32_t *>(vo + ((place >> 4) * kG + gr) * 8 + (i >> 3) * 4) >> offset4_bit(i & 7) & 15u;
+  }
   if (live && tid < 64 * kG) {
     const int g = tid & 3, f = (tid >> 6) * 32 + ((tid >> 2) & 15);
     const u32x4 x = *reinterpret_cast<const u32x4 *>(vc + value4_at(f, g));
@@ -186,25 +201,23 @@ __global__ __launch_bounds__(256) void cache4_read_kernel(const CacheArgs c, con
     for (int i = 0; i < 4; ++i) *reinterpret_cast<uint32_t *>(vt + (f + (i >> 1) * 16) * kS + g * 8 + (i & 1) * 4) = x[i];
   }
   __syncthreads();
-  const int col = tid % kLanes * 8, gr = col / 32;
   T *ko = const_cast<T *>(static_cast<const T *>(r.k)) + (w.b * r.H + w.h) * r.T * D;
   T *vout = const_cast<T *>(static_cast<const T *>(r.v)) + (w.b * r.H + w.h) * r.T * D;
 #pragma unroll
-  for (int pass = 0; pass < kPage / kRows; ++pass) {
+  for (int pass = 0; pass < kPasses; ++pass) {
     const int row = pass * kRows + tid / kLanes;
     if (row < w.lo || row >= w.hi) continue;
     const int64_t t = w.j * kPage + row - w.s;
     float x[8] = {0, 0, 0, 0, 0, 0, 0, 0}, y[8] = {0, 0, 0, 0, 0, 0, 0, 0};
     if (live && t < n) {
       const int place = page_place(row), g = place >> 4, i = place & 15;
-      const uint32_t kb = ks[gr * kPage + key_place(row)];
-      const uint32_t off = *reinterpret_cast<const uint32_t *>(vo + (g * kG + gr) * 8 + (i >> 3) * 4) >> offset4_bit(i & 7) & 15u;
       // a slot that was never written has zeros throughout
-      const float ke = pow2_byte(kb), ve = kb == 255 ? ke : pow2_byte(max(static_cast<int>(vs[place] + off) - 15, 0));
+      const float ke = pow2_byte(kb[pass]);
+      const float ve = kb[pass] == 255 ? ke : pow2_byte(max(static_cast<int>(vb[pass] + off[pass]) - 15, 0));
       uint32_t vw = 0;
 #pragma unroll
       for (int e = 0; e < 8; ++e) vw |= (vt[(col + e) * kS + g * 8 + (i >> 1)] >> (4 * (i & 1)) & 15u) << (4 * e);
-      unpack_e2m1(*reinterpret_cast<const uint32_t *>(kc + key4_at<D>(row, col)), x);
+      unpack_e2m1(kw[pass], x);
       unpack_e2m1(vw, y);
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
