@@ -47,6 +47,9 @@ __global__ __launch_bounds__(256, 2) void cache4_attn_few_kernel(const AttnParam
   constexpr int kG = D / 32;   // groups of a row; 16-byte loads of a page's keys, or values, per lane; products of a key tile
   constexpr int kParts = __is_same(Q, __bf16) ? 1 : 2;
   constexpr int kOps = kParts * kG;
+  // Pages of a wave on their way. Two where that is 16 KB, single tokens of 16 sequences over up to 131072 keys (8 x 4 heads)
+  // 298 us with one, 285 with two; at D = 64 the registers cost a wave a SIMD (eight sequences up to 33312: 44.7 and 47.5).
+  constexpr int kAhead = D == 128 && kTiles == 1 ? 2 : 1;
   typedef float Sums[kRows][D + 2];
   constexpr size_t kQBytes = kTiles * kOps * 1024, kSBytes = (kWaves - 1) * sizeof(Sums);
   __shared__ __align__(16) uint8_t shared[kQBytes > kSBytes ? kQBytes : kSBytes];
@@ -84,34 +87,36 @@ __global__ __launch_bounds__(256, 2) void cache4_attn_few_kernel(const AttnParam
     int page, pid;  // lane i has those of entry base + i
     resolve(p, w, base + lane, page, pid);
     const int n = min(w.e1 - base, 64);
-    u32x4 kr[kG];
-    uint32_t kb = 0;
-    auto load_keys = [&](int i) {
+    // a page is asked for as soon as the one before it in its place has been used
+    struct Raw {
+      u32x4 kr[kG], vr[kG], vp[kG / 2], vb;
+      uint32_t kb;
+    } ahead[kAhead];
+    auto load_keys = [&](int i, Raw &r) {
       const int64_t at = static_cast<int64_t>(__builtin_amdgcn_readlane(pid, i)) * p.H;
 #pragma unroll
-      for (int y = 0; y < kG; ++y) kr[y] = *reinterpret_cast<const u32x4 *>(kbase + at * (kPage * D / 2) + y * 1024);
-      kb = *reinterpret_cast<const uint32_t *>(ksbase + at * (kPage * kG));
+      for (int y = 0; y < kG; ++y) r.kr[y] = *reinterpret_cast<const u32x4 *>(kbase + at * (kPage * D / 2) + y * 1024);
+      r.kb = *reinterpret_cast<const uint32_t *>(ksbase + at * (kPage * kG));
     };
-    if (wave < n) load_keys(wave);
-    for (int i = wave; i < n; i += kWaves) {
-      const int lpage = __builtin_amdgcn_readlane(page, i);
+    auto load_values = [&](int i, Raw &r) {
       const int64_t at = static_cast<int64_t>(__builtin_amdgcn_readlane(pid, i)) * p.H;
+#pragma unroll
+      for (int y = 0; y < kG; ++y) r.vr[y] = *reinterpret_cast<const u32x4 *>(vbase + at * (kPage * D / 2) + y * 1024);
+      r.vb = *reinterpret_cast<const u32x4 *>(vsbase + at * kPage);
+#pragma unroll
+      for (int y = 0; y < kG / 2; ++y) r.vp[y] = *reinterpret_cast<const u32x4 *>(vobase + at * (kG * 32) + y * 16);
+    };
+    auto step = [&](int i, Raw &r) {
+      const int lpage = __builtin_amdgcn_readlane(page, i);
       // the query operands are read again for every page: held over the loop they would cost 8 to 64 registers
       asm volatile("" ::: "memory");
-      u32x4 vr[kG], vp[kG / 2];
-#pragma unroll
-      for (int y = 0; y < kG; ++y) vr[y] = *reinterpret_cast<const u32x4 *>(vbase + at * (kPage * D / 2) + y * 1024);
-      const u32x4 vb = *reinterpret_cast<const u32x4 *>(vsbase + at * kPage);
-#pragma unroll
-      for (int y = 0; y < kG / 2; ++y) vp[y] = *reinterpret_cast<const u32x4 *>(vobase + at * (kG * 32) + y * 16);
-
       floatx4 s[kTiles][4];
 #pragma unroll
       for (int t = 0; t < 4; ++t) {
-        const float power = pow2_byte((kb >> (8 * t)) & 255u);
+        const float power = pow2_byte((r.kb >> (8 * t)) & 255u);
 #pragma unroll
         for (int y = 0; y < kG; ++y) {
-          const bf16x8 a = widen4_scaled(D == 128 ? kr[t][y] : kr[t >> 1][(t & 1) * 2 + y], power);
+          const bf16x8 a = widen4_scaled(D == 128 ? r.kr[t][y] : r.kr[t >> 1][(t & 1) * 2 + y], power);
 #pragma unroll
           for (int x = 0; x < kTiles; ++x)
 #pragma unroll
@@ -123,13 +128,12 @@ __global__ __launch_bounds__(256, 2) void cache4_attn_few_kernel(const AttnParam
             }
         }
       }
-      // the next page's keys arrive while this one's weights are made
-      if (i + kWaves < n) load_keys(i + kWaves);
+      if (i + kAhead * kWaves < n) load_keys(i + kAhead * kWaves, r);
 
       // exponents, in place: the byte's bias of 127 goes with the reference
 #pragma unroll
       for (int t = 0; t < 4; ++t) {
-        const uint32_t vw = vb[t];
+        const uint32_t vw = r.vb[t];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const float ev = static_cast<float>((vw >> (8 * j)) & 255u);
@@ -142,18 +146,18 @@ __global__ __launch_bounds__(256, 2) void cache4_attn_few_kernel(const AttnParam
       static_assert(kSmall + 0x1f == 128, "the bytes' test");
       uint32_t top = 0;
 #pragma unroll
-      for (int t = 0; t < 4; ++t) top |= (vb[t] + 0x3d3d3d3du) & ~(vb[t] + 0x1f1f1f1fu);
+      for (int t = 0; t < 4; ++t) top |= (r.vb[t] + 0x3d3d3d3du) & ~(r.vb[t] + 0x1f1f1f1fu);
       rows.weights(s, lpage, g, inv_c, __ballot(top & 0x80808080u) != 0, [&](int t) {
-        const uint32_t iw = 0xfefefefeu - vb[t];  // the opposite powers
+        const uint32_t iw = 0xfefefefeu - r.vb[t];  // the opposite powers
         return floatx4{pow2_byte(iw & 255u), pow2_byte((iw >> 8) & 255u), pow2_byte((iw >> 16) & 255u), pow2_byte(iw >> 24)};
       }, wt);
 #pragma unroll
       for (int y = 0; y < kG; ++y) {
-        const halfx8 p0 = powers8(vp[y >> 1][(y & 1) * 2]), p1 = powers8(vp[y >> 1][(y & 1) * 2 + 1]);
+        const halfx8 p0 = powers8(r.vp[y >> 1][(y & 1) * 2]), p1 = powers8(r.vp[y >> 1][(y & 1) * 2 + 1]);
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
           const int d = y * 2 + half;
-          const halfx8 a0 = widen4(vr[y][half * 2], p0), a1 = widen4(vr[y][half * 2 + 1], p1);
+          const halfx8 a0 = widen4(r.vr[y][half * 2], p0), a1 = widen4(r.vr[y][half * 2 + 1], p1);
 #pragma unroll
           for (int x = 0; x < kTiles; ++x) {
             rows.acc[x][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a0, wt[x][0], rows.acc[x][d], 0, 0, 0);
@@ -161,7 +165,18 @@ __global__ __launch_bounds__(256, 2) void cache4_attn_few_kernel(const AttnParam
           }
         }
       }
-    }
+      if (i + kAhead * kWaves < n) load_values(i + kAhead * kWaves, r);
+    };
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k)
+      if (wave + k * kWaves < n) {
+        load_keys(wave + k * kWaves, ahead[k]);
+        load_values(wave + k * kWaves, ahead[k]);
+      }
+    for (int i = wave; i < n; i += kAhead * kWaves)
+#pragma unroll
+      for (int k = 0; k < kAhead; ++k)
+        if (i + k * kWaves < n) step(i + k * kWaves, ahead[k]);
   }
   float m[kTiles];
   rows.finish(m);
