@@ -348,3 +348,102 @@ def test_copied_pool(how):
     table = torch.full((1, 2), -1, device="cuda", dtype=torch.int32)
     ops.pages_reserve(other, table, _i32([0]), 128)
     assert table.tolist() == [[0, 1]] and (pool.refs[0].item() == 1) == (how == "copy")
+
+
+# ------------------------------------------------------------------ the stream
+def _model(axes):
+    from vasc_amd.aggregator import Aggregator, RotaryPositionEmbeddingAxes
+    torch.manual_seed(4)
+    model = Aggregator(dim=512, depth=2, num_heads=8, intermediate_layer_idx=(0, 1)).cuda().to(torch.bfloat16)
+    if axes == 3:
+        rope = RotaryPositionEmbeddingAxes((16, 24, 24), (1e4, 100.0, 100.0))
+        for blk in (*model.frame_blocks, *model.global_blocks):
+            blk.attn.rope = rope
+    return model
+
+
+@pytest.mark.parametrize("axes", [2, 3])
+@pytest.mark.parametrize("bits", [4, 8])
+def test_stream_forks(bits, axes):
+    """Branches of a stream that push frames of their own give what streams of their own give, bit for bit; so does the one
+    they come from, and one that is forked after another has been closed."""
+    from vasc_amd.streaming import AggregatorStream
+    model = _model(axes)
+    images = torch.rand(2, 7, 3, 112, 140, generator=_gen(73)).cuda()
+
+    def alone(order):
+        s = AggregatorStream(model, 5, sparse_ratio=0.5, bits=bits)
+        return [s.push(images[:, list(part)])[0] for part in order]
+
+    def same(got, want):
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+    trunk = AggregatorStream(model, 5, sparse_ratio=0.5, bits=bits, branches=3)
+    with pytest.raises(ValueError, match="nothing"):
+        trunk.fork()
+    trunk.push(images[:, [0, 1]])
+    left, right = trunk.fork(), trunk.fork()
+    with pytest.raises(ValueError, match="branches"):
+        trunk.fork()
+    l1, r1 = left.push(images[:, [2]])[0], right.push(images[:, [3, 4]])[0]
+    t1 = trunk.push(images[:, [5]])[0]
+    l2, t2 = left.push(images[:, [6]])[0], trunk.push(images[:, [2]])[0]
+    want = alone([(0, 1), (2,), (6,)])
+    same(l1, want[1])
+    same(l2, want[2])
+    same(r1, alone([(0, 1), (3, 4)])[1])
+    want = alone([(0, 1), (5,), (2,)])
+    same(t1, want[1])
+    same(t2, want[2])
+    right.close()
+    right.close()
+    with pytest.raises(ValueError, match="closed"):
+        right.push(images[:, [0]])
+    again = left.fork()
+    same(again.push(images[:, [0]])[0], alone([(0, 1), (2,), (6,), (0,)])[3])
+    same(left.push(images[:, [3]])[0], alone([(0, 1), (2,), (6,), (3,)])[3])
+    for s in (trunk, left, again):
+        s.close()
+    assert trunk.pool.available() == trunk.pool.pages
+
+
+@pytest.mark.parametrize("axes", [2, 3])
+@pytest.mark.parametrize("bits", [4, 8])
+def test_stream_keeps_frames(bits, axes):
+    """After keep() the caches hold the listed frames' tokens, and a push attends to those and its own."""
+    from vasc_amd.streaming import AggregatorStream
+    model = _model(axes)
+    images = torch.rand(2, 6, 3, 112, 140, generator=_gen(79)).cuda()
+    s = AggregatorStream(model, 8, sparse_ratio=0.0, bits=bits)
+    for part in ((0,), (1, 2), (3, 4)):
+        s.push(images[:, list(part)])
+    P, S = 85, 5
+    spans = [[(0, P - S), (P - S, S)]]
+    for first in (P, 3 * P):
+        spans += [[(first + j * (P - S), P - S), (first + 2 * (P - S) + j * S, S)] for j in range(2)]
+    rows = [torch.cat([torch.arange(a, a + n) for a, n in spans[f]]) for f in range(5)]
+    before = [ops.cache_read(c, s.page_table, _i32([0, 0]), 5 * P) for c in s.caches]
+    for bad in ((), (0, 0), (3, 1), (-1,), (5,)):
+        with pytest.raises(ValueError, match="ascending"):
+            s.keep(bad)
+    s.keep((0, 2, 3))
+    kept = torch.cat([rows[f] for f in (0, 2, 3)]).cuda()
+    for c, (k, v) in zip(s.caches, before):
+        k2, v2 = ops.cache_read(c, s.page_table, _i32([0, 0]), 3 * P)
+        assert torch.equal(k2, k[:, :, kept]) and torch.equal(v2, v[:, :, kept])
+    assert s.frames == 3 and s.pool.available() == s.pool.pages - 2 * -(-3 * P // 64)
+    s.keep((1, 2))
+    s.keep((0, 1))  # all of them: nothing to do
+    out, _ = s.push(images[:, [5]])
+    assert s.frames == 3 and s.lengths.tolist() == [3 * P] * 2 and all(o.isfinite().all() for o in out)
+    for c, (k, v) in zip(s.caches, before):
+        k2, v2 = ops.cache_read(c, s.page_table, _i32([0, 0]), 2 * P)
+        assert torch.equal(k2, k[:, :, kept[P:]]) and torch.equal(v2, v[:, :, kept[P:]])
+    full = AggregatorStream(model, 3, sparse_ratio=0.0, bits=bits)
+    for part in ((0,), (1, 2)):
+        full.push(images[:, list(part)])
+    with pytest.raises(ValueError, match="free pages"):
+        full.keep((0, 1))
+    full.reset()
+    assert full.pool.available() == full.pool.pages
+    full.push(images[:, [0, 1, 2]])

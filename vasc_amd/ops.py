@@ -1147,19 +1147,16 @@ def _same_gpu(owner, name: str, dev: int) -> None:
         raise ValueError(f"the {name} is on cuda:{owner.device_index}, the tensors on cuda:{dev}")
 
 
-def _in_place(t, name: str, shape: tuple, dev: int) -> torch.Tensor:
-    """An int32 tensor that a call changes: rows apart from one another, unit stride within."""
-    _gpu(t, name, dev)
-    if t.dtype is not torch.int32 or t.dim() != len(shape) or any(n not in (s, -1) for s, n in zip(t.shape, shape)):
-        raise ValueError(f"{name} is changed in place and must be int32 {list(shape)}, got {t.dtype} {tuple(t.shape)}")
-    strides = t.stride()
-    if (t.shape[-1] > 1 and strides[-1] != 1) or (len(shape) == 2 and t.shape[0] > 1 and strides[0] < t.shape[1]):
-        raise ValueError(f"{name} is changed in place and needs contiguous rows that do not overlap")
-    return t
-
-
-def _row_stride(t: torch.Tensor) -> int:
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+def _own_table(t, dev: int) -> tuple:
+    """(sequences, pages a sequence, row stride) of a page table that a call changes: rows apart, unit stride within."""
+    shape, strides = t.shape, t.stride()
+    if t.dtype is not torch.int32 or len(shape) != 2 or t.get_device() != dev:
+        raise ValueError(f"page_table is changed in place and must be [B, max_pages] int32 on cuda:{dev}, got {t.dtype} "
+                         f"{tuple(shape)} on {t.device}")
+    B, mp = shape
+    if (mp > 1 and strides[1] != 1) or (B > 1 and strides[0] < mp):
+        raise ValueError("page_table is changed in place and needs contiguous rows that do not overlap")
+    return B, mp, strides[0] if B > 1 else mp
 
 
 def cache_copy(cache, src: torch.Tensor, dst: torch.Tensor) -> None:
@@ -1238,8 +1235,7 @@ def pages_fork(pool, page_table: torch.Tensor, lengths: torch.Tensor, source: to
         raise ValueError("lengths and source [n] are required")
     n = source.shape[0]
     source = _int_rows(source, "source", n, dev)
-    out = torch.empty(n, mp, device=table.device, dtype=torch.int32)
-    out_lengths = torch.empty(n, device=table.device, dtype=torch.int32)
+    out, out_lengths = table.new_empty((n, mp)), table.new_empty(n)
     if not B:
         out.fill_(-1)
         out_lengths.zero_()
@@ -1259,12 +1255,13 @@ def pages_free(pool, page_table: torch.Tensor, lengths: torch.Tensor, keep: torc
     """
     dev = _gpu(page_table, "page_table")
     _same_gpu(pool, "pool", dev)
-    _in_place(page_table, "page_table", (-1, -1), dev)
-    B, mp = page_table.shape
-    _in_place(lengths, "lengths", (B,), dev)
+    B, mp, stride = _own_table(page_table, dev)
+    _gpu(lengths, "lengths", dev)
+    if lengths.dtype is not torch.int32 or lengths.shape != (B,) or not lengths.is_contiguous():
+        raise ValueError(f"lengths is changed in place and must be [{B}] int32, contiguous, got {lengths.dtype} {tuple(lengths.shape)}")
     keep = _int_rows(keep, "keep", B, dev)
     if B and mp:
-        _launch(dev, "vasc_pages_free", pool.pointer, pool.pages, page_table.data_ptr(), _row_stride(page_table), mp,
+        _launch(dev, "vasc_pages_free", pool.pointer, pool.pages, page_table.data_ptr(), stride, mp,
                 lengths.data_ptr(), B, _ptr(keep))
 
 
@@ -1292,22 +1289,21 @@ def pages_reserve(pool, page_table: torch.Tensor, lengths: torch.Tensor, tokens:
     """
     dev = _gpu(page_table, "page_table")
     _same_gpu(pool, "pool", dev)
-    _in_place(page_table, "page_table", (-1, -1), dev)
-    B, mp = page_table.shape
+    B, mp, stride = _own_table(page_table, dev)
     tokens = int(tokens)
     if tokens < 0:
         raise ValueError(f"tokens must not be negative, got {tokens}")
     lengths, count = _int_rows(lengths, "lengths", B, dev), _int_rows(count, "count", B, dev)
     if lengths is None:
         raise ValueError("lengths is required")
-    granted, src, dst = out = torch.empty(3, B, device=page_table.device, dtype=torch.int32).unbind(0)
+    granted, src, dst = out = page_table.new_empty((3, B)).unbind(0)
     if not (B and mp and tokens):
         granted.zero_()
         src.fill_(-1)
         dst.fill_(-1)
         return out
     size = _reserve_workspace(pool.pages, mp, B, tokens)
-    ws = torch.empty(max(size, 0), device=page_table.device, dtype=torch.uint8)
-    _launch(dev, "vasc_pages_reserve", pool.pointer, pool.pages, page_table.data_ptr(), _row_stride(page_table), mp,
+    ws = page_table.new_empty(max(size, 0) // 4)
+    _launch(dev, "vasc_pages_reserve", pool.pointer, pool.pages, page_table.data_ptr(), stride, mp,
             lengths.data_ptr(), B, tokens, _ptr(count), granted.data_ptr(), src.data_ptr(), dst.data_ptr(), ws.data_ptr(), size)
     return out

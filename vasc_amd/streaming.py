@@ -1,14 +1,16 @@
 """Streamed global attention: frames arrive one after another.
 
-* ``BlockCache`` holds the keys and values of what was seen, in 8 bits, in
-  pages of 64 tokens that a page table hands to the sequences.
+* ``BlockCache`` holds the keys and values of what was seen, in 8 bits or 4,
+  in pages of 64 tokens that a page table hands to the sequences;
+  ``PagePool`` counts who holds which page, so that sequences can share them.
 * ``stream_attention`` is a global layer over the new frames' tokens: their
   keys and values are written into the cache, patch queries attend to the
   pages that a cheap score chooses for each block of 128 of them, special
   tokens to everything seen (as in ``adaptive_sparse_attention_forward``,
   which needs the whole clip at once).
 * ``AggregatorStream`` runs a VGGT-shaped ``Aggregator`` that way: ``push``
-  takes the next frames, whose global blocks see all frames so far.
+  takes the next frames, whose global blocks see all frames so far; ``fork``
+  branches off, ``keep`` forgets frames.
 """
 from __future__ import annotations
 
@@ -198,36 +200,117 @@ class AggregatorStream:
 
     ``push(images)`` takes the next frames ``[B,n,3,H,W]`` (the same B, H and W
     every time) and returns what the aggregator returns for them. Frame blocks
-    see their frame, global blocks all frames so far, through a cache a layer;
-    a block of 128 patch queries keeps ``1 - sparse_ratio`` of the pages. The
-    model's own global attention (``Attention`` or an installed sparse one) is
-    not used. ``reset()`` starts over.
+    see their frame, global blocks all frames held, through a cache a layer
+    (``bits`` 8 or 4); a block of 128 patch queries keeps ``1 - sparse_ratio`` of
+    the pages. The model's own global attention (``Attention`` or an installed
+    sparse one) is not used. ``reset()`` starts over.
+
+    ``fork()`` gives another stream that goes on from here, with the frames so
+    far in pages that both share; up to ``branches`` streams at once, each of
+    at most ``max_frames`` frames (the caches hold so many), until
+    ``close()``. ``keep(frames)`` forgets the frames that it does not list.
     """
 
-    def __init__(self, model, max_frames: int, *, sparse_ratio: float = 0.75, sink: int = 1, recent: int = 1):
+    def __init__(self, model, max_frames: int, *, sparse_ratio: float = 0.75, sink: int = 1, recent: int = 1, bits: int = 8,
+                 branches: int = 1):
         if max_frames < 1 or not 0.0 <= sparse_ratio < 1.0:
             raise ValueError(f"max_frames {max_frames} must be positive, sparse_ratio {sparse_ratio} in [0, 1)")
+        if bits not in (4, 8) or branches < 1:
+            raise ValueError(f"bits {bits} must be 4 or 8, branches {branches} positive")
         self.model, self.max_frames, self.sparse_ratio = model, int(max_frames), float(sparse_ratio)
-        self.sink, self.recent = sink, recent
+        self.sink, self.recent, self.bits, self.branches = sink, recent, int(bits), int(branches)
         self.caches: list[BlockCache] = []
+        self.pool: PagePool | None = None
         self.frames, self._shape = 0, None
+        self._seen = 0      # frames pushed, those that were forgotten among them: the next one's time
+        self._tokens = []   # of each frame held, the (first, number) of its runs of tokens
+        self._streams = [1]  # open streams of these caches, shared among them
+        self._forked = False  # whether another stream may hold this one's last page
+
+    def _open(self) -> None:
+        if self._streams is None:
+            raise ValueError("the stream is closed")
 
     def reset(self) -> None:
-        self.frames = 0
+        self._open()
+        if self.frames:
+            with ops.on_device(self.pool.device_index):
+                ops.pages_free(self.pool, self.page_table, self.lengths)
+        self.frames = self._seen = 0
+        self._tokens, self._forked = [], False
+
+    def close(self) -> None:
+        """Gives the stream's pages back; of no use after it."""
+        if self._streams is not None:
+            self.reset()
+            self._streams[0] -= 1
+            self._streams = None
+
+    def fork(self) -> "AggregatorStream":
+        """Another stream with the frames so far; pages are copied where one of the two goes on in them."""
+        self._open()
+        if not self.frames:
+            raise ValueError("nothing to fork: no frame has been pushed")
+        if self._streams[0] >= self.branches:
+            raise ValueError(f"the stream was made for {self.branches} branches")
+        other = AggregatorStream.__new__(AggregatorStream)
+        other.__dict__.update(self.__dict__, _tokens=list(self._tokens))
+        with ops.on_device(self.pool.device_index):
+            source = torch.arange(self.page_table.shape[0], device=self.page_table.device, dtype=torch.int32)
+            other.page_table, other.lengths = ops.pages_fork(self.pool, self.page_table, self.lengths, source)
+        self._streams[0] += 1
+        self._forked = other._forked = True
+        return other
+
+    def keep(self, frames) -> None:
+        """Forgets all frames but the listed ones (places among those held, ascending); their tokens move to free pages."""
+        self._open()
+        frames = [int(f) for f in frames]
+        if not frames or any(b <= a for a, b in zip(frames, frames[1:])) or frames[0] < 0 or frames[-1] >= self.frames:
+            raise ValueError(f"frames {frames} must be some of the {self.frames} held, ascending")
+        if len(frames) == self.frames:
+            return
+        B, mp = self.page_table.shape
+        P = self._shape[1]
+        n = len(frames) * P
+        with torch.no_grad(), ops.on_device(self.pool.device_index):
+            need = B * math.ceil(n / ops.BLOCK_K)
+            free = self.pool.available()
+            if need > free:
+                raise ValueError(f"{len(frames)} frames need {need} free pages to move to, {free} are: allow more frames")
+            runs = [run for f in frames for run in self._tokens[f]]
+            index = torch.cat([torch.arange(at, at + m, dtype=torch.int32) for at, m in runs]).to(self.page_table.device)
+            table, lengths = torch.full_like(self.page_table, -1), torch.zeros_like(self.lengths)
+            granted, _, _ = ops.pages_reserve(self.pool, table, lengths, n)
+            for cache in self.caches:
+                ops.cache_compact(cache, self.page_table, index.expand(B, n), table)
+            ops.pages_free(self.pool, self.page_table, self.lengths)
+            self.page_table, self.lengths = table, granted.clone()
+        at, tokens = 0, []
+        for f in frames:
+            tokens.append([])
+            for _, m in self._tokens[f]:
+                tokens[-1].append((at, m))
+                at += m
+        self.frames, self._tokens, self._forked = len(frames), tokens, False
 
     def _begin(self, B: int, P: int, hw: tuple, device) -> None:
         if self._shape is None or self._shape[:3] != (B, P, hw) or self._shape[3] != device:
-            if self.frames:
+            if self.frames or self._streams[0] > 1:
                 raise ValueError(f"frames of another batch, size or device: {(B, P, hw, device)} after {self._shape}")
             pages = math.ceil(self.max_frames * P / ops.BLOCK_K)
             attn = self.model.global_blocks[0].attn
-            self.caches = [BlockCache(B * pages, attn.num_heads, attn.head_dim, device) for _ in self.model.global_blocks]
-            self.page_table = torch.arange(B * pages, device=device, dtype=torch.int32).view(B, pages)
+            total = B * pages * self.branches
+            self.caches = [BlockCache(total, attn.num_heads, attn.head_dim, device, self.bits) for _ in self.model.global_blocks]
+            self.pool = PagePool(total, device)
+            self.page_table = torch.full((B, pages), -1, device=device, dtype=torch.int32)
+            self.lengths = torch.zeros(B, device=device, dtype=torch.int32)
             self._shape = (B, P, hw, device)
 
     @torch.no_grad()
     def push(self, images: torch.Tensor):
         """images ``[B,n,3,H,W]`` in [0, 1] -> (list of per-layer outputs, patch_start_idx)."""
+        self._open()
         with ops.on_device(ops._gpu(images, "images")):
             return self._push(images)
 
@@ -241,7 +324,7 @@ class AggregatorStream:
         tokens = patch_tokens(m.patch_embed, x)
 
         def expand(token):  # the stream's first frame has tokens of its own
-            if self.frames == 0:
+            if self._seen == 0:
                 return m._expand(token, B, n)
             return token[:, 1:].expand(B, n, *token.shape[2:]).reshape(B * n, *token.shape[2:])
 
@@ -255,12 +338,17 @@ class AggregatorStream:
         pos = grid_positions(B * n, h, w, S, images.device).to(torch.int32).contiguous()
         if isinstance(m.global_blocks[0].attn.rope, RotaryPositionEmbeddingAxes):
             # (frame, row, column)
-            t = torch.arange(self.frames, self.frames + n, device=images.device, dtype=torch.int32)
+            t = torch.arange(self._seen, self._seen + n, device=images.device, dtype=torch.int32)
             pos = torch.cat([t.repeat(B).view(B * n, 1, 1).expand(-1, P, -1), pos], -1).contiguous()
         pos_global = pos.view(B, n * P, -1)
         before, after = self.frames * P, (self.frames + n) * P
-        start = torch.full((B,), before, device=tokens.device, dtype=torch.int32)
-        lengths = torch.full((B,), after, device=tokens.device, dtype=torch.int32)
+        start = self.lengths
+        # there are pages for `branches` streams of max_frames frames: everything is granted
+        granted, src, dst = ops.pages_reserve(self.pool, self.page_table, start, n * P)
+        if self._forked:
+            for cache in self.caches:
+                ops.cache_copy(cache, src, dst)
+        lengths = start + granted
         pages = math.ceil(after / ops.BLOCK_K)
         keep = None if self.sparse_ratio == 0 else max(0, ratio_to_topk(pages, self.sparse_ratio) - self.sink - self.recent)
         outputs, normed = [], None
@@ -279,5 +367,9 @@ class AggregatorStream:
             if normed is not None:
                 normed = normed.view(B * n, P, C)
             outputs.append(torch.cat([frame_out, tokens.view(B, n, P, C)], dim=-1) if i in m.intermediate_layer_idx else None)
+        # a call's tokens are held all patches before all special tokens
+        self._tokens += [[(before + j * (P - S), P - S), (before + n * (P - S) + j * S, S)] for j in range(n)]
+        self.lengths, self._forked = lengths, False
         self.frames += n
+        self._seen += n
         return outputs, S
