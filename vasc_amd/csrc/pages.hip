@@ -575,8 +575,10 @@ extern "C" int64_t vasc_pages_reserve_workspace_size(int64_t pages, int64_t max_
   if (!(pages > 0 && pages < (int64_t(1) << 26) && max_pages > 0 && max_pages < (int64_t(1) << 24) && B > 0 && B <= 65536 &&
         tokens > 0 && tokens < (int64_t(1) << 30)))
     return -1;
+  const int64_t span = reserve_span(tokens, max_pages);
+  if (B * span >= (int64_t(1) << 31)) return -1;
   int64_t at[4];
-  return reserve_bytes(pages, B, reserve_span(tokens, max_pages), at);
+  return reserve_bytes(pages, B, span, at);
 }
 
 extern "C" int vasc_pages_reserve(int32_t *refs, int64_t pages, int32_t *page_table, int64_t table_stride, int64_t max_pages,
@@ -593,6 +595,7 @@ extern "C" int vasc_pages_reserve(int32_t *refs, int64_t pages, int32_t *page_ta
   p.lengths = lengths; p.count = count; p.tokens = tokens;
   p.B = static_cast<int32_t>(B);
   p.span = static_cast<int32_t>(reserve_span(tokens, max_pages));
+  VASC_REQUIRE(B * p.span < (int64_t(1) << 31), "too many pages for one call");  // ranks are 32 bits
   p.chunks = static_cast<int32_t>(cdiv(pages, kChunk));
   p.granted = granted; p.src = src; p.dst = dst;
   int64_t at[4];
