@@ -39,16 +39,31 @@ __device__ __forceinline__ halfx8 widen4(uint32_t w, const halfx8 &power) {
   return __builtin_bit_cast(halfx8, x) * power;
 }
 
+// A lane's 16 bytes of each kilobyte. kOnce: no other unit reads them, and they go past the caches. Measured, in us: single
+// tokens of 16 sequences up to 131072 long 285 with plain loads, 253 so; eight units of 16 tokens over the same pages 32.2
+// with plain loads, 34.1 so.
+template <bool kOnce, int n>
+__device__ __forceinline__ void load_codes(u32x4 (&x)[n], const uint8_t *at) {
+  if constexpr (kOnce) {
+#pragma unroll
+    for (int y = 0; y < n; ++y) x[y] = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(at + y * 1024));
+  } else {
+#pragma unroll
+    for (int y = 0; y < n; ++y) x[y] = *reinterpret_cast<const u32x4 *>(at + y * 1024);
+  }
+}
+
 // Few rows (up to 32): the cache's bytes bound the kernel. Each of the 4 waves holds all of the unit's rows, kTiles tiles of
 // 16, and takes every fourth page straight from memory to its registers; their sums are joined in LDS.
-template <typename Q, int D, int kTiles>
+// Measured: single tokens of 16 sequences of 39000 to 131072 tokens, 8 x 4 heads of 128, 1.46 GB in 254 us (5.8 TB/s).
+template <typename Q, int D, int kTiles, bool kOnce>
 __global__ __launch_bounds__(256, 2) void cache4_attn_few_kernel(const AttnParams p) {
   constexpr int kWaves = 4, kDT = D / 16, kRows = kTiles * 16;
   constexpr int kG = D / 32;   // groups of a row; 16-byte loads of a page's keys, or values, per lane; products of a key tile
   constexpr int kParts = __is_same(Q, __bf16) ? 1 : 2;
   constexpr int kOps = kParts * kG;
-  // Pages of a wave on their way. Two where that is 16 KB, single tokens of 16 sequences over up to 131072 keys (8 x 4 heads)
-  // 298 us with one, 285 with two; at D = 64 the registers cost a wave a SIMD (eight sequences up to 33312: 44.7 and 47.5).
+  // Pages of a wave on their way. D = 128: single tokens of 16 sequences over up to 131072 keys (8 x 4 heads) 268 us with one,
+  // 254 with two. At D = 64 two cost a wave a SIMD: eight sequences of up to 33312 tokens 45.0 us with one, 50.5 with two.
   constexpr int kAhead = D == 128 && kTiles == 1 ? 2 : 1;
   typedef float Sums[kRows][D + 2];
   constexpr size_t kQBytes = kTiles * kOps * 1024, kSBytes = (kWaves - 1) * sizeof(Sums);
@@ -94,14 +109,12 @@ __global__ __launch_bounds__(256, 2) void cache4_attn_few_kernel(const AttnParam
     } ahead[kAhead];
     auto load_keys = [&](int i, Raw &r) {
       const int64_t at = static_cast<int64_t>(__builtin_amdgcn_readlane(pid, i)) * p.H;
-#pragma unroll
-      for (int y = 0; y < kG; ++y) r.kr[y] = *reinterpret_cast<const u32x4 *>(kbase + at * (kPage * D / 2) + y * 1024);
+      load_codes<kOnce>(r.kr, kbase + at * (kPage * D / 2));
       r.kb = *reinterpret_cast<const uint32_t *>(ksbase + at * (kPage * kG));
     };
     auto load_values = [&](int i, Raw &r) {
       const int64_t at = static_cast<int64_t>(__builtin_amdgcn_readlane(pid, i)) * p.H;
-#pragma unroll
-      for (int y = 0; y < kG; ++y) r.vr[y] = *reinterpret_cast<const u32x4 *>(vbase + at * (kPage * D / 2) + y * 1024);
+      load_codes<kOnce>(r.vr, vbase + at * (kPage * D / 2));
       r.vb = *reinterpret_cast<const u32x4 *>(vsbase + at * kPage);
 #pragma unroll
       for (int y = 0; y < kG / 2; ++y) r.vp[y] = *reinterpret_cast<const u32x4 *>(vobase + at * (kG * 32) + y * 16);
@@ -186,6 +199,13 @@ __global__ __launch_bounds__(256, 2) void cache4_attn_few_kernel(const AttnParam
 
 // Many rows (up to 128): the vector and matrix pipes bound the kernel. As for the 8-bit cache the kWaves waves lie side by
 // side over the rows, and a page is widened once for all of them, in LDS, two buffers and one barrier a page.
+// Measured: a frame of 1041 queries over 522 of 2082 pages, 16 heads of 64, 142 GFLOP in 238 us with the join (600 TFLOP/s);
+// 250 causal tokens of 32 heads of 128 over 20001, 163 GFLOP in 201 us (810). The frame's parts, each left out of a copy for
+// its time alone: the softmax 79 us, the operands' reads from LDS 27, the pages' loads 23; what stays, widening, products and
+// barriers, 110, where the products by themselves need 65. Also built, and no faster: the softmax without a maximum
+// beforehand (weights checked in half, sums by a product with ones, one power for the values of a page, a third fewer vector
+// instructions: 283 to 330 us, as pages are done again where a row's maximum grows, and 241 had none been), loads two pages
+// ahead (238), every wave widening its pages itself without LDS (306).
 template <typename Q, int D, int kTiles, int kWaves>
 __global__ __launch_bounds__(kWaves * 64, D == 64 && kWaves == 4 ? 3 : 2) void cache4_attn_many_kernel(const AttnParams p) {
   constexpr int kDT = D / 16, kG = D / 32;
@@ -329,8 +349,14 @@ int launch_attn4(const AttnParams &p, const Shape &s, hipStream_t st) {
   // float16 queries of 128 features are two operands: 16 rows a wave
   constexpr int kWaves = D == 128 && !__is_same(Q, __bf16) ? 8 : 4;
   switch (s.kind) {
-    case 0: hipLaunchKernelGGL((cache4_attn_few_kernel<Q, D, 1>), grid, dim3(256), 0, st, p); break;
-    case 1: hipLaunchKernelGGL((cache4_attn_few_kernel<Q, D, 2>), grid, dim3(256), 0, st, p); break;
+    case 0:
+      if (p.U == 1) hipLaunchKernelGGL((cache4_attn_few_kernel<Q, D, 1, true>), grid, dim3(256), 0, st, p);
+      else hipLaunchKernelGGL((cache4_attn_few_kernel<Q, D, 1, false>), grid, dim3(256), 0, st, p);
+      break;
+    case 1:
+      if (p.U == 1) hipLaunchKernelGGL((cache4_attn_few_kernel<Q, D, 2, true>), grid, dim3(256), 0, st, p);
+      else hipLaunchKernelGGL((cache4_attn_few_kernel<Q, D, 2, false>), grid, dim3(256), 0, st, p);
+      break;
     case 2: hipLaunchKernelGGL((cache4_attn_many_kernel<Q, D, 1, 4>), grid, dim3(256), 0, st, p); break;
     default: hipLaunchKernelGGL((cache4_attn_many_kernel<Q, D, 8 / kWaves, kWaves>), grid, dim3(kWaves * 64), 0, st, p); break;
   }
