@@ -25,13 +25,14 @@ def _fill(cache, g, table, lens, k=None, v=None):
     return [O.quantise4(_np(k[b, :, :n]), _np(v[b, :, :n])) for b, n in enumerate(lens)]
 
 
+@pytest.mark.parametrize("dtype,powers", [(torch.float32, (-60, 0, 37)), (torch.bfloat16, (-60, 0, 37)), (torch.float16, (-12, 0, 9))])
 @pytest.mark.parametrize("D", [64, 128])
-def test_every_code_and_tie(D):
+def test_every_code_and_tie(D, dtype, powers):
     """Each e2m1 value, each tie between two and one step beside it, both signs, under several powers: the conversion's
     rounding. A value of 6 (or 7) beside them holds the power in place."""
     codes = [0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0]
     ties = [(a + b) / 2 for a, b in zip(codes, codes[1:])]
-    near = [t * (1 + s * 2.0 ** -22) for t in ties + codes for s in (-1, 1)]
+    near = [t * (1 + s * 2.0 ** -k) for t in ties + codes for s in (-1, 1) for k in (22, 10, 7)]
     values = [s * x for x in codes + ties + near for s in (1, -1)]
     values += [6.5, -6.5, 7.0, 6.9999995]
     rows = [values[i:i + 31] for i in range(0, len(values), 31)]
@@ -40,11 +41,12 @@ def test_every_code_and_tie(D):
     at = 0
     for row in rows:
         for top in tops:
-            for e in (-60, 0, 37):
+            for e in powers:
                 for gr in range(D // 32):
                     x[0, 0, at, gr * 32:gr * 32 + len(row)] = torch.tensor(row) * 2.0 ** e
                     x[0, 0, at, gr * 32 + 31] = top * 2.0 ** e
                 at += 1
+    x = x.to(dtype)
     table = _i32([list(range(-(-at // 64)))])
     cache = BlockCache(8, 1, D, bits=4)
     ops.cache_write(cache, x.cuda(), x.flip(3).contiguous().cuda(), table, _i32([0]))
@@ -96,8 +98,9 @@ def test_write_then_read(dtype, D, H):
         assert torch.equal(getattr(cache, n)[rest], t[rest]), n
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("D", [64, 128])
-def test_write_edge_values(D):
+def test_write_edge_values(D, dtype):
     """Groups at the borders of the format: 7 * 2^e and one step past it, the exponents' ends, groups of a value row farther
     apart than the offsets reach, zeros, float32's largest and smallest; tokens that are not finite."""
     step = 1 + 2.0 ** -10
@@ -110,6 +113,7 @@ def test_write_edge_values(D):
         # the next group 13, 14, 15 and more powers lower, in turn
         x[0, 0, i, 32:32 + len(r)] = x[0, 0, i, :len(r)] * 2.0 ** -(11 + i % 7)
         x[0, 0, i, D - 1] = x[0, 0, i, 0]
+    x = x.to(dtype)
     y = torch.full_like(x, 0.5)
     y[0, 0, 2, 5] = float("nan")  # a value that is not finite marks the token's key too
     table = _i32([[1]])

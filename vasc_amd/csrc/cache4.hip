@@ -14,23 +14,82 @@
 namespace vasc {
 namespace {
 
-// Eight values over 2^(byte - 127) as e2m1 codes: to nearest, ties to even, at most 6.
-__device__ __forceinline__ uint32_t quantise8_e2m1(const float (&x)[8], int byte) {
-  const float inv = __uint_as_float(static_cast<uint32_t>(254 - byte) << 23);
-  float y[8];
+// Eight consecutive elements of a row as they come. Half types stay packed: magnitudes are compared as integers, and the
+// conversion takes pairs and the power, so that a value costs two instructions, not ten (the kernel's bound had been those:
+// 128 frames of 16 heads of 64 at 89% of what the vector pipes issue).
+template <typename T>
+struct Eight {
+  typedef uint32_t words __attribute__((ext_vector_type(sizeof(T) == 4 ? 8 : 4)));
+  words w;
+
+  __device__ __forceinline__ void load(const T *src) {
+    const u32x4 *from = reinterpret_cast<const u32x4 *>(src);
+    const u32x4 a = __builtin_nontemporal_load(from);
+    if constexpr (sizeof(T) == 2) {
+      w = a;
+    } else {
+      const u32x4 b = __builtin_nontemporal_load(from + 1);
+      w = words{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+    }
+  }
+
+  // The bits of the largest magnitude, of an infinity or a NaN if there is one.
+  __device__ __forceinline__ uint32_t top() const {
+    if constexpr (sizeof(T) == 2) {
+      typedef uint16_t pair __attribute__((ext_vector_type(2)));
+      pair m = {0, 0};
 #pragma unroll
-  for (int i = 0; i < 8; ++i) y[i] = fminf(fmaxf(x[i] * inv, -6.f), 6.f);
-  uint32_t w = 0;
-  w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, y[0], y[1], 1.0f, 0);
-  w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, y[2], y[3], 1.0f, 1);
-  w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, y[4], y[5], 1.0f, 2);
-  return __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, y[6], y[7], 1.0f, 3);
-}
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t x = w[i] & 0x7fff7fffu;
+        m = __builtin_elementwise_max(m, __builtin_bit_cast(pair, x));
+      }
+      return max(static_cast<uint32_t>(m[0]), static_cast<uint32_t>(m[1]));
+    } else {
+      uint32_t m = 0;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) m = max(m, w[i] & 0x7fffffffu);
+      return m;
+    }
+  }
+  static __device__ __forceinline__ bool finite(uint32_t top) {
+    return top < (sizeof(T) == 4 ? 0x7f800000u : __is_same(T, __bf16) ? 0x7f80u : 0x7c00u);
+  }
+  static __device__ __forceinline__ float value(uint32_t top) {
+    if constexpr (sizeof(T) == 4) return __uint_as_float(top);
+    else if constexpr (__is_same(T, __bf16)) return __uint_as_float(top << 16);
+    else return static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(top)));
+  }
+
+  // Over 2^(byte - 127) as e2m1 codes: to nearest, ties to even, at most 6 (the conversion saturates).
+  __device__ __forceinline__ uint32_t codes(int byte) const {
+    const float power = pow2_byte(byte);
+    uint32_t r = 0;
+    if constexpr (sizeof(T) == 4) {
+      r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, __uint_as_float(w[0]), __uint_as_float(w[1]), power, 0);
+      r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, __uint_as_float(w[2]), __uint_as_float(w[3]), power, 1);
+      r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, __uint_as_float(w[4]), __uint_as_float(w[5]), power, 2);
+      r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, __uint_as_float(w[6]), __uint_as_float(w[7]), power, 3);
+    } else if constexpr (__is_same(T, __bf16)) {
+      const uint32_t a = w[0], b = w[1], c = w[2], d = w[3];  // copies: a bit cast of an element itself reads element 0
+      r = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(r, __builtin_bit_cast(bf16x2, a), power, 0);
+      r = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(r, __builtin_bit_cast(bf16x2, b), power, 1);
+      r = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(r, __builtin_bit_cast(bf16x2, c), power, 2);
+      r = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(r, __builtin_bit_cast(bf16x2, d), power, 3);
+    } else {
+      const uint32_t a = w[0], b = w[1], c = w[2], d = w[3];
+      r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(r, __builtin_bit_cast(halfx2, a), power, 0);
+      r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(r, __builtin_bit_cast(halfx2, b), power, 1);
+      r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(r, __builtin_bit_cast(halfx2, c), power, 2);
+      r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(r, __builtin_bit_cast(halfx2, d), power, 3);
+    }
+    return r;
+  }
+};
 
 // Max over the four neighbouring lanes of a group.
-__device__ __forceinline__ float group4_max(float v) {
-  v = fmaxf(v, dpp<kQuadXor1>(v));
-  return fmaxf(v, dpp<kQuadXor2>(v));
+__device__ __forceinline__ uint32_t group4_max(uint32_t v) {
+  v = max(v, xor_lane(v, 1));
+  return max(v, xor_lane(v, 2));
 }
 
 // Max over the groups of a row, which agree within.
@@ -67,25 +126,17 @@ __global__ __launch_bounds__(256) void cache4_write_kernel(const CacheArgs c, co
       if ((col & 31) == 0) ke[row][gr] = ks[gr * kPage + key_place(row)];
     } else if (row < w.hi) {
       const int64_t t = w.j * kPage + row - w.s;
-      float x[8], y[8];
-      load8(kin + t * r.kst + col, x);
-      load8(vin + t * r.vst + col, y);
-      float kmax = 0.f, vmax = 0.f, bad = 0.f;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        kmax = fmaxf(kmax, fabsf(x[i]));
-        vmax = fmaxf(vmax, fabsf(y[i]));
-        // all ones in the exponent: infinity or NaN (a maximum drops NaN)
-        if ((__float_as_uint(x[i]) & 0x7f800000u) == 0x7f800000u || (__float_as_uint(y[i]) & 0x7f800000u) == 0x7f800000u)
-          bad = 1.f;
-      }
-      int kb = power_of<2>(group4_max(kmax), -60, 60) + 127, vb = power_of<2>(group4_max(vmax), -60, 60) + 127;
+      Eight<T> x, y;
+      x.load(kin + t * r.kst + col);
+      y.load(vin + t * r.vst + col);
+      const uint32_t ktop = group4_max(x.top()), vtop = group4_max(y.top());
+      int kb = power_of<2>(Eight<T>::value(ktop), -60, 60) + 127, vb = power_of<2>(Eight<T>::value(vtop), -60, 60) + 127;
       int row_b = groups_max<D>(vb);
       vb = max(vb, row_b - 14);
       uint32_t kw = 0, vw = 0;
-      if (groups_max<D>(static_cast<int>(group4_max(bad))) == 0) {
-        kw = quantise8_e2m1(x, kb);
-        vw = quantise8_e2m1(y, vb);
+      if (groups_max<D>(Eight<T>::finite(max(ktop, vtop)) ? 0 : 1) == 0) {
+        kw = x.codes(kb);
+        vw = y.codes(vb);
       } else {
         kb = 255;
         vb = row_b = 127;
@@ -105,24 +156,26 @@ __global__ __launch_bounds__(256) void cache4_write_kernel(const CacheArgs c, co
   // values, transposed: 16 bytes hold a lane group's 16 tokens of two features
   if (tid < 64 * kG) {
     const int g = tid & 3, f = (tid >> 6) * 32 + ((tid >> 2) & 15);
-    uint32_t cover[2] = {0, 0}, out[4] = {0, 0, 0, 0};
+    uint32_t out[4] = {0, 0, 0, 0};
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      const int t = token4_of(g, i);
-      if (t < w.lo || t >= w.hi) continue;
-      cover[i >> 3] |= 15u << (4 * (i & 7));
+    for (int i = 0; i < 16; ++i)
 #pragma unroll
       for (int half = 0; half < 2; ++half)
-        out[half * 2 + (i >> 3)] |= (vt[t][(f >> 3) + half * 2] >> (4 * (f & 7)) & 15u) << (4 * (i & 7));
-    }
-    if (cover[0] | cover[1]) {
-      u32x4 *at = reinterpret_cast<u32x4 *>(vc + value4_at(f, g));
-      u32x4 x = {out[0], out[1], out[2], out[3]};
-      if ((cover[0] & cover[1]) != 0xffffffffu) {
+        out[half * 2 + (i >> 3)] |= (vt[token4_of(g, i)][(f >> 3) + half * 2] >> (4 * (f & 7)) & 15u) << (4 * (i & 7));
+    u32x4 *at = reinterpret_cast<u32x4 *>(vc + value4_at(f, g));
+    u32x4 x = {out[0], out[1], out[2], out[3]};
+    if (w.lo > 0 || w.hi < kPage) {  // what the call does not cover stays (and was not in vt)
+      uint32_t cover[2] = {0, 0};
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        if (token4_of(g, i) >= w.lo && token4_of(g, i) < w.hi) cover[i >> 3] |= 15u << (4 * (i & 7));
+      if (cover[0] | cover[1]) {
         const u32x4 old = *at;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) x[i] |= old[i] & ~cover[i & 1];
+        for (int i = 0; i < 4; ++i) x[i] = (x[i] & cover[i & 1]) | (old[i] & ~cover[i & 1]);
+        *at = x;
       }
+    } else {
       *at = x;
     }
   }
@@ -148,10 +201,9 @@ __global__ __launch_bounds__(256) void cache4_write_kernel(const CacheArgs c, co
     double s[8] = {0, 0, 0, 0, 0, 0, 0, 0};
     for (int row = grp; row < w.hi; row += kGroups) {
       float f[8];
-      unpack_e2m1(kt[row][word], f);
-      const float e = pow2_byte(ke[row][gr]);
+      unpack_e2m1(kt[row][word], f, pow2_byte(ke[row][gr]));
 #pragma unroll
-      for (int i = 0; i < 8; ++i) s[i] += static_cast<double>(f[i] * e);
+      for (int i = 0; i < 8; ++i) s[i] += static_cast<double>(f[i]);
     }
 #pragma unroll
     for (int i = 0; i < 8; ++i) part[grp][col + i] = s[i];
@@ -217,13 +269,8 @@ __global__ __launch_bounds__(256) void cache4_read_kernel(const CacheArgs c, con
       uint32_t vw = 0;
 #pragma unroll
       for (int e = 0; e < 8; ++e) vw |= (vt[(col + e) * kS + g * 8 + (i >> 1)] >> (4 * (i & 1)) & 15u) << (4 * e);
-      unpack_e2m1(kw[pass], x);
-      unpack_e2m1(vw, y);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        x[e] *= ke;
-        y[e] *= ve;
-      }
+      unpack_e2m1(kw[pass], x, ke);
+      unpack_e2m1(vw, y, ve);
     }
     store8(ko + t * D + col, x);
     store8(vout + t * D + col, y);

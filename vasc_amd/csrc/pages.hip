@@ -222,11 +222,16 @@ __global__ __launch_bounds__(256) void compact_kernel(const CompactArgs p) {
     for (int row = grp; row < hi; row += kGroups) {
       float f[kCodes];
       const uint32_t w = *reinterpret_cast<const uint32_t *>(kt + row * kS + word * 4);
-      if constexpr (kBits == 8) unpack_e4m3(w, f);
-      else unpack_e2m1(w, f);
       const float e = pow2_byte(ke[row][kBits == 8 ? 0 : word / 4]);
+      if constexpr (kBits == 8) {
+        unpack_e4m3(w, f);
 #pragma unroll
-      for (int i = 0; i < kCodes; ++i) s[i] += static_cast<double>(f[i] * e);
+        for (int i = 0; i < kCodes; ++i) f[i] *= e;
+      } else {
+        unpack_e2m1(w, f, e);
+      }
+#pragma unroll
+      for (int i = 0; i < kCodes; ++i) s[i] += static_cast<double>(f[i]);
     }
 #pragma unroll
     for (int i = 0; i < kCodes; ++i) part[grp][word * kCodes + i] = s[i];

@@ -61,10 +61,10 @@ __device__ __forceinline__ int token4_of(int g, int i) { return (i >> 2) * 16 + 
 // Bit of token k (of eight) in a word of value offsets: the even ones in the low half, the odd ones in the high.
 __device__ __forceinline__ int offset4_bit(int k) { return (k >> 1) * 4 + (k & 1) * 16; }
 
-// Eight e2m1 codes as floats.
-__device__ __forceinline__ void unpack_e2m1(uint32_t w, float (&f)[8]) {
-  const floatx2 a = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.0f, 0), b = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.0f, 1);
-  const floatx2 c = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.0f, 2), d = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.0f, 3);
+// Eight e2m1 codes times a power of two as floats (infinity: NaN).
+__device__ __forceinline__ void unpack_e2m1(uint32_t w, float (&f)[8], float power) {
+  const floatx2 a = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, power, 0), b = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, power, 1);
+  const floatx2 c = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, power, 2), d = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, power, 3);
   f[0] = a[0]; f[1] = a[1]; f[2] = b[0]; f[3] = b[1];
   f[4] = c[0]; f[5] = c[1]; f[6] = d[0]; f[7] = d[1];
 }
