@@ -6,8 +6,8 @@
 // the call touches that page, so partly covered words are merged with plain
 // loads and stores, and the page's key mean is recomputed from its codes, a
 // function of what the page holds whatever calls brought it there.
-// Measured (bf16, 16 heads of 64): 32 frames of 1041 tokens written in 47 us
-// (4.4 TB/s; a large copy reaches 4.75), read back in 32 us (6.4 TB/s, partly
+// Measured (bf16, 16 heads of 64): 32 frames of 1041 tokens written in 41 us
+// (5.0 TB/s; a large copy reaches 5.1), read back in 31 us (6.6 TB/s, partly
 // from the cache behind HBM); one token of 64 sequences, 8 heads of 128, in
 // 7.3 us: the latency of table, codes, barrier and merge.
 #include "cache_page.h"
