@@ -73,8 +73,8 @@ struct Work {
 __device__ __forceinline__ Work work_of(const AttnParams &p) {
   Work w;
   // The units of a part on one XCD, whose L2 then has their pages once; the parts in turn over the XCDs, which have the same
-  // work so however uneven the sequences are (a range of the parts each: 63 us for eight sequences of 12000 to 33000
-  // tokens over a 4-bit cache 59 us, so 45; over an 8-bit one 87 and 72). What does not fill all XCDs comes last.
+  // work so however uneven the sequences are. Measured, in us: eight sequences of 12000 to 33000 tokens, 59 with a range of the
+  // parts to each XCD and 45 so (4 bits), 87 and 72 (8 bits). What does not fill all XCDs comes last.
   int id = blockIdx.x;
   const int even = static_cast<int>(gridDim.x) / p.U / 8 * 8 * p.U;
   if (id < even) {

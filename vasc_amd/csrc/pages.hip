@@ -77,7 +77,7 @@ __device__ __forceinline__ uint32_t quad_transpose(uint32_t v) {
 // byte (or half of one) of a feature a token: a wave reads a feature of its 64 tokens at a time, which is one 64-byte line
 // where they are neighbours and never more than a line a token, and turns 4 x 4 bytes between lanes for the store.
 // Bound by HBM and by those lines: a quarter of the tokens of 16 sequences, others for each of 8 heads of 128 (4 bits), in
-// 51 us, four source pages' values read for each page written (155 MB, 3.0 TB/s); 32 of 128 frames, 16 heads of 64 (8 bits),
+// 51 us, four source pages' values read for each page written (126 MB of traffic by the counters); 32 of 128 frames, 16 heads of 64 (8 bits),
 // in 31 us (4.4 TB/s).
 template <int D, int kBits>
 __global__ __launch_bounds__(256) void compact_kernel(const CompactArgs p) {
