@@ -393,3 +393,72 @@ def test_rounding_of_normal_rows():
     for r in ops.cache_read(cache, table, _i32([0]), 256, dtype=torch.float32):
         err, size = (r.cpu() - x).double().view(-1, 32).abs(), x.double().view(-1, 32).abs()
         assert (err <= torch.maximum(size / 5, size.amax(-1, keepdim=True) / 14)).all()
+
+
+@pytest.mark.parametrize("D,G,T", [(64, 1, 1), (64, 2, 40), (128, 1, 1), (128, 4, 30)])
+def test_attend_strided_tensors_out_and_scales(D, G, T):
+    """Queries cut from wider rows, written to a strided `out` whose other elements stay; scales of both signs, 0 and large; a
+    causal chunk longer than its sequence, whose first rows see nothing."""
+    g = _gen(D + G + T)
+    H, lens = 2, [700, 9]
+    table, pages = _table(g, 2, 11)
+    cache = BlockCache(pages, H, D, bits=4)
+    held = _fill(cache, g, table, lens)
+    wide = _randn(g, 2, T, H * G + 3, D + 24).cuda()
+    q = wide[:, :, 1:1 + H * G, 8:8 + D].transpose(1, 2)
+    store = torch.full((2, T + 2, H * G, D + 8), 7.0, device="cuda", dtype=torch.bfloat16)
+    out = store[:, 1:T + 1, :, 4:4 + D].transpose(1, 2)
+    n_q = [T, max(1, T - 5)]
+    for causal in (False, True):
+        for scale in (None, -0.3, 0.0, 1.0):
+            got = ops.cache_attn(q, cache, table, _i32(lens), causal=causal, q_count=_i32(n_q), scale=scale, out=out)
+            assert got is out
+            # the bound's part of the logits is their size, scale times sum |q| |k|: below 0 for a negative scale, which would
+            # take 2 (D + 8) 2^-24 30 = 5e-4 from it here; the opposite queries have the same logits with the positive one
+            sign = -1 if scale is not None and scale < 0 else 1
+            _check_attend(got.contiguous(), sign * q.contiguous(), held, lens, None, 128 // G, causal,
+                          scale=None if scale is None else abs(scale), n_q=n_q, H=H)
+            if causal and T > lens[1]:
+                assert not got[1, :, :n_q[1] - lens[1]].any()
+            seen = store.clone()
+            seen[:, 1:T + 1, :, 4:4 + D] = 7.0
+            assert (seen == 7.0).all()
+
+
+def test_two_streams_at_once():
+    """Attention over one 4-bit cache and writes into another on streams of their own: as one after the other."""
+    g = _gen(53)
+    H, D, L = 2, 128, 4000
+    table, pages = _table(g, 2, 63)
+    cache, other = BlockCache(pages, H, D, bits=4), BlockCache(pages, H, D, bits=4)
+    k, v = _randn(g, 2, H, L, D).cuda(), _randn(g, 2, H, L, D).cuda()
+    ops.cache_write(cache, k, v, table, _i32([0, 0]))
+    q, n, start = _randn(g, 2, H, 1, D).cuda(), _i32([L]), _i32([0, 0])
+    want = [ops.cache_attn(q[b:b + 1], cache, table[b:b + 1], n) for b in range(2)]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in range(3)], [[], []]
+    for _ in range(6):
+        for b in range(2):
+            with torch.cuda.stream(streams[b]):
+                got[b].append(ops.cache_attn(q[b:b + 1], cache, table[b:b + 1], n))
+        with torch.cuda.stream(streams[2]):
+            ops.cache_write(other, k, v, table, start)
+    torch.cuda.synchronize()
+    for b in range(2):
+        assert all(torch.equal(x, want[b]) for x in got[b])
+    assert all(torch.equal(getattr(other, name), getattr(cache, name)) for name in BUFFERS)
+
+
+def test_inputs_that_need_a_gradient_are_refused():
+    cache = BlockCache(2, 1, 64, bits=4)
+    x = torch.zeros(1, 1, 3, 64, device="cuda", requires_grad=True)
+    table, n = _i32([[0, 1]]), _i32([0])
+    with pytest.raises(ValueError, match="gradient"):
+        ops.cache_write(cache, x, x, table, n)
+    with pytest.raises(ValueError, match="gradient"):
+        ops.cache_attn(x.bfloat16(), cache, table, n)
+    with pytest.raises(ValueError, match="heads"):
+        ops.cache_write(cache, x.detach().expand(1, 2, 3, 64), x.detach().expand(1, 2, 3, 64), table, n)
+    with torch.no_grad():
+        ops.cache_write(cache, x, x, table, n)
+    assert cache.nbytes == sum(getattr(cache, name).numel() * getattr(cache, name).element_size() for name in BUFFERS)

@@ -447,3 +447,31 @@ def test_stream_keeps_frames(bits, axes):
     full.reset()
     assert full.pool.available() == full.pool.pages
     full.push(images[:, [0, 1, 2]])
+
+
+def test_arguments_that_are_refused():
+    cache, pool = BlockCache(4, 2, 64, bits=4), PagePool(4)
+    table, n = _i32([[0, 1], [2, 3]]), _i32([5, 6])
+    for bad, match in (((table, n.cpu()), "GPU"), ((table.long(), n), "int32"), ((table[0], n), "int32"),
+                       ((table[:1].expand(2, 2), n), "overlap"), ((table.t(), n), "contiguous"), ((table, n.long()), "int32"),
+                       ((table, _i32([1, 2, 3])), "int32"), ((table, _i32([1, 2, 3, 4])[::2]), "contiguous")):
+        with pytest.raises(ValueError, match=match):
+            ops.pages_free(pool, *bad)
+    for bad, match in (((table.long(), n, 3), "int32"), ((table[:1].expand(2, 2), n, 3), "overlap"), ((table, n, -1), "negative"),
+                       ((table, None, 3), "lengths"), ((table, _i32([1]), 3), "lengths")):
+        with pytest.raises(ValueError, match=match):
+            ops.pages_reserve(pool, *bad)
+    for bad, match in (((table, n, None), "source"), ((table, n, table), "source"), ((table, n, n.float()), "integers"),
+                       ((table, _i32([1]), n), "lengths")):
+        with pytest.raises(ValueError, match=match):
+            ops.pages_fork(pool, *bad)
+    for bad, match in (((n, _i32([1])), "dst"), ((table, table), "src"), ((n, n.float()), "integers"), ((n, None), "dst")):
+        with pytest.raises(ValueError, match=match):
+            ops.cache_copy(cache, *bad)
+    index = torch.zeros(2, 3, device="cuda", dtype=torch.int32)
+    for bad, match in (((table, index[0], table), "index"), ((table, index.view(2, 1, 3).expand(2, 3, 3), table), "index"),
+                       ((table, index.expand(2, 3).float(), table), "integers"), ((table[:1], index, table), "page_table"),
+                       ((table, torch.zeros(2, 200, device="cuda", dtype=torch.int32), table), "out_table")):
+        with pytest.raises(ValueError, match=match):
+            ops.cache_compact(cache, *bad)
+    assert pool.refs.sum() == 0 and table.tolist() == [[0, 1], [2, 3]] and n.tolist() == [5, 6]

@@ -200,7 +200,7 @@ __global__ __launch_bounds__(256, 2) void cache4_attn_few_kernel(const AttnParam
 // Many rows (up to 128): the vector and matrix pipes bound the kernel. As for the 8-bit cache the kWaves waves lie side by
 // side over the rows, and a page is widened once for all of them, in LDS, two buffers and one barrier a page.
 // Measured: a frame of 1041 queries over 522 of 2082 pages, 16 heads of 64, 142 GFLOP in 238 us with the join (600 TFLOP/s);
-// 250 causal tokens of 32 heads of 128 over 20001, 163 GFLOP in 201 us (810). The frame's parts, each left out of a copy for
+// 250 causal tokens of 32 heads of 128 over 20001, 163 GFLOP in 193 us (840). The frame's parts, each left out of a copy for
 // its time alone: the softmax 79 us, the operands' reads from LDS 27, the pages' loads 23; what stays, widening, products and
 // barriers, 110, where the products by themselves need 65. Also built, and no faster: the softmax without a maximum
 // beforehand (weights checked in half, sums by a product with ones, one power for the values of a page, a third fewer vector
@@ -346,8 +346,9 @@ __global__ __launch_bounds__(kWaves * 64, D == 64 && kWaves == 4 ? 3 : 2) void c
 template <typename Q, int D>
 int launch_attn4(const AttnParams &p, const Shape &s, hipStream_t st) {
   const dim3 grid(static_cast<unsigned>(p.B * p.H * p.U * s.parts));
-  // float16 queries of 128 features are two operands: 16 rows a wave
-  constexpr int kWaves = D == 128 && !__is_same(Q, __bf16) ? 8 : 4;
+  // D = 128: 16 rows a wave, which leave registers for four waves a SIMD (32 rows: two; a causal chunk 201 and 193 us, and
+  // float16 queries are two operands). D = 64: 32, three waves (16 rows read the operands twice as often: a frame 311 and 238).
+  constexpr int kWaves = D == 128 ? 8 : 4;
   switch (s.kind) {
     case 0:
       if (p.U == 1) hipLaunchKernelGGL((cache4_attn_few_kernel<Q, D, 1, true>), grid, dim3(256), 0, st, p);
