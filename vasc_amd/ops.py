@@ -1188,8 +1188,9 @@ def cache_compact(cache, page_table: torch.Tensor, index: torch.Tensor, out_tabl
     Token ``index[b,i]`` of the sequence that ``page_table [B,max_pages]``
     holds becomes token ``i < count[b]`` (default all) of the one that
     ``out_table [B,pages]`` holds, k and v as they are held, with no rounding.
-    index ``[B,n]``, or ``[B,H,n]`` with a list for each head; an entry that is
-    no token of the table is held as zeros. Key means of the pages written
+    index ``[B,n]``, or ``[B,H,n]`` with a list for each head, in any order; an
+    entry outside the table's pages is held as zeros (one behind the sequence's
+    last token as whatever its slot has). Key means of the pages written
     are renewed over their tokens up to the last one; a page's slots behind
     that stay as they are. No page may occur twice among those written, nor
     be both written and read from; the pages of ``page_table`` still hold what
@@ -1276,9 +1277,10 @@ def pages_reserve(pool, page_table: torch.Tensor, lengths: torch.Tensor, tokens:
     """Pages for the next ``tokens`` tokens (``count[b]`` of them) of each sequence: ``(granted, src, dst)``.
 
     page_table ``[B,max_pages]``, int32, changes in place. Of the pages that
-    tokens ``lengths[b]..`` touch, the ones that a sequence lacks, or that
-    others hold too, are replaced by free pages, the lowest first, in the
-    order of sequences and tokens; a shared page then counts a holder less.
+    tokens ``lengths[b]..`` touch, the ones that a sequence lacks, that others
+    hold too, or that the pool does not count, are replaced by free pages, the
+    lowest first, in the order of sequences and tokens; a shared page then
+    counts a holder less.
     Where it holds tokens before ``lengths[b]`` it has to be copied before
     the write: from ``src[b]`` to ``dst[b]`` (-1: nothing to copy), which
     ``cache_copy`` takes, for every cache that the table serves.
