@@ -143,7 +143,7 @@ int vasc_cache_attn(const void *q, int64_t q_sb, int64_t q_sh, int64_t q_st, voi
                     const int32_t *q_count, int64_t block_q, const int32_t *index, int64_t width, const int32_t *count,
                     int32_t causal, float scale, void *workspace, int64_t workspace_bytes, void *stream);
 
-/* vasc_cache_write, vasc_cache_read and vasc_cache_attn for a 4-bit cache; the workspace is vasc_cache_attn's. */
+/* vasc_cache_write, vasc_cache_read, vasc_cache_attn and its workspace's size for a 4-bit cache. */
 int vasc_cache4_write(const void *k, int64_t k_sb, int64_t k_sh, int64_t k_st, const void *v, int64_t v_sb, int64_t v_sh,
                       int64_t v_st, int64_t B, int64_t H, int64_t T, int64_t D, int32_t dtype,
                       const int32_t *page_table, int64_t table_stride, int64_t max_pages, const int32_t *start,
@@ -153,6 +153,8 @@ int vasc_cache4_read(const uint8_t *kc, const uint8_t *vc, const uint8_t *ks, co
                      int64_t pages, const int32_t *page_table, int64_t table_stride, int64_t max_pages,
                      const int32_t *start, const int32_t *count, int64_t B, int64_t H, int64_t T, int64_t D,
                      int32_t dtype, void *k_out, void *v_out, void *stream);
+int64_t vasc_cache4_attn_workspace_size(int64_t B, int64_t Hq, int64_t H, int64_t T, int64_t D, int64_t block_q,
+                                        int64_t max_pages, int64_t width);
 int vasc_cache4_attn(const void *q, int64_t q_sb, int64_t q_sh, int64_t q_st, void *o, int64_t o_sb, int64_t o_sh,
                      int64_t o_st, int64_t B, int64_t Hq, int64_t H, int64_t T, int64_t D, int32_t dtype,
                      const uint8_t *kc, const uint8_t *vc, const uint8_t *ks, const uint8_t *vs, const uint8_t *vo,

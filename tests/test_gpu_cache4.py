@@ -1,6 +1,7 @@
 """The 4-bit block cache against its definitions in float64 (oracle/streaming.py), as tests/test_gpu_streaming.py has them for
 the 8-bit one; the attention's bound is that one's: the widened keys and values are exact here too."""
 import copy
+import math
 import pickle
 
 import numpy as np
@@ -9,7 +10,7 @@ import torch
 
 from oracle import streaming as O
 from test_gpu_streaming import _check_attend, _gen, _i32, _np, _randn, _same, _table
-from vasc_amd import ops
+from vasc_amd import _lib, ops
 from vasc_amd.streaming import BlockCache
 
 pytestmark = pytest.mark.gpu
@@ -462,3 +463,49 @@ def test_inputs_that_need_a_gradient_are_refused():
     with torch.no_grad():
         ops.cache_write(cache, x, x, table, n)
     assert cache.nbytes == sum(getattr(cache, name).numel() * getattr(cache, name).element_size() for name in BUFFERS)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("how", ["lists", "causal"])
+def test_attend_frame_with_short_last_unit(how, dtype):
+    """A frame of 1041 queries over many pages, whose last unit of 17 rows has a launch of its own: lists of every unit, or a
+    causal chunk with a shorter count, against float64 on the GPU. The bound is _check_attend's."""
+    g = _gen(7)
+    H, D, T, L, block = 16, 64, 1041, 133200, 128
+    table, pages = _table(g, 1, -(-L // 64))
+    cache = BlockCache(pages, H, D, bits=4)
+    k, v = _randn(g, 1, H, L, D).cuda(), _randn(g, 1, H, L, D).cuda()
+    ops.cache_write(cache, k, v, table, _i32([0]))
+    k, v = (x[0].double() for x in ops.cache_read(cache, table, _i32([0]), L))
+    q = _randn(g, 1, H, T, D, dtype=dtype).cuda()
+    n_q = T if how == "lists" else T - 9
+    size = _lib.fn("vasc_cache4_attn_workspace_size")
+    sizes = [size(1, H, H, t, D, block, table.shape[1], 522 if how == "lists" else 0) for t in (T, T + 15, T + 16, 9 * block)]
+    # 17 and 32 rows are a launch of their own, of other parts; 33 are not, and take what 128 do
+    assert sizes[0] != sizes[2] and sizes[1] != sizes[2] and sizes[2] == sizes[3]
+    if how == "lists":
+        index, count = ops.cache_select(q, cache, table, _i32([L]), 520, block_q=block)
+        o = ops.cache_attn(q, cache, table, _i32([L]), index, count, block_q=block)
+    else:
+        o = ops.cache_attn(q, cache, table, _i32([L]), causal=True, q_count=_i32([n_q]))
+    pos = torch.arange(L, device="cuda")
+    for h in range(H):
+        for u in range(-(-T // block)):
+            rows = torch.arange(u * block, min(T, (u + 1) * block), device="cuda")
+            if how == "lists":
+                listed = torch.zeros(table.shape[1], dtype=torch.bool, device="cuda")
+                listed[index[0, h, u, :count[0, h, u]].long()] = True
+                seen = listed[pos // 64].expand(len(rows), L)
+            else:
+                seen = (pos[None] <= (L - n_q + rows)[:, None]) & (rows < n_q)[:, None]
+            qd = q[0, h, rows].double()
+            x = torch.where(seen, qd @ k[h].T.contiguous() * D ** -0.5, -math.inf)
+            w = torch.nan_to_num(torch.softmax(x, -1))
+            ref, mag = w @ v[h], w @ v[h].abs()
+            logit = torch.where(seen, qd.abs() @ k[h].abs().T.contiguous() * D ** -0.5, 0.0).amax(-1, keepdim=True)
+            n = seen.sum(-1, keepdim=True)
+            rel = 2.0 ** -11 + 2 * ((D + 8) * 2.0 ** -24 * logit + n * 2.0 ** -24) + 2.0 ** -14.5
+            half = torch.finfo(dtype).eps / 2
+            bound = rel * mag + half * (ref.abs() + rel * mag) + n * 2.0 ** -36 * v[h].abs().max() + 2.0 ** -25
+            assert ((o[0, h, rows].double() - ref).abs() <= bound).all(), (h, u)
+    assert not o[:, :, n_q:].any()

@@ -141,6 +141,10 @@ def test_workspace_sizes():
     for bad in ((0, 8, 2, 5), (1 << 26, 8, 2, 5), (9, 0, 2, 5), (9, 8, 0, 5), (9, 8, 2, 0), (9, 8, 65537, 5), (9, 8, 2, 1 << 30),
                 (9, 1 << 23, 65536, 1 << 29)):
         assert size(*bad) == -1
+    attn = _lib.fn("vasc_cache4_attn_workspace_size")
+    assert attn(1, 4, 2, 1, 64, 1, 5000, 0) > 0 and attn(1, 4, 2, 1, 64, 1, 5000, 4) == 0
+    for bad in ((0, 4, 2, 1, 64, 1, 10, 0), (1, 5, 2, 1, 64, 1, 10, 0), (1, 4, 2, 1, 60, 1, 10, 0), (1, 4, 2, 1, 64, 65, 10, 0)):
+        assert attn(*bad) == -1
 
 
 def test_host_tensors_and_constructors():

@@ -96,6 +96,7 @@ SIGNATURES: dict[str, tuple] = {
     "vasc_cache4_write": (c_int32, [P, I64, I64, I64, P, I64, I64, I64, I64, I64, I64, I64, I32, P, I64, I64, P, P,
                                     P, P, P, P, P, P, I64, P]),
     "vasc_cache4_read": (c_int32, [P, P, P, P, P, I64, P, I64, I64, P, P, I64, I64, I64, I64, I32, P, P, P]),
+    "vasc_cache4_attn_workspace_size": (I64, [I64, I64, I64, I64, I64, I64, I64, I64]),
     "vasc_cache4_attn": (c_int32, [P, I64, I64, I64, P, I64, I64, I64, I64, I64, I64, I64, I64, I32, P, P, P, P, P, I64,
                                    P, I64, I64, P, P, I64, P, I64, P, I32, c_float, P, I64, P]),
     "vasc_cache_copy": (c_int32, [I32, P, P, P, P, P, P, I64, I64, I64, P, P, I64, P]),

@@ -351,11 +351,11 @@ int launch_attn4(const AttnParams &p, const Shape &s, hipStream_t st) {
   constexpr int kWaves = D == 128 ? 8 : 4;
   switch (s.kind) {
     case 0:
-      if (p.U == 1) hipLaunchKernelGGL((cache4_attn_few_kernel<Q, D, 1, true>), grid, dim3(256), 0, st, p);
+      if (p.list_U == 1) hipLaunchKernelGGL((cache4_attn_few_kernel<Q, D, 1, true>), grid, dim3(256), 0, st, p);
       else hipLaunchKernelGGL((cache4_attn_few_kernel<Q, D, 1, false>), grid, dim3(256), 0, st, p);
       break;
     case 1:
-      if (p.U == 1) hipLaunchKernelGGL((cache4_attn_few_kernel<Q, D, 2, true>), grid, dim3(256), 0, st, p);
+      if (p.list_U == 1) hipLaunchKernelGGL((cache4_attn_few_kernel<Q, D, 2, true>), grid, dim3(256), 0, st, p);
       else hipLaunchKernelGGL((cache4_attn_few_kernel<Q, D, 2, false>), grid, dim3(256), 0, st, p);
       break;
     case 2: hipLaunchKernelGGL((cache4_attn_many_kernel<Q, D, 1, 4>), grid, dim3(256), 0, st, p); break;
@@ -365,8 +365,42 @@ int launch_attn4(const AttnParams &p, const Shape &s, hipStream_t st) {
   return rc ? rc : launch_join<Q, D>(p, s, st, "vasc_cache4_attn");
 }
 
+// A call's units, and in a launch of its own the last one of each head where that is better.
+//
+// The last unit of a frame has few rows (1041 tokens: 17 of 128), but among the others it takes a workgroup's place for as long
+// as they do; by itself it is one of few rows, whose four waves share its pages. Measured, in us: a frame over 522 pages, 16
+// heads of 64, 246 in one launch and 235 in two (1152 tokens, nine full units, 249), two of 1036 float16 queries over 82 pages
+// 112 and 102. The second launch and its join take some 8 us however small, which the estimate has to win: a frame over 130
+// pages is 97 in one launch (106 in two), 270 queries over 152 pages 45 (53).
+struct Plan {
+  Shape body, tail;
+  int64_t body_units, tail_rows;  // units of a head in the first launch; rows of the second's one (0: none)
+};
+
+Plan attn_plan(int64_t heads, int64_t G, int64_t T, int64_t D, int64_t block_q, int64_t pages) {
+  Plan plan;
+  plan.body_units = cdiv(T, block_q);
+  plan.tail_rows = 0;
+  plan.body = attn_shape(heads * plan.body_units, block_q * G, pages, D);
+  const int64_t rows = (T - (plan.body_units - 1) * block_q) * G;
+  if (plan.body.kind < 2 || plan.body_units < 2 || rows > 32) return plan;
+  const Shape body = attn_shape(heads * (plan.body_units - 1), block_q * G, pages, D), tail = attn_shape(heads, rows, pages, D);
+  if (body.us + tail.us + 8.0 >= plan.body.us) return plan;
+  return {body, tail, plan.body_units - 1, rows};
+}
+
 }  // namespace
 }  // namespace vasc
+
+extern "C" int64_t vasc_cache4_attn_workspace_size(int64_t B, int64_t Hq, int64_t H, int64_t T, int64_t D,
+                                                   int64_t block_q, int64_t max_pages, int64_t width) {
+  using namespace vasc;
+  if (!attn_sizes(B, Hq, H, T, D, block_q, max_pages, width)) return -1;
+  const Plan plan = attn_plan(B * H, Hq / H, T, D, block_q, width ? width : max_pages);
+  int64_t bytes = workspace_bytes(B * H * plan.body_units, block_q * (Hq / H), D, plan.body.parts);
+  if (plan.tail_rows) bytes = (bytes + 15) / 16 * 16 + workspace_bytes(B * H, plan.tail_rows, D, plan.tail.parts);
+  return bytes;
+}
 
 extern "C" int vasc_cache4_attn(const void *q, int64_t q_sb, int64_t q_sh, int64_t q_st, void *o, int64_t o_sb,
                                 int64_t o_sh, int64_t o_st, int64_t B, int64_t Hq, int64_t H, int64_t T, int64_t D,
@@ -378,13 +412,26 @@ extern "C" int vasc_cache4_attn(const void *q, int64_t q_sb, int64_t q_sh, int64
   using namespace vasc;
   VASC_REQUIRE(vo && (reinterpret_cast<uintptr_t>(vo) & 15) == 0, "vo must be given and 16-byte aligned");
   AttnParams p = {};
-  Shape s;
-  const int rc = attn_params(q, q_sb, q_sh, q_st, o, o_sb, o_sh, o_st, B, Hq, H, T, D, dtype, kc, vc, ks, vs, pages, page_table,
-                             table_stride, max_pages, lengths, q_count, block_q, index, width, count, causal, scale, workspace,
-                             workspace_bytes_given, p, s);
+  int rc = attn_params(q, q_sb, q_sh, q_st, o, o_sb, o_sh, o_st, B, Hq, H, T, D, dtype, kc, vc, ks, vs, pages, page_table,
+                       table_stride, max_pages, lengths, q_count, block_q, index, width, count, causal, scale, p);
   if (rc) return rc;
   p.vo = vo;
+  const Plan plan = attn_plan(B * H, p.G, T, D, block_q, width ? width : max_pages);
+  p.U = static_cast<int>(plan.body_units);
+  int64_t used = 0;
+  if ((rc = take_workspace(p, plan.body, D, workspace, workspace_bytes_given, used))) return rc;
+  AttnParams last = p;
+  if (plan.tail_rows) {
+    last.u0 = p.U;
+    last.U = 1;
+    last.rows = static_cast<int>(plan.tail_rows);
+    if ((rc = take_workspace(last, plan.tail, D, workspace, workspace_bytes_given, used))) return rc;
+  }
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
-  if (D == 64) return dtype == 0 ? launch_attn4<__bf16, 64>(p, s, st) : launch_attn4<_Float16, 64>(p, s, st);
-  return dtype == 0 ? launch_attn4<__bf16, 128>(p, s, st) : launch_attn4<_Float16, 128>(p, s, st);
+  const auto launch = [&](const AttnParams &a, const Shape &s) {
+    if (D == 64) return dtype == 0 ? launch_attn4<__bf16, 64>(a, s, st) : launch_attn4<_Float16, 64>(a, s, st);
+    return dtype == 0 ? launch_attn4<__bf16, 128>(a, s, st) : launch_attn4<_Float16, 128>(a, s, st);
+  };
+  if ((rc = launch(p, plan.body)) || !plan.tail_rows) return rc;
+  return launch(last, plan.tail);
 }

@@ -18,7 +18,8 @@ struct AttnParams {
   void *o;
   int64_t osb, osh, ost;
   int64_t B, T;
-  int H, G, U;
+  int H, G, U;          // U: units of this launch, from u0 of the call's list_U on
+  int u0, list_U;
   const uint8_t *kc, *vc, *ks, *vs, *vo;  // vo: of the 4-bit cache
   int64_t pages;
   const int32_t *table;
@@ -92,7 +93,7 @@ __device__ __forceinline__ Work work_of(const AttnParams &p) {
   w.L = p.lengths[w.b];
   w.nq = p.n_q ? p.n_q[w.b] : p.T;
   w.nq = w.nq < 0 ? 0 : (w.nq < p.T ? w.nq : p.T);
-  w.t0 = static_cast<int64_t>(w.u) * p.block_q;
+  w.t0 = static_cast<int64_t>(p.u0 + w.u) * p.block_q;
   w.t1 = w.t0 + p.block_q < w.nq ? w.t0 + p.block_q : w.nq;
   const UnitView view = unit_view(w.L, w.nq, w.t0, w.t1, p.max_pages, p.causal);
   w.cut = static_cast<int>(clamp_tokens(w.L, p.max_pages));  // below 2^30
@@ -101,8 +102,9 @@ __device__ __forceinline__ Work work_of(const AttnParams &p) {
   w.entries = w.seen;
   w.list = nullptr;
   if (p.index) {
-    w.list = p.index + w.unit_row * p.width;
-    const int64_t n = p.count[w.unit_row];
+    const int64_t row = static_cast<int64_t>(bh) * p.list_U + p.u0 + w.u;
+    w.list = p.index + row * p.width;
+    const int64_t n = p.count[row];
     w.entries = w.seen == 0 ? 0 : static_cast<int>(n < 0 ? 0 : (n < p.width ? n : p.width));
   }
   const int share = (w.entries + p.parts - 1) / p.parts;
@@ -417,7 +419,7 @@ __global__ __launch_bounds__(256) void cache_join_kernel(const AttnParams p) {
   const int r = static_cast<int>(row - unit * p.rows), tl = r / p.G, gh = r - tl * p.G;
   const int u = static_cast<int>(unit % p.U);
   const int64_t bh = unit / p.U, b = bh / p.H, h = bh - b * p.H;
-  const int64_t t = static_cast<int64_t>(u) * p.block_q + tl;
+  const int64_t t = static_cast<int64_t>(p.u0 + u) * p.block_q + tl;
   if (t >= p.T) return;  // the same for a whole workgroup where it shares a row
   const float *o = p.ws + row * p.parts * D + d;
   const float *ml = p.ws + all * p.parts * D + row * p.parts * 2;
@@ -486,6 +488,7 @@ __global__ __launch_bounds__(256) void cache_join_kernel(const AttnParams p) {
 struct Shape {
   int kind;   // 16 rows a wave, 32, or 64 or 128 a workgroup
   int parts;
+  double us;  // estimated
 };
 
 // Few rows (up to 32) or many (64, 128), and how many workgroups share a unit's pages: as many as one to four rounds of
@@ -516,6 +519,7 @@ Shape attn_shape(int64_t units, int64_t rows, int64_t pages, int64_t D) {
       s.parts = static_cast<int>(parts);
     }
   }
+  s.us = best;
   return s;
 }
 
@@ -542,13 +546,12 @@ int launch_join(const AttnParams &p, const Shape &s, hipStream_t st, const char 
   return check_launch(what);
 }
 
-// Checks a call's arguments and fills what the kernels take (but p.vo).
+// Checks a call's arguments and fills what the kernels take (but vo, the parts and the workspace), for one launch.
 int attn_params(const void *q, int64_t q_sb, int64_t q_sh, int64_t q_st, void *o, int64_t o_sb, int64_t o_sh, int64_t o_st,
                 int64_t B, int64_t Hq, int64_t H, int64_t T, int64_t D, int32_t dtype, const uint8_t *kc, const uint8_t *vc,
                 const uint8_t *ks, const uint8_t *vs, int64_t pages, const int32_t *page_table, int64_t table_stride,
                 int64_t max_pages, const int32_t *lengths, const int32_t *q_count, int64_t block_q, const int32_t *index,
-                int64_t width, const int32_t *count, int32_t causal, float scale, void *workspace,
-                int64_t workspace_bytes_given, AttnParams &p, Shape &s) {
+                int64_t width, const int32_t *count, int32_t causal, float scale, AttnParams &p) {
   VASC_SUPPORTED(D == 64 || D == 128, "D %lld not built (64, 128)", (long long)D);
   VASC_SUPPORTED(dtype == 0 || dtype == 1, "dtype %d not built", dtype);
   VASC_REQUIRE(q && o && kc && vc && ks && vs && page_table && lengths, "a required pointer is NULL");
@@ -569,7 +572,7 @@ int attn_params(const void *q, int64_t q_sb, int64_t q_sh, int64_t q_st, void *o
   p.B = B; p.T = T;
   p.H = static_cast<int>(H);
   p.G = static_cast<int>(Hq / H);
-  p.U = static_cast<int>(cdiv(T, block_q));
+  p.U = p.list_U = static_cast<int>(cdiv(T, block_q));
   p.kc = kc; p.vc = vc; p.ks = ks; p.vs = vs; p.pages = pages;
   p.table = page_table; p.table_stride = table_stride; p.max_pages = max_pages;
   p.lengths = lengths; p.n_q = q_count;
@@ -581,15 +584,20 @@ int attn_params(const void *q, int64_t q_sb, int64_t q_sh, int64_t q_st, void *o
   // the reference is divided by c: a scale of 0 is one too small to show
   p.c = scale == 0.f ? 1e-30f : scale * 1.4426950408889634f;
   p.rows = p.block_q * p.G;
-  const int64_t units = B * H * p.U;
-  s = attn_shape(units, p.rows, width ? width : max_pages, D);
+  return VASC_OK;
+}
+
+// What a launch over p.U units takes of the workspace, from `used` bytes of it on.
+int take_workspace(AttnParams &p, const Shape &s, int64_t D, void *workspace, int64_t given, int64_t &used) {
+  const int64_t units = p.B * p.H * p.U;
   p.parts = s.parts;
   VASC_REQUIRE(units < (int64_t(1) << 31) / s.parts, "too many units");
-  const int64_t need = workspace_bytes(units, p.rows, D, s.parts);
-  VASC_REQUIRE(need == 0 || (workspace && workspace_bytes_given >= need), "workspace of %lld bytes, %lld needed",
-               (long long)workspace_bytes_given, (long long)need);
   VASC_REQUIRE((reinterpret_cast<uintptr_t>(workspace) & 15) == 0, "the workspace must be 16-byte aligned");
-  p.ws = static_cast<float *>(workspace);
+  const int64_t need = workspace_bytes(units, p.rows, D, s.parts);
+  VASC_REQUIRE(need == 0 || (workspace && given >= used + need), "workspace of %lld bytes, %lld needed", (long long)given,
+               (long long)(used + need));
+  p.ws = reinterpret_cast<float *>(static_cast<uint8_t *>(workspace) + used);
+  used += (need + 15) / 16 * 16;
   return VASC_OK;
 }
 

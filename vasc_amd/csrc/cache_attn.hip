@@ -362,11 +362,12 @@ extern "C" int vasc_cache_attn(const void *q, int64_t q_sb, int64_t q_sh, int64_
                                void *workspace, int64_t workspace_bytes_given, void *stream) {
   using namespace vasc;
   AttnParams p = {};
-  Shape s;
-  const int rc = attn_params(q, q_sb, q_sh, q_st, o, o_sb, o_sh, o_st, B, Hq, H, T, D, dtype, kc, vc, ks, vs, pages, page_table,
-                             table_stride, max_pages, lengths, q_count, block_q, index, width, count, causal, scale, workspace,
-                             workspace_bytes_given, p, s);
+  int rc = attn_params(q, q_sb, q_sh, q_st, o, o_sb, o_sh, o_st, B, Hq, H, T, D, dtype, kc, vc, ks, vs, pages, page_table,
+                       table_stride, max_pages, lengths, q_count, block_q, index, width, count, causal, scale, p);
   if (rc) return rc;
+  const Shape s = attn_shape(B * H * p.U, p.rows, width ? width : max_pages, D);
+  int64_t used = 0;
+  if ((rc = take_workspace(p, s, D, workspace, workspace_bytes_given, used))) return rc;
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   if (D == 64) return dtype == 0 ? launch_attn<__bf16, 64>(p, s, st) : launch_attn<_Float16, 64>(p, s, st);
   return dtype == 0 ? launch_attn<__bf16, 128>(p, s, st) : launch_attn<_Float16, 128>(p, s, st);

@@ -942,7 +942,7 @@ def rotary_axes(q: torch.Tensor, k: torch.Tensor | None, pos: torch.Tensor, sect
     return _rotary(q, k, pos, sections, inv_freq, False)
 
 
-_CACHE_ENTRIES = {(n, name): f"vasc_cache{four}_{name}" for n, four in ((4, ""), (5, "4")) for name in ("write", "read", "attn")}
+_CACHE_ENTRIES = {(n, name): f"vasc_cache{four}_{name}" for n, four in ((4, ""), (5, "4")) for name in ("write", "read", "attn", "attn_workspace_size")}
 
 
 def _cache_entry(cache, name: str) -> str:
@@ -1073,8 +1073,8 @@ def cache_select(q: torch.Tensor, cache, page_table: torch.Tensor, lengths: torc
 
 
 @functools.lru_cache(maxsize=256)
-def _attn_workspace(*sizes: int) -> int:
-    return _lib.fn("vasc_cache_attn_workspace_size")(*sizes)
+def _attn_workspace(entry: str, *sizes: int) -> int:
+    return _lib.fn(entry)(*sizes)
 
 
 def cache_attn(q: torch.Tensor, cache, page_table: torch.Tensor, lengths: torch.Tensor,
@@ -1134,7 +1134,7 @@ def cache_attn(q: torch.Tensor, cache, page_table: torch.Tensor, lengths: torch.
         return out
     if index is not None and width == 0:
         return out.zero_()
-    size = _attn_workspace(B, Hq, H, T, D, block_q, mp, width)
+    size = _attn_workspace(_cache_entry(cache, "attn_workspace_size"), B, Hq, H, T, D, block_q, mp, width)
     ws = torch.empty(size, device=q.device, dtype=torch.uint8) if size > 0 else None
     _launch(dev, _cache_entry(cache, "attn"), *qargs, out.data_ptr(), osb, osh, ost, B, Hq, H, T, D, _DTYPE[q.dtype],
             *cache.pointers, cache.pages, table.data_ptr(), ts, mp, lengths.data_ptr(), _ptr(q_count), block_q,
