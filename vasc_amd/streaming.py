@@ -98,7 +98,8 @@ class PagePool:
     ``ops.pages_reserve`` gives sequences the lowest free pages, ``pages_fork``
     lets sequences share pages, ``pages_free`` gives them back; a table starts
     as -1 throughout. Nothing is kept on the host, so that a captured call
-    serves every step.
+    serves every step. Calls on one pool go one after another: on one stream,
+    or on streams that wait for each other.
     """
 
     def __init__(self, pages: int, device="cuda"):
