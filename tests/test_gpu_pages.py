@@ -195,7 +195,7 @@ def test_pool_random_walk(seed):
                 lengths += granted
                 tokens = [n + c for n, c in zip(tokens, g2)]
         elif what == "fork":
-            source = [r.randint(-1, len(rows)) for _ in range(r.choice([1, 4, 13]))]
+            source = [r.randint(-1, len(rows)) for _ in range(r.choice([1, 4, 13, 40]))]
             new, new_lengths = ops.pages_fork(pool, table, lengths, _i32(source))
             new_rows, new_tokens = ref.fork(rows, tokens, source)
             ops.pages_free(pool, table, lengths)

@@ -4,8 +4,8 @@
 // The counts are all that is kept: a page is free where its count is not positive, and the lowest free pages are given out
 // first. So what a call gives does not depend on the order of earlier calls, of its own atomics, or of its workgroups.
 //
-// Measured, in us: 32 branches of four sequences of up to 64 pages: fork 2.6, reserve 3.3 and 5.4, copy 4.5, free 2.6, the
-// latency of a few loads that depend on one another; 256 branches of 64 sequences of up to 1024 pages, in a pool of 45000: 9.2,
+// Measured, in us: eight branches of four sequences of up to 64 pages: fork 2.6, reserve 6.4, copy 4.7, free 2.6, the latency
+// of a few loads that depend on one another; 256 branches of 64 sequences of up to 1024 pages, in a pool of 45000: 9.2,
 // 7.3 and 6.4, 5.5, 9.2. A host that calls them one by one takes longer for each (5 to 12).
 #include "cache_page.h"
 
@@ -327,35 +327,31 @@ __device__ __forceinline__ Growth growth(const ReserveArgs &p, int64_t b) {
   return w;
 }
 
-// First: what is free (a wave 1024 pages), and what each sequence needs (a wave a sequence). An entry whose page is missing
-// becomes -1, one whose page others hold too -2 less the page, until the second kernel has served or restored it.
-__global__ __launch_bounds__(256) void reserve_count_kernel(const ReserveArgs p) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  if (static_cast<int>(blockIdx.x) < p.chunks) {
-    __shared__ int sum[4];
-    const int64_t base = static_cast<int64_t>(blockIdx.x) * kChunk + wave * (kChunk / 4);
-    int n = 0;
-    int32_t r[16];
+// A wave's 1024 pages: the words of their free bits; returns how many are free.
+__device__ __forceinline__ int count_free(const ReserveArgs &p, int64_t base, uint64_t *free) {
+  const int lane = threadIdx.x & 63;
+  int n = 0;
+  int32_t r[16];
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      const int64_t at = base + i * 64 + lane;
-      r[i] = at < p.pages ? p.refs[at] : 1;
-    }
-    uint64_t mine = 0;
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      const uint64_t bits = __ballot(r[i] <= 0);
-      n += __popcll(bits);
-      if (lane == i) mine = bits;
-    }
-    if (lane < 16) p.free[base / 64 + lane] = mine;
-    if (lane == 0) sum[wave] = n;
-    __syncthreads();
-    if (threadIdx.x == 0) p.chunk[blockIdx.x] = sum[0] + sum[1] + sum[2] + sum[3];
-    return;
+  for (int i = 0; i < 16; ++i) {
+    const int64_t at = base + i * 64 + lane;
+    r[i] = at < p.pages ? p.refs[at] : 1;
   }
-  const int64_t b = (static_cast<int64_t>(blockIdx.x) - p.chunks) * 4 + wave;
-  if (b >= p.B) return;
+  uint64_t mine = 0;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    const uint64_t bits = __ballot(r[i] <= 0);
+    n += __popcll(bits);
+    if (lane == i) mine = bits;
+  }
+  if (lane < 16) free[base / 64 + lane] = mine;
+  return n;
+}
+
+// The pages that sequence b needs. An entry whose page is missing becomes -1, one whose page others hold too -2 less the page,
+// until the sequence has been served or they are restored.
+__device__ __forceinline__ int count_needs(const ReserveArgs &p, int64_t b) {
+  const int lane = threadIdx.x & 63;
   const Growth w = growth(p, b);
   int n = 0;
   for (int i0 = 0; i0 < w.n; i0 += 64) {
@@ -370,7 +366,7 @@ __global__ __launch_bounds__(256) void reserve_count_kernel(const ReserveArgs p)
     }
     n += __popcll(__ballot(need));
   }
-  if (lane == 0) p.need[b] = n;
+  return n;
 }
 
 __device__ __forceinline__ int wave_scan(int v) {  // inclusive
@@ -382,20 +378,19 @@ __device__ __forceinline__ int wave_scan(int v) {  // inclusive
   return v;
 }
 
-// Second: a wave a sequence. It has the free pages of ranks [before, before + need), if there are so many.
-__global__ __launch_bounds__(256) void reserve_take_kernel(const ReserveArgs p) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int64_t b = static_cast<int64_t>(blockIdx.x) * 4 + wave;
-  if (b >= p.B) return;
+// Serves sequence b: it has the free pages of ranks [before, before + need), if there are so many.
+__device__ __forceinline__ void take_pages(const ReserveArgs &p, int64_t b, const uint64_t *free, const int32_t *chunk,
+                                           const int32_t *needs) {
+  const int lane = threadIdx.x & 63;
   const Growth w = growth(p, b);
-  const int need = p.need[b];
+  const int need = needs[b];
   int32_t src = -1, dst = -1;
   int64_t granted = w.fit;
   if (need > 0) {
     int64_t before = 0;
     {
       int v = 0;
-      for (int i = lane; i < b; i += 64) v += p.need[i];
+      for (int i = lane; i < b; i += 64) v += needs[i];
       before = wave_sum_int(v);
     }
     const int64_t end = before + need;
@@ -403,7 +398,7 @@ __global__ __launch_bounds__(256) void reserve_take_kernel(const ReserveArgs p) 
     int64_t seen = 0;
     int32_t *list = p.list + b * p.span;
     for (int c0 = 0; c0 < p.chunks && seen < end; c0 += 64) {
-      const int mine = c0 + lane < p.chunks ? p.chunk[c0 + lane] : 0;
+      const int mine = c0 + lane < p.chunks ? chunk[c0 + lane] : 0;
       const int upto = wave_scan(mine);
       const int all = __shfl(upto, 63);
       uint64_t hit = __ballot(mine > 0 && seen + upto > before && seen + upto - mine < end);
@@ -411,7 +406,7 @@ __global__ __launch_bounds__(256) void reserve_take_kernel(const ReserveArgs p) 
         const int i = __ffsll(static_cast<unsigned long long>(hit)) - 1;
         hit &= hit - 1;
         const int64_t base = static_cast<int64_t>(c0 + i) * kChunk + lane * 64;
-        uint64_t bits = p.free[base / 64];
+        uint64_t bits = free[base / 64];
         const int n = __popcll(bits);
         int64_t rank = seen + __shfl(upto - mine, i) + wave_scan(n) - n;  // of this word's first
         if (rank + n <= before || rank >= end) continue;
@@ -454,6 +449,50 @@ __global__ __launch_bounds__(256) void reserve_take_kernel(const ReserveArgs p) 
     p.src[b] = src;
     p.dst[b] = dst;
   }
+}
+
+// First: what is free (a wave 1024 pages), and what each sequence needs (a wave a sequence).
+__global__ __launch_bounds__(256) void reserve_count_kernel(const ReserveArgs p) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  if (static_cast<int>(blockIdx.x) < p.chunks) {
+    __shared__ int sum[4];
+    const int n = count_free(p, static_cast<int64_t>(blockIdx.x) * kChunk + wave * (kChunk / 4), p.free);
+    if (lane == 0) sum[wave] = n;
+    __syncthreads();
+    if (threadIdx.x == 0) p.chunk[blockIdx.x] = sum[0] + sum[1] + sum[2] + sum[3];
+    return;
+  }
+  const int64_t b = (static_cast<int64_t>(blockIdx.x) - p.chunks) * 4 + wave;
+  if (b >= p.B) return;
+  const int n = count_needs(p, b);
+  if (lane == 0) p.need[b] = n;
+}
+
+// Second: a wave a sequence.
+__global__ __launch_bounds__(256) void reserve_take_kernel(const ReserveArgs p) {
+  const int64_t b = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
+  if (b < p.B) take_pages(p, b, p.free, p.chunk, p.need);
+}
+
+// Both in one workgroup, for small pools and batches, a wave a sequence. Measured, with a free of the same table, in us among
+// others and alone: 16 sequences, 4000 pages 15.0 and 26.3, in two launches 17.8 and 27.8; one sequence of 30000 tokens, 16000
+// pages 18.9 and 35.4, 19.5 and 36.2; 32 sequences of 100 tokens, two to a wave, 20.0 and 36.2, 17.8 and 31.9.
+constexpr int kFewPages = 4 * kChunk, kFewSequences = 16;
+
+__global__ __launch_bounds__(1024) void reserve_few_kernel(const ReserveArgs p) {
+  __shared__ uint64_t free[kFewPages / 64];
+  __shared__ int32_t sum[16], chunk[4], need[kFewSequences];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int n = count_free(p, wave * 1024, free);
+  if (lane == 0) sum[wave] = n;
+  if (wave < p.B) {
+    const int k = count_needs(p, wave);
+    if (lane == 0) need[wave] = k;
+  }
+  __syncthreads();
+  if (threadIdx.x < 4) chunk[threadIdx.x] = sum[threadIdx.x * 4] + sum[threadIdx.x * 4 + 1] + sum[threadIdx.x * 4 + 2] + sum[threadIdx.x * 4 + 3];
+  __syncthreads();
+  if (wave < p.B) take_pages(p, wave, free, chunk, need);
 }
 
 int check_pool(const void *refs, int64_t pages, const void *table, int64_t stride, int64_t max_pages, const void *lengths, int64_t B) {
@@ -620,6 +659,10 @@ extern "C" int vasc_pages_reserve(int32_t *refs, int64_t pages, int32_t *page_ta
   p.need = reinterpret_cast<int32_t *>(ws + at[2]);
   p.list = reinterpret_cast<int32_t *>(ws + at[3]);
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+  if (pages <= kFewPages && B <= kFewSequences) {
+    hipLaunchKernelGGL(reserve_few_kernel, dim3(1), dim3(1024), 0, s, p);
+    return check_launch("vasc_pages_reserve");
+  }
   const unsigned rows = static_cast<unsigned>(cdiv(B, 4));
   hipLaunchKernelGGL(reserve_count_kernel, dim3(static_cast<unsigned>(p.chunks) + rows), dim3(256), 0, s, p);
   if ((rc = check_launch("vasc_pages_reserve"))) return rc;
