@@ -475,3 +475,31 @@ def test_arguments_that_are_refused():
         with pytest.raises(ValueError, match=match):
             ops.cache_compact(cache, *bad)
     assert pool.refs.sum() == 0 and table.tolist() == [[0, 1], [2, 3]] and n.tolist() == [5, 6]
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+def test_full_pool_costs_tokens_not_pages(bits):
+    """Branches of a pool with one free page: the first gets it, the others are granted nothing, and their writes with that
+    count change neither the parent's page nor each other's."""
+    g = _gen(23)
+    H, D = 2, 64
+    pool, cache = PagePool(3), BlockCache(3, H, D, bits=bits)
+    table, n = torch.full((1, 4), -1, device="cuda", dtype=torch.int32), _i32([0])
+    k = _randn(g, 1, H, 100, D).cuda()
+    granted, _, _ = ops.pages_reserve(pool, table, n, 100)
+    ops.cache_write(cache, k, k, table, n, count=granted)
+    n += granted
+    q = _randn(g, 1, H, 1, D).cuda()
+    parent = ops.cache_attn(q, cache, table, n)
+    branch, m = ops.pages_fork(pool, table, n, _i32([0, 0, 0]))
+    granted, src, dst = ops.pages_reserve(pool, branch, m, 5)
+    assert granted.tolist() == [5, 0, 0] and src.tolist() == [1, -1, -1] and dst.tolist() == [2, -1, -1]
+    assert branch.tolist() == [[0, 2, -1, -1], [0, 1, -1, -1], [0, 1, -1, -1]] and pool.refs.tolist() == [4, 3, 1]
+    ops.cache_copy(cache, src, dst)
+    new = _randn(g, 3, H, 5, D).cuda()
+    ops.cache_write(cache, new, new, branch, m, count=granted)
+    assert torch.equal(ops.cache_attn(q, cache, table, n), parent)
+    o = ops.cache_attn(q.expand(3, -1, -1, -1), cache, branch, m)
+    assert all(torch.equal(o[i:i + 1], parent) for i in range(3))
+    ops.pages_free(pool, branch, m)
+    assert pool.refs.tolist() == [1, 1, 0] and m.tolist() == [0, 0, 0]
