@@ -140,11 +140,8 @@ class Pool:
             ok = not lacking or wanted <= len(free)
             granted.append(c if ok else 0)
             s = d = -1
-            for i, j in enumerate(lacking):
+            for i, j in enumerate(lacking if ok else ()):
                 held = 0 <= row[j] < len(before)
-                if not ok:
-                    row[j] = row[j] if held else -1
-                    continue
                 if held:
                     if before[row[j]] > 0:
                         self.refs[row[j]] -= 1

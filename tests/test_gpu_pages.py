@@ -252,6 +252,38 @@ def test_reserve_odd_tables():
     assert ops.pages_fork(pool, table, _i32(lengths), _i32([]))[0].shape == (0, 3)
 
 
+def _check_reserve(refs, rows, lengths, counts):
+    """One call against the oracle, and a second that gives none of the pages again that the first has given. Returns the first's
+    (granted, src, dst), the rows and the holders' counts after it."""
+    B, T = len(rows), max(max(counts), 1)
+    pool, ref = PagePool(len(refs)), O.Pool(refs)
+    pool.refs.copy_(_i32(refs))
+    table = _i32(rows)
+    got = [t.tolist() for t in ops.pages_reserve(pool, table, _i32(lengths), T, _i32(counts))]
+    new, *want = ref.reserve(rows, lengths, counts)
+    assert got == want and _state(pool, table) == [ref.refs, new]
+    other = torch.full((1, 3), -1, device="cuda", dtype=torch.int32)
+    ops.pages_reserve(pool, other, _i32([0]), 150)
+    for old, row, granted in zip(rows, new, got[0]):
+        if granted == 0:
+            assert row == old
+        assert not {p for p, o in zip(row, old) if p != o} & set(other[0].tolist())
+    return got, new, ref.refs
+
+
+# pools and batches that one workgroup serves, and those that take two launches
+@pytest.mark.parametrize("pages,idle", [(12, 0), (12, 20), (20000, 0), (20000, 20)])
+def test_reserve_refused_rows_keep_their_entries(pages, idle):
+    """A row that gets nothing stays as it is, its entries that name no page among them."""
+    refs = [1] * pages
+    refs[4] = refs[9] = 0
+    rows = [[0, -1], [1, 2 ** 31 - 1], [pages, -9], [3, 5]] + [[2, -1]] * idle
+    got, new, after = _check_reserve(refs, rows, [60, 64, 0, 40] + [0] * idle, [10, 20, 65, 30] + [0] * idle)
+    assert got[0] == [10, 20, 0, 30] + [0] * idle and new[:4] == [[0, 4], [1, 9], [pages, -9], [3, 5]]
+    got, new, after = _check_reserve([2] * pages, rows, [60, 64, 0, 40] + [0] * idle, [10, 20, 65, 30] + [0] * idle)
+    assert not any(got[0]) and new == rows and after == [2] * pages
+
+
 @pytest.mark.parametrize("bits", [4, 8])
 def test_branches_write_apart(bits):
     """Three sequences fork into seven; each branch reserves, copies, writes tokens of its own and attends: as a cache that

@@ -294,6 +294,8 @@ __global__ __launch_bounds__(256) void free_kernel(int32_t *refs, int64_t pages,
   table[row * stride + j] = -1;
 }
 
+constexpr int32_t kMissing = -1, kKept = -2;
+
 struct ReserveArgs {
   int32_t *refs;
   int64_t pages;
@@ -306,6 +308,7 @@ struct ReserveArgs {
   uint64_t *free;          // a bit a page
   int32_t *chunk, *need;   // free pages of each chunk, pages that each sequence needs
   int32_t *list;           // [B][span]: a sequence's new pages
+  int32_t *mark;           // [B][span]: of the pages that it touches, the one to be replaced, kMissing or kKept
 };
 
 constexpr int kChunk = 4096;  // pages of a chunk: a word of free bits a lane
@@ -348,23 +351,21 @@ __device__ __forceinline__ int count_free(const ReserveArgs &p, int64_t base, ui
   return n;
 }
 
-// The pages that sequence b needs. An entry whose page is missing becomes -1, one whose page others hold too -2 less the page,
-// until the sequence has been served or they are restored.
+// The pages that sequence b needs. The table keeps its entries until the sequence is served.
 __device__ __forceinline__ int count_needs(const ReserveArgs &p, int64_t b) {
   const int lane = threadIdx.x & 63;
   const Growth w = growth(p, b);
   int n = 0;
   for (int i0 = 0; i0 < w.n; i0 += 64) {
     const int i = i0 + lane;
-    bool need = false;
+    int32_t mark = kKept;
     if (i < w.n) {
-      int32_t *at = p.table + b * p.stride + w.first + i;
-      const int32_t e = *at;
+      const int32_t e = p.table[b * p.stride + w.first + i];
       const bool held = e >= 0 && e < p.pages;
-      need = !held || p.refs[e] != 1;
-      if (need) *at = held ? -2 - e : -1;
+      if (!held || p.refs[e] != 1) mark = held ? e : kMissing;
+      p.mark[b * p.span + i] = mark;
     }
-    n += __popcll(__ballot(need));
+    n += __popcll(__ballot(mark != kKept));
   }
   return n;
 }
@@ -420,25 +421,19 @@ __device__ __forceinline__ void take_pages(const ReserveArgs &p, int64_t b, cons
     const bool ok = seen >= end;
     if (!ok) granted = 0;
     int done = 0;
-    for (int i0 = 0; i0 < w.n; i0 += 64) {
+    for (int i0 = 0; ok && i0 < w.n; i0 += 64) {
       const int i = i0 + lane;
-      int32_t *at = p.table + b * p.stride + w.first + i;
-      const int32_t e = i < w.n ? *at : 0;
-      const uint64_t flags = __ballot(e < 0);
-      if (e < 0) {
-        const int32_t old = e < -1 ? -2 - e : -1;
-        if (!ok) {
-          *at = old;
-        } else {
-          const int32_t page = list[done + lanes_below(flags)];
-          *at = page;
-          p.refs[page] = 1;
-          // a page that nobody counts as held is not counted down
-          if (old >= 0 && p.refs[old] > 0) atomicSub(p.refs + old, 1);
-          if (i == 0 && w.L % kPage && old >= 0) {
-            src = old;
-            dst = page;
-          }
+      const int32_t old = i < w.n ? p.mark[b * p.span + i] : kKept;
+      const uint64_t flags = __ballot(old != kKept);
+      if (old != kKept) {
+        const int32_t page = list[done + lanes_below(flags)];
+        p.table[b * p.stride + w.first + i] = page;
+        p.refs[page] = 1;
+        // a page that nobody counts as held is not counted down
+        if (old >= 0 && p.refs[old] > 0) atomicSub(p.refs + old, 1);
+        if (i == 0 && w.L % kPage && old >= 0) {
+          src = old;
+          dst = page;
         }
       }
       done += __popcll(flags);
@@ -603,12 +598,12 @@ extern "C" int vasc_pages_free(int32_t *refs, int64_t pages, int32_t *page_table
 
 namespace vasc {
 namespace {
-// Workspace: free bits, free pages of the chunks, needs, lists.
-int64_t reserve_bytes(int64_t pages, int64_t B, int64_t span, int64_t (&at)[4]) {
+// Workspace: free bits, free pages of the chunks, needs, lists, marks.
+int64_t reserve_bytes(int64_t pages, int64_t B, int64_t span, int64_t (&at)[5]) {
   const int64_t chunks = cdiv(pages, kChunk);
-  const int64_t size[4] = {chunks * (kChunk / 8), chunks * 4, B * 4, B * span * 4};
+  const int64_t size[5] = {chunks * (kChunk / 8), chunks * 4, B * 4, B * span * 4, B * span * 4};
   int64_t sum = 0;
-  for (int i = 0; i < 4; ++i) {
+  for (int i = 0; i < 5; ++i) {
     at[i] = sum;
     sum += static_cast<int64_t>(align256(size[i]));
   }
@@ -628,7 +623,7 @@ extern "C" int64_t vasc_pages_reserve_workspace_size(int64_t pages, int64_t max_
     return -1;
   const int64_t span = reserve_span(tokens, max_pages);
   if (B * span >= (int64_t(1) << 31)) return -1;
-  int64_t at[4];
+  int64_t at[5];
   return reserve_bytes(pages, B, span, at);
 }
 
@@ -649,7 +644,7 @@ extern "C" int vasc_pages_reserve(int32_t *refs, int64_t pages, int32_t *page_ta
   VASC_REQUIRE(B * p.span < (int64_t(1) << 31), "too many pages for one call");  // ranks are 32 bits
   p.chunks = static_cast<int32_t>(cdiv(pages, kChunk));
   p.granted = granted; p.src = src; p.dst = dst;
-  int64_t at[4];
+  int64_t at[5];
   const int64_t need = reserve_bytes(pages, B, p.span, at);
   VASC_REQUIRE(workspace && workspace_bytes >= need, "workspace of %lld bytes, %lld needed", (long long)workspace_bytes, (long long)need);
   VASC_REQUIRE((reinterpret_cast<uintptr_t>(workspace) & 15) == 0, "the workspace must be 16-byte aligned");
@@ -658,6 +653,7 @@ extern "C" int vasc_pages_reserve(int32_t *refs, int64_t pages, int32_t *page_ta
   p.chunk = reinterpret_cast<int32_t *>(ws + at[1]);
   p.need = reinterpret_cast<int32_t *>(ws + at[2]);
   p.list = reinterpret_cast<int32_t *>(ws + at[3]);
+  p.mark = reinterpret_cast<int32_t *>(ws + at[4]);
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   if (pages <= kFewPages && B <= kFewSequences) {
     hipLaunchKernelGGL(reserve_few_kernel, dim3(1), dim3(1024), 0, s, p);
