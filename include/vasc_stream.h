@@ -205,11 +205,14 @@ int vasc_pages_free(int32_t *refs, int64_t pages, int32_t *page_table, int64_t t
  * Reserve: of the pages that tokens lengths[b] .. lengths[b] + count[b]
  * (NULL: tokens; cut to what max_pages hold) touch, those that are missing
  * (no page, or a count that is not 1) are replaced, in the order of sequences
- * and pages, by the free pages, lowest first; a replaced page counts a holder
- * less. granted[b]: those tokens, or 0 where the free pages do not suffice for
- * this sequence and all before it that lack some: its row is left as it is.
- * src[b], dst[b]: the replaced page that holds tokens before lengths[b], and
- * its replacement, or -1.
+ * and pages, by the free pages, lowest first; a replaced page that was counted
+ * counts a holder less. granted[b]: those tokens, or 0 where the free pages do
+ * not suffice for this sequence and all before it that lack some, or where
+ * tokens before lengths[b] lie in the page to be written and that page is free
+ * (it may be given to anyone): its row is left as it is, and takes no page
+ * from the others. All of it goes by the counts before the call. src[b],
+ * dst[b]: the replaced page that holds tokens before lengths[b], and its
+ * replacement, or -1.
  */
 int64_t vasc_pages_reserve_workspace_size(int64_t pages, int64_t max_pages, int64_t B, int64_t tokens);
 int vasc_pages_reserve(int32_t *refs, int64_t pages, int32_t *page_table, int64_t table_stride, int64_t max_pages,

@@ -130,21 +130,25 @@ class Pool:
         free = [p for p, r in enumerate(before) if r <= 0]
         table = [list(row) for row in table]
         granted, src, dst, wanted = [], [], [], 0
+
+        def held(p):
+            return 0 <= p < len(before) and before[p] > 0
+
         for row, n, c in zip(table, lengths, counts):
             mp = len(row)
             n = max(0, min(n, mp * PAGE))
             c = max(0, min(c, mp * PAGE - n))
+            if c and n % PAGE and 0 <= row[n // PAGE] < len(before) and not held(row[n // PAGE]):
+                c = 0  # the last page's tokens are in one that is free
             lacking = [j for j in range(n // PAGE, -(-(n + c) // PAGE) if c else 0)
-                       if not (0 <= row[j] < len(before) and before[row[j]] == 1)]
+                       if not (held(row[j]) and before[row[j]] == 1)]
             at, wanted = wanted, wanted + len(lacking)
             ok = not lacking or wanted <= len(free)
             granted.append(c if ok else 0)
             s = d = -1
             for i, j in enumerate(lacking if ok else ()):
-                held = 0 <= row[j] < len(before)
-                if held:
-                    if before[row[j]] > 0:
-                        self.refs[row[j]] -= 1
+                if held(row[j]):
+                    self.refs[row[j]] -= 1
                     if j * PAGE < n:
                         s, d = row[j], free[at + i]
                 row[j] = free[at + i]

@@ -284,6 +284,46 @@ def test_reserve_refused_rows_keep_their_entries(pages, idle):
     assert not any(got[0]) and new == rows and after == [2] * pages
 
 
+# (counts of the first pages, rows, lengths, counts) -> (granted, rows, counts of the first pages)
+UNCOUNTED = {
+    "given back to its row": (([0, 0], [[0, 1]], [0], [128]), ([128], [[0, 1]], [1, 1])),
+    "given to an earlier row": (([0, 0, 1], [[-1, -1], [0, -1]], [0, 0], [10, 10]), ([10, 10], [[0, -1], [1, -1]], [1, 1, 1])),
+    "given to a later row": (([0, 1, 0], [[2, -1], [-1, -1]], [0, 0], [10, 10]), ([10, 10], [[0, -1], [2, -1]], [1, 1, 1])),
+    "swapped": (([0, 0], [[1, -1], [0, -1]], [0, 0], [64, 1]), ([64, 1], [[0, -1], [1, -1]], [1, 1])),
+    "negative": (([-1, -3], [[1, 0]], [0], [128]), ([128], [[0, 1]], [1, 1])),
+    "behind the tokens held": (([1, 0, 0], [[0, 2]], [40], [50]), ([50], [[0, 1]], [1, 1, 0])),
+    # a free page may be anyone's: a row whose tokens lie there gets nothing, and takes none from the others
+    "holds tokens": (([0, 0, 1], [[1, -1], [2, -1]], [10, 60], [10, 10]), ([0, 10], [[1, -1], [2, 0]], [1, 0, 1])),
+    "hold each other's": (([0, 0], [[1, -1], [0, -1]], [10, 20], [1, 64]), ([0, 0], [[1, -1], [0, -1]], [0, 0])),
+}
+
+
+@pytest.mark.parametrize("pages,idle", [(5, 0), (4, 20), (20000, 0), (20000, 20)])
+@pytest.mark.parametrize("case", UNCOUNTED)
+def test_reserve_of_pages_that_nobody_counts(case, pages, idle):
+    """Pages that a row names and the pool holds for free: what a call gives is counted once, whichever row is served first."""
+    (refs, rows, lengths, counts), (granted, want, first) = UNCOUNTED[case]
+    refs = refs + [1] * (pages - len(refs))
+    more = [0] * idle
+    got, new, after = _check_reserve(refs, rows + [[-1, -1]] * idle, lengths + more, counts + more)
+    assert got == [granted + more, [-1] * len(granted + more), [-1] * len(granted + more)]
+    assert new[:len(rows)] == want and after[:len(first)] == first and set(after[len(first):]) <= {1}
+
+
+@pytest.mark.parametrize("seed", range(8))
+def test_reserve_of_any_table(seed):
+    """Counts and entries by chance, also ones that do not agree."""
+    r = random.Random(seed)
+    for pages, B, mp in ((9, 3, 3), (60, 16, 5), (60, 17, 5), (17000, 5, 90), (300, 40, 4)):
+        busy = r.choice([0.3, 0.9])
+        refs = [r.choice([1, 1, 2, 3]) if r.random() < busy else r.choice([0, 0, -1]) for _ in range(pages)]
+        near = min(pages, B * mp)
+        rows = [[r.choice([-1, -5, pages, r.randrange(near), r.randrange(near)]) for _ in range(mp)] for _ in range(B)]
+        lengths = [r.choice([0, 64, r.randint(-2, mp * 64 + 2)]) for _ in range(B)]
+        got, _, _ = _check_reserve(refs, rows, lengths, [r.randint(-1, mp * 40) for _ in range(B)])
+        assert not {p for p in got[1] if p >= 0} & {p for p in got[2] if p >= 0}
+
+
 @pytest.mark.parametrize("bits", [4, 8])
 def test_branches_write_apart(bits):
     """Three sequences fork into seven; each branch reserves, copies, writes tokens of its own and attends: as a cache that

@@ -240,3 +240,37 @@ def test_pool_counts_its_holders():
                 pool.free(rows, lengths, [0] * len(rows))
             named = np.bincount([p for rows, _ in tables for row in rows for p in row if p >= 0], minlength=pages)
             assert named.tolist() == pool.refs
+
+
+def test_oracle_reserve_of_any_table():
+    """Counts and entries that do not agree: what is given was free, is given once and counted once; refused rows stay; counted
+    pages lose a holder for each entry that is replaced; nothing is both copied from and given."""
+    g = np.random.default_rng(3)
+    for _ in range(200):
+        pages, B, mp = 12, int(g.integers(1, 6)), 3
+        before = g.choice([-1, 0, 0, 1, 1, 2, 3], pages).tolist()
+        rows = g.integers(-2, pages + 1, (B, mp)).tolist()
+        lengths, counts = g.integers(-1, mp * 64 + 2, B).tolist(), g.integers(-1, 150, B).tolist()
+        pool = O.Pool(before)
+        new, granted, src, dst = pool.reserve(rows, lengths, counts)
+        lost = np.zeros(pages, int)
+        for old, row, n, c in zip(rows, new, lengths, granted):
+            assert c > 0 or row == old
+            touched = range(max(n, 0) // 64, -(-(max(n, 0) + c) // 64) if c else 0)
+            for j in range(mp):
+                if j not in touched:
+                    assert row[j] == old[j]
+                elif not (0 <= old[j] < pages and before[old[j]] == 1):
+                    assert before[row[j]] <= 0 and pool.refs[row[j]] == 1
+                    if 0 <= old[j] < pages and before[old[j]] > 0:
+                        lost[old[j]] += 1
+                else:
+                    assert row[j] == old[j]
+        fresh = [row[j] for old, row, n, c in zip(rows, new, lengths, granted) if c
+                 for j in range(max(n, 0) // 64, -(-(max(n, 0) + c) // 64)) if before[row[j]] <= 0]
+        assert len(fresh) == len(set(fresh))
+        assert sorted(fresh) == [p for p in range(pages) if before[p] <= 0][:len(fresh)]
+        for p in range(pages):
+            assert pool.refs[p] == (1 if p in fresh else before[p] - lost[p])
+        copied = {p for p in src if p >= 0}
+        assert not copied & {p for p in dst if p >= 0} and not copied & set(fresh)

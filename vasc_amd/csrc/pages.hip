@@ -295,6 +295,7 @@ __global__ __launch_bounds__(256) void free_kernel(int32_t *refs, int64_t pages,
 }
 
 constexpr int32_t kMissing = -1, kKept = -2;
+constexpr int32_t kRefused = -1;
 
 struct ReserveArgs {
   int32_t *refs;
@@ -351,7 +352,10 @@ __device__ __forceinline__ int count_free(const ReserveArgs &p, int64_t base, ui
   return n;
 }
 
-// The pages that sequence b needs. The table keeps its entries until the sequence is served.
+// The pages that sequence b needs, or kRefused. All of it is decided here, on the holders before the call: a page that nobody
+// counts is free, so it may be given to any sequence of the call, and its count says nothing from then on. Such a page is
+// missing; where it is the one with the sequence's last tokens, they may be gone, and the sequence gets nothing.
+// The table keeps its entries until the sequence is served.
 __device__ __forceinline__ int count_needs(const ReserveArgs &p, int64_t b) {
   const int lane = threadIdx.x & 63;
   const Growth w = growth(p, b);
@@ -359,12 +363,16 @@ __device__ __forceinline__ int count_needs(const ReserveArgs &p, int64_t b) {
   for (int i0 = 0; i0 < w.n; i0 += 64) {
     const int i = i0 + lane;
     int32_t mark = kKept;
+    bool lost = false;
     if (i < w.n) {
       const int32_t e = p.table[b * p.stride + w.first + i];
-      const bool held = e >= 0 && e < p.pages;
-      if (!held || p.refs[e] != 1) mark = held ? e : kMissing;
+      const bool page = e >= 0 && e < p.pages;
+      const int32_t holders = page ? p.refs[e] : 0;
+      if (holders != 1) mark = holders > 0 ? e : kMissing;
       p.mark[b * p.span + i] = mark;
+      lost = page && holders <= 0 && i == 0 && w.L % kPage;
     }
+    if (__ballot(lost)) return kRefused;
     n += __popcll(__ballot(mark != kKept));
   }
   return n;
@@ -386,12 +394,12 @@ __device__ __forceinline__ void take_pages(const ReserveArgs &p, int64_t b, cons
   const Growth w = growth(p, b);
   const int need = needs[b];
   int32_t src = -1, dst = -1;
-  int64_t granted = w.fit;
+  int64_t granted = need == kRefused ? 0 : w.fit;
   if (need > 0) {
     int64_t before = 0;
     {
       int v = 0;
-      for (int i = lane; i < b; i += 64) v += needs[i];
+      for (int i = lane; i < b; i += 64) v += max(needs[i], 0);
       before = wave_sum_int(v);
     }
     const int64_t end = before + need;
@@ -428,9 +436,8 @@ __device__ __forceinline__ void take_pages(const ReserveArgs &p, int64_t b, cons
       if (old != kKept) {
         const int32_t page = list[done + lanes_below(flags)];
         p.table[b * p.stride + w.first + i] = page;
-        p.refs[page] = 1;
-        // a page that nobody counts as held is not counted down
-        if (old >= 0 && p.refs[old] > 0) atomicSub(p.refs + old, 1);
+        p.refs[page] = 1;  // it was free, and `old` was not: no other store of the call meets this one
+        if (old >= 0) atomicSub(p.refs + old, 1);
         if (i == 0 && w.L % kPage && old >= 0) {
           src = old;
           dst = page;

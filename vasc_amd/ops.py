@@ -1278,17 +1278,19 @@ def pages_reserve(pool, page_table: torch.Tensor, lengths: torch.Tensor, tokens:
 
     page_table ``[B,max_pages]``, int32, changes in place. Of the pages that
     tokens ``lengths[b]..`` touch, the ones that a sequence lacks, that others
-    hold too, or that the pool does not count, are replaced by free pages, the
-    lowest first, in the order of sequences and tokens; a shared page then
-    counts a holder less.
+    hold too, or that the pool does not count (they are free, and may be given
+    out), are replaced by free pages, the lowest first, in the order of
+    sequences and tokens; a shared page then counts a holder less.
     Where it holds tokens before ``lengths[b]`` it has to be copied before
     the write: from ``src[b]`` to ``dst[b]`` (-1: nothing to copy), which
     ``cache_copy`` takes, for every cache that the table serves.
 
     ``granted[b]``: the tokens that may be written, for ``cache_write``'s
     ``count``: all of them that the table's row can hold, or 0 where the pool
-    does not have enough for this sequence and those before it that lack some;
-    such a row stays as it is. All three ``[B]`` int32. Nothing waits for the GPU.
+    does not have enough for this sequence and those before it that lack some,
+    or where the sequence's last tokens lie in a page that the pool does not
+    count; such a row stays as it is. All three ``[B]`` int32. Nothing waits
+    for the GPU.
     """
     dev = _gpu(page_table, "page_table")
     _same_gpu(pool, "pool", dev)
