@@ -521,6 +521,50 @@ def test_stream_keeps_frames(bits, axes):
     full.push(images[:, [0, 1, 2]])
 
 
+def test_stream_gives_back_what_a_failed_push_reserved():
+    """A push that ends in an error leaves its pages with the stream, which gives them back when it is closed or starts over;
+    and the next push gives what it would have."""
+    from vasc_amd.streaming import AggregatorStream
+    model = _model(2)
+    images = torch.rand(1, 3, 3, 112, 140, generator=_gen(83)).cuda()
+    block = model.global_blocks[1]
+
+    def failing(*_args, **_kw):
+        raise RuntimeError("a block's own error")
+
+    def fail(stream, part):
+        block.forward = failing
+        try:
+            with pytest.raises(RuntimeError, match="own error"):
+                stream.push(images[:, part])
+        finally:
+            del block.forward
+
+    first = AggregatorStream(model, 3, sparse_ratio=0.0)
+    fail(first, [0])
+    first.reset()
+    assert first.pool.available() == first.pool.pages
+    fail(first, [0, 1])
+    first.close()
+    assert first.pool.available() == first.pool.pages
+
+    trunk = AggregatorStream(model, 3, sparse_ratio=0.0, branches=2)
+    trunk.push(images[:, [0]])
+    left = trunk.fork()
+    trunk.reset()
+    fail(trunk, [0, 1, 2])
+    trunk.close()
+    held = -(-left.lengths.item() // 64)
+    assert left.pool.available() == left.pool.pages - held
+    fail(left, [1])
+    got = left.push(images[:, [1]])[0]
+    alone = AggregatorStream(model, 3, sparse_ratio=0.0)
+    alone.push(images[:, [0]])
+    assert all(torch.equal(a, b) for a, b in zip(got, alone.push(images[:, [1]])[0]))
+    left.close()
+    assert left.pool.available() == left.pool.pages
+
+
 def test_arguments_that_are_refused():
     cache, pool = BlockCache(4, 2, 64, bits=4), PagePool(4)
     table, n = _i32([[0, 1], [2, 3]]), _i32([5, 6])

@@ -234,7 +234,7 @@ class AggregatorStream:
 
     def reset(self) -> None:
         self._open()
-        if self.frames:
+        if self.pool is not None:  # whatever is held: a push that failed has reserved pages, too
             with ops.on_device(self.pool.device_index):
                 ops.pages_free(self.pool, self.page_table, self.lengths)
         self.frames = self._seen = 0
@@ -344,7 +344,8 @@ class AggregatorStream:
         pos_global = pos.view(B, n * P, -1)
         before, after = self.frames * P, (self.frames + n) * P
         start = self.lengths
-        # there are pages for `branches` streams of max_frames frames: everything is granted
+        # there are pages for `branches` streams of max_frames frames, and no stream holds more, a failed push's among
+        # them: everything is granted
         granted, src, dst = ops.pages_reserve(self.pool, self.page_table, start, n * P)
         if self._forked:
             for cache in self.caches:
