@@ -334,6 +334,24 @@ def test_offsets_past_32_bits():
         assert _same(_np(rk[b]), held[b][0][:, :500:2]) and _same(_np(rv[b]), held[b][1][:, :500:2])
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("D,H", [(64, 16), (128, 8)])
+@pytest.mark.parametrize("bits", [4, 8])
+def test_reads_of_much_and_little(bits, D, H, dtype):
+    """Outputs of 128 MB and more are stored in another way than smaller ones; the rows are the same."""
+    T = (1 << 27) // (2 * H * D * dtype.itemsize)
+    cache = BlockCache(-(-T // 64) + 1, H, D, bits=bits)
+    g = torch.Generator(device="cuda").manual_seed(5)
+    k, v = (torch.randn(1, H, T, D, device="cuda", generator=g, dtype=torch.bfloat16) for _ in range(2))
+    table = torch.arange(1, cache.pages, device="cuda", dtype=torch.int32).view(1, -1)
+    ops.cache_write(cache, k, v, table, _i32([0]))
+    ko, vo = ops.cache_read(cache, table, _i32([0]), T, count=_i32([T - 5]), dtype=dtype)
+    for at, n in ((0, T // 2), (T // 2, T - 5 - T // 2)):
+        a, b = ops.cache_read(cache, table, _i32([at]), n, dtype=dtype)
+        assert torch.equal(ko[:, :, at:at + n], a) and torch.equal(vo[:, :, at:at + n], b)
+    assert not ko[:, :, -5:].any() and not vo[:, :, -5:].any()
+
+
 def test_step_captured_in_graphs():
     """Write, choice and attention in two graphs with their own memory, replayed in turn with eager work between."""
     g = _gen(3)

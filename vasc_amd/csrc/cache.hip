@@ -160,7 +160,7 @@ __global__ __launch_bounds__(256) void cache_write_kernel(const CacheArgs c, con
   }
 }
 
-template <typename T, int D>
+template <typename T, int D, bool kPast>
 __global__ __launch_bounds__(256) void cache_read_kernel(const CacheArgs c, const RowArgs r) {
   constexpr int kLanes = D / 8, kRows = 256 / kLanes, kS = tile_stride<D>();
   __shared__ __align__(16) uint8_t vt[kPage * kS];
@@ -211,8 +211,8 @@ __global__ __launch_bounds__(256) void cache_read_kernel(const CacheArgs c, cons
         }
       }
     }
-    store8(ko + t * D + col, x);
-    store8(vo + t * D + col, y);
+    store8<kPast>(ko + t * D + col, x);
+    store8<kPast>(vo + t * D + col, y);
   }
 }
 
@@ -629,7 +629,10 @@ void launch_write(const CacheArgs &c, const RowArgs &r, hipStream_t s) {
 }
 template <typename T, int D>
 void launch_read(const CacheArgs &c, const RowArgs &r, hipStream_t s) {
-  hipLaunchKernelGGL((cache_read_kernel<T, D>), dim3(static_cast<unsigned>(r.B * r.H * r.span)), dim3(256), 0, s, c, r);
+  const dim3 grid(static_cast<unsigned>(r.B * r.H * r.span));
+  const bool past = r.B * r.H * r.T * D * static_cast<int64_t>(2 * sizeof(T)) >= kReadPast;
+  if (past) hipLaunchKernelGGL((cache_read_kernel<T, D, true>), grid, dim3(256), 0, s, c, r);
+  else hipLaunchKernelGGL((cache_read_kernel<T, D, false>), grid, dim3(256), 0, s, c, r);
 }
 
 }  // namespace

@@ -220,7 +220,7 @@ __global__ __launch_bounds__(256) void cache4_write_kernel(const CacheArgs c, co
   }
 }
 
-template <typename T, int D>
+template <typename T, int D, bool kPast>
 __global__ __launch_bounds__(256) void cache4_read_kernel(const CacheArgs c, const RowArgs r) {
   constexpr int kLanes = D / 8, kRows = 256 / kLanes, kG = D / 32;
   constexpr int kS = 36;  // bytes of a feature in LDS: eight features on, eight banks on
@@ -275,8 +275,8 @@ __global__ __launch_bounds__(256) void cache4_read_kernel(const CacheArgs c, con
       unpack_e2m1(kw[pass], x, ke);
       unpack_e2m1(vw, y, ve);
     }
-    store8(ko + t * D + col, x);
-    store8(vout + t * D + col, y);
+    store8<kPast>(ko + t * D + col, x);
+    store8<kPast>(vout + t * D + col, y);
   }
 }
 
@@ -286,7 +286,10 @@ void launch_write4(const CacheArgs &c, const RowArgs &r, hipStream_t s) {
 }
 template <typename T, int D>
 void launch_read4(const CacheArgs &c, const RowArgs &r, hipStream_t s) {
-  hipLaunchKernelGGL((cache4_read_kernel<T, D>), dim3(static_cast<unsigned>(r.B * r.H * r.span)), dim3(256), 0, s, c, r);
+  const dim3 grid(static_cast<unsigned>(r.B * r.H * r.span));
+  const bool past = r.B * r.H * r.T * D * static_cast<int64_t>(2 * sizeof(T)) >= kReadPast;
+  if (past) hipLaunchKernelGGL((cache4_read_kernel<T, D, true>), grid, dim3(256), 0, s, c, r);
+  else hipLaunchKernelGGL((cache4_read_kernel<T, D, false>), grid, dim3(256), 0, s, c, r);
 }
 
 }  // namespace

@@ -24,8 +24,9 @@ struct RowArgs {
   int span;  // pages that T tokens can touch
 };
 
-// Eight consecutive elements as floats. The rows to be written into a cache are read once: past the caches (32 frames on
-// data that is not in them 73 us with the read back, 70 so).
+// Eight consecutive elements as floats. The rows to be written into a cache are read once: past the caches. Measured, 16 heads
+// of 64, in us with plain loads and so: two products that make the rows and the write after them, 1041 tokens 11.8 and 11.8,
+// 4164 22.3 and 21.1, 16656 44.7 and 45.1, 33312 84.4 and 82.9; 32 frames that are in no cache 73 and 70 with the read back.
 template <typename T>
 __device__ __forceinline__ void load8(const T *src, float (&x)[8]) {
   struct alignas(16) Eight { T v[8]; };
@@ -43,9 +44,16 @@ __device__ __forceinline__ void load8(const T *src, float (&x)[8]) {
   for (int i = 0; i < 8; ++i) x[i] = to_f32(e.v[i]);
 }
 
-// Past the caches: rows that are read back are mostly more than these hold (heads' quarter of the tokens of 16 sequences,
-// 268 MB: 71 us with plain stores, 50 so; 32 frames 28.0 and 26.6).
-template <typename T>
+// Rows that are read back are mostly used at once, and go past the caches (kPast) only where these would hardly hold them:
+// where the two outputs have 128 MB, half the cache behind HBM, which the codes and what is made of the rows want as well.
+// Measured (8 bits, 16 heads of 64), in us with plain stores and past the caches, the read and the sum k + v after it: one token
+// 5.8 and 6.4, 1041 tokens 8.8 and 9.4, 4164 15.6 and 16.0 (8 heads of 128: 16.6 and 16.3). Larger outputs, again and again
+// and after a fill of 100 us that empties the caches: 68 MB 34 and 36, 136 and 148; 98 MB 46 and 50, 155 and 170; 136 MB 71
+// and 65, 176 and 199; 205 MB 104 and 113, 217 and 233; 273 MB 161 and 155, 275 and 275. The read by itself: 98 MB 25 and 24,
+// 136 MB 33 and 32.5, 273 MB 87 and 62 (4 bits: 75 and 53).
+constexpr int64_t kReadPast = int64_t(1) << 27;
+
+template <bool kPast, typename T>
 __device__ __forceinline__ void store8(T *dst, const float (&x)[8]) {
   typedef uint32_t words __attribute__((ext_vector_type(sizeof(T) == 4 ? 8 : 4)));
   struct alignas(sizeof(words)) Eight { T v[8]; };
@@ -53,9 +61,13 @@ __device__ __forceinline__ void store8(T *dst, const float (&x)[8]) {
 #pragma unroll
   for (int i = 0; i < 8; ++i) e.v[i] = from_f32<T>(x[i]);
   const words w = __builtin_bit_cast(words, e);
+  const auto put = [&](u32x4 v, u32x4 *to) {
+    if constexpr (kPast) __builtin_nontemporal_store(v, to);
+    else *to = v;
+  };
   u32x4 *to = reinterpret_cast<u32x4 *>(dst);
-  __builtin_nontemporal_store(u32x4{w[0], w[1], w[2], w[3]}, to);
-  if constexpr (sizeof(T) == 4) __builtin_nontemporal_store(u32x4{w[4], w[5], w[6], w[7]}, to + 1);
+  put(u32x4{w[0], w[1], w[2], w[3]}, to);
+  if constexpr (sizeof(T) == 4) put(u32x4{w[4], w[5], w[6], w[7]}, to + 1);
 }
 
 struct PageWork {
