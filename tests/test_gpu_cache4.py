@@ -338,7 +338,7 @@ def test_offsets_past_32_bits():
 @pytest.mark.parametrize("D,H", [(64, 16), (128, 8)])
 @pytest.mark.parametrize("bits", [4, 8])
 def test_reads_of_much_and_little(bits, D, H, dtype):
-    """Outputs of 128 MB and more are stored in another way than smaller ones; the rows are the same."""
+    """Outputs of 128 MB and more are stored in another way than smaller ones (half types); the rows are the same."""
     T = (1 << 27) // (2 * H * D * dtype.itemsize)
     cache = BlockCache(-(-T // 64) + 1, H, D, bits=bits)
     g = torch.Generator(device="cuda").manual_seed(5)
@@ -350,6 +350,24 @@ def test_reads_of_much_and_little(bits, D, H, dtype):
         a, b = ops.cache_read(cache, table, _i32([at]), n, dtype=dtype)
         assert torch.equal(ko[:, :, at:at + n], a) and torch.equal(vo[:, :, at:at + n], b)
     assert not ko[:, :, -5:].any() and not vo[:, :, -5:].any()
+
+
+@pytest.mark.parametrize("D,H", [(64, 16), (128, 8)])
+@pytest.mark.parametrize("bits", [4, 8])
+def test_writes_of_much_and_little(bits, D, H):
+    """Float32 rows of 256 MB and more are loaded in another way than fewer; the cache's bytes are the same."""
+    T = (1 << 28) // (2 * H * D * 4)
+    a, b = (BlockCache(-(-T // 64), H, D, bits=bits) for _ in range(2))
+    g = torch.Generator(device="cuda").manual_seed(6)
+    k, v = (torch.randn(1, H, T, D, device="cuda", generator=g) for _ in range(2))
+    k[0, 1, 77, 3] = float("nan")
+    table = torch.arange(a.pages, device="cuda", dtype=torch.int32).view(1, -1)
+    ops.cache_write(a, k, v, table, _i32([0]))
+    for at, n in ((0, T // 2 + 9), (T // 2 + 9, T - T // 2 - 9)):
+        ops.cache_write(b, k[:, :, at:at + n], v[:, :, at:at + n], table, _i32([at]))
+    for name in ("kc", "vc", "ks", "vs", "vo", "mean"):
+        x, y = getattr(a, name), getattr(b, name)
+        assert x is None or torch.equal(x.view(torch.uint8), y.view(torch.uint8)), name
 
 
 def test_step_captured_in_graphs():

@@ -38,7 +38,7 @@ __device__ __forceinline__ void quantise8(const float (&x)[8], int byte, uint32_
 template <int D>
 constexpr int tile_stride() { return D + 4; }
 
-template <typename T, int D>
+template <typename T, int D, bool kPast>
 __global__ __launch_bounds__(256) void cache_write_kernel(const CacheArgs c, const RowArgs r) {
   constexpr int kLanes = D / 8, kRows = 256 / kLanes, kS = tile_stride<D>();
   constexpr int kGroups = 256 / (D / 4);  // row groups of the mean, four columns a thread
@@ -64,8 +64,8 @@ __global__ __launch_bounds__(256) void cache_write_kernel(const CacheArgs c, con
     } else if (row < w.hi) {
       const int64_t t = w.j * kPage + row - w.s;
       float x[8], y[8];
-      load8(kin + t * r.kst + col, x);
-      load8(vin + t * r.vst + col, y);
+      load8<kPast>(kin + t * r.kst + col, x);
+      load8<kPast>(vin + t * r.vst + col, y);
       float kmax = 0.f, vmax = 0.f, bad = 0.f;
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
@@ -625,14 +625,25 @@ __global__ __launch_bounds__(kWaves * 64) void cache_list_kernel(const SelectPar
 
 template <typename T, int D>
 void launch_write(const CacheArgs &c, const RowArgs &r, hipStream_t s) {
-  hipLaunchKernelGGL((cache_write_kernel<T, D>), dim3(static_cast<unsigned>(r.B * r.H * r.span)), dim3(256), 0, s, c, r);
+  const dim3 grid(static_cast<unsigned>(r.B * r.H * r.span));
+  if constexpr (sizeof(T) == 4) {
+    if (!floats_past(r, D)) {
+      hipLaunchKernelGGL((cache_write_kernel<T, D, false>), grid, dim3(256), 0, s, c, r);
+      return;
+    }
+  }
+  hipLaunchKernelGGL((cache_write_kernel<T, D, true>), grid, dim3(256), 0, s, c, r);
 }
 template <typename T, int D>
 void launch_read(const CacheArgs &c, const RowArgs &r, hipStream_t s) {
   const dim3 grid(static_cast<unsigned>(r.B * r.H * r.span));
-  const bool past = r.B * r.H * r.T * D * static_cast<int64_t>(2 * sizeof(T)) >= kReadPast;
-  if (past) hipLaunchKernelGGL((cache_read_kernel<T, D, true>), grid, dim3(256), 0, s, c, r);
-  else hipLaunchKernelGGL((cache_read_kernel<T, D, false>), grid, dim3(256), 0, s, c, r);
+  if constexpr (sizeof(T) == 2) {
+    if (halves_past(r, D)) {
+      hipLaunchKernelGGL((cache_read_kernel<T, D, true>), grid, dim3(256), 0, s, c, r);
+      return;
+    }
+  }
+  hipLaunchKernelGGL((cache_read_kernel<T, D, false>), grid, dim3(256), 0, s, c, r);
 }
 
 }  // namespace

@@ -25,13 +25,14 @@ struct Eight {
   typedef uint32_t words __attribute__((ext_vector_type(sizeof(T) == 4 ? 8 : 4)));
   words w;
 
+  template <bool kPast>
   __device__ __forceinline__ void load(const T *src) {
     const u32x4 *from = reinterpret_cast<const u32x4 *>(src);
-    const u32x4 a = __builtin_nontemporal_load(from);
+    const u32x4 a = load16<kPast>(from);
     if constexpr (sizeof(T) == 2) {
       w = a;
     } else {
-      const u32x4 b = __builtin_nontemporal_load(from + 1);
+      const u32x4 b = load16<kPast>(from + 1);
       w = words{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
     }
   }
@@ -102,7 +103,7 @@ __device__ __forceinline__ int groups_max(int v) {
   return D == 128 ? max(v, xor_lane(v, 8)) : v;
 }
 
-template <typename T, int D>
+template <typename T, int D, bool kPast>
 __global__ __launch_bounds__(256) void cache4_write_kernel(const CacheArgs c, const RowArgs r) {
   constexpr int kLanes = D / 8, kRows = 256 / kLanes, kG = D / 32;
   constexpr int kS = kLanes + 1;         // words of a value row in LDS: four rows on, four banks on
@@ -130,8 +131,8 @@ __global__ __launch_bounds__(256) void cache4_write_kernel(const CacheArgs c, co
     } else if (row < w.hi) {
       const int64_t t = w.j * kPage + row - w.s;
       Eight<T> x, y;
-      x.load(kin + t * r.kst + col);
-      y.load(vin + t * r.vst + col);
+      x.template load<kPast>(kin + t * r.kst + col);
+      y.template load<kPast>(vin + t * r.vst + col);
       const uint32_t ktop = group4_max(x.top()), vtop = group4_max(y.top());
       int kb = power_of<2>(Eight<T>::value(ktop), -60, 60) + 127, vb = power_of<2>(Eight<T>::value(vtop), -60, 60) + 127;
       int row_b = groups_max<D>(vb);
@@ -282,14 +283,25 @@ __global__ __launch_bounds__(256) void cache4_read_kernel(const CacheArgs c, con
 
 template <typename T, int D>
 void launch_write4(const CacheArgs &c, const RowArgs &r, hipStream_t s) {
-  hipLaunchKernelGGL((cache4_write_kernel<T, D>), dim3(static_cast<unsigned>(r.B * r.H * r.span)), dim3(256), 0, s, c, r);
+  const dim3 grid(static_cast<unsigned>(r.B * r.H * r.span));
+  if constexpr (sizeof(T) == 4) {
+    if (!floats_past(r, D)) {
+      hipLaunchKernelGGL((cache4_write_kernel<T, D, false>), grid, dim3(256), 0, s, c, r);
+      return;
+    }
+  }
+  hipLaunchKernelGGL((cache4_write_kernel<T, D, true>), grid, dim3(256), 0, s, c, r);
 }
 template <typename T, int D>
 void launch_read4(const CacheArgs &c, const RowArgs &r, hipStream_t s) {
   const dim3 grid(static_cast<unsigned>(r.B * r.H * r.span));
-  const bool past = r.B * r.H * r.T * D * static_cast<int64_t>(2 * sizeof(T)) >= kReadPast;
-  if (past) hipLaunchKernelGGL((cache4_read_kernel<T, D, true>), grid, dim3(256), 0, s, c, r);
-  else hipLaunchKernelGGL((cache4_read_kernel<T, D, false>), grid, dim3(256), 0, s, c, r);
+  if constexpr (sizeof(T) == 2) {
+    if (halves_past(r, D)) {
+      hipLaunchKernelGGL((cache4_read_kernel<T, D, true>), grid, dim3(256), 0, s, c, r);
+      return;
+    }
+  }
+  hipLaunchKernelGGL((cache4_read_kernel<T, D, false>), grid, dim3(256), 0, s, c, r);
 }
 
 }  // namespace

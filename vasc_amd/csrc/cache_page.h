@@ -24,20 +24,34 @@ struct RowArgs {
   int span;  // pages that T tokens can touch
 };
 
-// Eight consecutive elements as floats. The rows to be written into a cache are read once: past the caches. Measured, 16 heads
+// 16 bytes of a tensor that is read once; kPast: past the caches.
+template <bool kPast>
+__device__ __forceinline__ u32x4 load16(const u32x4 *from) {
+  if constexpr (kPast) return __builtin_nontemporal_load(from);
+  else return *from;
+}
+
+// The rows to be written into a cache are read past the caches (kPast), in half types whatever their number. Measured, 16 heads
 // of 64, in us with plain loads and so: two products that make the rows and the write after them, 1041 tokens 11.8 and 11.8,
 // 4164 22.3 and 21.1, 16656 44.7 and 45.1, 33312 84.4 and 82.9; 32 frames that are in no cache 73 and 70 with the read back.
-template <typename T>
+// A lane's eight floats are two loads, each of half of every 32 bytes, which fetch a line twice: float32 rows go past the
+// caches from 256 MB on, where these have lost them anyway: 34 MB 27 and 30, 68 MB 40.5 and 48, 136 MB 75 and 81, 273 MB 155
+// and 153.5, 546 MB 317 and 310; rows that are in no cache, with 100 us for emptying these, 123 and 115, 148 and 133, 194 and
+// 166, 260 and 236 from 68 MB on.
+bool floats_past(const RowArgs &r, int64_t D) { return r.B * r.H * r.T * D * 8 >= int64_t(1) << 28; }
+
+// Eight consecutive elements as floats.
+template <bool kPast, typename T>
 __device__ __forceinline__ void load8(const T *src, float (&x)[8]) {
   struct alignas(16) Eight { T v[8]; };
   const u32x4 *from = reinterpret_cast<const u32x4 *>(src);
-  const u32x4 a = __builtin_nontemporal_load(from);
+  const u32x4 a = load16<kPast>(from);
   Eight e;
   if constexpr (sizeof(T) == 2) {
     e = __builtin_bit_cast(Eight, a);
   } else {
     typedef uint32_t words __attribute__((ext_vector_type(8)));
-    const u32x4 b = __builtin_nontemporal_load(from + 1);
+    const u32x4 b = load16<kPast>(from + 1);
     e = __builtin_bit_cast(Eight, words{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]});
   }
 #pragma unroll
@@ -50,8 +64,10 @@ __device__ __forceinline__ void load8(const T *src, float (&x)[8]) {
 // 5.8 and 6.4, 1041 tokens 8.8 and 9.4, 4164 15.6 and 16.0 (8 heads of 128: 16.6 and 16.3). Larger outputs, again and again
 // and after a fill of 100 us that empties the caches: 68 MB 34 and 36, 136 and 148; 98 MB 46 and 50, 155 and 170; 136 MB 71
 // and 65, 176 and 199; 205 MB 104 and 113, 217 and 233; 273 MB 161 and 155, 275 and 275. The read by itself: 98 MB 25 and 24,
-// 136 MB 33 and 32.5, 273 MB 87 and 62 (4 bits: 75 and 53).
-constexpr int64_t kReadPast = int64_t(1) << 27;
+// 136 MB 33 and 32.5, 273 MB 87 and 62 (4 bits: 75 and 53). Float32 rows never do: their two stores a lane have half of every
+// 32 bytes each, which only the caches join (the read by itself 136 MB 30 and 59, 546 MB 169 and 226, with the sum 321 and 299;
+// 4 bits 151 and 229, 305 and 339).
+bool halves_past(const RowArgs &r, int64_t D) { return r.B * r.H * r.T * D * 4 >= int64_t(1) << 27; }
 
 template <bool kPast, typename T>
 __device__ __forceinline__ void store8(T *dst, const float (&x)[8]) {
@@ -61,13 +77,12 @@ __device__ __forceinline__ void store8(T *dst, const float (&x)[8]) {
 #pragma unroll
   for (int i = 0; i < 8; ++i) e.v[i] = from_f32<T>(x[i]);
   const words w = __builtin_bit_cast(words, e);
-  const auto put = [&](u32x4 v, u32x4 *to) {
-    if constexpr (kPast) __builtin_nontemporal_store(v, to);
-    else *to = v;
-  };
+  static_assert(!kPast || sizeof(T) == 2, "float32 rows stay in the caches");
   u32x4 *to = reinterpret_cast<u32x4 *>(dst);
-  put(u32x4{w[0], w[1], w[2], w[3]}, to);
-  if constexpr (sizeof(T) == 4) put(u32x4{w[4], w[5], w[6], w[7]}, to + 1);
+  const u32x4 a = {w[0], w[1], w[2], w[3]};
+  if constexpr (kPast) __builtin_nontemporal_store(a, to);
+  else *to = a;
+  if constexpr (sizeof(T) == 4) to[1] = u32x4{w[4], w[5], w[6], w[7]};
 }
 
 struct PageWork {
