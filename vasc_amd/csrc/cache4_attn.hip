@@ -39,9 +39,12 @@ __device__ __forceinline__ halfx8 widen4(uint32_t w, const halfx8 &power) {
   return __builtin_bit_cast(halfx8, x) * power;
 }
 
-// A lane's 16 bytes of each kilobyte. kOnce: no other unit reads them, and they go past the caches. Measured, in us: single
-// tokens of 16 sequences up to 131072 long 285 with plain loads, 253 so; eight units of 16 tokens over the same pages 32.2
-// with plain loads, 34.1 so.
+// A lane's 16 bytes of each kilobyte. kOnce: the call has one unit a head, so a sequence's pages are read once, and go past the
+// caches. Measured with plain loads and so, in us: single tokens of 16 sequences up to 131072 long 285 and 253; calls again and
+// again over 1 to 145 MB of codes the same to 3%, over 519 MB 102 and 92, and after the caches were emptied 5 MB 15.0 and 14.2,
+// 36 MB 27 and 21.5, 145 MB 71 and 46. Units that share pages want the caches (eight of 16 tokens 32.2 and 34.1), and so do
+// branches of one parent, whose tables the host does not see: eight each of four, 16384 tokens long, 80 and 82 (D = 64: 95 and
+// 100), 100000 long 438 and 443 to 455, 32 of one 181 and 190.
 template <bool kOnce, int n>
 __device__ __forceinline__ void load_codes(u32x4 (&x)[n], const uint8_t *at) {
   if constexpr (kOnce) {
@@ -197,8 +200,11 @@ __global__ __launch_bounds__(256, 2) void cache4_attn_few_kernel(const AttnParam
   if (wave == 0) rows.template store<Q>(p, w, 0, col, g, m);
 }
 
-// Many rows (up to 128): the vector and matrix pipes bound the kernel. As for the 8-bit cache the kWaves waves lie side by
-// side over the rows, and a page is widened once for all of them, in LDS, two buffers and one barrier a page.
+// Many rows (up to 128): no pipe is full (a frame: matrix 24 %, 39 % of the waves' cycles waiting, 2130 cycles a wave's page
+// where the same products and exponentials from registers take 1110); what binds is a page's chain of dependent steps, from
+// barrier and operands over product, maximum and exponentials to the second product, at two or three waves a SIMD. As for the
+// 8-bit cache the kWaves waves lie side by side over the rows, and a page is widened once for all of them, in LDS, two buffers
+// and one barrier a page.
 // Measured: a frame of 1041 queries over 522 of 2082 pages, 16 heads of 64, 142 GFLOP in 238 us with the join (600 TFLOP/s);
 // 250 causal tokens of 32 heads of 128 over 20001, 163 GFLOP in 193 us (840). The frame's parts, each left out of a copy for
 // its time alone: the softmax 79 us, the operands' reads from LDS 27, the pages' loads 23; what stays, widening, products and

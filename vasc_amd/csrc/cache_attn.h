@@ -498,7 +498,9 @@ struct Shape {
 // rule's, in us: 144 units of a frame (the rule takes 5) 234 with 5, 279 with 4, 289 with 6, 237 with 10, 259 with 16;
 // a causal chunk of 128 units (4) 208 with 4, 303 with 2, 219 with 8; 128 units of single tokens, 258 pages (4) 108 with 4,
 // 138 with 1, 107 with 2, 112 with 8; of 521 pages (8) 85 with 8, 82 with 4, 83 with 16. The pages are the list's width or the
-// table's, as the lengths are on the device: short sequences in a long table leave parts empty.
+// table's, as the lengths are on the device: short sequences in a long table leave parts empty. The 0.3 holds where the loads
+// of all CUs' waves overlap; a page by itself takes longer: 16 units of 18 pages, five to a wave, 10 us where the estimate says
+// 4.5.
 Shape attn_shape(int64_t units, int64_t rows, int64_t pages, int64_t D) {
   Shape s;
   s.kind = rows <= 16 ? 0 : rows <= 32 ? 1 : rows <= 64 ? 2 : 3;

@@ -184,7 +184,8 @@ __global__ __launch_bounds__(256, 2) void cache_attn_few_kernel(const AttnParams
   if (wave == 0) rows.template store<Q>(p, w, 0, col, g, m);
 }
 
-// Many rows (up to 128): the vector and matrix pipes bound the kernel. The kWaves waves lie side by side over the rows, and
+// Many rows (up to 128): neither the vector nor the matrix pipe is full (63 % and 27 % of a frame's cycles); a page's chain of
+// dependent steps binds, at two or three waves a SIMD. The kWaves waves lie side by side over the rows, and
 // a page is widened once for all of them: each wave turns its share of the codes into operands in LDS (keys as bfloat16 with
 // their powers, values as half, and the values' exponents as floats), 16 bytes a lane in the order in which they are read.
 // Two buffers and one barrier a page: the next page's codes are on their way to registers while this one is computed.

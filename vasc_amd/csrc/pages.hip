@@ -4,9 +4,10 @@
 // The counts are all that is kept: a page is free where its count is not positive, and the lowest free pages are given out
 // first. So what a call gives does not depend on the order of earlier calls, of its own atomics, or of its workgroups.
 //
-// Measured, in us: eight branches of four sequences of up to 64 pages: fork 2.6, reserve 6.4, copy 4.7, free 2.6, the latency
+// Measured, in us: eight branches of four sequences of up to 64 pages: fork 2.6, reserve 6.6, copy 4.5, free 2.5, the latency
 // of a few loads that depend on one another; 256 branches of 64 sequences of up to 1024 pages, in a pool of 45000: 9.2,
-// 7.3 and 6.4, 5.5, 9.2. A host that calls them one by one takes longer for each (5 to 12).
+// 7.2 and 5.8, 5.8, 9.3. A host that calls them one by one takes longer for each (5 to 12): the four calls 32 and 37, in a
+// graph 14.5 and 35.
 #include "cache_page.h"
 
 namespace vasc {
@@ -76,9 +77,9 @@ __device__ __forceinline__ uint32_t quad_transpose(uint32_t v) {
 // One workgroup writes one (page, head), 64 chosen tokens from wherever they lie. Keys are rows. Values lie transposed, a
 // byte (or half of one) of a feature a token: a wave reads a feature of its 64 tokens at a time, which is one 64-byte line
 // where they are neighbours and never more than a line a token, and turns 4 x 4 bytes between lanes for the store.
-// Bound by HBM and by those lines: a quarter of the tokens of 16 sequences, others for each of 8 heads of 128 (4 bits), in
-// 51 us, four source pages' values read for each page written (126 MB of traffic by the counters); 32 of 128 frames, 16 heads of 64 (8 bits),
-// in 31 us (4.4 TB/s).
+// Bound by the accesses to the first cache where single tokens are kept, and by HBM where runs are: a quarter of the tokens of
+// 16 sequences, others for each of 8 heads of 128 (4 bits), in 51 us, 24.1e6 accesses (94000 in a CU's 141000 cycles, some 30 a
+// load of a feature) and 126 MB of traffic (2.5 TB/s); 32 of 128 frames, 16 heads of 64 (8 bits), in 31 us (4.4 TB/s).
 template <int D, int kBits>
 __global__ __launch_bounds__(256) void compact_kernel(const CompactArgs p) {
   constexpr int kG = D / 32, kRowBytes = D * kBits / 8;

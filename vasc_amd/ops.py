@@ -960,10 +960,11 @@ def cache_write(cache, k: torch.Tensor, v: torch.Tensor, page_table: torch.Tenso
     (entries outside the cache: nothing is written there); no page may occur
     twice among the pages one call writes. Each (token, head) row is rounded
     to e4m3 values times a power of two (4 bits: each 32 features of it to
-    e2m1 values times one), and every touched page's key mean is renewed over its tokens up to the last one written, so the tokens before
-    ``start`` in its page must be there, and writing further back drops what
-    came after. A token whose k or v row holds a value that is not finite is
-    held as NaN in both. Nothing here waits for the GPU.
+    e2m1 values times one), and every touched page's key mean is renewed over
+    its tokens up to the last one written, so the tokens before ``start`` in
+    its page must be there, and writing further back drops what came after. A
+    token whose k or v row holds a value that is not finite is held as NaN in
+    both. Nothing here waits for the GPU.
     """
     dev = _gpu(k, "k")
     _gpu(v, "v", dev)

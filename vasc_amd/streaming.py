@@ -94,7 +94,8 @@ class PagePool:
     """Who holds the pages of one or more block caches that a page table serves.
 
     ``refs [pages]`` int32 on the GPU counts each page's holders, the entries
-    of page tables that name it: a page is free where it is 0.
+    of page tables that name it: a page is free where it is not positive, also
+    where an entry names it that no operator has put there.
     ``ops.pages_reserve`` gives sequences the lowest free pages, ``pages_fork``
     lets sequences share pages, ``pages_free`` gives them back; a table starts
     as -1 throughout. Nothing is kept on the host, so that a captured call
@@ -209,7 +210,11 @@ class AggregatorStream:
     ``fork()`` gives another stream that goes on from here, with the frames so
     far in pages that both share; up to ``branches`` streams at once, each of
     at most ``max_frames`` frames (the caches hold so many), until
-    ``close()``. ``keep(frames)`` forgets the frames that it does not list.
+    ``close()``. ``keep(frames)`` forgets the frames that it does not list; it
+    needs free pages for those that stay, so a stream that forgets when it
+    holds n frames and keeps m of them wants ``max_frames`` n + m + 1 (frames of
+    64 tokens or more). Streams that share caches are called one after another,
+    as the pool's operators; the pool is theirs alone.
     """
 
     def __init__(self, model, max_frames: int, *, sparse_ratio: float = 0.75, sink: int = 1, recent: int = 1, bits: int = 8,
@@ -264,7 +269,8 @@ class AggregatorStream:
         return other
 
     def keep(self, frames) -> None:
-        """Forgets all frames but the listed ones (places among those held, ascending); their tokens move to free pages."""
+        """Forgets all frames but the listed ones (places among those held, ascending); their tokens move to free pages, of
+        which there must be enough for them beside all that are held. Waits for the GPU."""
         self._open()
         frames = [int(f) for f in frames]
         if not frames or any(b <= a for a, b in zip(frames, frames[1:])) or frames[0] < 0 or frames[-1] >= self.frames:
