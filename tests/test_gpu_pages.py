@@ -565,6 +565,33 @@ def test_stream_gives_back_what_a_failed_push_reserved():
     assert left.pool.available() == left.pool.pages
 
 
+def test_stream_keeps_everything_if_forgetting_fails(monkeypatch):
+    """keep() that ends in an error between two layers leaves the stream and the pool as they were."""
+    from vasc_amd.streaming import AggregatorStream
+    model = _model(2)
+    images = torch.rand(1, 4, 3, 112, 140, generator=_gen(89)).cuda()
+    s, alone = (AggregatorStream(model, 7, sparse_ratio=0.0) for _ in range(2))
+    for stream in (s, alone):
+        stream.push(images[:, :3])
+    free, calls, compact = s.pool.available(), [], ops.cache_compact
+
+    def second_fails(*args):
+        calls.append(args)
+        if len(calls) == 2:
+            raise RuntimeError("an error of its own")
+        compact(*args)
+
+    monkeypatch.setattr(ops, "cache_compact", second_fails)
+    with pytest.raises(RuntimeError, match="of its own"):
+        s.keep((0, 2))
+    monkeypatch.undo()
+    assert s.pool.available() == free and s.frames == 3
+    assert all(torch.equal(a, b) for a, b in zip(s.push(images[:, 3:])[0], alone.push(images[:, 3:])[0]))
+    s.keep((1, 3))
+    alone.keep((1, 3))
+    assert all(torch.equal(a, b) for a, b in zip(s.push(images[:, :1])[0], alone.push(images[:, :1])[0]))
+
+
 def test_arguments_that_are_refused():
     cache, pool = BlockCache(4, 2, 64, bits=4), PagePool(4)
     table, n = _i32([[0, 1], [2, 3]]), _i32([5, 6])

@@ -289,8 +289,12 @@ class AggregatorStream:
             index = torch.cat([torch.arange(at, at + m, dtype=torch.int32) for at, m in runs]).to(self.page_table.device)
             table, lengths = torch.full_like(self.page_table, -1), torch.zeros_like(self.lengths)
             granted, _, _ = ops.pages_reserve(self.pool, table, lengths, n)
-            for cache in self.caches:
-                ops.cache_compact(cache, self.page_table, index.expand(B, n), table)
+            try:
+                for cache in self.caches:
+                    ops.cache_compact(cache, self.page_table, index.expand(B, n), table)
+            except BaseException:  # the frames are still where they were
+                ops.pages_free(self.pool, table, lengths)
+                raise
             ops.pages_free(self.pool, self.page_table, self.lengths)
             self.page_table, self.lengths = table, granted.clone()
         at, tokens = 0, []
